@@ -704,6 +704,198 @@ int brx_moe_block_forward_noalloc(const brx_layer_desc* d, brx_pool* p, const vo
                               out_w, flags, stream, sp, BRX_NOALLOC_SCRATCH_BYTES);
 }
 
+// ------------------------------------------------------------------ MXFP4 activations
+static int check_rows(int dtype, int64_t batch, int64_t rows, int64_t cols) {
+    if (dtype != BRX_DT_F32 && dtype != BRX_DT_BF16 && dtype != BRX_DT_F16) return fail(BRX_EINVAL, "dtype %d unknown", dtype);
+    if (batch < 0 || rows < 0 || cols < 0)
+        return fail(BRX_EINVAL, "negative size (batch=%lld, rows=%lld, cols=%lld)", (long long)batch, (long long)rows, (long long)cols);
+    if (cols % 32) return fail(BRX_EINVAL, "cols %lld must be a multiple of 32 (MXFP4's groups)", (long long)cols);
+    const int64_t most = (int64_t)1 << 40;
+    if (cols > (1 << 30) || (cols && rows > most / cols) || (cols && rows && batch > most / (rows * cols)))
+        return fail(BRX_EINVAL, "%lld x %lld x %lld values are more than 2^40, or cols is more than 2^30", (long long)batch,
+                    (long long)rows, (long long)cols);
+    return BRX_OK;
+}
+
+int brx_mx_quantize(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int64_t x_batch_stride,
+                    int64_t x_row_stride, void* codes, int64_t codes_batch_stride, void* scales,
+                    int64_t scales_batch_stride, void* stream) {
+    int rc = check_rows(dtype, batch, rows, cols);
+    if (rc) return rc;
+    if ((rc = ensure_device())) return rc;
+    if (!batch || !rows || !cols) return BRX_OK;
+    if (!x || !codes || !scales) return fail(BRX_EINVAL, "x, codes and scales are required");
+    if ((uintptr_t)x & (dtype == BRX_DT_F32 ? 3 : 1)) return fail(BRX_EINVAL, "x is not aligned to its type");
+    if (batch > 1 && (codes_batch_stride < rows * (cols / 2) || scales_batch_stride < rows * (cols / 32)))
+        return fail(BRX_EINVAL, "the matrices' codes or scales overlap: strides of %lld and %lld bytes for %lld x %lld values",
+                    (long long)codes_batch_stride, (long long)scales_batch_stride, (long long)rows, (long long)cols);
+    MxRows m{const_cast<void*>(x), (uint8_t*)codes, (uint8_t*)scales, batch * rows * (cols / 32), rows, x_batch_stride,
+             x_row_stride, codes_batch_stride, scales_batch_stride, (int32_t)cols};
+    hipError_t e = launch_mx_quantize(m, dtype, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "quantize launch");
+    return BRX_OK;
+}
+
+int brx_mx_dequantize(const void* codes, int64_t codes_batch_stride, const void* scales, int64_t scales_batch_stride,
+                      int64_t batch, int64_t rows, int64_t cols, int dtype, void* out, void* stream) {
+    int rc = check_rows(dtype, batch, rows, cols);
+    if (rc) return rc;
+    if ((rc = ensure_device())) return rc;
+    if (!batch || !rows || !cols) return BRX_OK;
+    if (!out || !codes || !scales) return fail(BRX_EINVAL, "codes, scales and out are required");
+    if ((uintptr_t)out & (dtype == BRX_DT_F32 ? 3 : 1)) return fail(BRX_EINVAL, "out is not aligned to its type");
+    MxRows m{out, (uint8_t*)const_cast<void*>(codes), (uint8_t*)const_cast<void*>(scales), batch * rows * (cols / 32), rows,
+             rows * cols, cols, codes_batch_stride, scales_batch_stride, (int32_t)cols};
+    hipError_t e = launch_mx_dequantize(m, dtype, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "dequantize launch");
+    return BRX_OK;
+}
+
+// Most (token, expert) pairs of one call: its tiles and grids stay far inside 32-bit counts.
+constexpr int64_t kMxMaxPairs = (int64_t)1 << 21;
+
+static int check_mx_desc(const brx_layer_desc* d) {
+    int rc = check_desc(d);
+    if (rc) return rc;
+    if (d->quant_mode != BRX_QUANT_MXFP4)
+        return fail(BRX_EINVAL, "MXFP4 activations need MXFP4 experts (quant_mode %d)", d->quant_mode);
+    return BRX_OK;
+}
+
+static int check_mx_sizes(int T, int64_t n_pairs, bool shared) {
+    if (T < 0 || n_pairs < 0) return fail(BRX_EINVAL, "negative size (T=%d, n_pairs=%lld)", T, (long long)n_pairs);
+    if (n_pairs + (shared ? T : 0) > kMxMaxPairs)
+        return fail(BRX_EINVAL, "%lld pairs in one call: at most %lld", (long long)n_pairs + (shared ? T : 0), (long long)kMxMaxPairs);
+    return BRX_OK;
+}
+
+int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int shared, int product, size_t* out) {
+    int rc = check_mx_desc(d);
+    if (rc) return rc;
+    if (!out) return fail(BRX_EINVAL, "out is NULL");
+    if (shared && !d->shared_inter) return fail(BRX_EINVAL, "layer descriptor has no shared expert");
+    if ((rc = check_mx_sizes(T, n_pairs, shared != 0))) return rc;
+    // a layer call and the pairs form (whose shared pairs are among n_pairs) share the count
+    brx_pool none{};
+    none.d = *d;
+    none.lay = make_layout(*d, d->inter);
+    static const uint8_t some = 0;
+    FwdArgs a = make_args(d, &none, nullptr, T, (int)n_pairs, nullptr, nullptr, nullptr, 0, nullptr,
+                          shared ? &some : nullptr, nullptr, nullptr, nullptr);
+    *out = mx_workspace_bytes(a, !product, 0);
+    if (product) {
+        const size_t down = mx_workspace_bytes(a, false, 2);
+        if (down > *out) *out = down;
+    }
+    return BRX_OK;
+}
+
+// Ahead of a call's launches: its workspace checked, the stream behind the pool's refills (as run_forward).
+static int mx_begin(brx_pool* p, size_t need, void* workspace, size_t workspace_bytes, hipStream_t s) {
+    if (!workspace || ((uintptr_t)workspace & 255)) return fail(BRX_EINVAL, "workspace must be a 256-byte aligned device buffer");
+    if (workspace_bytes < need) return fail(BRX_EINVAL, "this call needs %zu bytes of workspace, %zu given", need, workspace_bytes);
+    if (p->refill_pending) {
+        HIP_TRY(hipStreamWaitEvent(s, p->refill_done, 0));
+        p->refill_pending = false;
+    }
+    return BRX_OK;
+}
+
+// After them: the pool marked read.
+static int mx_end(brx_pool* p, hipError_t e, hipStream_t s) {
+    if (e != hipSuccess) return hip_fail(e, "MXFP4 launch");
+    HIP_TRY(hipEventRecord(p->last_read, s));
+    p->read_recorded = true;
+    return BRX_OK;
+}
+
+static int check_mx_forward(const brx_layer_desc* d, brx_pool* p) {
+    int rc = check_mx_desc(d);
+    if (rc) return rc;
+    if ((rc = ensure_device())) return rc;
+    if (!p) return fail(BRX_EINVAL, "pool is NULL");
+    if (memcmp(&p->d, d, sizeof(brx_layer_desc)) != 0)
+        return fail(BRX_EINVAL, "descriptor differs from the one the pool was built with");
+    return BRX_OK;
+}
+
+static int check_pairs(int T, int n_pairs, int n_rows, const int32_t* pair_token, const int32_t* pair_expert,
+                       const int32_t* pair_row, const void* y_rows) {
+    if (T == 0) return fail(BRX_EINVAL, "pairs given but x has no rows");
+    if (!pair_token || !pair_expert || !y_rows) return fail(BRX_EINVAL, "pair_token, pair_expert and y_rows are required");
+    if ((uintptr_t)y_rows & 15) return fail(BRX_EINVAL, "y_rows must be 16-byte aligned");
+    if (pair_row ? n_rows < 1 : n_rows < n_pairs) return fail(BRX_EINVAL, "y_rows has %d rows for %d pairs", n_rows, n_pairs);
+    return BRX_OK;
+}
+
+int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* codes, const void* scales, int T,
+                          const int32_t* pair_token, const int32_t* pair_expert, const int32_t* pair_row, int n_pairs,
+                          int n_rows, int proj, void* y_rows, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_mx_forward(d, p);
+    if (rc) return rc;
+    if ((rc = check_mx_sizes(T, n_pairs, false))) return rc;
+    if (proj < 0 || proj > 2) return fail(BRX_EINVAL, "proj %d outside [0, 2]", proj);
+    if (proj == 1 && d->act == BRX_ACT_SILU_MLP) return fail(BRX_EINVAL, "a two-layer expert has no projection 1");
+    if (n_pairs == 0) return BRX_OK;
+    if (!codes || !scales) return fail(BRX_EINVAL, "codes and scales are required");
+    if ((uintptr_t)codes & 15) return fail(BRX_EINVAL, "codes must be 16-byte aligned");
+    if ((rc = check_pairs(T, n_pairs, n_rows, pair_token, pair_expert, pair_row, y_rows))) return rc;
+    FwdArgs a = make_args(d, p, nullptr, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, nullptr, nullptr,
+                          nullptr, y_rows);
+    hipStream_t s = (hipStream_t)stream;
+    if ((rc = mx_begin(p, mx_workspace_bytes(a, false, proj), workspace, workspace_bytes, s))) return rc;
+    return mx_end(p, launch_mx_product(a, (const uint8_t*)codes, (const uint8_t*)scales, proj, workspace, s), s);
+}
+
+static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T, int P, const int32_t* pexp,
+                      const int32_t* ptok, const int32_t* prow, int yrows, const float* w, const void* shared_expert,
+                      const float* shared_gate, void* out, void* y_rows, unsigned flags, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    if (!x) return fail(BRX_EINVAL, "x is required");
+    if ((uintptr_t)x & 15) return fail(BRX_EINVAL, "x must be 16-byte aligned");
+    if (shared_expert && !d->shared_inter) return fail(BRX_EINVAL, "layer descriptor has no shared expert");
+    if (shared_expert && ((uintptr_t)shared_expert & 15)) return fail(BRX_EINVAL, "shared expert must be 16-byte aligned");
+    if (flags & ~(BRX_FWD_FORCE_DECODE | BRX_FWD_FORCE_PREFILL))
+        return fail(BRX_EINVAL, "flags 0x%x: only FORCE_DECODE and FORCE_PREFILL here", flags);
+    if ((flags & BRX_FWD_FORCE_DECODE) && (flags & BRX_FWD_FORCE_PREFILL))
+        return fail(BRX_EINVAL, "FORCE_DECODE and FORCE_PREFILL are exclusive");
+    FwdArgs a = make_args(d, p, x, T, P, pexp, ptok, prow, yrows, w, shared_expert, shared_gate, out, y_rows);
+    hipStream_t s = (hipStream_t)stream;
+    const int rc = mx_begin(p, mx_workspace_bytes(a, true, 0), workspace, workspace_bytes, s);
+    if (rc) return rc;
+    return mx_end(p, launch_mx_layer(a, workspace, s), s);
+}
+
+int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, const int32_t* idx, const float* w,
+                       const void* shared_expert, const float* shared_gate, int T, void* out, void* y_unreduced,
+                       unsigned flags, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_mx_forward(d, p);
+    if (rc) return rc;
+    if (T < 0 || T > 65535) return fail(BRX_EINVAL, "T %d outside [0, 65535]", T);
+    if ((rc = check_mx_sizes(T, (int64_t)T * d->top_k, shared_expert != nullptr))) return rc;
+    if (T == 0) return BRX_OK;
+    if (!idx) return fail(BRX_EINVAL, "idx is required");
+    if (out && !w) return fail(BRX_EINVAL, "a combined output needs routing weights w");
+    if (!out && !y_unreduced) return fail(BRX_EINVAL, "nothing to write: out and y_unreduced are both NULL");
+    if (((uintptr_t)out | (uintptr_t)y_unreduced) & 15) return fail(BRX_EINVAL, "out and y_unreduced must be 16-byte aligned");
+    if (shared_expert && out && !shared_gate) return fail(BRX_EINVAL, "shared expert given without its gate values");
+    return mx_forward(d, p, x, T, T * d->top_k, idx, nullptr, nullptr, T * d->top_k, w, shared_expert, shared_gate, out,
+                      y_unreduced, flags, workspace, workspace_bytes, stream);
+}
+
+int brx_mx_moe_forward_pairs(const brx_layer_desc* d, brx_pool* p, const void* x, int T, const int32_t* pair_token,
+                             const int32_t* pair_expert, const int32_t* pair_row, int n_pairs, int n_rows,
+                             const void* shared_expert, void* y_rows, unsigned flags, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+    int rc = check_mx_forward(d, p);
+    if (rc) return rc;
+    if ((rc = check_mx_sizes(T, n_pairs, false))) return rc;
+    if (n_pairs == 0) return BRX_OK;
+    if ((rc = check_pairs(T, n_pairs, n_rows, pair_token, pair_expert, pair_row, y_rows))) return rc;
+    return mx_forward(d, p, x, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, shared_expert, nullptr,
+                      nullptr, y_rows, flags, workspace, workspace_bytes, stream);
+}
+
 int brx_combine(const brx_layer_desc* d, const void* y_routed, const float* w, const void* y_shared,
                 const float* shared_gate, int T, void* out, void* stream) {
     int rc = check_desc(d);

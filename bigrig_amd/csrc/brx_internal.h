@@ -663,6 +663,25 @@ hipError_t launch_dequant(const brx_layer_desc& d, const Layout& L, const uint8_
 hipError_t launch_sort_pairs(const int32_t* pexp, int P, int E, int E_ext, int T_shared, int BM,
                              int32_t* order, int32_t* offsets, int32_t* tile_start,
                              hipStream_t s);
+// Rows of MXFP4 and the values they come from (quantize) or go to (dequantize): `batch` matrices of rows x
+// cols values, each matrix's codes and scales contiguous, `groups` groups of 32 in all.
+struct MxRows {
+    void* x;
+    uint8_t* codes;
+    uint8_t* scales;
+    int64_t groups, rows;
+    int64_t x_batch, x_row;                 // values between matrices and rows of x
+    int64_t codes_batch, scales_batch;      // bytes between matrices
+    int32_t cols;
+};
+hipError_t launch_mx_quantize(const MxRows& m, int dtype, hipStream_t s);
+hipError_t launch_mx_dequantize(const MxRows& m, int dtype, hipStream_t s);
+// the expert layer with MXFP4 activations, and one projection's rows of quantized activations; `ws`
+// holds mx_workspace_bytes (layer: a whole layer, else an expert product of `proj`)
+size_t mx_workspace_bytes(const FwdArgs& a, bool layer, int proj);
+hipError_t launch_mx_layer(const FwdArgs& a, void* ws, hipStream_t s);
+hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, void* ws,
+                             hipStream_t s);
 hipError_t launch_combine(const uint16_t* y_routed, const uint16_t* y_shared, const float* w,
                           const float* sg, int T, int k, int H, uint16_t* out, hipStream_t s);
 

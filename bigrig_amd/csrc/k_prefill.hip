@@ -926,6 +926,8 @@ hipError_t launch_gemm(const FwdArgs& a, const PfWs& w, int E_ext, int Imax, uin
     return hipSuccess;
 }
 
+}  // namespace
+
 hipError_t launch_bucket(const int32_t* pexp, int P, int E, int E_ext, int T_sh, int BM,
                          const int32_t* g2s, int capacity, int host, int32_t* err, int32_t* order,
                          int32_t* offsets, int32_t* tile_start, int4* tinfo, hipStream_t s) {
@@ -943,8 +945,6 @@ hipError_t launch_bucket(const int32_t* pexp, int P, int E, int E_ext, int T_sh,
 #undef BRX_BUCKET
     return hipGetLastError();
 }
-
-}  // namespace
 
 // The M tile height of a call whose tiles all go to the thin-tile GEMM (k_thin.hip), or 0 for
 // k_pf_gemm. The line is the mean number of pairs an expert: both kernels within 2% at 48 (777

@@ -1,0 +1,75 @@
+// MXFP4 on the device: rounding a group of 32 values to e2m1 codes under one e8m0 scale, and the
+// operand layout of the scaled matrix instructions.
+//
+// A group's shared exponent is floor(log2(max |v|)) - 2 (2 is the exponent of e2m1's largest value,
+// 6), clamped to [-127, 127]; an element is v / 2^e rounded to the nearest e2m1 value, ties to the
+// even code, saturating at 6 (OCP Microscaling v1.0, section 6.3). The codes are those of
+// formats.quantize_mxfp4: no negative zero. A group that holds a NaN or an infinity gets the NaN
+// scale (255) and zero codes, so that every product it enters is NaN.
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 with fp4 operands: lane l holds row (or column) l % 16 and the 32
+// values of K group l / 16, sixteen bytes as the rows are packed, and that group's scale byte. So a
+// packed row and its scale array are operands as they stand: nothing is converted. The instruction
+// multiplies exactly and accumulates in fp32; a scale of 255 makes the lane's outputs NaN.
+#pragma once
+
+#include "brx_internal.h"
+
+namespace brx {
+
+// What the GEMM launches take beside the forward's arguments (FwdArgs::x is unused).
+struct MxArgs {
+    const uint8_t* xq;          // activation rows: codes [T, n_in / 2]
+    const uint8_t* xs;          // ... and scales [T, n_in / 32]
+    uint8_t* hq;                // intermediate rows in bucketed order: codes, `hstride` values apart
+    uint8_t* hs;                // ... and scales
+    const int32_t* order;
+    const int32_t* tile_start;
+    const int4* tinfo;
+    uint16_t* y_routed;
+    uint16_t* y_shared;
+    int32_t hstride;            // values between h rows
+    int32_t E_ext, ntn;
+    int32_t proj;               // the projection of an expert product
+};
+
+namespace {
+
+typedef uint32_t mx_u32x4 __attribute__((ext_vector_type(4)));
+typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
+
+// |v|'s bits: their unsigned order is the order of the magnitudes, infinities and NaN on top.
+__device__ __forceinline__ uint32_t mx_mag(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
+
+// The scale byte of a group whose largest magnitude has these bits (subnormal: floor(log2) - 2 is
+// below -127).
+__device__ __forceinline__ uint32_t mx_scale(uint32_t top) {
+    return top >= 0x7F800000u ? 255u : (uint32_t)max((int)(top >> 23) - 2, 0);
+}
+
+// The codes of 8 consecutive values of a group with scale byte `sb`, the first in the low bits. The
+// hardware conversion divides by the scale, rounds to nearest even and saturates; it keeps the
+// sign of a zero, which is cleared here: (m + 7) of a code's magnitude m has bit 3 set unless m is 0,
+// and never carries into the next code.
+__device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t sb) {
+    const float sc = __builtin_bit_cast(float, sb == 0u ? 0x00400000u : sb << 23);
+    uint32_t o = 0u;
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[0], v[1], sc, 0);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[2], v[3], sc, 1);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[4], v[5], sc, 2);
+    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[6], v[7], sc, 3);
+    const uint32_t m = o & 0x77777777u;
+    o = m | (o & (m + 0x77777777u) & 0x88888888u);
+    return sb == 255u ? 0u : o;
+}
+
+// acc += W (16 rows) . X (16 rows) over 128 K: lane l ends with W rows 4 (l / 16) .. + 3 of X row l % 16.
+__device__ __forceinline__ f32x4_t mx_mfma(const mx_u32x4& w, uint32_t ws, const mx_u32x4& x, uint32_t xs,
+                                           const f32x4_t& acc) {
+    const mx_i32x8 a{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    const mx_i32x8 b{(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, (int)ws, 0, (int)xs);
+}
+
+}  // namespace
+}  // namespace brx

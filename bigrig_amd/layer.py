@@ -148,10 +148,19 @@ def sort_pairs(spec: LayerSpec, idx, stream=None):
 class StreamingSwitchGLU:
     """Drop-in semantics of the reference's StreamingSwitchGLU over an HBM ExpertPool."""
 
-    def __init__(self, pool: ExpertPool, fetcher, shared=None, host_served: bool = False):
+    def __init__(self, pool: ExpertPool, fetcher, shared=None, host_served: bool = False,
+                 activations: str = "bf16"):
         """host_served: give the (fresh) pool host backing so misses are served by the kernels
         from the fetcher's pinned host store and residency is kept behind the forwards
-        (`hostserve.HostServedPool`); the operator is then always on the sync-free path."""
+        (`hostserve.HostServedPool`); the operator is then always on the sync-free path.
+        activations: "bf16", or "mxfp4" (layers of MXFP4 experts only): both projections' inputs are
+        rounded to MXFP4 and the products run on the scaled matrix instructions (`mx`)."""
+        if activations not in ("bf16", "mxfp4"):
+            raise ValueError(f"activations {activations!r} not in ('bf16', 'mxfp4')")
+        if activations == "mxfp4" and pool.spec.quant.mode != "mxfp4":
+            raise ValueError(f"MXFP4 activations need MXFP4 experts, the layer's are "
+                             f"{pool.spec.quant.mode}")
+        self.activations = activations
         self._pool = pool
         self._fetcher = fetcher
         self.spec = pool.spec
@@ -170,6 +179,26 @@ class StreamingSwitchGLU:
             from .hostserve import HostServedPool
             self._serve = HostServedPool(pool, store)
             self._sync_free = True
+
+    # -- the kernels of the chosen activations ------------------------------------------------
+    def _forward(self, x2, idx, w=None, shared=None, sgate=None, out=None, y_unreduced=None,
+                 flags=None, stream=None):
+        if self.activations == "mxfp4":
+            from . import mx
+            mx.moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced, flags,
+                           stream)
+        else:
+            moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced, flags,
+                        stream)
+
+    def _forward_pairs(self, x2, pair_tok, pair_exp, pair_row, y_rows, flags, shared=None, stream=None):
+        if self.activations == "mxfp4":
+            from . import mx
+            mx.forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, flags,
+                             shared, stream)
+        else:
+            forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, flags, shared,
+                          stream)
 
     # -- residency (stream.py:922-978) -------------------------------------------------------
     def ensure(self, indices, ranks=None) -> np.ndarray:
@@ -252,8 +281,7 @@ class StreamingSwitchGLU:
             t_tok = torch.from_numpy(tok[lo:hi].astype(np.int32)).to(dev)
             t_exp = torch.from_numpy(spe[lo:hi].astype(np.int32)).to(dev)
             t_row = torch.from_numpy(order[lo:hi].astype(np.int32)).to(dev)
-            forward_pairs(self.spec, self._pool, x2, t_tok, t_exp, t_row, y_rows, flags,
-                          stream=stream)
+            self._forward_pairs(x2, t_tok, t_exp, t_row, y_rows, flags, stream=stream)
 
     def __call__(self, x, indices, stream=None):
         """Unreduced expert rows [..., k, H] (bf16) for `indices` [..., k]."""
@@ -266,7 +294,7 @@ class StreamingSwitchGLU:
         y = torch.empty((T, k, H), dtype=torch.bfloat16, device=x2.device)
         if self._sync_free:
             self._before(stream)
-            moe_forward(self.spec, self._pool, x2, idx, y_unreduced=y, flags=flags, stream=stream)
+            self._forward(x2, idx, y_unreduced=y, flags=flags, stream=stream)
             self._after(idx, stream)
             return y.reshape(*indices.shape[:-1], k, H)
         gi = self._host_routing(idx)
@@ -277,7 +305,7 @@ class StreamingSwitchGLU:
         if len(np.unique(gi)) <= self._pool.capacity:
             self.ensure(gi)
             self._pool.g2s_device(_stream(stream))
-            moe_forward(self.spec, self._pool, x2, idx, y_unreduced=y, flags=flags, stream=stream)
+            self._forward(x2, idx, y_unreduced=y, flags=flags, stream=stream)
         else:
             self.chunked_calls += 1
             self._spans(x2, gi, y.view(T * k, H), flags, stream)
@@ -294,8 +322,7 @@ class StreamingSwitchGLU:
         shared = self.shared
         if self._sync_free:
             self._before(stream)
-            moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out=out, flags=flags,
-                        stream=stream)
+            self._forward(x2, idx, w, shared, sgate, out=out, flags=flags, stream=stream)
             self._after(idx, stream)
             return out
         gi = self._host_routing(idx)
@@ -306,8 +333,7 @@ class StreamingSwitchGLU:
         if len(np.unique(gi)) <= self._pool.capacity:
             self.ensure(gi)
             self._pool.g2s_device(_stream(stream))
-            moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out=out, flags=flags,
-                        stream=stream)
+            self._forward(x2, idx, w, shared, sgate, out=out, flags=flags, stream=stream)
             return out
         self.chunked_calls += 1
         y = torch.empty((T * k, H), dtype=torch.bfloat16, device=x2.device)
@@ -317,8 +343,7 @@ class StreamingSwitchGLU:
             ysh = torch.empty((T, H), dtype=torch.bfloat16, device=x2.device)
             tt = torch.arange(T, dtype=torch.int32, device=x2.device)
             te = torch.full((T,), self.spec.n_experts, dtype=torch.int32, device=x2.device)
-            forward_pairs(self.spec, self._pool, x2, tt, te, None, ysh, flags, shared=shared,
-                          stream=stream)
+            self._forward_pairs(x2, tt, te, None, ysh, flags, shared=shared, stream=stream)
         combine(self.spec, y, w, out, ysh, sgate, stream=stream)
         return out
 
@@ -342,7 +367,7 @@ class MoELayer:
     def __call__(self, x, stream=None):
         x2 = x.reshape(-1, self.spec.hidden).contiguous()
         sw = self.switch
-        if sw._sync_free:
+        if sw._sync_free and sw.activations == "bf16":
             # every expert resident (or served from host memory): routing, experts and combine
             # in one library call, the routing never waited for by the host (stream.py:1377-1394)
             sw._before(stream)

@@ -18,7 +18,7 @@ SCALE_BF16, SCALE_F16 = 0, 1
 ACT_SWIGLU, ACT_SWIGLU_CLAMPED = 0, 1
 ROUTE_SOFTMAX_TOPK, ROUTE_SOFTMAX_TOPK_RENORM, ROUTE_TOPK_SOFTMAX = 0, 1, 2
 ROUTE_SIGMOID_TOPK, ROUTE_SIGMOID_TOPK_RENORM = 3, 4
-DT_F32, DT_BF16 = 0, 1
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 FWD_FORCE_DECODE, FWD_FORCE_PREFILL, FWD_PHASE_A, FWD_PHASE_B, FWD_PHASE_R = 1, 2, 4, 8, 16
 ABI_VERSION = 2         # brx_abi_version() of the library this binding matches (BRX_ABI_VERSION)
 NOALLOC_SCRATCH_BYTES = 16 << 20
@@ -31,7 +31,9 @@ EXPORTS = (
     "brx_moe_forward_pairs", "brx_moe_block_forward", "brx_combine", "brx_dequant",
     "brx_sort_pairs", "brx_pool_set_host_backing", "brx_pool_publish_async",
     "brx_pool_admit_async", "brx_pool_refill_range_async", "brx_pool_check",
-    "brx_moe_block_forward_noalloc",
+    "brx_moe_block_forward_noalloc", "brx_mx_quantize", "brx_mx_dequantize",
+    "brx_mx_workspace_bytes", "brx_mx_expert_product", "brx_mx_moe_forward",
+    "brx_mx_moe_forward_pairs",
 )
 
 
@@ -63,6 +65,7 @@ _lock = threading.Lock()
 _init_device = None
 
 _vp, _i32p, _f32p = C.c_void_p, C.POINTER(C.c_int32), C.POINTER(C.c_float)
+_i64 = C.c_int64
 _SIGS = {
     "brx_abi_version": ([], C.c_int),
     "brx_last_error": ([], C.c_char_p),
@@ -93,6 +96,17 @@ _SIGS = {
                                _vp, _vp, C.c_uint, _vp], C.c_int),
     "brx_moe_block_forward_noalloc": ([C.POINTER(LayerDesc), _vp, _vp, _vp, _vp, _vp, _vp, C.c_int,
                                        _vp, _vp, _vp, C.c_uint, _vp], C.c_int),
+    "brx_mx_quantize": ([_vp, C.c_int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp],
+                        C.c_int),
+    "brx_mx_dequantize": ([_vp, _i64, _vp, _i64, _i64, _i64, _i64, C.c_int, _vp, _vp], C.c_int),
+    "brx_mx_workspace_bytes": ([C.POINTER(LayerDesc), C.c_int, _i64, C.c_int, C.c_int,
+                                C.POINTER(C.c_size_t)], C.c_int),
+    "brx_mx_expert_product": ([C.POINTER(LayerDesc), _vp, _vp, _vp, C.c_int, _vp, _vp, _vp, C.c_int,
+                               C.c_int, C.c_int, _vp, _vp, C.c_size_t, _vp], C.c_int),
+    "brx_mx_moe_forward": ([C.POINTER(LayerDesc), _vp, _vp, _vp, _vp, _vp, _vp, C.c_int, _vp, _vp,
+                            C.c_uint, _vp, C.c_size_t, _vp], C.c_int),
+    "brx_mx_moe_forward_pairs": ([C.POINTER(LayerDesc), _vp, _vp, C.c_int, _vp, _vp, _vp, C.c_int,
+                                  C.c_int, _vp, _vp, C.c_uint, _vp, C.c_size_t, _vp], C.c_int),
     "brx_combine": ([C.POINTER(LayerDesc), _vp, _vp, _vp, _vp, C.c_int, _vp, _vp], C.c_int),
     "brx_dequant": ([C.POINTER(LayerDesc), _vp, C.c_int, C.c_int, _vp, _vp], C.c_int),
     "brx_sort_pairs": ([C.POINTER(LayerDesc), _vp, C.c_int, _vp, _vp, _vp], C.c_int),

@@ -1,0 +1,359 @@
+"""MXFP4 rows, and expert layers whose activations are MXFP4 too, on libbrx.
+
+The reference keeps gpt-oss-style experts in MXFP4 and multiplies them by unquantized activations
+(bigrig_engine/stream.py:1623-1625); so do `layer.moe_forward` and the blocks built on it. Here both
+operands are MXFP4 and the products run on the scaled matrix instructions of gfx950 as the rows are
+packed. That is a choice of precision, made per operator (`StreamingSwitchGLU(...,
+activations="mxfp4")`): a group of 32 activations keeps e2m1's one mantissa bit under a common power
+of two.
+
+* `quantize` / `dequantize`: rows into MXFP4 and back;
+* `pack_experts`: unquantized expert weights into the packed bytes of MXFP4 experts, on the GPU
+  (`formats.quantize_mxfp4` of every projection, in blob layout);
+* `expert_product`: one projection's rows for a list of (token, expert) pairs;
+* `moe_forward` / `forward_pairs`: the layer forms of `layer.moe_forward` / `layer.forward_pairs`.
+
+A row [K] is K / 2 bytes of e2m1 codes (two a byte, the low nibble first) and K / 32 e8m0 scale
+bytes, as an expert's `weight` and `scales` components hold it. A group that holds a NaN or an
+infinity is held as NaN.
+
+Tensors live on the current device. Scratch is allocated per call by torch, on the call's stream, so
+calls on several streams do not share any, and a captured graph keeps its own.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+from . import formats as F
+from . import lib as L
+from .layer import _stream, path_flag
+from .pool import ExpertPool
+from .spec import LayerSpec
+
+MAX_TOKENS = 65535      # token rows of one layer call
+MAX_PAIRS = 1 << 21     # (token, expert) pairs of one call
+
+
+@dataclass(frozen=True)
+class MXRows:
+    """Rows [..., K] in MXFP4: `codes` uint8 [..., K / 2], `scales` uint8 [..., K / 32]."""
+    codes: object
+    scales: object
+
+    @property
+    def shape(self) -> tuple:
+        return (*self.codes.shape[:-1], 2 * self.codes.shape[-1])
+
+
+def _dtype(t) -> int:
+    import torch
+    dt = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}.get(t)
+    if dt is None:
+        raise ValueError(f"{t}: MXFP4 rows are made of float32, bfloat16 or float16 values")
+    return dt
+
+
+def _on_device(*tensors) -> None:
+    """Every tensor given is on the current device."""
+    import torch
+    cur = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("tensors must be on the GPU")
+        if cur is None:
+            cur = torch.cuda.current_device()
+        if t.device.index != cur:
+            raise ValueError(f"tensor on cuda:{t.device.index}, the current device is cuda:{cur}")
+
+
+def _matrices(t, what: str):
+    """(batch, rows, batch stride, row stride) of t [..., rows, n] seen as a run of matrices, in
+    elements; its innermost dimension must be contiguous and the leading ones collapse to one."""
+    if t.dim() == 0:
+        raise ValueError(f"{what} has no dimensions")
+    if t.numel() == 0:
+        return 0, 0, 0, 0
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{what}'s innermost dimension must be contiguous (stride {t.stride(-1)})")
+    if t.dim() == 1:
+        return 1, 1, 0, 0
+    if t.dim() == 2:
+        return 1, t.shape[0], 0, t.stride(0)
+    if t.is_contiguous():
+        return 1, t.numel() // t.shape[-1], 0, t.shape[-1]
+    if t.dim() > 3:
+        try:
+            t = t.view(-1, *t.shape[-2:])
+        except RuntimeError:
+            raise ValueError(f"{what}'s leading dimensions {tuple(t.shape[:-2])} do not collapse "
+                             f"into one: make it contiguous") from None
+    return t.shape[0], t.shape[1], t.stride(0), t.stride(1)
+
+
+def _packed(t, what: str):
+    """(batch, rows, batch stride) of packed bytes [..., rows, n] whose matrices are contiguous."""
+    import torch
+    if t.dtype != torch.uint8:
+        raise ValueError(f"{what} are uint8, got {t.dtype}")
+    b, r, bs, rs = _matrices(t, what)
+    if r > 1 and rs != t.shape[-1]:
+        raise ValueError(f"{what}: the rows of a matrix must follow one another")
+    return b, r, bs
+
+
+def _keep(stream, *tensors) -> None:
+    """Memory allocated for a call that runs on `stream` is not handed out again before it ends."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
+def _run_quantize(x, codes, codes_bs, scales, scales_bs, stream) -> None:
+    b, r, bs, rs = _matrices(x, "x")
+    if b == 0:
+        return
+    L.check(L.load().brx_mx_quantize(x.data_ptr(), _dtype(x.dtype), b, r, x.shape[-1], bs, rs,
+                                     codes, codes_bs, scales, scales_bs, _stream(stream)))
+
+
+def quantize(x, stream=None) -> MXRows:
+    """x [..., K] (float32, bfloat16 or float16; K a multiple of 32; rows may be strided) in MXFP4:
+    per group of 32, e = floor(log2(max |v|)) - 2 and codes v / 2^e rounded to nearest even,
+    saturating at 6 -- the codes of `formats.quantize_mxfp4`. A group with a NaN or an infinity is
+    held as NaN (scale byte 255)."""
+    import torch
+    _on_device(x)
+    _dtype(x.dtype)
+    if x.dim() == 0 or x.shape[-1] % 32:
+        raise ValueError(f"rows of {tuple(x.shape)}: the innermost dimension must be a multiple of 32")
+    K = x.shape[-1]
+    codes = torch.empty((*x.shape[:-1], K // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], K // 32), dtype=torch.uint8, device=x.device)
+    b, r, _, _ = _matrices(x, "x")
+    _run_quantize(x, codes.data_ptr(), r * (K // 2), scales.data_ptr(), r * (K // 32), stream)
+    _keep(stream, codes, scales)
+    return MXRows(codes, scales)
+
+
+def dequantize(q: MXRows, dtype=None, stream=None):
+    """The values of q as a contiguous [..., K] tensor of `dtype` (default bfloat16; exact in
+    float32 and bfloat16, rounded to nearest even in float16)."""
+    import torch
+    dtype = torch.bfloat16 if dtype is None else dtype
+    dt = _dtype(dtype)
+    _on_device(q.codes, q.scales)
+    K = 2 * q.codes.shape[-1] if q.codes.dim() else 0
+    if K % 32 or tuple(q.scales.shape) != (*q.codes.shape[:-1], K // 32):
+        raise ValueError(f"codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} are not "
+                         f"[..., K / 2] and [..., K / 32] of one K")
+    out = torch.empty((*q.codes.shape[:-1], K), dtype=dtype, device=q.codes.device)
+    if out.numel() == 0:
+        return out
+    b, r, cbs = _packed(q.codes, "codes")
+    b2, r2, sbs = _packed(q.scales, "scales")
+    if (b, r) != (b2, r2):      # one of the two is contiguous as a whole, the other is not
+        if b == 1:
+            b, r, cbs = b2, r2, r2 * (K // 2)
+        else:
+            sbs = r * (K // 32)
+    L.check(L.load().brx_mx_dequantize(q.codes.data_ptr(), cbs, q.scales.data_ptr(), sbs, b, r, K, dt,
+                                       out.data_ptr(), _stream(stream)))
+    _keep(stream, out)
+    return out
+
+
+def pack_experts(spec: LayerSpec, weights: dict, biases: dict | None = None, shared: bool = False,
+                 stream=None):
+    """uint8 [E, bytes_per_expert]: the packed MXFP4 experts of a layer whose unquantized weights
+    are weights[projection] [E, n_out, n_in] (and biases[projection] [E, n_out]), in the layout
+    `ExpertPool.admit_device` and `HostStore` take. `shared`: the shared expert's width."""
+    import torch
+    if spec.quant.mode != "mxfp4":
+        raise ValueError(f"the layer's experts are {spec.quant.mode}, not mxfp4")
+    es = spec.expert_spec(shared)
+    if set(weights) != set(es):
+        raise ValueError(f"weights for {sorted(weights)}, the layer's projections are {sorted(es)}")
+    if bool(biases) != spec.has_bias or (biases and set(biases) != set(es)):
+        raise ValueError(f"biases for {sorted(biases or {})}: the layer has "
+                         f"{'one a projection' if spec.has_bias else 'none'}")
+    E = next(iter(weights.values())).shape[0]
+    for p, comps in es.items():
+        n, kb = comps["scales"]["shape"]
+        if tuple(weights[p].shape) != (E, n, kb * 32):
+            raise ValueError(f"{p}: weights {tuple(weights[p].shape)}, the layer has {(E, n, kb * 32)}")
+        if biases and tuple(biases[p].shape) != (E, n):
+            raise ValueError(f"{p}: bias {tuple(biases[p].shape)}, the layer has {(E, n)}")
+        _dtype(weights[p].dtype)
+    _on_device(*weights.values(), *(biases or {}).values())
+    offs, per = F.spec_offsets(es), F.spec_bytes(es)
+    with torch.cuda.stream(stream):      # (None: the current stream)
+        out = torch.empty((E, per), dtype=torch.uint8, device=next(iter(weights.values())).device)
+        for p in es:
+            w = weights[p]
+            if w.dim() == 3 and w.is_contiguous():
+                # seen as one run of rows, but every expert's codes have a place of their own
+                args = (E, w.shape[1], w.shape[2], w.stride(0), w.stride(1))
+            else:
+                b, r, bs, rs = _matrices(w, p)
+                args = (b, r, w.shape[2], bs, rs)
+            if out.numel():
+                L.check(L.load().brx_mx_quantize(w.data_ptr(), _dtype(w.dtype), *args,
+                                                 out.data_ptr() + offs[(p, "weight")], per,
+                                                 out.data_ptr() + offs[(p, "scales")], per, _stream(stream)))
+            if biases:
+                o = offs[(p, "bias")]
+                b16 = biases[p].to(torch.bfloat16).contiguous().view(torch.uint8)
+                out[:, o:o + b16.shape[1]] = b16
+    return out
+
+
+# ------------------------------------------------------------------ products
+def _check_spec(spec: LayerSpec) -> None:
+    if spec.quant.mode != "mxfp4":
+        raise ValueError(f"MXFP4 activations need MXFP4 experts, the layer's are {spec.quant.mode}")
+
+
+def _index(t, n: int, what: str):
+    import torch
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {n} entries, got "
+                         f"{t.dtype} {tuple(t.shape)}")
+
+
+def _workspace(spec: LayerSpec, T: int, pairs: int, shared: bool, product: bool, device):
+    """Scratch for one call, from torch's allocator."""
+    import torch
+    known = spec.__dict__.setdefault("_mx_workspace", {})     # sizes, not memory
+    key = (T, pairs, shared, product)
+    n = known.get(key)
+    if n is None:
+        out = C.c_size_t()
+        L.check(L.load().brx_mx_workspace_bytes(C.byref(spec.c_desc), T, pairs, int(shared),
+                                                int(product), C.byref(out)))
+        if len(known) > 4096:
+            known.clear()
+        n = known[key] = out.value
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pair_expert, proj: str,
+                   pair_row=None, out=None, stream=None):
+    """Rows W_proj[pair_expert[i]] . q[pair_token[i]] (+ bias) of one projection ("gate_proj",
+    "up_proj", "down_proj"; "fc1", "fc2"), bf16 [n_pairs, n_out]. q: the activations [T, n_in];
+    pair_token and pair_expert int32 [n_pairs]. With `out` [n_rows, n_out] and pair_row (distinct
+    rows), row pair_row[i] is written and the others are left as they are."""
+    import torch
+    _check_spec(spec)
+    es = spec.expert_spec()
+    if proj not in es:
+        raise ValueError(f"projection {proj!r} not in {list(es)}")
+    n_out, groups = es[proj]["scales"]["shape"]
+    n = pair_expert.numel()
+    _on_device(q.codes, q.scales, pair_token, pair_expert, pair_row, out)
+    if (q.codes.dim() != 2 or q.codes.shape[1] != groups * 16 or
+            tuple(q.scales.shape) != (q.codes.shape[0], groups)):
+        raise ValueError(f"activations {tuple(q.codes.shape)} / {tuple(q.scales.shape)}: {proj} takes rows "
+                         f"of {groups * 32} values")
+    if (q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8 or not q.codes.is_contiguous() or
+            not q.scales.is_contiguous()):
+        raise ValueError("activations must be contiguous uint8 codes and scales")
+    _index(pair_token, n, "pair_token")
+    _index(pair_expert, n, "pair_expert")
+    if pair_row is not None:
+        _index(pair_row, n, "pair_row")
+        if out is None:
+            raise ValueError("pair_row names rows of an `out` that is not given")
+    if out is None:
+        out = torch.empty((n, n_out), dtype=torch.bfloat16, device=q.codes.device)
+    elif out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[1] != n_out or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous bfloat16 [n_rows, {n_out}]")
+    ws = _workspace(spec, q.codes.shape[0], n, False, True, q.codes.device)
+    j = list(F.MLP_PROJECTIONS if not spec.gated else F.PROJECTIONS).index(proj)
+    L.check(L.load().brx_mx_expert_product(
+        C.byref(spec.c_desc), pool.device.handle, q.codes.data_ptr(), q.scales.data_ptr(),
+        q.codes.shape[0], pair_token.data_ptr(), pair_expert.data_ptr(),
+        None if pair_row is None else pair_row.data_ptr(), n, out.shape[0],
+        j if spec.gated else 2 * j, out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(stream)))
+    _keep(stream, ws, out)
+    return out
+
+
+def _rows_of(spec: LayerSpec, x):
+    import torch
+    if x.dtype != torch.bfloat16 or x.shape[-1] != spec.hidden:
+        raise ValueError(f"x must be bfloat16 [..., {spec.hidden}], got {x.dtype} {tuple(x.shape)}")
+    return x.reshape(-1, spec.hidden).contiguous()
+
+
+def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, sgate=None, out=None,
+                y_unreduced=None, flags=None, stream=None):
+    """The routed experts of tokens x [T, H] (bf16) under a routing idx [T, k] (int32) with both
+    projections' activations in MXFP4. With weights w [T, k] (fp32): out [T, H] = sum_j w[t, j] *
+    y[t, j] (+ sgate[t] * shared(x_t)); without: the unreduced rows [T, k, H]. The pool's table must
+    be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`."""
+    import torch
+    _check_spec(spec)
+    x2 = _rows_of(spec, x)
+    T, H, k = x2.shape[0], spec.hidden, spec.top_k
+    _on_device(x2, idx, w, shared, sgate, out, y_unreduced)
+    _index(idx, T * k, "idx")
+    if w is not None and (w.dtype != torch.float32 or w.numel() != T * k or not w.is_contiguous()):
+        raise ValueError(f"w must be contiguous float32 [{T}, {k}]")
+    if sgate is not None and (sgate.dtype != torch.float32 or sgate.numel() != T or not sgate.is_contiguous()):
+        raise ValueError(f"sgate must be contiguous float32 [{T}]")
+    _check_shared(spec, shared)
+    if w is not None and out is None:
+        out = torch.empty((T, H), dtype=torch.bfloat16, device=x2.device)
+    if w is None and y_unreduced is None:
+        y_unreduced = torch.empty((T, k, H), dtype=torch.bfloat16, device=x2.device)
+    for t, n in ((out, T * H), (y_unreduced, T * k * H)):
+        if t is not None and (t.dtype != torch.bfloat16 or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"out and y_unreduced must be contiguous bfloat16 [{T}, {H}] and [{T}, {k}, {H}]")
+    ws = _workspace(spec, T, T * k, shared is not None, False, x2.device)
+    ptr = L.ptr
+    L.check(L.load().brx_mx_moe_forward(
+        C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), idx.data_ptr(), ptr(w), ptr(shared),
+        ptr(sgate), T, ptr(out), ptr(y_unreduced), path_flag(T, k) if flags is None else flags,
+        ws.data_ptr(), ws.numel(), _stream(stream)))
+    _keep(stream, ws, out, y_unreduced, x2)
+    return out if w is not None else y_unreduced
+
+
+def _check_shared(spec: LayerSpec, shared) -> None:
+    import torch
+    if shared is None:
+        return
+    if not spec.shared_inter:
+        raise ValueError("the layer has no shared expert")
+    per = F.spec_bytes(spec.expert_spec(True))
+    if shared.dtype != torch.uint8 or shared.numel() != per or not shared.is_contiguous():
+        raise ValueError(f"the shared expert is {per} contiguous bytes")
+
+
+def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair_row, y_rows, flags: int,
+                  shared=None, stream=None) -> None:
+    """`layer.forward_pairs` with MXFP4 activations."""
+    import torch
+    _check_spec(spec)
+    x2 = _rows_of(spec, x)
+    n = pair_exp.numel()
+    _on_device(x2, pair_tok, pair_exp, pair_row, y_rows, shared)
+    _index(pair_tok, n, "pair_tok")
+    _index(pair_exp, n, "pair_exp")
+    if pair_row is not None:
+        _index(pair_row, n, "pair_row")
+    _check_shared(spec, shared)
+    if (y_rows.dtype != torch.bfloat16 or y_rows.dim() != 2 or y_rows.shape[1] != spec.hidden or
+            not y_rows.is_contiguous()):
+        raise ValueError(f"y_rows must be contiguous bfloat16 [n_rows, {spec.hidden}]")
+    ws = _workspace(spec, x2.shape[0], n, shared is not None, False, x2.device)
+    ptr = L.ptr
+    L.check(L.load().brx_mx_moe_forward_pairs(
+        C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), x2.shape[0], ptr(pair_tok), ptr(pair_exp),
+        ptr(pair_row), n, y_rows.shape[0], ptr(shared), y_rows.data_ptr(), flags, ws.data_ptr(), ws.numel(),
+        _stream(stream)))
+    _keep(stream, ws, x2)

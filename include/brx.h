@@ -57,8 +57,8 @@ enum { BRX_ROUTE_SOFTMAX_TOPK = 0,        /* p=softmax(logits); w=p[idx] (OLMoE)
        BRX_ROUTE_SIGMOID_TOPK = 3,        /* s=sigmoid(logits); select on s + bias;
                                              w = s[idx] (DeepSeek-V3-style scoring)        */
        BRX_ROUTE_SIGMOID_TOPK_RENORM = 4 };/* ... then w /= sum(w)                          */
-/* router weight dtype */
-enum { BRX_DT_F32 = 0, BRX_DT_BF16 = 1 };
+/* router weight dtype (F32, BF16), dtype of the values of MXFP4 rows (all three) */
+enum { BRX_DT_F32 = 0, BRX_DT_BF16 = 1, BRX_DT_F16 = 2 };
 
 /* One MoE layer's shape and quantization: the manifest's per-layer
  * {n_experts, spec, quant} record (stream.py:133-151) plus the block's routing rule. */
@@ -304,6 +304,67 @@ int brx_moe_block_forward_noalloc(const brx_layer_desc* d, brx_pool* p, const vo
                                   const void* shared_gate_w, const void* shared_expert, int T,
                                   void* out, int32_t* out_idx, float* out_w, unsigned flags,
                                   void* stream);
+
+/* ---- MXFP4 activations
+ * The reference multiplies MXFP4 experts by unquantized activations (mx.gather_qmm,
+ * stream.py:1623-1625); these entry points have no counterpart there. Activations are rounded to
+ * MXFP4 as the weights are, and the products run on the scaled matrix instructions with both operands
+ * as packed. A row of K values (K a multiple of 32) is K / 2 bytes of e2m1 codes, two a byte, the low
+ * nibble first, and K / 32 e8m0 scale bytes: a projection's `weight` and `scales` components, row by
+ * row. Per group of 32: e = floor(log2(max |v|)) - 2 clamped to [-127, 127] (all zero: -127), scale
+ * byte e + 127, codes v / 2^e rounded to nearest even, saturating at 6, no negative zero. A group that
+ * holds a NaN or an infinity gets scale byte 255 and zero codes: it reads as NaN, and so does every
+ * product it enters. None of these calls uses the library workspace: scratch comes from the caller,
+ * so calls on several streams and captured graphs do not meet as long as their scratch does not. */
+
+/* Round `batch` matrices of rows x cols values to MXFP4.
+ *   x       device, BRX_DT_* values; matrix b's row r starts x_batch_stride * b + x_row_stride * r
+ *           values after x, its values are contiguous (strides may be 0 or negative, x any address
+ *           its type is aligned to)
+ *   codes   matrix b's [rows, cols / 2] bytes start codes_batch_stride bytes after matrix b - 1's
+ *   scales  ... its [rows, cols / 32] bytes scales_batch_stride bytes after
+ * With the strides and offsets of an expert's layout this packs unquantized weights into MXFP4
+ * experts in place. cols a multiple of 32; batch * rows * cols at most 2^40. */
+int brx_mx_quantize(const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols,
+                    int64_t x_batch_stride, int64_t x_row_stride, void* codes,
+                    int64_t codes_batch_stride, void* scales, int64_t scales_batch_stride, void* stream);
+/* The values of MXFP4 matrices (laid out as above) as one contiguous [batch, rows, cols] tensor `out`
+ * of `dtype`: exact in fp32 and bf16, rounded to nearest even in fp16. */
+int brx_mx_dequantize(const void* codes, int64_t codes_batch_stride, const void* scales,
+                      int64_t scales_batch_stride, int64_t batch, int64_t rows, int64_t cols, int dtype,
+                      void* out, void* stream);
+
+/* Bytes of scratch the calls below need for T token rows and n_pairs routed pairs (a layer: T * top_k):
+ * `product` nonzero for brx_mx_expert_product, zero for the layer calls (shared != 0: given a shared
+ * expert). What a call needs never exceeds this. */
+int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int shared, int product,
+                           size_t* out);
+
+/* One projection's rows for a list of (token, expert) pairs, activations already quantized:
+ *   y_rows[pair_row[i]] = W_proj[pair_expert[i]] . x[pair_token[i]] (+ bias)      (fp32 sums, bf16)
+ * proj 0 gate (fc1), 1 up, 2 down (fc2); codes [T, n_in / 2] and scales [T, n_in / 32] of the projection's
+ * inputs; y_rows [n_rows, n_out], pair_row NULL or distinct rows as in brx_moe_forward_pairs. Routed
+ * experts only, read through the pool's table; an absent one yields NaN rows and the pool's error.
+ * codes, y_rows and workspace 16-byte aligned; at most 2^21 pairs. */
+int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* codes, const void* scales,
+                          int T, const int32_t* pair_token, const int32_t* pair_expert,
+                          const int32_t* pair_row, int n_pairs, int n_rows, int proj, void* y_rows,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* brx_moe_forward with MXFP4 activations, for layers of MXFP4 experts: x is rounded to MXFP4, the
+ * activation is applied to the fp32 sums and its result h rounded to MXFP4 (once, from fp32), so
+ *   y[t, j] = down(Q(act(gate(Q(x_t)), up(Q(x_t)))))
+ * and out / y_unreduced as there. T at most 65535, out and y_unreduced 16-byte aligned. */
+int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, const int32_t* idx,
+                       const float* w, const void* shared_expert, const float* shared_gate, int T,
+                       void* out, void* y_unreduced, unsigned flags, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* brx_moe_forward_pairs with MXFP4 activations. */
+int brx_mx_moe_forward_pairs(const brx_layer_desc* d, brx_pool* p, const void* x, int T,
+                             const int32_t* pair_token, const int32_t* pair_expert,
+                             const int32_t* pair_row, int n_pairs, int n_rows,
+                             const void* shared_expert, void* y_rows, unsigned flags, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /* The caller's router-weighted combine of unreduced rows (stream.py:1523-1525):
  *   out[t] = bf16( sum_j w[t, j] * y_routed[t, j]  (+ shared_gate[t] * y_shared[t]) )
