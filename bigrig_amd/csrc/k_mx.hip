@@ -20,7 +20,9 @@ constexpr int kMxWaves = 4;
 constexpr int kMxThreads = 64 * kMxWaves;
 constexpr int kMxRows = 64;                      // weight rows of a wave: four fragments
 constexpr int kMxBlockN = kMxWaves * kMxRows;
-constexpr int kMxNR = 4;                         // steps of weights a wave has in registers
+// pairs of steps of weights a wave has in registers
+template <int MP>
+constexpr int kMxNH = MP == 4 ? 2 : 4;
 
 // LDS bytes of a staged A row's codes and scales. One zero chunk (scale 127) follows the row's
 // last: what the lanes of K groups past the row's end read. The code pitch is an odd number of 16-byte
@@ -49,35 +51,50 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
 
-    // ---- weight rows: fragment f's row l16 is row 8 (l16 / 4) + 4 (f % 2) + l16 % 4 of its 32, so a
-    // lane's outputs of two fragments are 8 consecutive rows
+    // ---- weight rows. Fragment f's row m is row 8 (m / 4) + 4 (f % 2) + m % 4 of the 32 rows from c0 on
+    // (fragments 2 and 3: the same 32 of the up matrix, or the next 32), so a lane's outputs of two
+    // fragments are 8 consecutive rows. (Widths are multiples of 64: a wave's rows are all there or
+    // none is; a wave with none works on the last ones and stores nothing.)
     const int c0 = nt * (gated ? kMxBlockN / 2 : kMxBlockN) + wv * (gated ? kMxRows / 2 : kMxRows);
+    const int cr = min(c0, N - (gated ? kMxRows / 2 : kMxRows));
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(base, (uint32_t)L.bytes);
-    uint32_t vw[4], vs[4];
-#pragma unroll
-    for (int f = 0; f < 4; ++f) {
-        const Proj& P = f < 2 ? P0 : P1;
-        const int r = min(c0 + (gated ? 0 : 32 * (f >> 1)) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3), N - 1);
-        vw[f] = (uint32_t)P.w + (uint32_t)r * (uint32_t)(K / 2);
-        vs[f] = (uint32_t)P.s + (uint32_t)r * (uint32_t)G;
-    }
-    struct Ring {
-        mx_u32x4 w[4];
+    // Codes: a load instruction reads 128 bytes (256 K) of 8 rows, lane (g, m) chunk 4 (m / 8) + g of row
+    // m % 8: whole cache lines. Two of them (rows 0-7 and 8-15 of a fragment) hold two steps, and the
+    // halves of each 16-lane group trade places to make the operands (mx_pair).
+    const uint32_t vw = (uint32_t)P0.w + (uint32_t)(cr + 8 * ((l16 & 7) >> 2) + (l16 & 3)) * (uint32_t)(K / 2);
+    const uint32_t dw = gated ? (uint32_t)(P1.w - P0.w) : 16u * (uint32_t)K;
+    // Scales: a load reads the 16 scale bytes of 512 K of 16 rows, lane (g, m) the four of step g of row m;
+    // the last four of a row where there are fewer left.
+    const uint32_t vs = (uint32_t)P0.s + (uint32_t)(cr + 8 * (l16 >> 2) + (l16 & 3)) * (uint32_t)G;
+    const uint32_t ds = gated ? (uint32_t)(P1.s - P0.s) : 32u * (uint32_t)G;
+    struct Half {
+        mx_u32x4 w[4][2];
+    };
+    struct Scales {
         uint32_t s[4];
     };
-    // (groups past the row's end read its last one: their A codes are zero)
-    auto issue = [&](int s, Ring& q) __attribute__((always_inline)) {
-        const int gi = min(4 * s + g, G - 1);
+    // (chunks past the row's end read its last one: their A codes are zero)
+    auto issue = [&](int hs, Half& q) __attribute__((always_inline)) {
+        const uint32_t v = vw + 16u * (uint32_t)min(8 * hs + 4 * (l16 >> 3) + g, G - 1);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(rw, vw[f] + 16 * gi, 0, 0);
-            q.w[f] = mx_u32x4{v[0], v[1], v[2], v[3]};
-            q.s[f] = __builtin_amdgcn_raw_buffer_load_b8(rw, vs[f] + gi, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                q.w[f][i] = __builtin_amdgcn_raw_buffer_load_b128(rw, v, (f >> 1) * dw + (f & 1) * 2u * K + i * 8u * K, 0);
         }
     };
-    Ring q[kMxNR];
+    auto issue_s = [&](int ss, Scales& q) __attribute__((always_inline)) {
+        const uint32_t v = vs + (uint32_t)min(16 * ss + 4 * g, G - 4);
 #pragma unroll
-    for (int s = 0; s < kMxNR - 1; ++s) issue(s, q[s]);
+        for (int f = 0; f < 4; ++f)
+            q.s[f] = __builtin_amdgcn_raw_buffer_load_b32(rw, v, (f >> 1) * ds + (f & 1) * 4u * G, 0);
+    };
+    constexpr int NH = kMxNH<MP>;
+    Half q[NH];
+    Scales qs[2];
+    issue_s(0, qs[0]);
+#pragma unroll
+    for (int h = 0; h < NH - 1; ++h) issue(h, q[h]);
 
     // ---- A rows, whole, into LDS
     const int PC = mx_code_pitch(K), PS = mx_scale_pitch(K);
@@ -114,21 +131,38 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
         for (int f = 0; f < 4; ++f) acc[p][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     const uint8_t* const ac = smem + l16 * PC;
     const uint8_t* const as = sc + l16 * PS;
-    const int nsteps = (G + 3) / 4;
-    for (int s0 = 0; s0 < nsteps; s0 += kMxNR) {
+    // one round: 8 steps, two loads of scales, four of codes; steps past the last multiply the zero chunk
+    const int rounds = (G + 31) / 32;
+    for (int r0 = 0; r0 < rounds; ++r0) {
 #pragma unroll
-        for (int v = 0; v < kMxNR; ++v) {
-            const int s = s0 + v;      // steps past the last multiply the zero chunk
-            issue(s + kMxNR - 1, q[(v + kMxNR - 1) % kMxNR]);
-            const int gi = min(4 * s + g, G);
+        for (int h = 0; h < 4; ++h) {
+            const int hs = 4 * r0 + h;
+            if ((h & 1) == 0) issue_s(hs / 2 + 1, qs[((h >> 1) + 1) & 1]);
+            issue(hs + NH - 1, q[(h + NH - 1) % NH]);
+            __builtin_amdgcn_sched_barrier(0);     // (or the loads sink to where they are used)
+            mx_u32x4 w[2][4];
 #pragma unroll
-            for (int p = 0; p < MP; ++p) {
-                const u32x4_t xv = *reinterpret_cast<const u32x4_t*>(ac + p * 16 * PC + 16 * gi);
-                const uint32_t xe = as[p * 16 * PS + gi];
+            for (int f = 0; f < 4; ++f) mx_pair(q[h % NH].w[f], w[0][f], w[1][f]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int s = 2 * hs + j;
+                uint32_t ws[4];
+                // (a mask, not a select: that becomes a branch; only the low byte counts)
+                const uint32_t sh = 8u * (uint32_t)(g + max(0, 4 * s + 4 - G)), in = (uint32_t)((4 * s + g - G) >> 31);
 #pragma unroll
                 for (int f = 0; f < 4; ++f)
-                    acc[p][f] = mx_mfma(q[v].w[f], q[v].s[f], mx_u32x4{xv[0], xv[1], xv[2], xv[3]}, xe, acc[p][f]);
+                    ws[f] = (mx_group(qs[(h >> 1) & 1].s[f], 2 * (h & 1) + j) >> (sh & 31u)) & in;
+                const int gi = min(4 * s + g, G);
+#pragma unroll
+                for (int p = 0; p < MP; ++p) {
+                    const u32x4_t xv = *reinterpret_cast<const u32x4_t*>(ac + p * 16 * PC + 16 * gi);
+                    const uint32_t xe = as[p * 16 * PS + gi];
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+                        acc[p][f] = mx_mfma(w[j][f], ws[f], mx_u32x4{xv[0], xv[1], xv[2], xv[3]}, xe, acc[p][f]);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 

@@ -63,6 +63,26 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t sb) {
     return sb == 255u ? 0u : o;
 }
 
+// Two loads of 8 rows x 8 chunks, lane (g, m) holding chunk 4 (m / 8) + g of row m % 8 (+ 8 in the second), as
+// two operands of 16 rows x 4 chunks: lanes 8-15 of each 16 trade the first load's second half of
+// chunks for the second load's first half (row_ror:8, written to one half of the lanes).
+__device__ __forceinline__ void mx_pair(const mx_u32x4 (&in)[2], mx_u32x4& o0,
+                                        mx_u32x4& o1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        o0[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)in[0][i], (int)in[1][i], 0x128, 0xF, 0xC, false);
+        o1[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)in[1][i], (int)in[0][i], 0x128, 0xF, 0x3, false);
+    }
+}
+
+// The value of lane group j (16 lanes) in every group, lane by lane: the lane swaps of gfx950.
+__device__ __forceinline__ uint32_t mx_group(uint32_t v, int j) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);    // groups 0 0 2 2, 1 1 3 3
+    const uint32_t e = (j & 1) ? a[1] : a[0];
+    const auto b = __builtin_amdgcn_permlane32_swap(e, e, false, false);
+    return (j & 2) ? b[1] : b[0];
+}
+
 // acc += W (16 rows) . X (16 rows) over 128 K: lane l ends with W rows 4 (l / 16) .. + 3 of X row l % 16.
 __device__ __forceinline__ f32x4_t mx_mfma(const mx_u32x4& w, uint32_t ws, const mx_u32x4& x, uint32_t xs,
                                            const f32x4_t& acc) {
