@@ -838,7 +838,7 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
     if (proj == 1 && d->act == BRX_ACT_SILU_MLP) return fail(BRX_EINVAL, "a two-layer expert has no projection 1");
     if (n_pairs == 0) return BRX_OK;
     if (!codes || !scales) return fail(BRX_EINVAL, "codes and scales are required");
-    if ((uintptr_t)codes & 15) return fail(BRX_EINVAL, "codes must be 16-byte aligned");
+    if (((uintptr_t)codes & 15) || ((uintptr_t)scales & 1)) return fail(BRX_EINVAL, "codes must be 16-byte, scales 2-byte aligned");
     if ((rc = check_pairs(T, n_pairs, n_rows, pair_token, pair_expert, pair_row, y_rows))) return rc;
     FwdArgs a = make_args(d, p, nullptr, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, nullptr, nullptr,
                           nullptr, y_rows);

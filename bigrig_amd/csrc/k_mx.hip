@@ -22,13 +22,14 @@ constexpr int kMxRows = 64;                      // weight rows of a wave: four 
 constexpr int kMxBlockN = kMxWaves * kMxRows;
 // pairs of steps of weights a wave has in registers
 template <int MP>
-constexpr int kMxNH = MP == 4 ? 2 : 4;
+constexpr int kMxNH = 2;
 
-// LDS bytes of a staged A row's codes and scales. One zero chunk (scale 127) follows the row's
-// last: what the lanes of K groups past the row's end read. The code pitch is an odd number of 16-byte
-// chunks and the scale pitch an odd number of words, so that 16 rows spread over the banks.
+// LDS bytes of a staged A row's codes and scales. One zero chunk follows the row's last: what the lanes
+// of K groups past the row's end read. The code pitch is an odd number of 16-byte chunks and the scale
+// pitch an odd number of words, so that 16 rows spread over the banks. A 16-bit copy into LDS fills a
+// word, so a word holds two groups' scales.
 __host__ __device__ inline int mx_code_pitch(int K) { return K / 2 + 16; }
-__host__ __device__ inline int mx_scale_pitch(int K) { return ((K / 32 + 1 + 3) / 4 | 1) * 4; }
+__host__ __device__ inline int mx_scale_pitch(int K) { return (K / 64 | 1) * 4; }
 __host__ __device__ inline int mx_row_lds(int K) { return mx_code_pitch(K) + mx_scale_pitch(K); }
 
 __device__ __forceinline__ float mx_act(const FwdArgs& a, float g, float u) {
@@ -89,40 +90,60 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
         for (int f = 0; f < 4; ++f)
             q.s[f] = __builtin_amdgcn_raw_buffer_load_b32(rw, v, (f >> 1) * ds + (f & 1) * 4u * G, 0);
     };
+    // ---- the tile's pairs, one a lane, and what follows from them: the A row (gathered rows) and the
+    // row the outputs go to (>= 0 routed, -2 - t shared)
+    int arow = m0 + lane, drow = 0;
+    if constexpr (KIND != 1) {
+        const int pair = m.order[m0 + min(lane, rows - 1)];
+        arow = pair_token(a, pair);
+        if constexpr (KIND == 2) drow = pair_row(a, pair);
+    } else {
+        const int pair = m.order[m0 + min(lane, rows - 1)];
+        drow = pair < a.P ? pair_row(a, pair) : -2 - (pair - a.P);
+    }
+    // the outputs' biases, and the first steps' scales and codes under the A rows' round trip
+    const bool biased = P0.bias >= 0;              // uniform
+    u32x4_t bias[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        bias[h] = u32x4_t{0u, 0u, 0u, 0u};
+        if (biased)
+            bias[h] = __builtin_amdgcn_raw_buffer_load_b128(
+                rw, (uint32_t)P0.bias + 2u * (uint32_t)(cr + 8 * g), gated ? h * (P1.bias - P0.bias) : 64 * h, 0);
+    }
     constexpr int NH = kMxNH<MP>;
     Half q[NH];
     Scales qs[2];
     issue_s(0, qs[0]);
-#pragma unroll
-    for (int h = 0; h < NH - 1; ++h) issue(h, q[h]);
+    issue(0, q[0]);
+    asm volatile("" ::: "memory");
 
-    // ---- A rows, whole, into LDS
+    // ---- A rows, whole, copied into LDS: row r by wave r % 4, a 1 KB run of codes or 64 scale pairs an
+    // instruction. Lanes past the row, and rows past the tile's pairs, read past their buffer's end: zeros.
     const int PC = mx_code_pitch(K), PS = mx_scale_pitch(K);
     uint8_t* const sc = smem + 16 * MP * PC;
-    for (int r = wv; r < 16 * MP; r += kMxWaves) {
-        const uint8_t *xc = nullptr, *xs = nullptr;
-        if (r < rows) {
-            if constexpr (KIND == 1) {
-                xc = m.hq + (int64_t)(m0 + r) * (m.hstride / 2);
-                xs = m.hs + (int64_t)(m0 + r) * (m.hstride / 32);
-            } else {
-                const int64_t t = pair_token(a, m.order[m0 + r]);
-                xc = m.xq + t * (K / 2);
-                xs = m.xs + t * G;
-            }
-        }
-        for (int c = lane; c <= G; c += 64) {
-            u32x4_t v{0u, 0u, 0u, 0u};
-            uint8_t s = 127;
-            if (c < G && r < rows) {
-                v = *reinterpret_cast<const u32x4_t*>(xc + 16 * c);
-                s = xs[c];
-            }
-            *reinterpret_cast<u32x4_t*>(smem + r * PC + 16 * c) = v;
-            sc[r * PS + c] = s;
-        }
+    const uint8_t* const srcc = KIND == 1 ? m.hq : m.xq;
+    const uint8_t* const srcs = KIND == 1 ? m.hs : m.xs;
+    const int64_t stride = KIND == 1 ? m.hstride : K;
+#pragma unroll 1
+    for (int i = 0; i < 4 * MP; ++i) {
+        const int r = 4 * i + wv;
+        const int64_t row = __builtin_amdgcn_readlane(arow, r);
+        const __amdgpu_buffer_rsrc_t rc = make_rsrc(srcc + row * (stride / 2), r < rows ? (uint32_t)(K / 2) : 0u);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(srcs + row * (stride / 32), r < rows ? (uint32_t)G : 0u);
+#pragma unroll 1
+        for (int c = 0; c <= G; c += 64)
+            if (c + lane <= G)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, (LDS_PTR)(smem + r * PC + 16 * c), 16, 16 * (c + lane), 0, 0, 0);
+#pragma unroll 1
+        for (int c = 0; 2 * c < G; c += 64)
+            if (2 * (c + lane) < G)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_PTR)(sc + r * PS + 4 * c), 2, 2 * (c + lane), 0, 0, 0);
     }
-    __syncthreads();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int h = 1; h < NH - 1; ++h) issue(h, q[h]);
+    dma_wait_barrier<8 * (NH - 2)>();
 
     f32x4_t acc[MP][4];
 #pragma unroll
@@ -152,11 +173,11 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
 #pragma unroll
                 for (int f = 0; f < 4; ++f)
                     ws[f] = (mx_group(qs[(h >> 1) & 1].s[f], 2 * (h & 1) + j) >> (sh & 31u)) & in;
-                const int gi = min(4 * s + g, G);
+                const int gi = min(4 * s + g, G), gs = min(4 * s + g, G - 1);
 #pragma unroll
                 for (int p = 0; p < MP; ++p) {
                     const u32x4_t xv = *reinterpret_cast<const u32x4_t*>(ac + p * 16 * PC + 16 * gi);
-                    const uint32_t xe = as[p * 16 * PS + gi];
+                    const uint32_t xe = as[p * 16 * PS + 4 * (gs >> 1) + (gs & 1)];
 #pragma unroll
                     for (int f = 0; f < 4; ++f)
                         acc[p][f] = mx_mfma(w[j][f], ws[f], mx_u32x4{xv[0], xv[1], xv[2], xv[3]}, xe, acc[p][f]);
@@ -167,22 +188,20 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     }
 
     // ---- epilogue: lane (g, l16) has rows 8 g .. 8 g + 7 of each 32-row group for pair l16
-    auto bias8 = [&](const Proj& P, int r, float (&b)[8]) __attribute__((always_inline)) {
-        u32x4_t w{0u, 0u, 0u, 0u};
-        if (P.bias >= 0) w = *reinterpret_cast<const u32x4_t*>(base + P.bias + 2 * r);
+    auto bias8 = [&](const u32x4_t& w, float (&b)[8]) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) b[i] = bf2f((i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu);
     };
+    if (c0 >= N) return;                           // (a wave past the last rows)
     const float nan = absent_nan();
     if constexpr (KIND == 0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {             // gated: one group; else fragments 2 h, 2 h + 1
             if (gated && h == 1) break;
             const int col = c0 + 32 * h + 8 * g;
-            if (c0 + 32 * h >= N) break;           // uniform
             float b0[8], b1[8];
-            bias8(P0, col, b0);
-            if (gated) bias8(P1, col, b1);
+            bias8(bias[h], b0);
+            bias8(bias[1], b1);
 #pragma unroll
             for (int p = 0; p < MP; ++p) {
                 float hv[8];
@@ -209,20 +228,14 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
         uint16_t* dst[MP];
 #pragma unroll
         for (int p = 0; p < MP; ++p) {
-            dst[p] = nullptr;
-            const int r = p * 16 + l16;
-            if (r < rows) {
-                const int pair = m.order[m0 + r];
-                dst[p] = pair < a.P ? m.y_routed + (int64_t)pair_row(a, pair) * N
-                                    : m.y_shared + (int64_t)(pair - a.P) * N;
-            }
+            const int d = __shfl(drow, p * 16 + l16, 64);
+            dst[p] = p * 16 + l16 >= rows ? nullptr : d >= 0 ? m.y_routed + (int64_t)d * N : m.y_shared + (int64_t)(-2 - d) * N;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int col = c0 + 32 * h + 8 * g;
-            if (c0 + 32 * h >= N) break;           // uniform
             float b[8];
-            bias8(P0, col, b);
+            bias8(bias[h], b);
 #pragma unroll
             for (int p = 0; p < MP; ++p) {
                 float y[8];
@@ -236,8 +249,10 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     }
 }
 
-template <int KIND>
-__global__ __launch_bounds__(kMxThreads, 2) void k_mx_gemm(FwdArgs a, MxArgs m) {
+// MPX: the call's tallest tiles, in 16 pairs (a launch of low tiles takes fewer registers).
+template <int KIND, int MPX>
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(MPX == 4 ? 2 : 3)))
+void k_mx_gemm(FwdArgs a, MxArgs m) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     prefetch_args(a);
     const int blk = blockIdx.x;
@@ -253,8 +268,8 @@ __global__ __launch_bounds__(kMxThreads, 2) void k_mx_gemm(FwdArgs a, MxArgs m) 
     const int N = pj == 0 ? L.p[0].n_out : pj == 1 ? L.p[1].n_out : L.p[2].n_out;
     const int per = KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxBlockN / 2 : kMxBlockN;
     if (nt * per >= N) return;
-    if (rows <= 16) mx_tile<KIND, 1>(a, m, smem, e, m0, rows, ti.w, nt);
-    else if (rows <= 32) mx_tile<KIND, 2>(a, m, smem, e, m0, rows, ti.w, nt);
+    if (MPX == 1 || rows <= 16) mx_tile<KIND, 1>(a, m, smem, e, m0, rows, ti.w, nt);
+    else if (MPX == 2 || rows <= 32) mx_tile<KIND, 2>(a, m, smem, e, m0, rows, ti.w, nt);
     else mx_tile<KIND, 4>(a, m, smem, e, m0, rows, ti.w, nt);
 }
 
@@ -309,7 +324,11 @@ template <int KIND>
 hipError_t launch_gemm(const FwdArgs& a, MxArgs m, const MxWs& w, int K, int N, hipStream_t s) {
     const int per = KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxBlockN / 2 : kMxBlockN;
     m.ntn = (N + per - 1) / per;
-    hipLaunchKernelGGL(k_mx_gemm<KIND>, dim3(w.mt_pad * m.ntn), dim3(kMxThreads), w.tile * mx_row_lds(K), s, a, m);
+    const dim3 grid(w.mt_pad * m.ntn);
+    const int lds = w.tile * mx_row_lds(K);
+    if (w.tile == 16) hipLaunchKernelGGL((k_mx_gemm<KIND, 1>), grid, dim3(kMxThreads), lds, s, a, m);
+    else if (w.tile == 32) hipLaunchKernelGGL((k_mx_gemm<KIND, 2>), grid, dim3(kMxThreads), lds, s, a, m);
+    else hipLaunchKernelGGL((k_mx_gemm<KIND, 4>), grid, dim3(kMxThreads), lds, s, a, m);
     return hipGetLastError();
 }
 

@@ -345,7 +345,7 @@ int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int 
  * proj 0 gate (fc1), 1 up, 2 down (fc2); codes [T, n_in / 2] and scales [T, n_in / 32] of the projection's
  * inputs; y_rows [n_rows, n_out], pair_row NULL or distinct rows as in brx_moe_forward_pairs. Routed
  * experts only, read through the pool's table; an absent one yields NaN rows and the pool's error.
- * codes, y_rows and workspace 16-byte aligned; at most 2^21 pairs. */
+ * codes and y_rows 16-byte, scales 2-byte, workspace 256-byte aligned; at most 2^21 pairs. */
 int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* codes, const void* scales,
                           int T, const int32_t* pair_token, const int32_t* pair_expert,
                           const int32_t* pair_row, int n_pairs, int n_rows, int proj, void* y_rows,
@@ -354,7 +354,7 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
 /* brx_moe_forward with MXFP4 activations, for layers of MXFP4 experts: x is rounded to MXFP4, the
  * activation is applied to the fp32 sums and its result h rounded to MXFP4 (once, from fp32), so
  *   y[t, j] = down(Q(act(gate(Q(x_t)), up(Q(x_t)))))
- * and out / y_unreduced as there. T at most 65535, out and y_unreduced 16-byte aligned. */
+ * and out / y_unreduced as there. T at most 65535; x, out and y_unreduced 16-byte, workspace 256-byte aligned. */
 int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, const int32_t* idx,
                        const float* w, const void* shared_expert, const float* shared_gate, int T,
                        void* out, void* y_unreduced, unsigned flags, void* workspace,
