@@ -782,11 +782,7 @@ int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int 
     static const uint8_t some = 0;
     FwdArgs a = make_args(d, &none, nullptr, T, (int)n_pairs, nullptr, nullptr, nullptr, 0, nullptr,
                           shared ? &some : nullptr, nullptr, nullptr, nullptr);
-    *out = mx_workspace_bytes(a, !product, 0);
-    if (product) {
-        const size_t down = mx_workspace_bytes(a, false, 2);
-        if (down > *out) *out = down;
-    }
+    *out = mx_workspace_bytes(a, !product);
     return BRX_OK;
 }
 
@@ -840,10 +836,12 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
     if (!codes || !scales) return fail(BRX_EINVAL, "codes and scales are required");
     if (((uintptr_t)codes & 15) || ((uintptr_t)scales & 1)) return fail(BRX_EINVAL, "codes must be 16-byte, scales 2-byte aligned");
     if ((rc = check_pairs(T, n_pairs, n_rows, pair_token, pair_expert, pair_row, y_rows))) return rc;
+    const int64_t k_in = proj == 2 ? d->inter : d->hidden;
+    if ((int64_t)T * (k_in / 2) >= (int64_t)0xFFFFFF00) return fail(BRX_EINVAL, "%d rows of %lld values: codes of at most 4 GB", T, (long long)k_in);
     FwdArgs a = make_args(d, p, nullptr, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, nullptr, nullptr,
                           nullptr, y_rows);
     hipStream_t s = (hipStream_t)stream;
-    if ((rc = mx_begin(p, mx_workspace_bytes(a, false, proj), workspace, workspace_bytes, s))) return rc;
+    if ((rc = mx_begin(p, mx_workspace_bytes(a, false), workspace, workspace_bytes, s))) return rc;
     return mx_end(p, launch_mx_product(a, (const uint8_t*)codes, (const uint8_t*)scales, proj, workspace, s), s);
 }
 
@@ -861,7 +859,7 @@ static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T
         return fail(BRX_EINVAL, "FORCE_DECODE and FORCE_PREFILL are exclusive");
     FwdArgs a = make_args(d, p, x, T, P, pexp, ptok, prow, yrows, w, shared_expert, shared_gate, out, y_rows);
     hipStream_t s = (hipStream_t)stream;
-    const int rc = mx_begin(p, mx_workspace_bytes(a, true, 0), workspace, workspace_bytes, s);
+    const int rc = mx_begin(p, mx_workspace_bytes(a, true), workspace, workspace_bytes, s);
     if (rc) return rc;
     return mx_end(p, launch_mx_layer(a, workspace, s), s);
 }

@@ -677,8 +677,8 @@ struct MxRows {
 hipError_t launch_mx_quantize(const MxRows& m, int dtype, hipStream_t s);
 hipError_t launch_mx_dequantize(const MxRows& m, int dtype, hipStream_t s);
 // the expert layer with MXFP4 activations, and one projection's rows of quantized activations; `ws`
-// holds mx_workspace_bytes (layer: a whole layer, else an expert product of `proj`)
-size_t mx_workspace_bytes(const FwdArgs& a, bool layer, int proj);
+// holds mx_workspace_bytes (layer: a whole layer, else an expert product)
+size_t mx_workspace_bytes(const FwdArgs& a, bool layer);
 hipError_t launch_mx_layer(const FwdArgs& a, void* ws, hipStream_t s);
 hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, void* ws,
                              hipStream_t s);

@@ -10,6 +10,8 @@
 //
 // y[n][m] = sum over K groups g of 2^(es_w[m][g] + es_x[n][g] - 254) * sum_k w[m][k] x[n][k], exact
 // products, fp32 sums in steps of 128 K in order. A row's bits do not depend on its tile.
+#include <type_traits>
+
 #include "mx_common.h"
 #include "pf_common.h"
 
@@ -20,20 +22,33 @@ constexpr int kMxWaves = 4;
 constexpr int kMxThreads = 64 * kMxWaves;
 constexpr int kMxRows = 64;                      // weight rows of a wave: four fragments
 constexpr int kMxBlockN = kMxWaves * kMxRows;
-// pairs of steps of weights a wave has in registers
-template <int MP>
-constexpr int kMxNH = 2;
 
-// LDS bytes of a staged A row's codes and scales. One zero chunk follows the row's last: what the lanes
-// of K groups past the row's end read. The code pitch is an odd number of 16-byte chunks and the scale
-// pitch an odd number of words, so that 16 rows spread over the banks. A 16-bit copy into LDS fills a
-// word, so a word holds two groups' scales.
-__host__ __device__ inline int mx_code_pitch(int K) { return K / 2 + 16; }
-__host__ __device__ inline int mx_scale_pitch(int K) { return (K / 64 | 1) * 4; }
-__host__ __device__ inline int mx_row_lds(int K) { return mx_code_pitch(K) + mx_scale_pitch(K); }
+// A rows pass through LDS in chunks of 512 K, two at a time: 256 bytes of codes a row (16-byte piece c
+// in slot c ^ (row % 16), so that 16 rows read at one piece fall into different banks), and the 16
+// scales two to a word (a 16-bit copy into LDS fills a word).
+template <int MP>
+constexpr int kMxA = 16 * MP * 256;
+template <int MP>
+constexpr int kMxBuf = kMxA<MP> + 16 * MP * 32;
+// Chunks of weights a wave has in registers.
+template <int MP>
+constexpr int kMxNQ = 1;
+// Copies of a chunk a wave issues: 1 KB runs of codes (4 rows), and 8 rows of scales (with 16 rows the
+// last two waves repeat the first two's).
+template <int MP>
+constexpr int kMxNS = MP == 1 ? 1 : MP / 2;
 
 __device__ __forceinline__ float mx_act(const FwdArgs& a, float g, float u) {
     return act_apply(a.act, g, u, a.alpha, a.limit);
+}
+
+// 16 or 2 bytes a lane from byte `off` of the buffer into LDS, lane after lane from `to` on (2 bytes fill
+// a word).
+__device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LDS_PTR)to, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void copy2(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LDS_PTR)to, 2, off, 0, 0, 0);
 }
 
 template <int KIND, int MP>
@@ -59,49 +74,58 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     const int c0 = nt * (gated ? kMxBlockN / 2 : kMxBlockN) + wv * (gated ? kMxRows / 2 : kMxRows);
     const int cr = min(c0, N - (gated ? kMxRows / 2 : kMxRows));
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(base, (uint32_t)L.bytes);
-    // Codes: a load instruction reads 128 bytes (256 K) of 8 rows, lane (g, m) chunk 4 (m / 8) + g of row
-    // m % 8: whole cache lines. Two of them (rows 0-7 and 8-15 of a fragment) hold two steps, and the
-    // halves of each 16-lane group trade places to make the operands (mx_pair).
-    const uint32_t vw = (uint32_t)P0.w + (uint32_t)(cr + 8 * ((l16 & 7) >> 2) + (l16 & 3)) * (uint32_t)(K / 2);
+    // Codes: four neighbouring lanes read 64 bytes in a row, the cache's coalescing width (one row a
+    // lane, 16 bytes each, costs it four times the lookups, and they bound the kernel): lane (g, m)
+    // piece 4 g + m % 4 of row 4 (m / 4) + t in load t, and the four transpose (mx_transpose).
+    const uint32_t vw = (uint32_t)P0.w + (uint32_t)(cr + 8 * (l16 >> 2)) * (uint32_t)(K / 2);
     const uint32_t dw = gated ? (uint32_t)(P1.w - P0.w) : 16u * (uint32_t)K;
-    // Scales: a load reads the 16 scale bytes of 512 K of 16 rows, lane (g, m) the four of step g of row m;
-    // the last four of a row where there are fewer left.
+    // Scales: lane (g, m) the four bytes of its groups of row m; where a row has fewer left, its last four.
     const uint32_t vs = (uint32_t)P0.s + (uint32_t)(cr + 8 * (l16 >> 2) + (l16 & 3)) * (uint32_t)G;
     const uint32_t ds = gated ? (uint32_t)(P1.s - P0.s) : 32u * (uint32_t)G;
-    struct Half {
-        mx_u32x4 w[4][2];
-    };
-    struct Scales {
+    struct Chunk {
+        mx_u32x4 w[4][4];
         uint32_t s[4];
     };
-    // (chunks past the row's end read its last one: their A codes are zero)
-    auto issue = [&](int hs, Half& q) __attribute__((always_inline)) {
-        const uint32_t v = vw + 16u * (uint32_t)min(8 * hs + 4 * (l16 >> 3) + g, G - 1);
+    // (pieces past the row's end read its last one: their A codes are zero)
+    auto issue = [&](int ch, Chunk& q) __attribute__((always_inline)) {
+        const uint32_t u = vs + (uint32_t)min(16 * ch + 4 * g, G - 4);
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+            q.s[f] = __builtin_amdgcn_raw_buffer_load_b32(rw, u, (f >> 1) * ds + (f & 1) * 4u * G, 0);
+        const uint32_t v = vw + 16u * (uint32_t)min(16 * ch + 4 * g + (l16 & 3), G - 1);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                q.w[f][i] = __builtin_amdgcn_raw_buffer_load_b128(rw, v, (f >> 1) * dw + (f & 1) * 2u * K + i * 8u * K, 0);
+            for (int t = 0; t < 4; ++t)
+                q.w[f][t] = __builtin_amdgcn_raw_buffer_load_b128(
+                    rw, v, (f >> 1) * dw + (f & 1) * 2u * K + t * (uint32_t)(K / 2), 0);
         }
     };
-    auto issue_s = [&](int ss, Scales& q) __attribute__((always_inline)) {
-        const uint32_t v = vs + (uint32_t)min(16 * ss + 4 * g, G - 4);
-#pragma unroll
-        for (int f = 0; f < 4; ++f)
-            q.s[f] = __builtin_amdgcn_raw_buffer_load_b32(rw, v, (f >> 1) * ds + (f & 1) * 4u * G, 0);
-    };
-    // ---- the tile's pairs, one a lane, and what follows from them: the A row (gathered rows) and the
-    // row the outputs go to (>= 0 routed, -2 - t shared)
-    int arow = m0 + lane, drow = 0;
+
+    // ---- what this lane copies of the A rows: piece lc of tile row r at byte va of the codes, slot ls of
+    // row r at byte vx of the scales; rows past the tile's pairs have pieces past every row's end
+    constexpr int NC = MP, NS = kMxNS<MP>;
+    constexpr int kNone = 1 << 28;
+    const uint8_t* const srcc = KIND == 1 ? m.hq + (int64_t)m0 * (m.hstride / 2) : m.xq;
+    const uint8_t* const srcs = KIND == 1 ? m.hs + (int64_t)m0 * (m.hstride / 32) : m.xs;
+    const uint32_t sa = (uint32_t)(KIND == 1 ? m.hstride : K) / 2;
+    const int64_t nrow = KIND == 1 ? rows : a.T;
+    const __amdgpu_buffer_rsrc_t rc = make_rsrc(srcc, (uint32_t)(nrow * sa));
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(srcs, (uint32_t)(nrow * (sa / 16)));
+    int pc[NC], px[NS], pd[MP];
+    auto crow = [&](int i) { return 4 * (wv * NC + i) + (lane >> 4); };
+    auto srow = [&](int i) { return 8 * ((wv * NS + i) % (2 * MP)) + (lane >> 3); };
     if constexpr (KIND != 1) {
-        const int pair = m.order[m0 + min(lane, rows - 1)];
-        arow = pair_token(a, pair);
-        if constexpr (KIND == 2) drow = pair_row(a, pair);
-    } else {
-        const int pair = m.order[m0 + min(lane, rows - 1)];
-        drow = pair < a.P ? pair_row(a, pair) : -2 - (pair - a.P);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) pc[i] = m.order[m0 + min(crow(i), rows - 1)];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) px[i] = m.order[m0 + min(srow(i), rows - 1)];
     }
-    // the outputs' biases, and the first steps' scales and codes under the A rows' round trip
+    if constexpr (KIND != 0) {
+#pragma unroll
+        for (int p = 0; p < MP; ++p) pd[p] = m.order[m0 + min(16 * p + l16, rows - 1)];
+    }
+    // the outputs' biases, and the first steps' scales and codes under the pair list's round trip
     const bool biased = P0.bias >= 0;              // uniform
     u32x4_t bias[2];
 #pragma unroll
@@ -111,80 +135,87 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
             bias[h] = __builtin_amdgcn_raw_buffer_load_b128(
                 rw, (uint32_t)P0.bias + 2u * (uint32_t)(cr + 8 * g), gated ? h * (P1.bias - P0.bias) : 64 * h, 0);
     }
-    constexpr int NH = kMxNH<MP>;
-    Half q[NH];
-    Scales qs[2];
-    issue_s(0, qs[0]);
+    constexpr int NQ = kMxNQ<MP>;
+    Chunk q[NQ];
     issue(0, q[0]);
     asm volatile("" ::: "memory");
-
-    // ---- A rows, whole, copied into LDS: row r by wave r % 4, a 1 KB run of codes or 64 scale pairs an
-    // instruction. Lanes past the row, and rows past the tile's pairs, read past their buffer's end: zeros.
-    const int PC = mx_code_pitch(K), PS = mx_scale_pitch(K);
-    uint8_t* const sc = smem + 16 * MP * PC;
-    const uint8_t* const srcc = KIND == 1 ? m.hq : m.xq;
-    const uint8_t* const srcs = KIND == 1 ? m.hs : m.xs;
-    const int64_t stride = KIND == 1 ? m.hstride : K;
-#pragma unroll 1
-    for (int i = 0; i < 4 * MP; ++i) {
-        const int r = 4 * i + wv;
-        const int64_t row = __builtin_amdgcn_readlane(arow, r);
-        const __amdgpu_buffer_rsrc_t rc = make_rsrc(srcc + row * (stride / 2), r < rows ? (uint32_t)(K / 2) : 0u);
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(srcs + row * (stride / 32), r < rows ? (uint32_t)G : 0u);
-#pragma unroll 1
-        for (int c = 0; c <= G; c += 64)
-            if (c + lane <= G)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, (LDS_PTR)(smem + r * PC + 16 * c), 16, 16 * (c + lane), 0, 0, 0);
-#pragma unroll 1
-        for (int c = 0; 2 * c < G; c += 64)
-            if (2 * (c + lane) < G)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_PTR)(sc + r * PS + 4 * c), 2, 2 * (c + lane), 0, 0, 0);
-    }
-    asm volatile("" ::: "memory");
+    uint32_t va[NC], vx[NS];
+    int lc[NC], ls[NS];
 #pragma unroll
-    for (int h = 1; h < NH - 1; ++h) issue(h, q[h]);
-    dma_wait_barrier<8 * (NH - 2)>();
+    for (int i = 0; i < NC; ++i) {
+        const int r = crow(i);
+        lc[i] = r < rows ? (lane & 15) ^ (r & 15) : kNone;
+        va[i] = (uint32_t)(KIND == 1 ? min(r, rows - 1) : pair_token(a, pc[i])) * sa + 16u * (uint32_t)((lane & 15) ^ (r & 15));
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int r = srow(i);
+        ls[i] = r < rows ? 2 * (lane & 7) : kNone;
+        vx[i] = (uint32_t)(KIND == 1 ? min(r, rows - 1) : pair_token(a, px[i])) * (sa / 16) + 2u * (uint32_t)(lane & 7);
+    }
+    // pieces past a row's end are copied from past the buffer's end: the range check writes zeros
+    auto issue_a = [&](int ch) __attribute__((always_inline)) {
+        uint8_t* const buf = smem + (ch & 1) * kMxBuf<MP>;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            copy16(rc, buf + (wv * NC + i) * 1024, lc[i] + 16 * ch < G ? va[i] + 256u * ch : 0xFFFFFF00u);
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            copy2(rs, buf + kMxA<MP> + (wv * NS + i) % (2 * MP) * 256,
+                        ls[i] + 16 * ch < G ? vx[i] + 16u * ch : 0xFFFFFF00u);
+    };
+    issue_a(0);
+    asm volatile("" ::: "memory");
+    if constexpr (NQ == 2) issue(1, q[1]);
 
     f32x4_t acc[MP][4];
 #pragma unroll
     for (int p = 0; p < MP; ++p)
 #pragma unroll
         for (int f = 0; f < 4; ++f) acc[p][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const uint8_t* const ac = smem + l16 * PC;
-    const uint8_t* const as = sc + l16 * PS;
-    // one round: 8 steps, two loads of scales, four of codes; steps past the last multiply the zero chunk
-    const int rounds = (G + 31) / 32;
-    for (int r0 = 0; r0 < rounds; ++r0) {
+    dma_wait_barrier<(NQ - 1) * 20>();             // (all but the second chunk of weights)
+    const int nch = (G + 15) / 16;
+    auto chunk = [&](int ch, Chunk& c) __attribute__((always_inline)) {
+        issue_a(ch + 1);                           // (every wave is done with the chunk that was there)
+        asm volatile("" ::: "memory");
+        const uint8_t* const buf = smem + (ch & 1) * kMxBuf<MP>;
+        uint32_t ws[4];
+        // the lane's first group is byte `off` of its word; none of its groups is there: zeros
+        const int first = 16 * ch + 4 * g, off = max(first - (G - 4), 0);
+        const uint32_t in = (uint32_t)((first - G) >> 31);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const int hs = 4 * r0 + h;
-            if ((h & 1) == 0) issue_s(hs / 2 + 1, qs[((h >> 1) + 1) & 1]);
-            issue(hs + NH - 1, q[(h + NH - 1) % NH]);
-            __builtin_amdgcn_sched_barrier(0);     // (or the loads sink to where they are used)
-            mx_u32x4 w[2][4];
-#pragma unroll
-            for (int f = 0; f < 4; ++f) mx_pair(q[h % NH].w[f], w[0][f], w[1][f]);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int s = 2 * hs + j;
-                uint32_t ws[4];
-                // (a mask, not a select: that becomes a branch; only the low byte counts)
-                const uint32_t sh = 8u * (uint32_t)(g + max(0, 4 * s + 4 - G)), in = (uint32_t)((4 * s + g - G) >> 31);
-#pragma unroll
-                for (int f = 0; f < 4; ++f)
-                    ws[f] = (mx_group(qs[(h >> 1) & 1].s[f], 2 * (h & 1) + j) >> (sh & 31u)) & in;
-                const int gi = min(4 * s + g, G), gs = min(4 * s + g, G - 1);
-#pragma unroll
-                for (int p = 0; p < MP; ++p) {
-                    const u32x4_t xv = *reinterpret_cast<const u32x4_t*>(ac + p * 16 * PC + 16 * gi);
-                    const uint32_t xe = as[p * 16 * PS + 4 * (gs >> 1) + (gs & 1)];
-#pragma unroll
-                    for (int f = 0; f < 4; ++f)
-                        acc[p][f] = mx_mfma(w[j][f], ws[f], mx_u32x4{xv[0], xv[1], xv[2], xv[3]}, xe, acc[p][f]);
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int f = 0; f < 4; ++f) {
+            ws[f] = (c.s[f] >> ((8 * off) & 31)) & in;
+            mx_transpose(c.w[f]);
         }
+        uint32_t xe[MP];       // the lane's four scales of its pairs' rows
+#pragma unroll
+        for (int p = 0; p < MP; ++p) {
+            const u32x2_t v = *reinterpret_cast<const u32x2_t*>(buf + kMxA<MP> + p * 512 + l16 * 32 + 8 * g);
+            xe[p] = v[0] | (v[1] << 16);
+        }
+        auto step = [&](auto t_) __attribute__((always_inline)) {
+            constexpr int t = decltype(t_)::value;
+#pragma unroll
+            for (int p = 0; p < MP; ++p) {
+                const mx_u32x4 xv = *reinterpret_cast<const mx_u32x4*>(buf + p * 4096 + l16 * 256 + 16 * ((4 * g + t) ^ l16));
+#pragma unroll
+                for (int f = 0; f < 4; ++f) acc[p][f] = mx_mfma<t>(c.w[f][t], ws[f], xv, xe[p], acc[p][f]);
+            }
+        };
+        step(std::integral_constant<int, 0>{});
+        step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 2>{});
+        step(std::integral_constant<int, 3>{});
+        issue(ch + NQ, c);
+        __builtin_amdgcn_sched_barrier(0);
+        // the next chunk of A has landed (the weights were issued after its copies), and every wave is done
+        // reading this one
+        thin_wait_barrier<20>();
+    };
+    for (int ch = 0; ch < nch; ch += NQ) {
+#pragma unroll
+        for (int v = 0; v < NQ; ++v) chunk(ch + v, q[v]);      // (zeros past the last)
     }
 
     // ---- epilogue: lane (g, l16) has rows 8 g .. 8 g + 7 of each 32-row group for pair l16
@@ -228,7 +259,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
         uint16_t* dst[MP];
 #pragma unroll
         for (int p = 0; p < MP; ++p) {
-            const int d = __shfl(drow, p * 16 + l16, 64);
+            const int d = KIND == 2 || pd[p] < a.P ? pair_row(a, pd[p]) : -2 - (pd[p] - a.P);
             dst[p] = p * 16 + l16 >= rows ? nullptr : d >= 0 ? m.y_routed + (int64_t)d * N : m.y_shared + (int64_t)(-2 - d) * N;
         }
 #pragma unroll
@@ -251,7 +282,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
 
 // MPX: the call's tallest tiles, in 16 pairs (a launch of low tiles takes fewer registers).
 template <int KIND, int MPX>
-__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(MPX == 4 ? 2 : 3)))
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(MPX == 8 ? 2 : MPX == 4 ? 2 : MPX == 2 ? 3 : 4)))
 void k_mx_gemm(FwdArgs a, MxArgs m) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     prefetch_args(a);
@@ -270,17 +301,15 @@ void k_mx_gemm(FwdArgs a, MxArgs m) {
     if (nt * per >= N) return;
     if (MPX == 1 || rows <= 16) mx_tile<KIND, 1>(a, m, smem, e, m0, rows, ti.w, nt);
     else if (MPX == 2 || rows <= 32) mx_tile<KIND, 2>(a, m, smem, e, m0, rows, ti.w, nt);
-    else mx_tile<KIND, 4>(a, m, smem, e, m0, rows, ti.w, nt);
+    else if (MPX == 4 || rows <= 64) mx_tile<KIND, 4>(a, m, smem, e, m0, rows, ti.w, nt);
+    else mx_tile<KIND, 8>(a, m, smem, e, m0, rows, ti.w, nt);
 }
 
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// Pairs of the call's tallest M tile: what the mean expert's pairs fit in, while a tile's A rows, held
-// whole, leave room in LDS.
-int mx_tile_rows(int64_t pairs, int64_t experts, int K) {
-    int r = pairs <= 8 * experts ? 16 : pairs <= 24 * experts ? 32 : 64;
-    while (r > 16 && r * mx_row_lds(K) > 150 * 1024) r /= 2;
-    return r;
+// Pairs of the call's tallest M tile: what the mean expert's pairs fit in.
+int mx_tile_rows(int64_t pairs, int64_t experts) {
+    return pairs <= 8 * experts ? 16 : pairs <= 24 * experts ? 32 : pairs <= 48 * experts ? 64 : 128;
 }
 
 struct MxWs {
@@ -294,12 +323,11 @@ struct MxWs {
 
 // The scratch of a call over P routed pairs (and T shared ones) of T token rows; `layer`: a whole layer
 // (else an expert product, whose activations and rows are the caller's).
-MxWs carve(const FwdArgs& a, bool layer, int proj, void* ws) {
+MxWs carve(const FwdArgs& a, bool layer, void* ws) {
     const int T_sh = a.auto_shared ? a.T : 0, P_ext = a.P + T_sh, E_ext = a.E + (a.shared ? 1 : 0);
     MxWs w{};
     w.Imax = a.shared && a.I_sh > a.I ? a.I_sh : a.I;
-    const int Kmax = layer ? (a.H > w.Imax ? a.H : w.Imax) : proj == 2 ? w.Imax : a.H;
-    w.tile = mx_tile_rows(P_ext, E_ext, Kmax);
+    w.tile = mx_tile_rows(P_ext, E_ext);
     w.mt_pad = ((P_ext + w.tile - 1) / w.tile + E_ext + kXcd - 1) / kXcd * kXcd;
     char* b = reinterpret_cast<char*>(ws);
     size_t off = 0;
@@ -321,14 +349,16 @@ MxWs carve(const FwdArgs& a, bool layer, int proj, void* ws) {
 }
 
 template <int KIND>
-hipError_t launch_gemm(const FwdArgs& a, MxArgs m, const MxWs& w, int K, int N, hipStream_t s) {
+hipError_t launch_gemm(const FwdArgs& a, MxArgs m, const MxWs& w, int N, hipStream_t s) {
     const int per = KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxBlockN / 2 : kMxBlockN;
     m.ntn = (N + per - 1) / per;
     const dim3 grid(w.mt_pad * m.ntn);
-    const int lds = w.tile * mx_row_lds(K);
-    if (w.tile == 16) hipLaunchKernelGGL((k_mx_gemm<KIND, 1>), grid, dim3(kMxThreads), lds, s, a, m);
-    else if (w.tile == 32) hipLaunchKernelGGL((k_mx_gemm<KIND, 2>), grid, dim3(kMxThreads), lds, s, a, m);
-    else hipLaunchKernelGGL((k_mx_gemm<KIND, 4>), grid, dim3(kMxThreads), lds, s, a, m);
+#define BRX_MX(MPX) hipLaunchKernelGGL((k_mx_gemm<KIND, MPX>), grid, dim3(kMxThreads), 2 * kMxBuf<MPX>, s, a, m)
+    if (w.tile == 16) BRX_MX(1);
+    else if (w.tile == 32) BRX_MX(2);
+    else if (w.tile == 64) BRX_MX(4);
+    else BRX_MX(8);
+#undef BRX_MX
     return hipGetLastError();
 }
 
@@ -348,10 +378,10 @@ hipError_t bucket(const FwdArgs& a, const MxWs& w, hipStream_t s) {
 
 }  // namespace
 
-size_t mx_workspace_bytes(const FwdArgs& a, bool layer, int proj) { return carve(a, layer, proj, nullptr).bytes; }
+size_t mx_workspace_bytes(const FwdArgs& a, bool layer) { return carve(a, layer, nullptr).bytes; }
 
 hipError_t launch_mx_layer(const FwdArgs& a, void* ws, hipStream_t s) {
-    const MxWs w = carve(a, true, 0, ws);
+    const MxWs w = carve(a, true, ws);
     MxRows x{};
     x.x = const_cast<uint16_t*>(a.x);
     x.codes = w.xq;
@@ -371,15 +401,15 @@ hipError_t launch_mx_layer(const FwdArgs& a, void* ws, hipStream_t s) {
     m.hstride = w.Imax;
     m.y_routed = a.yun ? a.yun : w.y_routed;
     m.y_shared = w.y_shared;
-    if ((e = launch_gemm<0>(a, m, w, a.H, w.Imax, s)) != hipSuccess) return e;
-    if ((e = launch_gemm<1>(a, m, w, w.Imax, a.H, s)) != hipSuccess) return e;
+    if ((e = launch_gemm<0>(a, m, w, w.Imax, s)) != hipSuccess) return e;
+    if ((e = launch_gemm<1>(a, m, w, a.H, s)) != hipSuccess) return e;
     if (!a.out) return hipSuccess;
     return launch_combine(m.y_routed, a.auto_shared ? w.y_shared : nullptr, a.w, a.sgate, a.T, a.k, a.H, a.out, s);
 }
 
 hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, void* ws,
                              hipStream_t s) {
-    const MxWs w = carve(a, false, proj, ws);
+    const MxWs w = carve(a, false, ws);
     hipError_t e = bucket(a, w, s);
     if (e != hipSuccess) return e;
     MxArgs m = gemm_args(a, w);
@@ -387,7 +417,7 @@ hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8
     m.xs = scales;
     m.y_routed = a.yun;
     m.proj = proj;
-    return launch_gemm<2>(a, m, w, proj == 2 ? w.Imax : a.H, proj == 2 ? a.H : w.Imax, s);
+    return launch_gemm<2>(a, m, w, proj == 2 ? a.H : w.Imax, s);
 }
 
 }  // namespace brx

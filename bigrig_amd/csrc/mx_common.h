@@ -9,8 +9,11 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 with fp4 operands: lane l holds row (or column) l % 16 and the 32
 // values of K group l / 16, sixteen bytes as the rows are packed, and that group's scale byte. So a
-// packed row and its scale array are operands as they stand: nothing is converted. The instruction
-// multiplies exactly and accumulates in fp32; a scale of 255 makes the lane's outputs NaN.
+// packed row and its scale array are operands as they stand: nothing is converted. Which 128 K a step
+// takes is free, the same on both sides: in a chunk of 512 K (256 bytes of a row, 16 groups), step t
+// takes groups 4 g + t, so that the four scales of lane group g are one word of the row, a byte a step
+// (the instruction selects it). The instruction multiplies exactly and accumulates in fp32; a scale of
+// 255 makes the lane's outputs NaN.
 #pragma once
 
 #include "brx_internal.h"
@@ -63,32 +66,40 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t sb) {
     return sb == 255u ? 0u : o;
 }
 
-// Two loads of 8 rows x 8 chunks, lane (g, m) holding chunk 4 (m / 8) + g of row m % 8 (+ 8 in the second), as
-// two operands of 16 rows x 4 chunks: lanes 8-15 of each 16 trade the first load's second half of
-// chunks for the second load's first half (row_ror:8, written to one half of the lanes).
-__device__ __forceinline__ void mx_pair(const mx_u32x4 (&in)[2], mx_u32x4& o0,
-                                        mx_u32x4& o1) {
+// The 4 x 4 transpose of 16-byte pieces over each four neighbouring lanes: lane q comes in with piece q of
+// rows 0 to 3 (in[t]: row t) and goes out with pieces 0 to 3 of row q. Two rounds of exchanges, with the
+// lane one away and with the lane two away.
+template <int CTRL>
+__device__ __forceinline__ uint32_t mx_quad(uint32_t v) {     // (every lane of a quad has a source)
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
+}
+__device__ __forceinline__ void mx_transpose(mx_u32x4 (&v)[4]) {
+    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        o0[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)in[0][i], (int)in[1][i], 0x128, 0xF, 0xC, false);
-        o1[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)in[1][i], (int)in[0][i], 0x128, 0xF, 0x3, false);
+#pragma unroll
+        for (int t = 0; t < 4; t += 2) {       // quad_perm [1, 0, 3, 2]
+            const uint32_t a = v[t][i], b = v[t + 1][i], s = mx_quad<0xB1>(odd ? a : b);
+            v[t][i] = odd ? s : a;
+            v[t + 1][i] = odd ? b : s;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {          // quad_perm [2, 3, 0, 1]
+            const uint32_t a = v[t][i], b = v[t + 2][i], s = mx_quad<0x4E>(high ? a : b);
+            v[t][i] = high ? s : a;
+            v[t + 2][i] = high ? b : s;
+        }
     }
 }
 
-// The value of lane group j (16 lanes) in every group, lane by lane: the lane swaps of gfx950.
-__device__ __forceinline__ uint32_t mx_group(uint32_t v, int j) {
-    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);    // groups 0 0 2 2, 1 1 3 3
-    const uint32_t e = (j & 1) ? a[1] : a[0];
-    const auto b = __builtin_amdgcn_permlane32_swap(e, e, false, false);
-    return (j & 2) ? b[1] : b[0];
-}
-
-// acc += W (16 rows) . X (16 rows) over 128 K: lane l ends with W rows 4 (l / 16) .. + 3 of X row l % 16.
+// acc += W (16 rows) . X (16 rows) over 128 K under byte S of each side's scales: lane l ends with W rows
+// 4 (l / 16) .. + 3 of X row l % 16.
+template <int S>
 __device__ __forceinline__ f32x4_t mx_mfma(const mx_u32x4& w, uint32_t ws, const mx_u32x4& x, uint32_t xs,
                                            const f32x4_t& acc) {
     const mx_i32x8 a{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     const mx_i32x8 b{(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, (int)ws, 0, (int)xs);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, S, (int)ws, S, (int)xs);
 }
 
 }  // namespace

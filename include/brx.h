@@ -345,7 +345,8 @@ int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int 
  * proj 0 gate (fc1), 1 up, 2 down (fc2); codes [T, n_in / 2] and scales [T, n_in / 32] of the projection's
  * inputs; y_rows [n_rows, n_out], pair_row NULL or distinct rows as in brx_moe_forward_pairs. Routed
  * experts only, read through the pool's table; an absent one yields NaN rows and the pool's error.
- * codes and y_rows 16-byte, scales 2-byte, workspace 256-byte aligned; at most 2^21 pairs. */
+ * codes and y_rows 16-byte, scales 2-byte, workspace 256-byte aligned; at most 2^21 pairs and codes of
+ * less than 2^32 - 256 bytes. */
 int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* codes, const void* scales,
                           int T, const int32_t* pair_token, const int32_t* pair_expert,
                           const int32_t* pair_row, int n_pairs, int n_rows, int proj, void* y_rows,
