@@ -18,25 +18,27 @@
 namespace brx {
 namespace {
 
-constexpr int kMxWaves = 4;
-constexpr int kMxThreads = 64 * kMxWaves;
 constexpr int kMxRows = 64;                      // weight rows of a wave: four fragments
-constexpr int kMxBlockN = kMxWaves * kMxRows;
 
 // A rows pass through LDS in chunks of 512 K, two at a time: 256 bytes of codes a row (16-byte piece c
 // in slot c ^ (row % 16), so that 16 rows read at one piece fall into different banks), and the 16
-// scales two to a word (a 16-bit copy into LDS fills a word).
+// scales two to a word (a 16-bit copy into LDS fills a word). The scales of a wave's weight rows are
+// in LDS whole, as they lie in memory.
 template <int MP>
 constexpr int kMxA = 16 * MP * 256;
 template <int MP>
 constexpr int kMxBuf = kMxA<MP> + 16 * MP * 32;
-// Chunks of weights a wave has in registers.
-template <int MP>
-constexpr int kMxNQ = 1;
-// Copies of a chunk a wave issues: 1 KB runs of codes (4 rows), and 8 rows of scales (with 16 rows the
-// last two waves repeat the first two's).
-template <int MP>
-constexpr int kMxNS = MP == 1 ? 1 : MP / 2;
+__host__ __device__ constexpr int mx_table(int waves, int K) { return waves * kMxRows * (K / 32) + 16; }
+// Waves of a block by its tallest tiles: four, and eight on tiles of 128 pairs, whose A chunks take half a
+// CU's LDS.
+template <int MPX>
+constexpr int kMxWaves = MPX == 8 ? 8 : 4;
+// Copies of a chunk a wave issues: 1 KB runs of codes (4 rows), and 8 rows of scales (of low tiles the last
+// waves repeat the first ones').
+template <int MP, int W>
+constexpr int kMxNC = (4 * MP + W - 1) / W;
+template <int MP, int W>
+constexpr int kMxNS = (2 * MP + W - 1) / W;
 
 __device__ __forceinline__ float mx_act(const FwdArgs& a, float g, float u) {
     return act_apply(a.act, g, u, a.alpha, a.limit);
@@ -51,7 +53,7 @@ __device__ __forceinline__ void copy2(__amdgpu_buffer_rsrc_t r, uint8_t* to, uin
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LDS_PTR)to, 2, off, 0, 0, 0);
 }
 
-template <int KIND, int MP>
+template <int KIND, int MP, int W>
 __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8_t* smem, int e, int m0, int rows,
                                         int slot, int nt) {
     const bool sh = e >= a.E;
@@ -71,7 +73,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     // (fragments 2 and 3: the same 32 of the up matrix, or the next 32), so a lane's outputs of two
     // fragments are 8 consecutive rows. (Widths are multiples of 64: a wave's rows are all there or
     // none is; a wave with none works on the last ones and stores nothing.)
-    const int c0 = nt * (gated ? kMxBlockN / 2 : kMxBlockN) + wv * (gated ? kMxRows / 2 : kMxRows);
+    const int c0 = (nt * W + wv) * (gated ? kMxRows / 2 : kMxRows);
     const int cr = min(c0, N - (gated ? kMxRows / 2 : kMxRows));
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(base, (uint32_t)L.bytes);
     // Codes: four neighbouring lanes read 64 bytes in a row, the cache's coalescing width (one row a
@@ -79,19 +81,11 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     // piece 4 g + m % 4 of row 4 (m / 4) + t in load t, and the four transpose (mx_transpose).
     const uint32_t vw = (uint32_t)P0.w + (uint32_t)(cr + 8 * (l16 >> 2)) * (uint32_t)(K / 2);
     const uint32_t dw = gated ? (uint32_t)(P1.w - P0.w) : 16u * (uint32_t)K;
-    // Scales: lane (g, m) the four bytes of its groups of row m; where a row has fewer left, its last four.
-    const uint32_t vs = (uint32_t)P0.s + (uint32_t)(cr + 8 * (l16 >> 2) + (l16 & 3)) * (uint32_t)G;
-    const uint32_t ds = gated ? (uint32_t)(P1.s - P0.s) : 32u * (uint32_t)G;
     struct Chunk {
         mx_u32x4 w[4][4];
-        uint32_t s[4];
     };
     // (pieces past the row's end read its last one: their A codes are zero)
     auto issue = [&](int ch, Chunk& q) __attribute__((always_inline)) {
-        const uint32_t u = vs + (uint32_t)min(16 * ch + 4 * g, G - 4);
-#pragma unroll
-        for (int f = 0; f < 4; ++f)
-            q.s[f] = __builtin_amdgcn_raw_buffer_load_b32(rw, u, (f >> 1) * ds + (f & 1) * 4u * G, 0);
         const uint32_t v = vw + 16u * (uint32_t)min(16 * ch + 4 * g + (l16 & 3), G - 1);
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
@@ -104,7 +98,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
 
     // ---- what this lane copies of the A rows: piece lc of tile row r at byte va of the codes, slot ls of
     // row r at byte vx of the scales; rows past the tile's pairs have pieces past every row's end
-    constexpr int NC = MP, NS = kMxNS<MP>;
+    constexpr int NC = kMxNC<MP, W>, NS = kMxNS<MP, W>;
     constexpr int kNone = 1 << 28;
     const uint8_t* const srcc = KIND == 1 ? m.hq + (int64_t)m0 * (m.hstride / 2) : m.xq;
     const uint8_t* const srcs = KIND == 1 ? m.hs + (int64_t)m0 * (m.hstride / 32) : m.xs;
@@ -113,7 +107,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     const __amdgpu_buffer_rsrc_t rc = make_rsrc(srcc, (uint32_t)(nrow * sa));
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(srcs, (uint32_t)(nrow * (sa / 16)));
     int pc[NC], px[NS], pd[MP];
-    auto crow = [&](int i) { return 4 * (wv * NC + i) + (lane >> 4); };
+    auto crow = [&](int i) { return 4 * ((wv * NC + i) % (4 * MP)) + (lane >> 4); };
     auto srow = [&](int i) { return 8 * ((wv * NS + i) % (2 * MP)) + (lane >> 3); };
     if constexpr (KIND != 1) {
 #pragma unroll
@@ -135,9 +129,14 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
             bias[h] = __builtin_amdgcn_raw_buffer_load_b128(
                 rw, (uint32_t)P0.bias + 2u * (uint32_t)(cr + 8 * g), gated ? h * (P1.bias - P0.bias) : 64 * h, 0);
     }
-    constexpr int NQ = kMxNQ<MP>;
-    Chunk q[NQ];
-    issue(0, q[0]);
+    Chunk q;
+    issue(0, q);
+    // the scales of the wave's rows: two runs of 32 rows, 16 bytes a lane
+    uint8_t* const tbl = smem + 2 * kMxBuf<MP> + wv * kMxRows * G;
+    const uint32_t ts = (uint32_t)P0.s + (uint32_t)(cr * G), ds = (gated ? (uint32_t)(P1.s - P0.s) : 32u * (uint32_t)G) - 32u * (uint32_t)G;
+#pragma unroll 1
+    for (int c = 0; c < 4 * G; c += 64)
+        if (c + lane < 4 * G) copy16(rw, tbl + 16 * c, ts + 16u * (uint32_t)(c + lane) + (c + lane >= 2 * G ? ds : 0u));
     asm volatile("" ::: "memory");
     uint32_t va[NC], vx[NS];
     int lc[NC], ls[NS];
@@ -158,7 +157,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
         uint8_t* const buf = smem + (ch & 1) * kMxBuf<MP>;
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-            copy16(rc, buf + (wv * NC + i) * 1024, lc[i] + 16 * ch < G ? va[i] + 256u * ch : 0xFFFFFF00u);
+            copy16(rc, buf + (wv * NC + i) % (4 * MP) * 1024, lc[i] + 16 * ch < G ? va[i] + 256u * ch : 0xFFFFFF00u);
 #pragma unroll
         for (int i = 0; i < NS; ++i)
             copy2(rs, buf + kMxA<MP> + (wv * NS + i) % (2 * MP) * 256,
@@ -166,27 +165,28 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     };
     issue_a(0);
     asm volatile("" ::: "memory");
-    if constexpr (NQ == 2) issue(1, q[1]);
 
     f32x4_t acc[MP][4];
 #pragma unroll
     for (int p = 0; p < MP; ++p)
 #pragma unroll
         for (int f = 0; f < 4; ++f) acc[p][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    dma_wait_barrier<(NQ - 1) * 20>();             // (all but the second chunk of weights)
+    dma_wait_barrier<0>();
     const int nch = (G + 15) / 16;
-    auto chunk = [&](int ch, Chunk& c) __attribute__((always_inline)) {
+    for (int ch = 0; ch < nch; ++ch) {
         issue_a(ch + 1);                           // (every wave is done with the chunk that was there)
         asm volatile("" ::: "memory");
         const uint8_t* const buf = smem + (ch & 1) * kMxBuf<MP>;
         uint32_t ws[4];
-        // the lane's first group is byte `off` of its word; none of its groups is there: zeros
-        const int first = 16 * ch + 4 * g, off = max(first - (G - 4), 0);
-        const uint32_t in = (uint32_t)((first - G) >> 31);
+        // groups past the row's end: zeros (another row's byte might be a NaN)
+        const int left = G - (16 * ch + 4 * g);
+        const uint32_t in = left >= 4 ? 0xFFFFFFFFu : left >= 2 ? 0xFFFFu : 0u;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
-            ws[f] = (c.s[f] >> ((8 * off) & 31)) & in;
-            mx_transpose(c.w[f]);
+            const uint16_t* const t =
+                reinterpret_cast<const uint16_t*>(tbl + (32 * (f >> 1) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3)) * G + 16 * ch + 4 * g);
+            ws[f] = (t[0] | ((uint32_t)t[1] << 16)) & in;
+            mx_transpose(q.w[f]);
         }
         uint32_t xe[MP];       // the lane's four scales of its pairs' rows
 #pragma unroll
@@ -200,22 +200,18 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
             for (int p = 0; p < MP; ++p) {
                 const mx_u32x4 xv = *reinterpret_cast<const mx_u32x4*>(buf + p * 4096 + l16 * 256 + 16 * ((4 * g + t) ^ l16));
 #pragma unroll
-                for (int f = 0; f < 4; ++f) acc[p][f] = mx_mfma<t>(c.w[f][t], ws[f], xv, xe[p], acc[p][f]);
+                for (int f = 0; f < 4; ++f) acc[p][f] = mx_mfma<t>(q.w[f][t], ws[f], xv, xe[p], acc[p][f]);
             }
         };
         step(std::integral_constant<int, 0>{});
         step(std::integral_constant<int, 1>{});
         step(std::integral_constant<int, 2>{});
         step(std::integral_constant<int, 3>{});
-        issue(ch + NQ, c);
+        issue(ch + 1, q);
         __builtin_amdgcn_sched_barrier(0);
         // the next chunk of A has landed (the weights were issued after its copies), and every wave is done
         // reading this one
-        thin_wait_barrier<20>();
-    };
-    for (int ch = 0; ch < nch; ch += NQ) {
-#pragma unroll
-        for (int v = 0; v < NQ; ++v) chunk(ch + v, q[v]);      // (zeros past the last)
+        thin_wait_barrier<16>();
     }
 
     // ---- epilogue: lane (g, l16) has rows 8 g .. 8 g + 7 of each 32-row group for pair l16
@@ -282,7 +278,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
 
 // MPX: the call's tallest tiles, in 16 pairs (a launch of low tiles takes fewer registers).
 template <int KIND, int MPX>
-__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(MPX == 8 ? 2 : MPX == 4 ? 2 : MPX == 2 ? 3 : 4)))
+__global__ __launch_bounds__(64 * kMxWaves<MPX>) __attribute__((amdgpu_waves_per_eu(MPX == 8 ? 2 : MPX == 4 ? 2 : MPX == 2 ? 3 : 4)))
 void k_mx_gemm(FwdArgs a, MxArgs m) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     prefetch_args(a);
@@ -297,19 +293,23 @@ void k_mx_gemm(FwdArgs a, MxArgs m) {
     const Layout& L = e >= a.E ? a.lay_sh : a.lay;
     const int pj = KIND == 0 ? 0 : KIND == 1 ? 2 : m.proj;
     const int N = pj == 0 ? L.p[0].n_out : pj == 1 ? L.p[1].n_out : L.p[2].n_out;
-    const int per = KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxBlockN / 2 : kMxBlockN;
-    if (nt * per >= N) return;
-    if (MPX == 1 || rows <= 16) mx_tile<KIND, 1>(a, m, smem, e, m0, rows, ti.w, nt);
-    else if (MPX == 2 || rows <= 32) mx_tile<KIND, 2>(a, m, smem, e, m0, rows, ti.w, nt);
-    else if (MPX == 4 || rows <= 64) mx_tile<KIND, 4>(a, m, smem, e, m0, rows, ti.w, nt);
-    else mx_tile<KIND, 8>(a, m, smem, e, m0, rows, ti.w, nt);
+    constexpr int W = kMxWaves<MPX>;
+    if (nt * W * (KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxRows / 2 : kMxRows) >= N) return;
+    if (MPX == 1 || rows <= 16) mx_tile<KIND, 1, W>(a, m, smem, e, m0, rows, ti.w, nt);
+    else if (MPX == 2 || rows <= 32) mx_tile<KIND, 2, W>(a, m, smem, e, m0, rows, ti.w, nt);
+    else if (MPX == 4 || rows <= 64) mx_tile<KIND, 4, W>(a, m, smem, e, m0, rows, ti.w, nt);
+    else mx_tile<KIND, 8, W>(a, m, smem, e, m0, rows, ti.w, nt);
 }
 
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// Pairs of the call's tallest M tile: what the mean expert's pairs fit in.
-int mx_tile_rows(int64_t pairs, int64_t experts) {
-    return pairs <= 8 * experts ? 16 : pairs <= 24 * experts ? 32 : pairs <= 48 * experts ? 64 : 128;
+constexpr int kMxLds = 160 * 1024;
+
+// Pairs of the call's tallest M tile: what the mean expert's pairs fit in, 128 while LDS holds them beside
+// the scales of rows of K.
+int mx_tile_rows(int64_t pairs, int64_t experts, int K) {
+    if (pairs > 48 * experts) return 2 * kMxBuf<8> + mx_table(8, K) <= kMxLds ? 128 : 64;
+    return pairs <= 8 * experts ? 16 : pairs <= 24 * experts ? 32 : 64;
 }
 
 struct MxWs {
@@ -327,7 +327,7 @@ MxWs carve(const FwdArgs& a, bool layer, void* ws) {
     const int T_sh = a.auto_shared ? a.T : 0, P_ext = a.P + T_sh, E_ext = a.E + (a.shared ? 1 : 0);
     MxWs w{};
     w.Imax = a.shared && a.I_sh > a.I ? a.I_sh : a.I;
-    w.tile = mx_tile_rows(P_ext, E_ext);
+    w.tile = mx_tile_rows(P_ext, E_ext, a.H > w.Imax ? a.H : w.Imax);
     w.mt_pad = ((P_ext + w.tile - 1) / w.tile + E_ext + kXcd - 1) / kXcd * kXcd;
     char* b = reinterpret_cast<char*>(ws);
     size_t off = 0;
@@ -348,18 +348,23 @@ MxWs carve(const FwdArgs& a, bool layer, void* ws) {
     return w;
 }
 
-template <int KIND>
-hipError_t launch_gemm(const FwdArgs& a, MxArgs m, const MxWs& w, int N, hipStream_t s) {
-    const int per = KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxBlockN / 2 : kMxBlockN;
+template <int KIND, int MPX>
+hipError_t launch_tall(const FwdArgs& a, MxArgs m, const MxWs& w, int K, int N, hipStream_t s) {
+    constexpr int W = kMxWaves<MPX>;
+    const int per = W * (KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxRows / 2 : kMxRows);
     m.ntn = (N + per - 1) / per;
-    const dim3 grid(w.mt_pad * m.ntn);
-#define BRX_MX(MPX) hipLaunchKernelGGL((k_mx_gemm<KIND, MPX>), grid, dim3(kMxThreads), 2 * kMxBuf<MPX>, s, a, m)
-    if (w.tile == 16) BRX_MX(1);
-    else if (w.tile == 32) BRX_MX(2);
-    else if (w.tile == 64) BRX_MX(4);
-    else BRX_MX(8);
-#undef BRX_MX
+    hipLaunchKernelGGL((k_mx_gemm<KIND, MPX>), dim3(w.mt_pad * m.ntn), dim3(64 * W), 2 * kMxBuf<MPX> + mx_table(W, K), s, a, m);
     return hipGetLastError();
+}
+
+template <int KIND>
+hipError_t launch_gemm(const FwdArgs& a, const MxArgs& m, const MxWs& w, int K, int N, hipStream_t s) {
+    switch (w.tile) {
+        case 16: return launch_tall<KIND, 1>(a, m, w, K, N, s);
+        case 32: return launch_tall<KIND, 2>(a, m, w, K, N, s);
+        case 64: return launch_tall<KIND, 4>(a, m, w, K, N, s);
+        default: return launch_tall<KIND, 8>(a, m, w, K, N, s);
+    }
 }
 
 MxArgs gemm_args(const FwdArgs& a, const MxWs& w) {
@@ -401,8 +406,8 @@ hipError_t launch_mx_layer(const FwdArgs& a, void* ws, hipStream_t s) {
     m.hstride = w.Imax;
     m.y_routed = a.yun ? a.yun : w.y_routed;
     m.y_shared = w.y_shared;
-    if ((e = launch_gemm<0>(a, m, w, w.Imax, s)) != hipSuccess) return e;
-    if ((e = launch_gemm<1>(a, m, w, a.H, s)) != hipSuccess) return e;
+    if ((e = launch_gemm<0>(a, m, w, a.H, w.Imax, s)) != hipSuccess) return e;
+    if ((e = launch_gemm<1>(a, m, w, w.Imax, a.H, s)) != hipSuccess) return e;
     if (!a.out) return hipSuccess;
     return launch_combine(m.y_routed, a.auto_shared ? w.y_shared : nullptr, a.w, a.sgate, a.T, a.k, a.H, a.out, s);
 }
@@ -417,7 +422,7 @@ hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8
     m.xs = scales;
     m.y_routed = a.yun;
     m.proj = proj;
-    return launch_gemm<2>(a, m, w, proj == 2 ? a.H : w.Imax, s);
+    return launch_gemm<2>(a, m, w, proj == 2 ? w.Imax : a.H, proj == 2 ? a.H : w.Imax, s);
 }
 
 }  // namespace brx
