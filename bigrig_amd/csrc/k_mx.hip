@@ -17,7 +17,8 @@
 
 namespace brx {
 namespace {
-
+constexpr int kMxWaves = 4;
+constexpr int kMxThreads = 64 * kMxWaves;
 constexpr int kMxRows = 64;                      // weight rows of a wave: four fragments
 
 // A rows pass through LDS in chunks of 512 K, two at a time: 256 bytes of codes a row (16-byte piece c
@@ -28,21 +29,11 @@ template <int MP>
 constexpr int kMxA = 16 * MP * 256;
 template <int MP>
 constexpr int kMxBuf = kMxA<MP> + 16 * MP * 32;
-__host__ __device__ constexpr int mx_table(int waves, int K) { return waves * kMxRows * (K / 32) + 16; }
-// Waves of a block by its tallest tiles: four, and eight on tiles of 128 pairs, whose A chunks take half a
-// CU's LDS.
-template <int MPX>
-constexpr int kMxWaves = MPX == 8 ? 8 : 4;
-// Copies of a chunk a wave issues: 1 KB runs of codes (4 rows), and 8 rows of scales (of low tiles the last
-// waves repeat the first ones').
-template <int MP, int W>
-constexpr int kMxNC = (4 * MP + W - 1) / W;
-template <int MP, int W>
-constexpr int kMxNS = (2 * MP + W - 1) / W;
-
-__device__ __forceinline__ float mx_act(const FwdArgs& a, float g, float u) {
-    return act_apply(a.act, g, u, a.alpha, a.limit);
-}
+__host__ __device__ constexpr int mx_table(int K) { return kMxWaves * kMxRows * (K / 32) + 16; }
+// Copies of a chunk's scales a wave issues, 8 rows each (of 16-row tiles the last two waves repeat the first
+// two's); its codes are MP copies of 1 KB (4 rows) a wave.
+template <int MP>
+constexpr int kMxNS = MP == 1 ? 1 : MP / 2;
 
 // 16 or 2 bytes a lane from byte `off` of the buffer into LDS, lane after lane from `to` on (2 bytes fill
 // a word).
@@ -53,7 +44,7 @@ __device__ __forceinline__ void copy2(__amdgpu_buffer_rsrc_t r, uint8_t* to, uin
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LDS_PTR)to, 2, off, 0, 0, 0);
 }
 
-template <int KIND, int MP, int W>
+template <int KIND, int MP>
 __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8_t* smem, int e, int m0, int rows,
                                         int slot, int nt) {
     const bool sh = e >= a.E;
@@ -73,7 +64,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     // (fragments 2 and 3: the same 32 of the up matrix, or the next 32), so a lane's outputs of two
     // fragments are 8 consecutive rows. (Widths are multiples of 64: a wave's rows are all there or
     // none is; a wave with none works on the last ones and stores nothing.)
-    const int c0 = (nt * W + wv) * (gated ? kMxRows / 2 : kMxRows);
+    const int c0 = (nt * kMxWaves + wv) * (gated ? kMxRows / 2 : kMxRows);
     const int cr = min(c0, N - (gated ? kMxRows / 2 : kMxRows));
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(base, (uint32_t)L.bytes);
     // Codes: four neighbouring lanes read 64 bytes in a row, the cache's coalescing width (one row a
@@ -98,7 +89,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
 
     // ---- what this lane copies of the A rows: piece lc of tile row r at byte va of the codes, slot ls of
     // row r at byte vx of the scales; rows past the tile's pairs have pieces past every row's end
-    constexpr int NC = kMxNC<MP, W>, NS = kMxNS<MP, W>;
+    constexpr int NC = MP, NS = kMxNS<MP>;
     constexpr int kNone = 1 << 28;
     const uint8_t* const srcc = KIND == 1 ? m.hq + (int64_t)m0 * (m.hstride / 2) : m.xq;
     const uint8_t* const srcs = KIND == 1 ? m.hs + (int64_t)m0 * (m.hstride / 32) : m.xs;
@@ -107,7 +98,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     const __amdgpu_buffer_rsrc_t rc = make_rsrc(srcc, (uint32_t)(nrow * sa));
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(srcs, (uint32_t)(nrow * (sa / 16)));
     int pc[NC], px[NS], pd[MP];
-    auto crow = [&](int i) { return 4 * ((wv * NC + i) % (4 * MP)) + (lane >> 4); };
+    auto crow = [&](int i) { return 4 * (wv * NC + i) + (lane >> 4); };
     auto srow = [&](int i) { return 8 * ((wv * NS + i) % (2 * MP)) + (lane >> 3); };
     if constexpr (KIND != 1) {
 #pragma unroll
@@ -131,12 +122,6 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     }
     Chunk q;
     issue(0, q);
-    // the scales of the wave's rows: two runs of 32 rows, 16 bytes a lane
-    uint8_t* const tbl = smem + 2 * kMxBuf<MP> + wv * kMxRows * G;
-    const uint32_t ts = (uint32_t)P0.s + (uint32_t)(cr * G), ds = (gated ? (uint32_t)(P1.s - P0.s) : 32u * (uint32_t)G) - 32u * (uint32_t)G;
-#pragma unroll 1
-    for (int c = 0; c < 4 * G; c += 64)
-        if (c + lane < 4 * G) copy16(rw, tbl + 16 * c, ts + 16u * (uint32_t)(c + lane) + (c + lane >= 2 * G ? ds : 0u));
     asm volatile("" ::: "memory");
     uint32_t va[NC], vx[NS];
     int lc[NC], ls[NS];
@@ -157,13 +142,19 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
         uint8_t* const buf = smem + (ch & 1) * kMxBuf<MP>;
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-            copy16(rc, buf + (wv * NC + i) % (4 * MP) * 1024, lc[i] + 16 * ch < G ? va[i] + 256u * ch : 0xFFFFFF00u);
+            copy16(rc, buf + (wv * NC + i) * 1024, lc[i] + 16 * ch < G ? va[i] + 256u * ch : 0xFFFFFF00u);
 #pragma unroll
         for (int i = 0; i < NS; ++i)
             copy2(rs, buf + kMxA<MP> + (wv * NS + i) % (2 * MP) * 256,
                         ls[i] + 16 * ch < G ? vx[i] + 16u * ch : 0xFFFFFF00u);
     };
     issue_a(0);
+    // the scales of the wave's rows: two runs of 32 rows, 16 bytes a lane
+    uint8_t* const tbl = smem + 2 * kMxBuf<MP> + wv * kMxRows * G;
+    const uint32_t ts = (uint32_t)P0.s + (uint32_t)(cr * G), ds = (gated ? (uint32_t)(P1.s - P0.s) : 32u * (uint32_t)G) - 32u * (uint32_t)G;
+#pragma unroll 1
+    for (int c = 0; c < 4 * G; c += 64)
+        if (c + lane < 4 * G) copy16(rw, tbl + 16 * c, ts + 16u * (uint32_t)(c + lane) + (c + lane >= 2 * G ? ds : 0u));
     asm volatile("" ::: "memory");
 
     f32x4_t acc[MP][4];
@@ -222,6 +213,10 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     if (c0 >= N) return;                           // (a wave past the last rows)
     const float nan = absent_nan();
     if constexpr (KIND == 0) {
+        // act_apply's values with the rule picked by selects (one copy of the code) and the limits by
+        // comparisons, which leave a NaN as it is
+        const bool clamped = a.act == BRX_ACT_SWIGLU_CLAMPED;
+        const float alpha = clamped ? a.alpha : 1.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {             // gated: one group; else fragments 2 h, 2 h + 1
             if (gated && h == 1) break;
@@ -236,8 +231,13 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float gv = acc[p][2 * h + (i >> 2)][i & 3] + b0[i];
-                    const float uv = gated ? acc[p][2 + (i >> 2)][i & 3] + b1[i] : 0.f;
-                    hv[i] = absent ? nan : mx_act(a, gv, uv);
+                    float uv = 1.0f;
+                    if (gated) {
+                        uv = acc[p][2 + (i >> 2)][i & 3] + b1[i];
+                        if (clamped) uv = (uv > a.limit ? a.limit : uv < -a.limit ? -a.limit : uv) + 1.0f;
+                    }
+                    hv[i] = x_sigmoid(clamped && gv > a.limit ? a.limit : gv, alpha) * uv;
+                    hv[i] = absent ? nan : hv[i];
                     top = max(top, mx_mag(hv[i]));
                 }
                 top = max(top, lane_xor16(top));
@@ -278,14 +278,15 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
 
 // MPX: the call's tallest tiles, in 16 pairs (a launch of low tiles takes fewer registers).
 template <int KIND, int MPX>
-__global__ __launch_bounds__(64 * kMxWaves<MPX>) __attribute__((amdgpu_waves_per_eu(MPX == 8 ? 2 : MPX == 4 ? 2 : MPX == 2 ? 3 : 4)))
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(MPX == 4 ? 2 : MPX == 2 ? 3 : 4)))
 void k_mx_gemm(FwdArgs a, MxArgs m) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     prefetch_args(a);
     const int blk = blockIdx.x;
     const int loc = blk / kXcd;
-    const int nt = loc % m.ntn;
-    const int mt = (loc / m.ntn) * kXcd + blk % kXcd;
+    const int of = loc / (m.group * m.ntn), in = loc % (m.group * m.ntn);
+    const int nt = in / m.group;
+    const int mt = (of * kXcd + blk % kXcd) * m.group + in % m.group;
     const int total = m.tile_start[m.E_ext];
     const int4 ti = m.tinfo[mt];
     if (mt >= total) return;
@@ -293,31 +294,29 @@ void k_mx_gemm(FwdArgs a, MxArgs m) {
     const Layout& L = e >= a.E ? a.lay_sh : a.lay;
     const int pj = KIND == 0 ? 0 : KIND == 1 ? 2 : m.proj;
     const int N = pj == 0 ? L.p[0].n_out : pj == 1 ? L.p[1].n_out : L.p[2].n_out;
-    constexpr int W = kMxWaves<MPX>;
-    if (nt * W * (KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxRows / 2 : kMxRows) >= N) return;
-    if (MPX == 1 || rows <= 16) mx_tile<KIND, 1, W>(a, m, smem, e, m0, rows, ti.w, nt);
-    else if (MPX == 2 || rows <= 32) mx_tile<KIND, 2, W>(a, m, smem, e, m0, rows, ti.w, nt);
-    else if (MPX == 4 || rows <= 64) mx_tile<KIND, 4, W>(a, m, smem, e, m0, rows, ti.w, nt);
-    else mx_tile<KIND, 8, W>(a, m, smem, e, m0, rows, ti.w, nt);
+    if (nt * kMxWaves * (KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxRows / 2 : kMxRows) >= N) return;
+    if (MPX == 1 || rows <= 16) mx_tile<KIND, 1>(a, m, smem, e, m0, rows, ti.w, nt);
+    else if (MPX == 2 || rows <= 32) mx_tile<KIND, 2>(a, m, smem, e, m0, rows, ti.w, nt);
+    else mx_tile<KIND, 4>(a, m, smem, e, m0, rows, ti.w, nt);
 }
 
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-constexpr int kMxLds = 160 * 1024;
-
-// Pairs of the call's tallest M tile: what the mean expert's pairs fit in, 128 while LDS holds them beside
-// the scales of rows of K.
-int mx_tile_rows(int64_t pairs, int64_t experts, int K) {
-    if (pairs > 48 * experts) return 2 * kMxBuf<8> + mx_table(8, K) <= kMxLds ? 128 : 64;
+// Pairs of the call's tallest M tile: what the mean expert's pairs fit in (tiles of 128 pairs leave one wave a
+// SIMD its registers: a 2048-token layer 195 us, 184 with 64).
+int mx_tile_rows(int64_t pairs, int64_t experts) {
     return pairs <= 8 * experts ? 16 : pairs <= 24 * experts ? 32 : 64;
 }
+// Consecutive M tiles whose runs of columns an XCD takes in turn: an expert's tall tiles then read its weights
+// from one L2 (a 2048-token layer 183 us one by one, 180 by two, 179 by four).
+int mx_group(int tile) { return tile == 64 ? 4 : 1; }
 
 struct MxWs {
     uint8_t *xq, *xs, *hq, *hs;
     int32_t *order, *offsets, *tile_start;
     int4* tinfo;
     uint16_t *y_routed, *y_shared;
-    int mt_pad, tile, Imax;
+    int mt_pad, tile, group, Imax;
     size_t bytes;
 };
 
@@ -327,15 +326,17 @@ MxWs carve(const FwdArgs& a, bool layer, void* ws) {
     const int T_sh = a.auto_shared ? a.T : 0, P_ext = a.P + T_sh, E_ext = a.E + (a.shared ? 1 : 0);
     MxWs w{};
     w.Imax = a.shared && a.I_sh > a.I ? a.I_sh : a.I;
-    w.tile = mx_tile_rows(P_ext, E_ext, a.H > w.Imax ? a.H : w.Imax);
-    w.mt_pad = ((P_ext + w.tile - 1) / w.tile + E_ext + kXcd - 1) / kXcd * kXcd;
+    w.tile = mx_tile_rows(P_ext, E_ext);
+    w.group = mx_group(w.tile);
+    const int step = kXcd * w.group;
+    w.mt_pad = ((P_ext + w.tile - 1) / w.tile + (E_ext < P_ext ? E_ext : P_ext) + step - 1) / step * step;
     char* b = reinterpret_cast<char*>(ws);
     size_t off = 0;
     auto take = [&](size_t n) { char* p = b + off; off = align256(off + n); return p; };
     w.order = (int32_t*)take(sizeof(int32_t) * P_ext);
     w.offsets = (int32_t*)take(sizeof(int32_t) * (E_ext + 1));
     w.tile_start = (int32_t*)take(sizeof(int32_t) * (E_ext + 1));
-    w.tinfo = (int4*)take(sizeof(int4) * (P_ext / 16 + E_ext + kXcd));   // (any tile height's)
+    w.tinfo = (int4*)take(sizeof(int4) * (P_ext / 16 + E_ext + 4 * kXcd));   // (any tile height's)
     if (layer) {
         w.xq = (uint8_t*)take((size_t)a.T * (a.H / 2));
         w.xs = (uint8_t*)take((size_t)a.T * (a.H / 32));
@@ -349,21 +350,19 @@ MxWs carve(const FwdArgs& a, bool layer, void* ws) {
 }
 
 template <int KIND, int MPX>
-hipError_t launch_tall(const FwdArgs& a, MxArgs m, const MxWs& w, int K, int N, hipStream_t s) {
-    constexpr int W = kMxWaves<MPX>;
-    const int per = W * (KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxRows / 2 : kMxRows);
+hipError_t launch_tiles(const FwdArgs& a, MxArgs m, const MxWs& w, int K, int N, hipStream_t s) {
+    const int per = kMxWaves * (KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxRows / 2 : kMxRows);
     m.ntn = (N + per - 1) / per;
-    hipLaunchKernelGGL((k_mx_gemm<KIND, MPX>), dim3(w.mt_pad * m.ntn), dim3(64 * W), 2 * kMxBuf<MPX> + mx_table(W, K), s, a, m);
+    hipLaunchKernelGGL((k_mx_gemm<KIND, MPX>), dim3(w.mt_pad * m.ntn), dim3(kMxThreads), 2 * kMxBuf<MPX> + mx_table(K), s, a, m);
     return hipGetLastError();
 }
 
 template <int KIND>
 hipError_t launch_gemm(const FwdArgs& a, const MxArgs& m, const MxWs& w, int K, int N, hipStream_t s) {
     switch (w.tile) {
-        case 16: return launch_tall<KIND, 1>(a, m, w, K, N, s);
-        case 32: return launch_tall<KIND, 2>(a, m, w, K, N, s);
-        case 64: return launch_tall<KIND, 4>(a, m, w, K, N, s);
-        default: return launch_tall<KIND, 8>(a, m, w, K, N, s);
+        case 16: return launch_tiles<KIND, 1>(a, m, w, K, N, s);
+        case 32: return launch_tiles<KIND, 2>(a, m, w, K, N, s);
+        default: return launch_tiles<KIND, 4>(a, m, w, K, N, s);
     }
 }
 
@@ -371,6 +370,7 @@ MxArgs gemm_args(const FwdArgs& a, const MxWs& w) {
     MxArgs m{};
     m.order = w.order;
     m.tile_start = w.tile_start;
+    m.group = w.group;
     m.tinfo = w.tinfo;
     m.E_ext = a.E + (a.shared ? 1 : 0);
     return m;

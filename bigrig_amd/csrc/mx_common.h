@@ -33,6 +33,7 @@ struct MxArgs {
     uint16_t* y_shared;
     int32_t hstride;            // values between h rows
     int32_t E_ext, ntn;
+    int32_t group;              // M tiles an XCD takes together
     int32_t proj;               // the projection of an expert product
 };
 
