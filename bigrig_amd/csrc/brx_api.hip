@@ -782,13 +782,15 @@ int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int 
     static const uint8_t some = 0;
     FwdArgs a = make_args(d, &none, nullptr, T, (int)n_pairs, nullptr, nullptr, nullptr, 0, nullptr,
                           shared ? &some : nullptr, nullptr, nullptr, nullptr);
-    *out = mx_workspace_bytes(a, !product);
+    // (of whichever kernels a call may take)
+    const size_t all = mx_workspace_bytes(a, !product, false), few = mx_workspace_bytes(a, !product, true);
+    *out = T <= 8 && n_pairs <= 64 && few > all ? few : all;
     return BRX_OK;
 }
 
 // Ahead of a call's launches: its workspace checked, the stream behind the pool's refills (as run_forward).
 static int mx_begin(brx_pool* p, size_t need, void* workspace, size_t workspace_bytes, hipStream_t s) {
-    if (!workspace || ((uintptr_t)workspace & 255)) return fail(BRX_EINVAL, "workspace must be a 256-byte aligned device buffer");
+    if (need && (!workspace || ((uintptr_t)workspace & 255))) return fail(BRX_EINVAL, "workspace must be a 256-byte aligned device buffer");
     if (workspace_bytes < need) return fail(BRX_EINVAL, "this call needs %zu bytes of workspace, %zu given", need, workspace_bytes);
     if (p->refill_pending) {
         HIP_TRY(hipStreamWaitEvent(s, p->refill_done, 0));
@@ -841,7 +843,7 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
     FwdArgs a = make_args(d, p, nullptr, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, nullptr, nullptr,
                           nullptr, y_rows);
     hipStream_t s = (hipStream_t)stream;
-    if ((rc = mx_begin(p, mx_workspace_bytes(a, false), workspace, workspace_bytes, s))) return rc;
+    if ((rc = mx_begin(p, mx_workspace_bytes(a, false, false), workspace, workspace_bytes, s))) return rc;
     return mx_end(p, launch_mx_product(a, (const uint8_t*)codes, (const uint8_t*)scales, proj, workspace, s), s);
 }
 
@@ -859,9 +861,12 @@ static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T
         return fail(BRX_EINVAL, "FORCE_DECODE and FORCE_PREFILL are exclusive");
     FwdArgs a = make_args(d, p, x, T, P, pexp, ptok, prow, yrows, w, shared_expert, shared_gate, out, y_rows);
     hipStream_t s = (hipStream_t)stream;
-    const int rc = mx_begin(p, mx_workspace_bytes(a, true), workspace, workspace_bytes, s);
+    const bool few = (flags & BRX_FWD_FORCE_DECODE) || (!(flags & BRX_FWD_FORCE_PREFILL) && T <= 8 && P <= 64);
+    if (few && (T > 8 || P > 64))
+        return fail(BRX_EINVAL, "the decode path takes at most 8 token rows and 64 pairs (T=%d, P=%d)", T, P);
+    const int rc = mx_begin(p, mx_workspace_bytes(a, true, few), workspace, workspace_bytes, s);
     if (rc) return rc;
-    return mx_end(p, launch_mx_layer(a, workspace, s), s);
+    return mx_end(p, launch_mx_layer(a, few, workspace, s), s);
 }
 
 int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, const int32_t* idx, const float* w,

@@ -213,8 +213,6 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     if (c0 >= N) return;                           // (a wave past the last rows)
     const float nan = absent_nan();
     if constexpr (KIND == 0) {
-        // act_apply's values with the rule picked by selects (one copy of the code) and the limits by
-        // comparisons, which leave a NaN as it is
         const bool clamped = a.act == BRX_ACT_SWIGLU_CLAMPED;
         const float alpha = clamped ? a.alpha : 1.0f;
 #pragma unroll
@@ -230,14 +228,8 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float gv = acc[p][2 * h + (i >> 2)][i & 3] + b0[i];
-                    float uv = 1.0f;
-                    if (gated) {
-                        uv = acc[p][2 + (i >> 2)][i & 3] + b1[i];
-                        if (clamped) uv = (uv > a.limit ? a.limit : uv < -a.limit ? -a.limit : uv) + 1.0f;
-                    }
-                    hv[i] = x_sigmoid(clamped && gv > a.limit ? a.limit : gv, alpha) * uv;
-                    hv[i] = absent ? nan : hv[i];
+                    hv[i] = mx_act(a, gated, clamped, alpha, acc[p][2 * h + (i >> 2)][i & 3] + b0[i],
+                                   acc[p][2 + (i >> 2)][i & 3] + b1[i], absent);
                     top = max(top, mx_mag(hv[i]));
                 }
                 top = max(top, lane_xor16(top));
@@ -383,9 +375,13 @@ hipError_t bucket(const FwdArgs& a, const MxWs& w, hipStream_t s) {
 
 }  // namespace
 
-size_t mx_workspace_bytes(const FwdArgs& a, bool layer) { return carve(a, layer, nullptr).bytes; }
+size_t mx_workspace_bytes(const FwdArgs& a, bool layer, bool few) {
+    if (!layer && a.P <= kMxFewPairs) return 0;
+    return few ? mx_few_workspace_bytes(a) : carve(a, layer, nullptr).bytes;
+}
 
-hipError_t launch_mx_layer(const FwdArgs& a, void* ws, hipStream_t s) {
+hipError_t launch_mx_layer(const FwdArgs& a, bool few, void* ws, hipStream_t s) {
+    if (few) return launch_mx_few_layer(a, ws, s);
     const MxWs w = carve(a, true, ws);
     MxRows x{};
     x.x = const_cast<uint16_t*>(a.x);
@@ -414,6 +410,7 @@ hipError_t launch_mx_layer(const FwdArgs& a, void* ws, hipStream_t s) {
 
 hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, void* ws,
                              hipStream_t s) {
+    if (a.P <= kMxFewPairs) return launch_mx_few_product(a, codes, scales, proj, s);
     const MxWs w = carve(a, false, ws);
     hipError_t e = bucket(a, w, s);
     if (e != hipSuccess) return e;

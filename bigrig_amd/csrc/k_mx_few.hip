@@ -1,0 +1,435 @@
+// MXFP4 products of few (token, expert) pairs: a decode step's expert layer in two launches, a short
+// list's expert product in one.
+//
+//   k_mx_few_up    grid (32 features, entry): the entry's token rows rounded to MXFP4 in LDS, the gate and up
+//                  rows of its expert, act() and h in MXFP4; also writes the entry table.
+//   k_mx_few_rows  <true>: 16 output columns of every entry's down rows and, in the epilogue, their weighted
+//                  sum (grid H / 16). <false>: one projection's rows for a list of pairs (grid
+//                  (n_out / 16, entries / 8)).
+// An entry is an expert with up to 16 of the step's pairs, in order of its first pair; the shared
+// expert's comes last. The arithmetic is k_mx_gemm's to the bit: the same 512-K chunks in the same order, the
+// same roundings.
+//
+// What bounds it: the weights are read once, and a wave requests the whole of its 16 rows (up to 6 chunks,
+// 24 KB) before it multiplies anything, so a call is a few dependent round trips -- the routing, the
+// table, the weights -- and little else.
+#include <type_traits>
+
+#include "mx_common.h"
+#include "pf_common.h"
+
+namespace brx {
+namespace {
+
+constexpr int kUpWaves = 4;
+constexpr int kRowWaves = 8;
+
+// Pairs of an entry, and what the second launch reads of it.
+struct MxEntry {
+    int32_t slot, n;
+    int32_t pair[16];
+};
+struct MxTable {
+    int32_t n, pad[3];
+    MxEntry ent[kMxFewPairs + 1];
+};
+
+// One entry as a wave holds it: its expert, slot code, pairs (column c's pair in lanes c, c + 16, ..; the last
+// one again past the end), and the step's number of entries. Returns false past the last entry.
+struct MxPlan {
+    int e, slot, n, pair, entries;
+};
+__device__ __forceinline__ bool mx_plan(const FwdArgs& a, int u, int32_t* s_pair, MxPlan& o) {
+    const int lane = threadIdx.x & 63;
+    const int P = a.P, emax = a.shared ? a.E : a.E - 1;
+    const int e = lane < P ? min(max(a.pexp[min(lane, P - 1)], 0), emax) : -1 - lane;
+    uint64_t same = 0;
+    for (int r = 0; r < P; ++r) {
+        const bool eq = e == __builtin_amdgcn_readlane(e, r);
+        const uint64_t b = __ballot(eq);
+        if (eq) same = b;
+    }
+    const uint64_t below = (1ull << lane) - 1ull;
+    const int rank = __popcll(same & below);
+    const uint64_t leads = __ballot(lane < P && (rank & 15) == 0);
+    const int routed = __popcll(leads);
+    o.entries = routed + (a.auto_shared ? 1 : 0);
+    if (u >= o.entries) return false;
+    if (u == routed) {                             // every token of the shared expert (at most 8)
+        o.e = a.E;
+        o.slot = -1;
+        o.n = a.T;
+        o.pair = P + min(lane & 15, a.T - 1);
+        return true;
+    }
+    const int lead = __builtin_ctzll(__ballot(((leads >> lane) & 1) && __popcll(leads & below) == u));
+    o.e = __builtin_amdgcn_readlane(e, lead);
+    const int r0 = __builtin_amdgcn_readlane(rank, lead);
+    const bool in = e == o.e && rank >= r0 && rank < r0 + 16;
+    o.n = __popcll(__ballot(in));
+    if (in) s_pair[rank - r0] = lane;              // (the wave's own words)
+    __builtin_amdgcn_wave_barrier();
+    o.pair = s_pair[min(lane & 15, o.n - 1)];
+    o.slot = o.e < a.E ? slot_code(a, o.e, a.g2s[o.e]) : -1;
+    o.slot = __builtin_amdgcn_readfirstlane(o.slot);
+    if (o.slot == kAbsentCode && lane == 0) note_absent(a, o.e);
+    return true;
+}
+
+// NB chunks of 16 weight rows as a wave loads them: the codes as k_mx_gemm, and each row's 16 scale bytes by
+// four neighbouring lanes.
+template <int NB>
+struct FewW {
+    mx_u32x4 w[NB][4];
+    uint32_t s[NB];
+};
+// w0 and s0: byte offsets of the fragment's codes row and scales row 0; row m of the fragment is `step` rows
+// apart in blocks of four (8: rows 8 (m / 4) + m % 4; 4: the rows in order).
+template <int NB>
+__device__ __forceinline__ void few_load(__amdgpu_buffer_rsrc_t r, uint32_t w0, uint32_t s0, int step, int K, int ch0,
+                                         FewW<NB>& o) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15, G = K / 32;
+    const uint32_t row = (uint32_t)(K / 2);
+    const uint32_t vw = w0 + (uint32_t)(step * (l16 >> 2)) * row;
+    const uint32_t vs = s0 + (uint32_t)(step * (lane >> 4) + ((lane >> 2) & 3)) * (uint32_t)G;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int ch = ch0 + j;
+        o.s[j] = __builtin_amdgcn_raw_buffer_load_b32(r, vs + (uint32_t)min(16 * ch + 4 * (lane & 3), G - 4), 0, 0);
+        const uint32_t v = vw + 16u * (uint32_t)min(16 * ch + 4 * g + (l16 & 3), G - 1);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o.w[j][t] = __builtin_amdgcn_raw_buffer_load_b128(r, v, t * row, 0);
+    }
+}
+// acc += the fragment's chunk ch times X's (pieces xv of this lane's K groups, their scales xe).
+__device__ __forceinline__ void few_mul(mx_u32x4 (&w)[4], uint32_t s, int ch, int K, const mx_u32x4 (&xv)[4], uint32_t xe,
+                                        f32x4_t& acc) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, G = K / 32;
+    // lane (g, m) takes word g of row m's scales from lane 4 m + g; its first group is byte `off` of the word,
+    // and groups past the row's end are zeros
+    s = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (4 * (lane & 15) + g), (int)s);
+    const int first = 16 * ch + 4 * g, off = max(first - (G - 4), 0);
+    const uint32_t ws = (s >> ((8 * off) & 31)) & (uint32_t)((first - G) >> 31);
+    mx_transpose(w);
+    acc = mx_mfma<0>(w[0], ws, xv[0], xe, acc);
+    acc = mx_mfma<1>(w[1], ws, xv[1], xe, acc);
+    acc = mx_mfma<2>(w[2], ws, xv[2], xe, acc);
+    acc = mx_mfma<3>(w[3], ws, xv[3], xe, acc);
+}
+
+// LDS of a staged token row of nch chunks: an odd number of 16-byte pieces, an odd number of words of scales.
+__host__ __device__ inline int few_code_pitch(int nch) { return nch * 256 + 16; }
+__host__ __device__ inline int few_scale_pitch(int nch) { return nch * 16 + 4; }
+
+template <int NB>
+__global__ __launch_bounds__(64 * kUpWaves) void k_mx_few_up(FwdArgs a, MxArgs m, MxTable* __restrict__ table) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ __attribute__((aligned(16))) f32x4_t red[4][64];
+    __shared__ int32_t s_pair[kUpWaves][16];
+    prefetch_args(a);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, l16 = lane & 15;
+    MxPlan pl;
+    if (!mx_plan(a, blockIdx.y, s_pair[wv], pl)) return;
+    const bool gated = a.act != BRX_ACT_SILU_MLP, sh = pl.e >= a.E;
+    const Layout& L = sh ? a.lay_sh : a.lay;
+    const int K = a.H, N = L.p[0].n_out, G = K / 32, nch = (G + 15) / 16;
+    const int c0 = blockIdx.x * (gated ? 32 : 64);
+    if (blockIdx.x == 0 && wv == 0) {
+        MxEntry& en = table->ent[blockIdx.y];
+        if (lane == 0) {
+            en.slot = pl.slot;
+            en.n = pl.n;
+            if (blockIdx.y == 0) table->n = pl.entries;
+        }
+        if (lane < 16) en.pair[lane] = pl.pair;
+    }
+    if (c0 >= N) return;
+    const uint8_t* base = sh ? a.shared : code_base(a, clamp_code(a, pl.slot));
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(base, (uint32_t)L.bytes);
+    // wave f: fragment f (0, 1: the first 32 rows' blocks of four in turn; 2, 3: the up rows, or the next 32)
+    const bool second = wv >= 2;
+    const Proj& P = gated && second ? L.p[1] : L.p[0];
+    const int r0 = c0 + (gated || !second ? 0 : 32) + 4 * (wv & 1);
+    FewW<NB> q;
+    // (x first: its rounding goes on while the weights come)
+    const int token = pl.pair >= a.P ? pl.pair - a.P : pair_tok(a, pl.pair);
+    if (lane < 16) s_pair[wv][lane] = token;
+    __builtin_amdgcn_wave_barrier();
+    const int pieces = pl.n * (K / 8);             // 8 values each
+    const int PC = few_code_pitch(nch), PS = few_scale_pitch(nch);
+    uint8_t* const sc = smem + pl.n * PC;
+    constexpr int U = 4;
+    u32x4_t xr[U];
+    auto x_at = [&](int i) __attribute__((always_inline)) {
+        const int r = min(i, pieces - 1) / (K / 8), c = min(i, pieces - 1) - r * (K / 8);
+        return *reinterpret_cast<const u32x4_t*>(a.x + (int64_t)s_pair[wv][r] * K + 8 * c);
+    };
+    auto x_put = [&](int i, const u32x4_t& v4) __attribute__((always_inline)) {
+        const int r = min(i, pieces - 1) / (K / 8), c = min(i, pieces - 1) - r * (K / 8);
+        float v[8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = bf2f((k & 1) ? v4[k >> 1] >> 16 : v4[k >> 1] & 0xFFFFu);
+            top = max(top, mx_mag(v[k]));
+        }
+        top = max(top, dpp_u<0xB1>(top));
+        top = max(top, dpp_u<0x4E>(top));
+        const uint32_t sb = mx_scale(top), o = mx_codes(v, sb);
+        if (i < pieces) {
+            *reinterpret_cast<uint32_t*>(smem + r * PC + 4 * c) = o;
+            if ((c & 3) == 0) sc[r * PS + c / 4] = (uint8_t)sb;
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < U; ++k) xr[k] = x_at(tid + k * 64 * kUpWaves);
+    asm volatile("" ::: "memory");
+    const uint32_t w0 = (uint32_t)P.w + (uint32_t)r0 * (uint32_t)(K / 2), s0 = (uint32_t)P.s + (uint32_t)r0 * (uint32_t)G;
+    few_load<NB>(rw, w0, s0, 8, K, 0, q);
+    // the biases of this block's outputs (used by the first wave)
+    u32x4_t bias[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        bias[h] = u32x4_t{0u, 0u, 0u, 0u};
+        const Proj& B = gated && h ? L.p[1] : L.p[0];
+        if (B.bias >= 0)
+            bias[h] = __builtin_amdgcn_raw_buffer_load_b128(rw, (uint32_t)(B.bias + 2 * (c0 + (gated || !h ? 0 : 32) + 8 * g)), 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) x_put(tid + k * 64 * kUpWaves, xr[k]);
+    for (int i0 = U * 64 * kUpWaves; i0 < pieces; i0 += U * 64 * kUpWaves) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) xr[k] = x_at(i0 + tid + k * 64 * kUpWaves);
+#pragma unroll
+        for (int k = 0; k < U; ++k) x_put(i0 + tid + k * 64 * kUpWaves, xr[k]);
+    }
+    // zeros past the rows' ends, up to whole chunks
+    const int padp = 16 * nch - G;
+    for (int i = tid; i < pl.n * padp; i += 64 * kUpWaves) {
+        const int r = i / padp, c = G + i % padp;
+        *reinterpret_cast<u32x4_t*>(smem + r * PC + 16 * c) = u32x4_t{0u, 0u, 0u, 0u};
+        sc[r * PS + c] = 0;
+    }
+    lds_barrier();
+    f32x4_t acc{0.f, 0.f, 0.f, 0.f};
+    const int xrow = min(l16, pl.n - 1);
+    for (int ch0 = 0; ch0 < nch; ch0 += NB) {
+        if (ch0) few_load<NB>(rw, w0, s0, 8, K, ch0, q);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            if (ch0 + j < nch) {                   // uniform
+                mx_u32x4 xv[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    xv[t] = *reinterpret_cast<const mx_u32x4*>(smem + xrow * PC + (ch0 + j) * 256 + 16 * (4 * g + t));
+                const uint32_t xe = *reinterpret_cast<const uint32_t*>(sc + xrow * PS + (ch0 + j) * 16 + 4 * g);
+                few_mul(q.w[j], q.s[j], ch0 + j, K, xv, xe, acc);
+            }
+        }
+    }
+    red[wv][lane] = acc;
+    lds_barrier();
+    if (wv != 0) return;
+    // lane (g, n): columns 8 g .. 8 g + 7 of each 32 for pair n, as in k_mx_gemm's epilogue
+    const f32x4_t d[4] = {red[0][lane], red[1][lane], red[2][lane], red[3][lane]};
+    const bool clamped = a.act == BRX_ACT_SWIGLU_CLAMPED;
+    const float alpha = clamped ? a.alpha : 1.0f;
+    float b[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[h][i] = bf2f((i & 1) ? bias[h][i >> 1] >> 16 : bias[h][i >> 1] & 0xFFFFu);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (gated && h == 1) break;
+        float hv[8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            hv[i] = mx_act(a, gated, clamped, alpha, d[2 * h + (i >> 2)][i & 3] + b[h][i], d[2 + (i >> 2)][i & 3] + b[1][i],
+                           pl.slot == kAbsentCode);
+            top = max(top, mx_mag(hv[i]));
+        }
+        top = max(top, lane_xor16(top));
+        top = max(top, lane_xor32(top));
+        const uint32_t sb = mx_scale(top);
+        if (l16 < pl.n) {
+            const int64_t row = pl.pair;
+            const int col = c0 + 32 * h + 8 * g;
+            *reinterpret_cast<uint32_t*>(m.hq + row * (m.hstride / 2) + col / 2) = mx_codes(hv, sb);
+            if (g == 0) m.hs[row * (m.hstride / 32) + col / 32] = (uint8_t)sb;
+        }
+    }
+}
+
+// DOWN: the second launch of a layer, over the entry table; else one projection's rows.
+template <bool DOWN, int NB>
+__global__ __launch_bounds__(64 * kRowWaves) void k_mx_few_rows(FwdArgs a, MxArgs m, const MxTable* __restrict__ table) {
+    __shared__ __attribute__((aligned(16))) float ys[DOWN ? kMxFewPairs + kMxFewTokens : 1][16];
+    __shared__ int32_t s_pair[kRowWaves][16];
+    prefetch_args(a);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, l16 = lane & 15;
+    const int c0 = blockIdx.x * 16;
+    const int entries = DOWN ? __builtin_amdgcn_readfirstlane(table->n) : 0;
+    for (int u = DOWN ? wv : blockIdx.y * kRowWaves + wv; DOWN ? u < entries : true; u += DOWN ? kRowWaves : 1 << 20) {
+        MxPlan pl;
+        if constexpr (DOWN) {
+            pl.slot = __builtin_amdgcn_readfirstlane(table->ent[u].slot);
+            pl.n = __builtin_amdgcn_readfirstlane(table->ent[u].n);
+            pl.pair = table->ent[u].pair[l16];
+            pl.e = pl.slot == -1 ? a.E : 0;
+        } else {
+            if (!mx_plan(a, u, s_pair[wv], pl)) break;
+        }
+        const bool sh = pl.e >= a.E, absent = pl.slot == kAbsentCode;
+        const Layout& L = sh ? a.lay_sh : a.lay;
+        const Proj P = DOWN ? L.p[2] : m.proj == 0 ? L.p[0] : m.proj == 1 ? L.p[1] : L.p[2];
+        const uint8_t* base = sh ? a.shared : code_base(a, clamp_code(a, pl.slot));
+        const __amdgpu_buffer_rsrc_t rw = make_rsrc(base, (uint32_t)L.bytes);
+        const int K = P.n_in, N = P.n_out, G = K / 32, nch = (G + 15) / 16;
+        const uint32_t w0 = (uint32_t)P.w + (uint32_t)c0 * (uint32_t)(K / 2), s0 = (uint32_t)P.s + (uint32_t)c0 * (uint32_t)G;
+        const int64_t xr = DOWN ? pl.pair : pair_tok(a, pl.pair);
+        const int64_t stride = DOWN ? m.hstride : K;
+        const uint8_t* const xc = (DOWN ? m.hq : m.xq) + xr * (stride / 2);
+        const uint8_t* const xs = (DOWN ? m.hs : m.xs) + xr * (stride / 32);
+        f32x4_t acc{0.f, 0.f, 0.f, 0.f};
+        u32x2_t bias{0u, 0u};
+        if (P.bias >= 0) bias = *reinterpret_cast<const u32x2_t*>(base + P.bias + 2 * (c0 + 4 * g));
+        for (int ch0 = 0; ch0 < nch; ch0 += NB) {
+            FewW<NB> q;
+            mx_u32x4 xv[NB][4];
+            uint32_t xe[NB];
+            few_load<NB>(rw, w0, s0, 4, K, ch0, q);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int first = 16 * (ch0 + j) + 4 * g;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    // (pieces past the row's end: any, and zeros below)
+                    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(xc + 16 * min(first + t, G - 1));
+                    xv[j][t] = mx_u32x4{v[0], v[1], v[2], v[3]};
+                }
+                // two groups at a time: rows of scales are 2-byte aligned
+                const uint32_t lo = *reinterpret_cast<const uint16_t*>(xs + min(first, G - 2));
+                const uint32_t hi = *reinterpret_cast<const uint16_t*>(xs + min(first + 2, G - 2));
+                xe[j] = lo | (hi << 16);
+            }
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                if (ch0 + j < nch) {               // uniform
+                    const int first = 16 * (ch0 + j) + 4 * g;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const uint32_t in = (uint32_t)((first + t - G) >> 31);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) xv[j][t][i] &= in;
+                    }
+                    few_mul(q.w[j], q.s[j], ch0 + j, K, xv[j], xe[j], acc);
+                }
+            }
+        }
+        // lane (g, n): columns 4 g .. 4 g + 3 of pair n
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            y[i] = absent ? absent_nan() : acc[i] + bf2f((i & 1) ? bias[i >> 1] >> 16 : bias[i >> 1] & 0xFFFFu);
+        if (l16 < pl.n) {
+            if constexpr (DOWN) {
+                *reinterpret_cast<f32x4_t*>(&ys[pl.pair][4 * g]) = f32x4_t{y[0], y[1], y[2], y[3]};
+            } else {
+                *reinterpret_cast<u32x2_t*>(m.y_routed + (int64_t)pair_row(a, pl.pair) * N + c0 + 4 * g) =
+                    u32x2_t{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+            }
+        }
+    }
+    if constexpr (DOWN) {
+        lds_barrier();
+        // two columns a thread, each pair's row rounded to bf16
+        const int c = 2 * (tid & 7);
+        if (a.yun) {
+            for (int q = tid >> 3; q < a.P; q += 8 * kRowWaves)
+                *reinterpret_cast<uint32_t*>(a.yun + (int64_t)pair_row(a, q) * a.H + c0 + c) = pk_bf16(ys[q][c], ys[q][c + 1]);
+        }
+        if (a.out && tid < 8 * a.T) {
+            const int t = tid >> 3;
+            float o0 = 0.f, o1 = 0.f;
+            auto add = [&](float w, int q) __attribute__((always_inline)) {
+                const uint32_t v = pk_bf16(ys[q][c], ys[q][c + 1]);
+                o0 = fmaf(w, bf2f(v & 0xFFFFu), o0);
+                o1 = fmaf(w, bf2f(v >> 16), o1);
+            };
+            for (int j = 0; j < a.k; ++j) add(a.w[t * a.k + j], t * a.k + j);
+            if (a.auto_shared && a.sgate) add(a.sgate[t], a.P + t);
+            *reinterpret_cast<uint32_t*>(a.out + (int64_t)t * a.H + c0 + c) = f2bf(o0) | (f2bf(o1) << 16);
+        }
+    }
+}
+
+inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+struct FewWs {
+    MxTable* table;
+    uint8_t *hq, *hs;
+    int Imax;
+    size_t bytes;
+};
+FewWs carve_few(const FwdArgs& a, void* ws) {
+    FewWs w{};
+    w.Imax = a.shared && a.I_sh > a.I ? a.I_sh : a.I;
+    const size_t rows = (size_t)a.P + (a.auto_shared ? a.T : 0);
+    uint8_t* b = reinterpret_cast<uint8_t*>(ws);
+    w.table = reinterpret_cast<MxTable*>(b);
+    size_t off = align256(sizeof(MxTable));
+    w.hq = b + off; off = align256(off + rows * (w.Imax / 2));
+    w.hs = b + off; off = align256(off + rows * (w.Imax / 32));
+    w.bytes = off;
+    return w;
+}
+
+// Chunks a wave loads at once: all of a row's, up to six.
+inline int few_batch(int K) { const int nch = (K + 511) / 512; return nch <= 2 ? 2 : nch <= 4 ? 4 : 6; }
+
+}  // namespace
+
+size_t mx_few_workspace_bytes(const FwdArgs& a) { return carve_few(a, nullptr).bytes; }
+
+hipError_t launch_mx_few_layer(const FwdArgs& a, void* ws, hipStream_t s) {
+    const FewWs w = carve_few(a, ws);
+    MxArgs m{};
+    m.hq = w.hq;
+    m.hs = w.hs;
+    m.hstride = w.Imax;
+    const int per = a.act == BRX_ACT_SILU_MLP ? 64 : 32, nch = (a.H + 511) / 512;
+    int most = a.P < 16 ? a.P : 16;                // pairs of an entry, at most
+    if (a.auto_shared && a.T > most) most = a.T;
+    const dim3 grid((w.Imax + per - 1) / per, a.P + (a.auto_shared ? 1 : 0));
+    const size_t lds = (size_t)most * (few_code_pitch(nch) + few_scale_pitch(nch));
+#define BRX_UP(NB) hipLaunchKernelGGL((k_mx_few_up<NB>), grid, dim3(64 * kUpWaves), lds, s, a, m, w.table)
+    switch (few_batch(a.H)) { case 2: BRX_UP(2); break; case 4: BRX_UP(4); break; default: BRX_UP(6); }
+#undef BRX_UP
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+#define BRX_DOWN(NB) hipLaunchKernelGGL((k_mx_few_rows<true, NB>), dim3(a.H / 16), dim3(64 * kRowWaves), 0, s, a, m, w.table)
+    switch (few_batch(w.Imax)) { case 2: BRX_DOWN(2); break; case 4: BRX_DOWN(4); break; default: BRX_DOWN(6); }
+#undef BRX_DOWN
+    return hipGetLastError();
+}
+
+hipError_t launch_mx_few_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, hipStream_t s) {
+    MxArgs m{};
+    m.xq = codes;
+    m.xs = scales;
+    m.y_routed = a.yun;
+    m.proj = proj;
+    const dim3 grid((proj == 2 ? a.H : a.I) / 16, (a.P + kRowWaves - 1) / kRowWaves);
+#define BRX_ROWS(NB) hipLaunchKernelGGL((k_mx_few_rows<false, NB>), grid, dim3(64 * kRowWaves), 0, s, a, m, (const MxTable*)nullptr)
+    switch (few_batch(proj == 2 ? a.I : a.H)) { case 2: BRX_ROWS(2); break; case 4: BRX_ROWS(4); break; default: BRX_ROWS(6); }
+#undef BRX_ROWS
+    return hipGetLastError();
+}
+
+}  // namespace brx

@@ -20,6 +20,10 @@
 
 namespace brx {
 
+// Most tokens and (token, expert) pairs of the few-pair kernels (a step is planned by one wave).
+constexpr int kMxFewTokens = 8;
+constexpr int kMxFewPairs = 64;
+
 // What the GEMM launches take beside the forward's arguments (FwdArgs::x is unused).
 struct MxArgs {
     const uint8_t* xq;          // activation rows: codes [T, n_in / 2]
@@ -91,6 +95,18 @@ __device__ __forceinline__ void mx_transpose(mx_u32x4 (&v)[4]) {
             v[t + 2][i] = high ? b : s;
         }
     }
+}
+
+// The activation of one output: act_apply's values with the rule picked by selects (one copy of the code)
+// and the limits by comparisons, which leave a NaN as it is; NaN for an absent expert.
+__device__ __forceinline__ float mx_act(const FwdArgs& a, bool gated, bool clamped, float alpha, float g, float u,
+                                        bool absent) {
+    if (clamped) {
+        g = g > a.limit ? a.limit : g;
+        u = (u > a.limit ? a.limit : u < -a.limit ? -a.limit : u) + 1.0f;
+    }
+    const float h = x_sigmoid(g, alpha) * (gated ? u : 1.0f);
+    return absent ? absent_nan() : h;
 }
 
 // acc += W (16 rows) . X (16 rows) over 128 K under byte S of each side's scales: lane l ends with W rows

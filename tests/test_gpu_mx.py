@@ -299,9 +299,18 @@ def test_product_refusals(gpu):
         return lib.brx_mx_expert_product(C.byref(d), pool.device.handle, codes, q.scales.data_ptr(), T, t.data_ptr(),
                                          e.data_ptr(), None, n, 8, proj, out, w, nb, None)
     for kw in (dict(codes=None), dict(codes=q.codes.data_ptr() + 8), dict(T=0), dict(T=-1), dict(n=-1), dict(proj=3),
-               dict(w=None), dict(w=ws.data_ptr() + 16), dict(nb=64), dict(out=None), dict(out=y.data_ptr() + 2)):
+               dict(out=None), dict(out=y.data_ptr() + 2)):
         assert raw(**kw) == L.BRX_EINVAL, kw
     assert raw() == 0
+    # more pairs take scratch
+    t, e = t.repeat(10), e.repeat(10)
+    y = torch.zeros(80, 192, dtype=torch.bfloat16, device=gpu)
+    more = lambda w, nb: lib.brx_mx_expert_product(   # noqa: E731
+        C.byref(d), pool.device.handle, q.codes.data_ptr(), q.scales.data_ptr(), 3, t.data_ptr(), e.data_ptr(), None,
+        80, 80, 0, y.data_ptr(), w, nb, None)
+    for w, nb in ((None, ws.numel()), (ws.data_ptr() + 16, ws.numel() - 256), (ws.data_ptr(), 64)):
+        assert more(w, nb) == L.BRX_EINVAL
+    assert more(ws.data_ptr(), ws.numel()) == 0
     torch.cuda.synchronize()
 
 
@@ -389,6 +398,41 @@ def test_a_row_does_not_depend_on_its_call(gpu, T):
     for t in (0, T // 2, T - 1):
         one = bits(mx.moe_forward(spec, pool, xd[t:t + 1], idd[t:t + 1], flags=flags))
         assert np.array_equal(one[0], rows[t])
+
+
+@pytest.mark.parametrize("name", ["swiglu", "shared", "clamped", "mlp", "wide", "long"])
+@pytest.mark.parametrize("T", [1, 3, 8])
+def test_both_kernel_families_give_the_same_bits(gpu, name, T):
+    spec, lay, sw, pool = built(name, gpu)
+    x, idx, w, sg = _layer_inputs(spec, lay, gpu, T, seed=40 + T)
+    if T == 8 and name == "clamped":
+        idx[:, 1:] = 3                   # an expert with more pairs than a tile's smallest height
+    xd, idd, wd = to_dev_bits(x, gpu), dev(idx, gpu), dev(w, gpu)
+    kw = dict(shared=sw.shared, sgate=None if sg is None else dev(sg, gpu))
+    out = [bits(mx.moe_forward(spec, pool, xd, idd, wd, flags=f, **kw)) for f in (L.FWD_FORCE_DECODE, L.FWD_FORCE_PREFILL)]
+    rows = [bits(mx.moe_forward(spec, pool, xd, idd, flags=f)) for f in (L.FWD_FORCE_DECODE, L.FWD_FORCE_PREFILL)]
+    assert np.array_equal(*rows)
+    assert np.array_equal(*out)
+
+
+@pytest.mark.parametrize("name, proj", [("swiglu", "down_proj"), ("clamped", "gate_proj"), ("mlp", "fc1"), ("wide", "up_proj"),
+                                        ("long", "down_proj")])
+def test_short_and_long_lists_give_the_same_bits(gpu, name, proj):
+    spec, pool, q, tok, ex, _, _ = _product(gpu, name, proj, 11, 80, seed=6)
+    t, e = dev(tok, gpu), dev(ex, gpu)
+    want = bits(mx.expert_product(spec, pool, q, t, e, proj))
+    for a, b in ((0, 64), (3, 4), (10, 47)):
+        got = bits(mx.expert_product(spec, pool, q, t[a:b].contiguous(), e[a:b].contiguous(), proj))
+        assert np.array_equal(got, want[a:b])
+
+
+@pytest.mark.parametrize("T", [4, 40])
+def test_nan_passes_the_clamped_activation(gpu, T):
+    spec, lay, sw, pool = built("clamped", gpu)
+    x, idx, w, _ = _layer_inputs(spec, lay, gpu, T, seed=9)
+    x[2, 100] = 0x7F80
+    out = f64(bits(mx.moe_forward(spec, pool, to_dev_bits(x, gpu), dev(idx, gpu), dev(w, gpu))))
+    assert np.isnan(out[2]).all() and np.isfinite(out[np.r_[:2, 3:T]]).all()
 
 
 # ------------------------------------------------------------------ as a program uses them
