@@ -55,17 +55,20 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t top) {
     return top >= 0x7F800000u ? 255u : (uint32_t)max((int)(top >> 23) - 2, 0);
 }
 
-// The codes of 8 consecutive values of a group with scale byte `sb`, the first in the low bits. The
+// The codes of N = 4 or 8 consecutive values of a group with scale byte `sb`, the first in the low bits. The
 // hardware conversion divides by the scale, rounds to nearest even and saturates; it keeps the
 // sign of a zero, which is cleared here: (m + 7) of a code's magnitude m has bit 3 set unless m is 0,
 // and never carries into the next code.
-__device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t sb) {
+template <int N>
+__device__ __forceinline__ uint32_t mx_codes(const float (&v)[N], uint32_t sb) {
     const float sc = __builtin_bit_cast(float, sb == 0u ? 0x00400000u : sb << 23);
     uint32_t o = 0u;
     o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[0], v[1], sc, 0);
     o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[2], v[3], sc, 1);
-    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[4], v[5], sc, 2);
-    o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[6], v[7], sc, 3);
+    if constexpr (N == 8) {
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[4], v[5], sc, 2);
+        o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[6], v[7], sc, 3);
+    }
     const uint32_t m = o & 0x77777777u;
     o = m | (o & (m + 0x77777777u) & 0x88888888u);
     return sb == 255u ? 0u : o;

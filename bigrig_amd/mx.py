@@ -23,16 +23,18 @@ calls on several streams do not share any, and a captured graph keeps its own.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 from . import formats as F
 from . import lib as L
-from .layer import _stream, path_flag
+from .layer import _stream
 from .pool import ExpertPool
 from .spec import LayerSpec
 
 MAX_TOKENS = 65535      # token rows of one layer call
 MAX_PAIRS = 1 << 21     # (token, expert) pairs of one call
+FEW_PAIRS = 64          # pairs an expert product runs without scratch
 
 
 @dataclass(frozen=True)
@@ -46,6 +48,7 @@ class MXRows:
         return (*self.codes.shape[:-1], 2 * self.codes.shape[-1])
 
 
+@functools.lru_cache(maxsize=None)
 def _dtype(t) -> int:
     import torch
     dt = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}.get(t)
@@ -61,30 +64,32 @@ def _on_device(*tensors) -> None:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError("tensors must be on the GPU")
-        if cur is None:
+        d = t.get_device()
+        if d != cur:
+            if not t.is_cuda:
+                raise ValueError("tensors must be on the GPU")
             cur = torch.cuda.current_device()
-        if t.device.index != cur:
-            raise ValueError(f"tensor on cuda:{t.device.index}, the current device is cuda:{cur}")
+            if d != cur:
+                raise ValueError(f"tensor on {t.device}, the current device is cuda:{cur}")
 
 
 def _matrices(t, what: str):
     """(batch, rows, batch stride, row stride) of t [..., rows, n] seen as a run of matrices, in
     elements; its innermost dimension must be contiguous and the leading ones collapse to one."""
-    if t.dim() == 0:
+    n = t.dim()
+    if n == 0:
         raise ValueError(f"{what} has no dimensions")
     if t.numel() == 0:
         return 0, 0, 0, 0
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{what}'s innermost dimension must be contiguous (stride {t.stride(-1)})")
-    if t.dim() == 1:
-        return 1, 1, 0, 0
-    if t.dim() == 2:
+    if n == 2:
         return 1, t.shape[0], 0, t.stride(0)
+    if n == 1:
+        return 1, 1, 0, 0
     if t.is_contiguous():
         return 1, t.numel() // t.shape[-1], 0, t.shape[-1]
-    if t.dim() > 3:
+    if n > 3:
         try:
             t = t.view(-1, *t.shape[-2:])
         except RuntimeError:
@@ -106,18 +111,9 @@ def _packed(t, what: str):
 
 def _keep(stream, *tensors) -> None:
     """Memory allocated for a call that runs on `stream` is not handed out again before it ends."""
-    if stream is not None:
-        for t in tensors:
-            if t is not None:
-                t.record_stream(stream)
-
-
-def _run_quantize(x, codes, codes_bs, scales, scales_bs, stream) -> None:
-    b, r, bs, rs = _matrices(x, "x")
-    if b == 0:
-        return
-    L.check(L.load().brx_mx_quantize(x.data_ptr(), _dtype(x.dtype), b, r, x.shape[-1], bs, rs,
-                                     codes, codes_bs, scales, scales_bs, _stream(stream)))
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
 
 
 def quantize(x, stream=None) -> MXRows:
@@ -127,15 +123,20 @@ def quantize(x, stream=None) -> MXRows:
     held as NaN (scale byte 255)."""
     import torch
     _on_device(x)
-    _dtype(x.dtype)
-    if x.dim() == 0 or x.shape[-1] % 32:
-        raise ValueError(f"rows of {tuple(x.shape)}: the innermost dimension must be a multiple of 32")
-    K = x.shape[-1]
-    codes = torch.empty((*x.shape[:-1], K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], K // 32), dtype=torch.uint8, device=x.device)
-    b, r, _, _ = _matrices(x, "x")
-    _run_quantize(x, codes.data_ptr(), r * (K // 2), scales.data_ptr(), r * (K // 32), stream)
-    _keep(stream, codes, scales)
+    dt = _dtype(x.dtype)
+    shape = x.shape
+    if not shape or shape[-1] % 32:
+        raise ValueError(f"rows of {tuple(shape)}: the innermost dimension must be a multiple of 32")
+    K = shape[-1]
+    b, r, bs, rs = _matrices(x, "x")
+    lead = shape[:-1]
+    codes = x.new_empty(lead + (K // 2,), dtype=torch.uint8)
+    scales = x.new_empty(lead + (K // 32,), dtype=torch.uint8)
+    if b:
+        L.check(L.load().brx_mx_quantize(x.data_ptr(), dt, b, r, K, bs, rs, codes.data_ptr(), r * (K // 2),
+                                         scales.data_ptr(), r * (K // 32), _stream(stream)))
+        if stream is not None:
+            _keep(stream, codes, scales)
     return MXRows(codes, scales)
 
 
@@ -145,24 +146,31 @@ def dequantize(q: MXRows, dtype=None, stream=None):
     import torch
     dtype = torch.bfloat16 if dtype is None else dtype
     dt = _dtype(dtype)
-    _on_device(q.codes, q.scales)
-    K = 2 * q.codes.shape[-1] if q.codes.dim() else 0
-    if K % 32 or tuple(q.scales.shape) != (*q.codes.shape[:-1], K // 32):
-        raise ValueError(f"codes {tuple(q.codes.shape)} and scales {tuple(q.scales.shape)} are not "
+    codes, scales = q.codes, q.scales
+    _on_device(codes, scales)
+    lead = codes.shape[:-1]
+    K = 2 * codes.shape[-1] if codes.dim() else 0
+    if K % 32 or scales.shape != lead + (K // 32,):
+        raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not "
                          f"[..., K / 2] and [..., K / 32] of one K")
-    out = torch.empty((*q.codes.shape[:-1], K), dtype=dtype, device=q.codes.device)
-    if out.numel() == 0:
+    out = codes.new_empty(lead + (K,), dtype=dtype)
+    n = out.numel()
+    if n == 0:
         return out
-    b, r, cbs = _packed(q.codes, "codes")
-    b2, r2, sbs = _packed(q.scales, "scales")
-    if (b, r) != (b2, r2):      # one of the two is contiguous as a whole, the other is not
-        if b == 1:
-            b, r, cbs = b2, r2, r2 * (K // 2)
-        else:
-            sbs = r * (K // 32)
-    L.check(L.load().brx_mx_dequantize(q.codes.data_ptr(), cbs, q.scales.data_ptr(), sbs, b, r, K, dt,
+    if codes.is_contiguous() and scales.is_contiguous() and codes.dtype == scales.dtype == torch.uint8:
+        b, r, cbs, sbs = 1, n // K, 0, 0
+    else:
+        b, r, cbs = _packed(codes, "codes")
+        b2, r2, sbs = _packed(scales, "scales")
+        if (b, r) != (b2, r2):      # one of the two is contiguous as a whole, the other is not
+            if b == 1:
+                b, r, cbs = b2, r2, r2 * (K // 2)
+            else:
+                sbs = r * (K // 32)
+    L.check(L.load().brx_mx_dequantize(codes.data_ptr(), cbs, scales.data_ptr(), sbs, b, r, K, dt,
                                        out.data_ptr(), _stream(stream)))
-    _keep(stream, out)
+    if stream is not None:
+        _keep(stream, out)
     return out
 
 
@@ -219,7 +227,7 @@ def _check_spec(spec: LayerSpec) -> None:
 
 def _index(t, n: int, what: str):
     import torch
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {n} entries, got "
                          f"{t.dtype} {tuple(t.shape)}")
 
@@ -240,26 +248,33 @@ def _workspace(spec: LayerSpec, T: int, pairs: int, shared: bool, product: bool,
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
+_PROJ = {"gate_proj": 0, "up_proj": 1, "down_proj": 2}
+_MLP_PROJ = {"fc1": 0, "fc2": 2}
+
+
 def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pair_expert, proj: str,
                    pair_row=None, out=None, stream=None):
     """Rows W_proj[pair_expert[i]] . q[pair_token[i]] (+ bias) of one projection ("gate_proj",
     "up_proj", "down_proj"; "fc1", "fc2"), bf16 [n_pairs, n_out]. q: the activations [T, n_in];
-    pair_token and pair_expert int32 [n_pairs]. With `out` [n_rows, n_out] and pair_row (distinct
-    rows), row pair_row[i] is written and the others are left as they are."""
+    pair_token and pair_expert int32 [n_pairs] (entries outside are clamped, as in the layer's pair
+    lists). With `out` [n_rows, n_out] and pair_row (distinct rows), row pair_row[i] is written and
+    the others are left as they are. Up to 64 pairs run as one launch, more as two and with scratch;
+    the rows are the same bits."""
     import torch
     _check_spec(spec)
-    es = spec.expert_spec()
-    if proj not in es:
-        raise ValueError(f"projection {proj!r} not in {list(es)}")
-    n_out, groups = es[proj]["scales"]["shape"]
+    j = (_PROJ if spec.gated else _MLP_PROJ).get(proj)
+    if j is None:
+        raise ValueError(f"projection {proj!r} not in {list(_PROJ if spec.gated else _MLP_PROJ)}")
+    n_out, n_in = (spec.hidden, spec.inter) if j == 2 else (spec.inter, spec.hidden)
+    codes, scales = q.codes, q.scales
     n = pair_expert.numel()
-    _on_device(q.codes, q.scales, pair_token, pair_expert, pair_row, out)
-    if (q.codes.dim() != 2 or q.codes.shape[1] != groups * 16 or
-            tuple(q.scales.shape) != (q.codes.shape[0], groups)):
-        raise ValueError(f"activations {tuple(q.codes.shape)} / {tuple(q.scales.shape)}: {proj} takes rows "
-                         f"of {groups * 32} values")
-    if (q.codes.dtype != torch.uint8 or q.scales.dtype != torch.uint8 or not q.codes.is_contiguous() or
-            not q.scales.is_contiguous()):
+    _on_device(codes, scales, pair_token, pair_expert, pair_row, out)
+    T = codes.shape[0] if codes.dim() else 0
+    if codes.shape != (T, n_in // 2) or scales.shape != (T, n_in // 32):
+        raise ValueError(f"activations {tuple(codes.shape)} / {tuple(scales.shape)}: {proj} takes rows "
+                         f"of {n_in} values")
+    if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_contiguous() or
+            not scales.is_contiguous()):
         raise ValueError("activations must be contiguous uint8 codes and scales")
     _index(pair_token, n, "pair_token")
     _index(pair_expert, n, "pair_expert")
@@ -268,25 +283,24 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
         if out is None:
             raise ValueError("pair_row names rows of an `out` that is not given")
     if out is None:
-        out = torch.empty((n, n_out), dtype=torch.bfloat16, device=q.codes.device)
+        out = torch.empty((n, n_out), dtype=torch.bfloat16, device=codes.device)
     elif out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[1] != n_out or not out.is_contiguous():
         raise ValueError(f"out must be contiguous bfloat16 [n_rows, {n_out}]")
-    ws = _workspace(spec, q.codes.shape[0], n, False, True, q.codes.device)
-    j = list(F.MLP_PROJECTIONS if not spec.gated else F.PROJECTIONS).index(proj)
+    ws = _workspace(spec, T, n, False, True, codes.device) if n > FEW_PAIRS else None
     L.check(L.load().brx_mx_expert_product(
-        C.byref(spec.c_desc), pool.device.handle, q.codes.data_ptr(), q.scales.data_ptr(),
-        q.codes.shape[0], pair_token.data_ptr(), pair_expert.data_ptr(),
-        None if pair_row is None else pair_row.data_ptr(), n, out.shape[0],
-        j if spec.gated else 2 * j, out.data_ptr(), ws.data_ptr(), ws.numel(), _stream(stream)))
-    _keep(stream, ws, out)
+        C.byref(spec.c_desc), pool.device.handle, codes.data_ptr(), scales.data_ptr(), T, pair_token.data_ptr(),
+        pair_expert.data_ptr(), None if pair_row is None else pair_row.data_ptr(), n, out.shape[0], j,
+        out.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream(stream)))
+    if stream is not None:
+        _keep(stream, ws, out)
     return out
 
 
 def _rows_of(spec: LayerSpec, x):
     import torch
-    if x.dtype != torch.bfloat16 or x.shape[-1] != spec.hidden:
+    if x.dtype != torch.bfloat16 or not x.shape or x.shape[-1] != spec.hidden:
         raise ValueError(f"x must be bfloat16 [..., {spec.hidden}], got {x.dtype} {tuple(x.shape)}")
-    return x.reshape(-1, spec.hidden).contiguous()
+    return x if x.dim() == 2 and x.is_contiguous() else x.reshape(-1, spec.hidden).contiguous()
 
 
 def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, sgate=None, out=None,
@@ -294,7 +308,8 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
     """The routed experts of tokens x [T, H] (bf16) under a routing idx [T, k] (int32) with both
     projections' activations in MXFP4. With weights w [T, k] (fp32): out [T, H] = sum_j w[t, j] *
     y[t, j] (+ sgate[t] * shared(x_t)); without: the unreduced rows [T, k, H]. The pool's table must
-    be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`."""
+    be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`. Up to 8 tokens and 64 pairs run
+    as two launches, more as the grouped GEMM; the outputs are the same bits."""
     import torch
     _check_spec(spec)
     x2 = _rows_of(spec, x)
@@ -305,31 +320,33 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
         raise ValueError(f"w must be contiguous float32 [{T}, {k}]")
     if sgate is not None and (sgate.dtype != torch.float32 or sgate.numel() != T or not sgate.is_contiguous()):
         raise ValueError(f"sgate must be contiguous float32 [{T}]")
-    _check_shared(spec, shared)
+    if shared is not None:
+        _check_shared(spec, shared)
+    for t, n in ((out, T * H), (y_unreduced, T * k * H)):
+        if t is not None and (t.dtype != torch.bfloat16 or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"out and y_unreduced must be contiguous bfloat16 [{T}, {H}] and [{T}, {k}, {H}]")
     if w is not None and out is None:
         out = torch.empty((T, H), dtype=torch.bfloat16, device=x2.device)
     if w is None and y_unreduced is None:
         y_unreduced = torch.empty((T, k, H), dtype=torch.bfloat16, device=x2.device)
-    for t, n in ((out, T * H), (y_unreduced, T * k * H)):
-        if t is not None and (t.dtype != torch.bfloat16 or t.numel() != n or not t.is_contiguous()):
-            raise ValueError(f"out and y_unreduced must be contiguous bfloat16 [{T}, {H}] and [{T}, {k}, {H}]")
     ws = _workspace(spec, T, T * k, shared is not None, False, x2.device)
     ptr = L.ptr
     L.check(L.load().brx_mx_moe_forward(
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), idx.data_ptr(), ptr(w), ptr(shared),
-        ptr(sgate), T, ptr(out), ptr(y_unreduced), path_flag(T, k) if flags is None else flags,
-        ws.data_ptr(), ws.numel(), _stream(stream)))
-    _keep(stream, ws, out, y_unreduced, x2)
+        ptr(sgate), T, ptr(out), ptr(y_unreduced), 0 if flags is None else flags, ws.data_ptr(), ws.numel(),
+        _stream(stream)))
+    if stream is not None:
+        _keep(stream, ws, out, y_unreduced, x2)
     return out if w is not None else y_unreduced
 
 
 def _check_shared(spec: LayerSpec, shared) -> None:
     import torch
-    if shared is None:
-        return
     if not spec.shared_inter:
         raise ValueError("the layer has no shared expert")
-    per = F.spec_bytes(spec.expert_spec(True))
+    per = spec.__dict__.get("_mx_shared_bytes")
+    if per is None:
+        per = spec.__dict__["_mx_shared_bytes"] = F.spec_bytes(spec.expert_spec(True))
     if shared.dtype != torch.uint8 or shared.numel() != per or not shared.is_contiguous():
         raise ValueError(f"the shared expert is {per} contiguous bytes")
 
@@ -346,7 +363,8 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
     _index(pair_exp, n, "pair_exp")
     if pair_row is not None:
         _index(pair_row, n, "pair_row")
-    _check_shared(spec, shared)
+    if shared is not None:
+        _check_shared(spec, shared)
     if (y_rows.dtype != torch.bfloat16 or y_rows.dim() != 2 or y_rows.shape[1] != spec.hidden or
             not y_rows.is_contiguous()):
         raise ValueError(f"y_rows must be contiguous bfloat16 [n_rows, {spec.hidden}]")
@@ -356,4 +374,5 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), x2.shape[0], ptr(pair_tok), ptr(pair_exp),
         ptr(pair_row), n, y_rows.shape[0], ptr(shared), y_rows.data_ptr(), flags, ws.data_ptr(), ws.numel(),
         _stream(stream)))
-    _keep(stream, ws, x2)
+    if stream is not None:
+        _keep(stream, ws, x2)

@@ -127,6 +127,7 @@ def test_every_border_of_a_code(gpu):
 
 
 def test_zeros_subnormals_and_the_largest(gpu):
+    import torch
     v = np.zeros((8, 32), dtype=np.float32)
     v[1] = -0.0
     v[2, 5] = np.float32(2.0 ** -149)
@@ -137,6 +138,8 @@ def test_zeros_subnormals_and_the_largest(gpu):
     v[7] = np.nextafter(np.float32(4.0), np.float32(0))      # just below a power of two
     q = mx.quantize(_tensor(v, "f32", gpu))
     _check_rows(q, v.astype(np.float64))
+    for dt in (torch.float32, torch.bfloat16):               # (their subnormals among them)
+        assert np.array_equal(mx.dequantize(q, dt).double().cpu().numpy(), O.held(v.astype(np.float64)))
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
