@@ -783,8 +783,8 @@ int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int 
     FwdArgs a = make_args(d, &none, nullptr, T, (int)n_pairs, nullptr, nullptr, nullptr, 0, nullptr,
                           shared ? &some : nullptr, nullptr, nullptr, nullptr);
     // (of whichever kernels a call may take)
-    const size_t all = mx_workspace_bytes(a, !product, false), few = mx_workspace_bytes(a, !product, true);
-    *out = T <= 8 && n_pairs <= 64 && few > all ? few : all;
+    const size_t all = mx_workspace_bytes(a, !product, kMxMany), own = mx_workspace_bytes(a, !product, mx_path(a));
+    *out = own > all ? own : all;
     return BRX_OK;
 }
 
@@ -843,7 +843,7 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
     FwdArgs a = make_args(d, p, nullptr, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, nullptr, nullptr,
                           nullptr, y_rows);
     hipStream_t s = (hipStream_t)stream;
-    if ((rc = mx_begin(p, mx_workspace_bytes(a, false, false), workspace, workspace_bytes, s))) return rc;
+    if ((rc = mx_begin(p, mx_workspace_bytes(a, false, kMxMany), workspace, workspace_bytes, s))) return rc;
     return mx_end(p, launch_mx_product(a, (const uint8_t*)codes, (const uint8_t*)scales, proj, workspace, s), s);
 }
 
@@ -861,12 +861,12 @@ static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T
         return fail(BRX_EINVAL, "FORCE_DECODE and FORCE_PREFILL are exclusive");
     FwdArgs a = make_args(d, p, x, T, P, pexp, ptok, prow, yrows, w, shared_expert, shared_gate, out, y_rows);
     hipStream_t s = (hipStream_t)stream;
-    const bool few = (flags & BRX_FWD_FORCE_DECODE) || (!(flags & BRX_FWD_FORCE_PREFILL) && T <= 8 && P <= 64);
-    if (few && (T > 8 || P > 64))
+    const MxPath path = flags & BRX_FWD_FORCE_PREFILL ? kMxMany : mx_path(a);
+    if ((flags & BRX_FWD_FORCE_DECODE) && path != kMxFew)
         return fail(BRX_EINVAL, "the decode path takes at most 8 token rows and 64 pairs (T=%d, P=%d)", T, P);
-    const int rc = mx_begin(p, mx_workspace_bytes(a, true, few), workspace, workspace_bytes, s);
+    const int rc = mx_begin(p, mx_workspace_bytes(a, true, path), workspace, workspace_bytes, s);
     if (rc) return rc;
-    return mx_end(p, launch_mx_layer(a, few, workspace, s), s);
+    return mx_end(p, launch_mx_layer(a, path, workspace, s), s);
 }
 
 int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, const int32_t* idx, const float* w,

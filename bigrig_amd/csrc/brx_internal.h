@@ -677,14 +677,16 @@ struct MxRows {
 hipError_t launch_mx_quantize(const MxRows& m, int dtype, hipStream_t s);
 hipError_t launch_mx_dequantize(const MxRows& m, int dtype, hipStream_t s);
 // the expert layer with MXFP4 activations, and one projection's rows of quantized activations; `ws`
-// holds mx_workspace_bytes (layer: a whole layer, else an expert product). few: the kernels of a decode
-// step (at most 8 tokens and 64 pairs), the same bits.
-size_t mx_workspace_bytes(const FwdArgs& a, bool layer, bool few);
-hipError_t launch_mx_layer(const FwdArgs& a, bool few, void* ws, hipStream_t s);
+// holds mx_workspace_bytes (layer: a whole layer, else an expert product). Which kernels run a layer: those
+// of few pairs (a decode step), the same behind a bucketing, or the grouped GEMM; the bits are the same.
+enum MxPath { kMxFew, kMxMid, kMxMany };
+MxPath mx_path(const FwdArgs& a);
+size_t mx_workspace_bytes(const FwdArgs& a, bool layer, MxPath path);
+hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, void* ws, hipStream_t s);
 hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, void* ws,
                              hipStream_t s);
-size_t mx_few_workspace_bytes(const FwdArgs& a);
-hipError_t launch_mx_few_layer(const FwdArgs& a, void* ws, hipStream_t s);
+size_t mx_few_workspace_bytes(const FwdArgs& a, bool tiles);
+hipError_t launch_mx_few_layer(const FwdArgs& a, bool tiles, void* ws, hipStream_t s);
 hipError_t launch_mx_few_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, hipStream_t s);
 hipError_t launch_combine(const uint16_t* y_routed, const uint16_t* y_shared, const float* w,
                           const float* sg, int T, int k, int H, uint16_t* out, hipStream_t s);

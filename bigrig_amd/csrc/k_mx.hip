@@ -375,13 +375,18 @@ hipError_t bucket(const FwdArgs& a, const MxWs& w, hipStream_t s) {
 
 }  // namespace
 
-size_t mx_workspace_bytes(const FwdArgs& a, bool layer, bool few) {
-    if (!layer && a.P <= kMxFewPairs) return 0;
-    return few ? mx_few_workspace_bytes(a) : carve(a, layer, nullptr).bytes;
+MxPath mx_path(const FwdArgs& a) {
+    if (a.T <= kMxFewTokens && a.P <= kMxFewPairs) return kMxFew;
+    return a.T <= kMxMidTokens && a.P <= kMxMidPairs ? kMxMid : kMxMany;
 }
 
-hipError_t launch_mx_layer(const FwdArgs& a, bool few, void* ws, hipStream_t s) {
-    if (few) return launch_mx_few_layer(a, ws, s);
+size_t mx_workspace_bytes(const FwdArgs& a, bool layer, MxPath path) {
+    if (!layer && a.P <= kMxFewPairs) return 0;
+    return layer && path != kMxMany ? mx_few_workspace_bytes(a, path == kMxMid) : carve(a, layer, nullptr).bytes;
+}
+
+hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, void* ws, hipStream_t s) {
+    if (path != kMxMany) return launch_mx_few_layer(a, path == kMxMid, ws, s);
     const MxWs w = carve(a, true, ws);
     MxRows x{};
     x.x = const_cast<uint16_t*>(a.x);

@@ -20,9 +20,10 @@
 
 namespace brx {
 
-// Most tokens and (token, expert) pairs of the few-pair kernels (a step is planned by one wave).
-constexpr int kMxFewTokens = 8;
-constexpr int kMxFewPairs = 64;
+// Most tokens and (token, expert) pairs of a step that every block of the few-pair kernels plans itself (one
+// wave, a pair a lane), and of one that is bucketed for them first.
+constexpr int kMxFewTokens = 8, kMxFewPairs = 64;
+constexpr int kMxMidTokens = 64, kMxMidPairs = 256;
 
 // What the GEMM launches take beside the forward's arguments (FwdArgs::x is unused).
 struct MxArgs {
