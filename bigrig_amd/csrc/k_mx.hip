@@ -12,6 +12,7 @@
 // products, fp32 sums in steps of 128 K in order. A row's bits do not depend on its tile.
 #include <type_traits>
 
+#include "bucket.h"
 #include "mx_common.h"
 #include "pf_common.h"
 
@@ -373,11 +374,69 @@ hipError_t bucket(const FwdArgs& a, const MxWs& w, hipStream_t s) {
                          a.host != nullptr, a.err, w.order, w.offsets, w.tile_start, w.tinfo, s);
 }
 
+// The first launch of a layer: blocks [0, E_ext) bucket the pairs, the others round x [n8 runs of 8 values] to
+// MXFP4, a group per four neighbouring lanes. (Two launches: 3 us more a 64-token layer.)
+template <int PER>
+__global__ __launch_bounds__(kBucketThreads) void k_mx_prepare(const int32_t* __restrict__ pexp, int P, int E, int E_ext,
+                                                               int T_sh, int lbm, const int32_t* __restrict__ g2s,
+                                                               int capacity, int host, int32_t* __restrict__ err,
+                                                               int32_t* __restrict__ order,
+                                                               int32_t* __restrict__ offsets,
+                                                               int32_t* __restrict__ tile_start,
+                                                               int4* __restrict__ tinfo, int lcap,
+                                                               const uint16_t* __restrict__ x, int64_t n8,
+                                                               uint8_t* __restrict__ xq, uint8_t* __restrict__ xs) {
+    if ((int)blockIdx.x < E_ext) {
+        bucket_block<PER>(blockIdx.x, pexp, P, E, E_ext, T_sh, lbm, g2s, capacity, host, err, order, offsets, tile_start,
+                          tinfo, lcap);
+        return;
+    }
+    const int64_t i = (int64_t)(blockIdx.x - E_ext) * kBucketThreads + threadIdx.x;
+    if (i >= n8) return;                           // (whole groups)
+    const u32x4_t q = *reinterpret_cast<const u32x4_t*>(x + 8 * i);
+    float v[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        v[k] = bf2f((k & 1) ? q[k >> 1] >> 16 : q[k >> 1] & 0xFFFFu);
+        top = max(top, mx_mag(v[k]));
+    }
+    top = max(top, dpp_u<0xB1>(top));
+    top = max(top, dpp_u<0x4E>(top));
+    const uint32_t sb = mx_scale(top);
+    reinterpret_cast<uint32_t*>(xq)[i] = mx_codes(v, sb);
+    if ((i & 3) == 0) xs[i >> 2] = (uint8_t)sb;
+}
+
+hipError_t prepare(const FwdArgs& a, const MxWs& w, hipStream_t s) {
+    const int E_ext = a.E + (a.shared ? 1 : 0), T_sh = a.auto_shared ? a.T : 0;
+    const int lcap = bucket_list(a.P + T_sh);
+    const int64_t n8 = (int64_t)a.T * (a.H / 8);
+    const dim3 grid((unsigned)(E_ext + (n8 + kBucketThreads - 1) / kBucketThreads));
+#define BRX_PREPARE(PER) hipLaunchKernelGGL(k_mx_prepare<PER>, grid, dim3(kBucketThreads), sizeof(int32_t) * (E_ext + lcap), s, \
+                                            a.pexp, a.P, a.E, E_ext, T_sh, __builtin_ctz(w.tile), a.g2s, a.capacity, \
+                                            a.host != nullptr ? 1 : 0, a.err, w.order, w.offsets, w.tile_start, w.tinfo, lcap, \
+                                            a.x, n8, w.xq, w.xs)
+    switch (bucket_per(a.P + T_sh)) {
+        case 2: BRX_PREPARE(2); break;
+        case 4: BRX_PREPARE(4); break;
+        default: BRX_PREPARE(16);
+    }
+#undef BRX_PREPARE
+    return hipGetLastError();
+}
+
 }  // namespace
 
+// The few-pair kernels have a block for every run of an expert's rows: they win while launches and round trips
+// set the time. The line past 8 tokens is the pairs times an expert's bytes (what the pairs could read), these
+// kernels against the grouped GEMM: 2048 x 768, top-8, 9 tokens (179 MB) 32.9 / 36.2 us, 12 (239 MB) 34.6 / 36.7,
+// 16 (318 MB) 39.2 / 37.6; 2048 x 512, 256 experts and a shared one, 16 tokens (214 MB) 34.9 / 37.8, 32 (428 MB)
+// 45.2 / 44.1; 2048 x 1024, top-8, 9 tokens (240 MB) 37.5 / 38.0, 16 (427 MB) 43.4 / 39.7; a 2048 x 128 MLP, 64
+// tokens (36 MB) 16.7 / 18.3.
 MxPath mx_path(const FwdArgs& a) {
     if (a.T <= kMxFewTokens && a.P <= kMxFewPairs) return kMxFew;
-    return a.T <= kMxMidTokens && a.P <= kMxMidPairs ? kMxMid : kMxMany;
+    return a.T <= kMxMidTokens && a.P <= kMxMidPairs && a.P * a.lay.bytes <= 260 * 1000 * 1000 ? kMxMid : kMxMany;
 }
 
 size_t mx_workspace_bytes(const FwdArgs& a, bool layer, MxPath path) {
@@ -388,17 +447,8 @@ size_t mx_workspace_bytes(const FwdArgs& a, bool layer, MxPath path) {
 hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, void* ws, hipStream_t s) {
     if (path != kMxMany) return launch_mx_few_layer(a, path == kMxMid, ws, s);
     const MxWs w = carve(a, true, ws);
-    MxRows x{};
-    x.x = const_cast<uint16_t*>(a.x);
-    x.codes = w.xq;
-    x.scales = w.xs;
-    x.rows = a.T;
-    x.cols = a.H;
-    x.x_row = a.H;
-    x.groups = (int64_t)a.T * (a.H / 32);
-    hipError_t e = launch_mx_quantize(x, BRX_DT_BF16, s);
+    hipError_t e = prepare(a, w, s);
     if (e != hipSuccess) return e;
-    if ((e = bucket(a, w, s)) != hipSuccess) return e;
     MxArgs m = gemm_args(a, w);
     m.xq = w.xq;
     m.xs = w.xs;

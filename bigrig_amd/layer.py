@@ -184,9 +184,9 @@ class StreamingSwitchGLU:
     def _forward(self, x2, idx, w=None, shared=None, sgate=None, out=None, y_unreduced=None,
                  flags=None, stream=None):
         if self.activations == "mxfp4":
-            from . import mx
-            mx.moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced, flags,
-                           stream)
+            from . import mx      # (its kernels agree bit for bit: no flag holds a chunk to one of them)
+            mx.moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced,
+                           stream=stream)
         else:
             moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced, flags,
                         stream)
@@ -194,8 +194,8 @@ class StreamingSwitchGLU:
     def _forward_pairs(self, x2, pair_tok, pair_exp, pair_row, y_rows, flags, shared=None, stream=None):
         if self.activations == "mxfp4":
             from . import mx
-            mx.forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, flags,
-                             shared, stream)
+            mx.forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, 0, shared,
+                             stream)
         else:
             forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, flags, shared,
                           stream)

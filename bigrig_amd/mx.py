@@ -309,7 +309,8 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
     projections' activations in MXFP4. With weights w [T, k] (fp32): out [T, H] = sum_j w[t, j] *
     y[t, j] (+ sgate[t] * shared(x_t)); without: the unreduced rows [T, k, H]. The pool's table must
     be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`. Up to 8 tokens and 64 pairs run
-    as two launches, more as the grouped GEMM; the outputs are the same bits."""
+    as two launches, some more as three and the rest as the grouped GEMM; the outputs are the same bits
+(`flags`: BRX_FWD_FORCE_DECODE or BRX_FWD_FORCE_PREFILL for the first or the last of these)."""
     import torch
     _check_spec(spec)
     x2 = _rows_of(spec, x)
@@ -353,7 +354,7 @@ def _check_shared(spec: LayerSpec, shared) -> None:
 
 def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair_row, y_rows, flags: int,
                   shared=None, stream=None) -> None:
-    """`layer.forward_pairs` with MXFP4 activations."""
+    """`layer.forward_pairs` with MXFP4 activations (any `flags` give the same bits)."""
     import torch
     _check_spec(spec)
     x2 = _rows_of(spec, x)

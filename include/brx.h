@@ -336,7 +336,7 @@ int brx_mx_dequantize(const void* codes, int64_t codes_batch_stride, const void*
 
 /* Bytes of scratch the calls below need for T token rows and n_pairs routed pairs (a layer: T * top_k):
  * `product` nonzero for brx_mx_expert_product, zero for the layer calls (shared != 0: given a shared
- * expert). What a call needs never exceeds this. */
+ * expert). What a call needs never exceeds this; a product of at most 64 pairs needs none. */
 int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int shared, int product,
                            size_t* out);
 
@@ -355,12 +355,15 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
 /* brx_moe_forward with MXFP4 activations, for layers of MXFP4 experts: x is rounded to MXFP4, the
  * activation is applied to the fp32 sums and its result h rounded to MXFP4 (once, from fp32), so
  *   y[t, j] = down(Q(act(gate(Q(x_t)), up(Q(x_t)))))
- * and out / y_unreduced as there. T at most 65535; x, out and y_unreduced 16-byte, workspace 256-byte aligned. */
+ * and out / y_unreduced as there. T at most 65535; x, out and y_unreduced 16-byte, workspace 256-byte aligned.
+ * Every output is the same bits whichever kernels run, so no flag is needed: FORCE_DECODE asks for the
+ * two-launch kernels (at most 8 token rows and 64 pairs, BRX_EINVAL above), FORCE_PREFILL for the grouped
+ * GEMM, any other flag is BRX_EINVAL. */
 int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, const int32_t* idx,
                        const float* w, const void* shared_expert, const float* shared_gate, int T,
                        void* out, void* y_unreduced, unsigned flags, void* workspace,
                        size_t workspace_bytes, void* stream);
-/* brx_moe_forward_pairs with MXFP4 activations. */
+/* brx_moe_forward_pairs with MXFP4 activations (flags as in brx_mx_moe_forward). */
 int brx_mx_moe_forward_pairs(const brx_layer_desc* d, brx_pool* p, const void* x, int T,
                              const int32_t* pair_token, const int32_t* pair_expert,
                              const int32_t* pair_row, int n_pairs, int n_rows,
