@@ -36,14 +36,14 @@ __device__ __forceinline__ void bucket_experts(const int32_t* __restrict__ pexp,
 
 // Block e of the bucketing (kBucketThreads threads, (E_ext + lcap) words of dynamic LDS).
 template <int PER>
-__device__ __forceinline__ void bucket_block(int e, const int32_t* __restrict__ pexp, int P, int E, int E_ext, int T_sh, int lbm,
-                                             const int32_t* __restrict__ g2s, int capacity, int host,
+__device__ __forceinline__ void bucket_block(int e, const int32_t* __restrict__ pexp, int P, int E, int E_ext, int T_sh,
+                                             int lbm, int slack, const int32_t* __restrict__ g2s, int capacity, int host,
                                              int32_t* __restrict__ err, int32_t* __restrict__ order,
                                              int32_t* __restrict__ offsets, int32_t* __restrict__ tile_start,
                                              int4* __restrict__ tinfo, int lcap) {
     // E_ext = E + 1 when a shared expert exists (id E); T_sh shared pairs follow the P routed; the M
-    // tile height is 1 << lbm. LDS: the histogram [E_ext], then a list of up to lcap of this
-    // expert's pairs.
+    // tile height is 1 << lbm, and an expert's last full tile takes up to `slack` rows more. LDS: the
+    // histogram [E_ext], then a list of up to lcap of this expert's pairs.
     extern __shared__ int32_t hist[];
     int32_t* list = hist + E_ext;
     constexpr int kNw = kBucketThreads / kWave;
@@ -93,6 +93,11 @@ __device__ __forceinline__ void bucket_block(int e, const int32_t* __restrict__ 
         __syncthreads();
         return total;
     };
+    // rows of the last tile of n pairs where it is not full; up to `slack` of them join the tile before
+    auto last_rows = [&](int n) __attribute__((always_inline)) {
+        const int r = n & (BM - 1);
+        return r <= slack && n >= BM ? 0 : r;
+    };
     int run = 0;
     for (int p0 = 0; p0 < P_ext; p0 += kPass)
         run += compact(p0, run, std::true_type{}, [&](int q, int p) { if (q < lcap) list[q] = p; });
@@ -104,7 +109,7 @@ __device__ __forceinline__ void bucket_block(int e, const int32_t* __restrict__ 
         // call has fewer than 2^16 small tiles, one an expert).
         int off = 0, below_e = 0, big_all = 0, small_all = 0, big = 0;
         for (int j = lane; j < E_ext; j += 64) {
-            const int n = hist[j], r = n & (BM - 1);
+            const int n = hist[j], r = last_rows(n);
             const int nb = (n >> lbm) + (r > BM / 2 ? 1 : 0), ns = (r > 0 && r <= BM / 2) ? 1 : 0;
             if (j < e) { off += n; big += nb; below_e += ns; }
             big_all += nb;
@@ -135,8 +140,9 @@ __device__ __forceinline__ void bucket_block(int e, const int32_t* __restrict__ 
             err[1] = e;
             err[0] = 1;
         }
-        for (int j = tid; j * BM < n; j += kBucketThreads) {
-            const int rows = min(BM, n - j * BM);
+        const int all = (n >> lbm) + (last_rows(n) > 0 ? 1 : 0);
+        for (int j = tid; j < all; j += kBucketThreads) {
+            const int rows = j == all - 1 ? n - j * BM : BM;
             tinfo[rows > BM / 2 ? big + j : small] = make_int4(e, off + j * BM, rows, slot);
         }
     }

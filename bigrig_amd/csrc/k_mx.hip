@@ -31,10 +31,10 @@ constexpr int kMxA = 16 * MP * 256;
 template <int MP>
 constexpr int kMxBuf = kMxA<MP> + 16 * MP * 32;
 __host__ __device__ constexpr int mx_table(int K) { return kMxWaves * kMxRows * (K / 32) + 16; }
-// Copies of a chunk's scales a wave issues, 8 rows each (of 16-row tiles the last two waves repeat the first
-// two's); its codes are MP copies of 1 KB (4 rows) a wave.
+// Copies of a chunk's scales a wave issues, 8 rows each (the last waves repeat the first ones' where rows run
+// out); its codes are MP copies of 1 KB (4 rows) a wave.
 template <int MP>
-constexpr int kMxNS = MP == 1 ? 1 : MP / 2;
+constexpr int kMxNS = (MP + 1) / 2;
 
 // 16 or 2 bytes a lane from byte `off` of the buffer into LDS, lane after lane from `to` on (2 bytes fill
 // a word).
@@ -166,7 +166,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     dma_wait_barrier<0>();
     const int nch = (G + 15) / 16;
     for (int ch = 0; ch < nch; ++ch) {
-        issue_a(ch + 1);                           // (every wave is done with the chunk that was there)
+        if (ch + 1 < nch) issue_a(ch + 1);         // (every wave is done with the chunk that was there)
         asm volatile("" ::: "memory");
         const uint8_t* const buf = smem + (ch & 1) * kMxBuf<MP>;
         uint32_t ws[4];
@@ -199,6 +199,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
         step(std::integral_constant<int, 1>{});
         step(std::integral_constant<int, 2>{});
         step(std::integral_constant<int, 3>{});
+        if (ch + 1 == nch) break;                  // (a request past the last chunk: 3% of a call)
         issue(ch + 1, q);
         __builtin_amdgcn_sched_barrier(0);
         // the next chunk of A has landed (the weights were issued after its copies), and every wave is done
@@ -271,7 +272,7 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
 
 // MPX: the call's tallest tiles, in 16 pairs (a launch of low tiles takes fewer registers).
 template <int KIND, int MPX>
-__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(MPX == 4 ? 2 : MPX == 2 ? 3 : 4)))
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(MPX == 5 ? 2 : MPX == 2 ? 3 : 4)))
 void k_mx_gemm(FwdArgs a, MxArgs m) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     prefetch_args(a);
@@ -290,7 +291,8 @@ void k_mx_gemm(FwdArgs a, MxArgs m) {
     if (nt * kMxWaves * (KIND == 0 && a.act != BRX_ACT_SILU_MLP ? kMxRows / 2 : kMxRows) >= N) return;
     if (MPX == 1 || rows <= 16) mx_tile<KIND, 1>(a, m, smem, e, m0, rows, ti.w, nt);
     else if (MPX == 2 || rows <= 32) mx_tile<KIND, 2>(a, m, smem, e, m0, rows, ti.w, nt);
-    else mx_tile<KIND, 4>(a, m, smem, e, m0, rows, ti.w, nt);
+    else if (rows <= 64) mx_tile<KIND, 4>(a, m, smem, e, m0, rows, ti.w, nt);
+    else mx_tile<KIND, 5>(a, m, smem, e, m0, rows, ti.w, nt);
 }
 
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -300,6 +302,9 @@ inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 int mx_tile_rows(int64_t pairs, int64_t experts) {
     return pairs <= 8 * experts ? 16 : pairs <= 24 * experts ? 32 : 64;
 }
+// Rows past a tile of 64 that join it (tiles of up to 80): the mean expert's pairs are near 64, 128, ..., and the
+// few that pass it would read the expert's weights once more.
+int mx_slack(int tile) { return tile == 64 ? 16 : 0; }
 // Consecutive M tiles whose runs of columns an XCD takes in turn: an expert's tall tiles then read its weights
 // from one L2 (a 2048-token layer 183 us one by one, 180 by two, 179 by four).
 int mx_group(int tile) { return tile == 64 ? 4 : 1; }
@@ -355,7 +360,7 @@ hipError_t launch_gemm(const FwdArgs& a, const MxArgs& m, const MxWs& w, int K, 
     switch (w.tile) {
         case 16: return launch_tiles<KIND, 1>(a, m, w, K, N, s);
         case 32: return launch_tiles<KIND, 2>(a, m, w, K, N, s);
-        default: return launch_tiles<KIND, 4>(a, m, w, K, N, s);
+        default: return launch_tiles<KIND, 5>(a, m, w, K, N, s);
     }
 }
 
@@ -371,14 +376,15 @@ MxArgs gemm_args(const FwdArgs& a, const MxWs& w) {
 
 hipError_t bucket(const FwdArgs& a, const MxWs& w, hipStream_t s) {
     return launch_bucket(a.pexp, a.P, a.E, a.E + (a.shared ? 1 : 0), a.auto_shared ? a.T : 0, w.tile, a.g2s, a.capacity,
-                         a.host != nullptr, a.err, w.order, w.offsets, w.tile_start, w.tinfo, s);
+                         a.host != nullptr, a.err, w.order, w.offsets, w.tile_start, w.tinfo, s, mx_slack(w.tile));
 }
 
 // The first launch of a layer: blocks [0, E_ext) bucket the pairs, the others round x [n8 runs of 8 values] to
 // MXFP4, a group per four neighbouring lanes. (Two launches: 3 us more a 64-token layer.)
 template <int PER>
 __global__ __launch_bounds__(kBucketThreads) void k_mx_prepare(const int32_t* __restrict__ pexp, int P, int E, int E_ext,
-                                                               int T_sh, int lbm, const int32_t* __restrict__ g2s,
+                                                               int T_sh, int lbm, int slack,
+                                                               const int32_t* __restrict__ g2s,
                                                                int capacity, int host, int32_t* __restrict__ err,
                                                                int32_t* __restrict__ order,
                                                                int32_t* __restrict__ offsets,
@@ -387,8 +393,8 @@ __global__ __launch_bounds__(kBucketThreads) void k_mx_prepare(const int32_t* __
                                                                const uint16_t* __restrict__ x, int64_t n8,
                                                                uint8_t* __restrict__ xq, uint8_t* __restrict__ xs) {
     if ((int)blockIdx.x < E_ext) {
-        bucket_block<PER>(blockIdx.x, pexp, P, E, E_ext, T_sh, lbm, g2s, capacity, host, err, order, offsets, tile_start,
-                          tinfo, lcap);
+        bucket_block<PER>(blockIdx.x, pexp, P, E, E_ext, T_sh, lbm, slack, g2s, capacity, host, err, order, offsets,
+                          tile_start, tinfo, lcap);
         return;
     }
     const int64_t i = (int64_t)(blockIdx.x - E_ext) * kBucketThreads + threadIdx.x;
@@ -414,7 +420,7 @@ hipError_t prepare(const FwdArgs& a, const MxWs& w, hipStream_t s) {
     const int64_t n8 = (int64_t)a.T * (a.H / 8);
     const dim3 grid((unsigned)(E_ext + (n8 + kBucketThreads - 1) / kBucketThreads));
 #define BRX_PREPARE(PER) hipLaunchKernelGGL(k_mx_prepare<PER>, grid, dim3(kBucketThreads), sizeof(int32_t) * (E_ext + lcap), s, \
-                                            a.pexp, a.P, a.E, E_ext, T_sh, __builtin_ctz(w.tile), a.g2s, a.capacity, \
+                                            a.pexp, a.P, a.E, E_ext, T_sh, __builtin_ctz(w.tile), mx_slack(w.tile), a.g2s, a.capacity, \
                                             a.host != nullptr ? 1 : 0, a.err, w.order, w.offsets, w.tile_start, w.tinfo, lcap, \
                                             a.x, n8, w.xq, w.xs)
     switch (bucket_per(a.P + T_sh)) {

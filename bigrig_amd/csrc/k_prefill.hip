@@ -46,15 +46,15 @@ constexpr int kThreads = 256;
 // ------------------------------------------------------------------ bucketing (bucket.h)
 template <int PER>
 __global__ __launch_bounds__(kBucketThreads) void k_bucket(const int32_t* __restrict__ pexp, int P, int E,
-                                                           int E_ext, int T_sh, int lbm,
+                                                           int E_ext, int T_sh, int lbm, int slack,
                                                            const int32_t* __restrict__ g2s, int capacity,
                                                            int host, int32_t* __restrict__ err,
                                                            int32_t* __restrict__ order,
                                                            int32_t* __restrict__ offsets,
                                                            int32_t* __restrict__ tile_start,
                                                            int4* __restrict__ tinfo, int lcap) {
-    bucket_block<PER>(blockIdx.x, pexp, P, E, E_ext, T_sh, lbm, g2s, capacity, host, err, order, offsets, tile_start,
-                      tinfo, lcap);
+    bucket_block<PER>(blockIdx.x, pexp, P, E, E_ext, T_sh, lbm, slack, g2s, capacity, host, err, order, offsets,
+                      tile_start, tinfo, lcap);
 }
 
 // ------------------------------------------------------------------ grouped GEMM
@@ -797,7 +797,7 @@ hipError_t launch_gemm(const FwdArgs& a, const PfWs& w, int E_ext, int Imax, uin
 
 hipError_t launch_bucket(const int32_t* pexp, int P, int E, int E_ext, int T_sh, int BM,
                          const int32_t* g2s, int capacity, int host, int32_t* err, int32_t* order,
-                         int32_t* offsets, int32_t* tile_start, int4* tinfo, hipStream_t s) {
+                         int32_t* offsets, int32_t* tile_start, int4* tinfo, hipStream_t s, int slack) {
     // each block lists its expert's pairs in LDS during the histogram pass, up to lcap of them;
     // an expert with more takes a second pass over the pairs
     const int P_ext = P + T_sh;
@@ -805,7 +805,7 @@ hipError_t launch_bucket(const int32_t* pexp, int P, int E, int E_ext, int T_sh,
     const size_t lds = sizeof(int32_t) * (E_ext + lcap);
     const int lbm = __builtin_ctz(BM);
 #define BRX_BUCKET(PER) hipLaunchKernelGGL(k_bucket<PER>, dim3(E_ext), dim3(kBucketThreads), lds, s, pexp, P, E, E_ext, \
-                                           T_sh, lbm, g2s, capacity, host, err, order, offsets, tile_start, tinfo, lcap)
+                                           T_sh, lbm, slack, g2s, capacity, host, err, order, offsets, tile_start, tinfo, lcap)
     switch (bucket_per(P_ext)) {
         case 2: BRX_BUCKET(2); break;
         case 4: BRX_BUCKET(4); break;              // (a list that holds every pair: no second pass)

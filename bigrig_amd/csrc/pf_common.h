@@ -20,10 +20,10 @@ struct ThinArgs {
     int E_ext, Imax, mt_pad, tile_rows;
 };
 // k_bucket over P routed pairs and T_sh shared ones: the stable order, each expert's run and the tile
-// descriptors of M tiles of BM rows (tinfo may be null)
+// descriptors of M tiles of BM rows (tinfo may be null; up to `slack` rows past a full tile join it)
 hipError_t launch_bucket(const int32_t* pexp, int P, int E, int E_ext, int T_sh, int BM, const int32_t* g2s,
                          int capacity, int host, int32_t* err, int32_t* order, int32_t* offsets, int32_t* tile_start,
-                         int4* tinfo, hipStream_t s);
+                         int4* tinfo, hipStream_t s, int slack = 0);
 hipError_t launch_thin(const FwdArgs& a, const ThinArgs& t, int phases, hipStream_t s);
 hipError_t launch_dense(const FwdArgs& a, const ThinArgs& t, int phases, hipStream_t s);   // bf16 weights
 

@@ -261,6 +261,34 @@ def test_expert_product_of_one_expert(gpu, P):
     close(f64(bits(got)), want, bound, f"one expert P={P}")
 
 
+COUNTS = [64, 80, 81, 65, 145, 144]      # a tile of 64; 16 and 17 pairs past one; 1 past; 16 and 17 past two
+
+
+def test_expert_product_of_tall_tiles(gpu):
+    """Pairs a little past whole tiles, which the last tile takes or does not."""
+    ex = np.random.default_rng(3).permutation(np.repeat(np.arange(6), COUNTS))
+    for proj in ("gate_proj", "down_proj"):
+        spec, pool, q, tok, ex, want, bound = _product(gpu, "swiglu", proj, 70, len(ex), seed=8, experts=ex)
+        got = mx.expert_product(spec, pool, q, dev(tok, gpu), dev(ex, gpu), proj)
+        close(f64(bits(got)), want, bound, f"tall tiles {proj}")
+
+
+def test_layer_of_tall_tiles(gpu):
+    """The pairs form over the same counts: the rows a call of one pair each gives, bit for bit."""
+    import torch
+    spec, lay, sw, pool = built("swiglu", gpu)
+    x = to_dev_bits(acts(8, spec.hidden, 31), gpu)
+    rng = np.random.default_rng(4)
+    ex = rng.permutation(np.repeat(np.arange(6), COUNTS)).astype(np.int32)
+    tok = rng.integers(0, 8, ex.size).astype(np.int32)
+    y = torch.zeros(ex.size, spec.hidden, dtype=torch.bfloat16, device=gpu)
+    mx.forward_pairs(spec, pool, x, dev(tok, gpu), dev(ex, gpu), None, y, 0)
+    each = torch.zeros(48, spec.hidden, dtype=torch.bfloat16, device=gpu)
+    t48, e48 = np.repeat(np.arange(8), 6).astype(np.int32), np.tile(np.arange(6), 8).astype(np.int32)
+    mx.forward_pairs(spec, pool, x, dev(t48, gpu), dev(e48, gpu), None, each, L.FWD_FORCE_DECODE)
+    assert np.array_equal(bits(y), bits(each)[tok * 6 + ex])
+
+
 def test_expert_product_rows(gpu):
     """pair_row scatters the rows; rows no pair names are left as they were."""
     import torch
