@@ -31,14 +31,13 @@ __device__ __forceinline__ void load_run(const void* p, float (&v)[kRun<DT>]) {
 }
 
 // A thread takes kUnit runs (its neighbours the others of a group), a wave 64 neighbouring runs at a time, all
-// loads before the first use. HBM sets the time of a large matrix: 131072
-// x 2048 fp32 read and held in MXFP4 QQ.
+// loads before the first use. HBM sets the time of a large matrix: 131072 x 2048 fp32 values take 195 us
+// to MXFP4 (6.2 TB/s) and 94 us from there to bf16 (7.3 TB/s).
 constexpr int kUnit = 2;
 constexpr int kBlocksMost = 1 << 22;
 
-// Run i of the matrices: matrix b, row r and run c of it. FLAT: one matrix whose rows follow one another, so
-// rows need no division.
-// `run` values each.
+// Run i of the matrices, `run` values each: matrix b, row r and run c of it. FLAT: one matrix whose rows
+// follow one another, so rows need no division.
 template <bool FLAT>
 __device__ __forceinline__ void find_run(const MxRows& m, int run, int64_t i, int64_t& b, int64_t& r, int64_t& c) {
     if constexpr (FLAT) {

@@ -41,6 +41,7 @@ struct MxArgs {
     int32_t group;              // M tiles an XCD takes together
     int32_t proj;               // the projection of an expert product
 };
+static_assert(sizeof(FwdArgs) + sizeof(MxArgs) <= 512, "kernel argument blocks must stay under 512 bytes");
 
 namespace {
 

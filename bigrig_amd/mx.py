@@ -18,7 +18,9 @@ bytes, as an expert's `weight` and `scales` components hold it. A group that hol
 infinity is held as NaN.
 
 Tensors live on the current device. Scratch is allocated per call by torch, on the call's stream, so
-calls on several streams do not share any, and a captured graph keeps its own.
+calls on several streams do not share any, and a captured graph keeps its own. Given a `stream`, the
+whole call runs there, its allocations and copies too; the inputs have to be ready on it, and its
+results may be read on the stream that was current once that waits for it.
 """
 from __future__ import annotations
 
@@ -109,11 +111,16 @@ def _packed(t, what: str):
     return b, r, bs
 
 
-def _keep(stream, *tensors) -> None:
-    """Memory allocated for a call that runs on `stream` is not handed out again before it ends."""
-    for t in tensors:
-        if t is not None:
-            t.record_stream(stream)
+def _on(stream, call, *args):
+    """call(*args) with `stream` current (memory that the current stream's last work may still use is
+    not handed to it, nor its results' memory reused under readers on the current stream)."""
+    import torch
+    here = torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        got = call(*args)
+    for t in (got.codes, got.scales) if isinstance(got, MXRows) else () if got is None else (got,):
+        t.record_stream(here)
+    return got
 
 
 def quantize(x, stream=None) -> MXRows:
@@ -122,6 +129,8 @@ def quantize(x, stream=None) -> MXRows:
     saturating at 6 -- the codes of `formats.quantize_mxfp4`. A group with a NaN or an infinity is
     held as NaN (scale byte 255)."""
     import torch
+    if stream is not None:
+        return _on(stream, quantize, x)
     _on_device(x)
     dt = _dtype(x.dtype)
     shape = x.shape
@@ -134,9 +143,7 @@ def quantize(x, stream=None) -> MXRows:
     scales = x.new_empty(lead + (K // 32,), dtype=torch.uint8)
     if b:
         L.check(L.load().brx_mx_quantize(x.data_ptr(), dt, b, r, K, bs, rs, codes.data_ptr(), r * (K // 2),
-                                         scales.data_ptr(), r * (K // 32), _stream(stream)))
-        if stream is not None:
-            _keep(stream, codes, scales)
+                                         scales.data_ptr(), r * (K // 32), _stream()))
     return MXRows(codes, scales)
 
 
@@ -144,6 +151,8 @@ def dequantize(q: MXRows, dtype=None, stream=None):
     """The values of q as a contiguous [..., K] tensor of `dtype` (default bfloat16; exact in
     float32 and bfloat16, rounded to nearest even in float16)."""
     import torch
+    if stream is not None:
+        return _on(stream, dequantize, q, dtype)
     dtype = torch.bfloat16 if dtype is None else dtype
     dt = _dtype(dtype)
     codes, scales = q.codes, q.scales
@@ -168,9 +177,7 @@ def dequantize(q: MXRows, dtype=None, stream=None):
             else:
                 sbs = r * (K // 32)
     L.check(L.load().brx_mx_dequantize(codes.data_ptr(), cbs, scales.data_ptr(), sbs, b, r, K, dt,
-                                       out.data_ptr(), _stream(stream)))
-    if stream is not None:
-        _keep(stream, out)
+                                       out.data_ptr(), _stream()))
     return out
 
 
@@ -180,6 +187,8 @@ def pack_experts(spec: LayerSpec, weights: dict, biases: dict | None = None, sha
     are weights[projection] [E, n_out, n_in] (and biases[projection] [E, n_out]), in the layout
     `ExpertPool.admit_device` and `HostStore` take. `shared`: the shared expert's width."""
     import torch
+    if stream is not None:
+        return _on(stream, pack_experts, spec, weights, biases, shared)
     if spec.quant.mode != "mxfp4":
         raise ValueError(f"the layer's experts are {spec.quant.mode}, not mxfp4")
     es = spec.expert_spec(shared)
@@ -198,24 +207,23 @@ def pack_experts(spec: LayerSpec, weights: dict, biases: dict | None = None, sha
         _dtype(weights[p].dtype)
     _on_device(*weights.values(), *(biases or {}).values())
     offs, per = F.spec_offsets(es), F.spec_bytes(es)
-    with torch.cuda.stream(stream):      # (None: the current stream)
-        out = torch.empty((E, per), dtype=torch.uint8, device=next(iter(weights.values())).device)
-        for p in es:
-            w = weights[p]
-            if w.dim() == 3 and w.is_contiguous():
-                # seen as one run of rows, but every expert's codes have a place of their own
-                args = (E, w.shape[1], w.shape[2], w.stride(0), w.stride(1))
-            else:
-                b, r, bs, rs = _matrices(w, p)
-                args = (b, r, w.shape[2], bs, rs)
-            if out.numel():
-                L.check(L.load().brx_mx_quantize(w.data_ptr(), _dtype(w.dtype), *args,
-                                                 out.data_ptr() + offs[(p, "weight")], per,
-                                                 out.data_ptr() + offs[(p, "scales")], per, _stream(stream)))
-            if biases:
-                o = offs[(p, "bias")]
-                b16 = biases[p].to(torch.bfloat16).contiguous().view(torch.uint8)
-                out[:, o:o + b16.shape[1]] = b16
+    out = torch.empty((E, per), dtype=torch.uint8, device=next(iter(weights.values())).device)
+    for p in es:
+        w = weights[p]
+        if w.dim() == 3 and w.is_contiguous():
+            # seen as one run of rows, but every expert's codes have a place of their own
+            args = (E, w.shape[1], w.shape[2], w.stride(0), w.stride(1))
+        else:
+            b, r, bs, rs = _matrices(w, p)
+            args = (b, r, w.shape[2], bs, rs)
+        if out.numel():
+            L.check(L.load().brx_mx_quantize(w.data_ptr(), _dtype(w.dtype), *args,
+                                             out.data_ptr() + offs[(p, "weight")], per,
+                                             out.data_ptr() + offs[(p, "scales")], per, _stream()))
+        if biases:
+            o = offs[(p, "bias")]
+            b16 = biases[p].to(torch.bfloat16).contiguous().view(torch.uint8)
+            out[:, o:o + b16.shape[1]] = b16
     return out
 
 
@@ -261,6 +269,8 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
     the others are left as they are. Up to 64 pairs run as one launch, more as two and with scratch;
     the rows are the same bits."""
     import torch
+    if stream is not None:
+        return _on(stream, expert_product, spec, pool, q, pair_token, pair_expert, proj, pair_row, out)
     _check_spec(spec)
     j = (_PROJ if spec.gated else _MLP_PROJ).get(proj)
     if j is None:
@@ -290,9 +300,7 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
     L.check(L.load().brx_mx_expert_product(
         C.byref(spec.c_desc), pool.device.handle, codes.data_ptr(), scales.data_ptr(), T, pair_token.data_ptr(),
         pair_expert.data_ptr(), None if pair_row is None else pair_row.data_ptr(), n, out.shape[0], j,
-        out.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream(stream)))
-    if stream is not None:
-        _keep(stream, ws, out)
+        out.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream()))
     return out
 
 
@@ -310,8 +318,10 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
     y[t, j] (+ sgate[t] * shared(x_t)); without: the unreduced rows [T, k, H]. The pool's table must
     be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`. Up to 8 tokens and 64 pairs run
     as two launches, some more as three and the rest as the grouped GEMM; the outputs are the same bits
-(`flags`: BRX_FWD_FORCE_DECODE or BRX_FWD_FORCE_PREFILL for the first or the last of these)."""
+    (`flags`: BRX_FWD_FORCE_DECODE or BRX_FWD_FORCE_PREFILL for the first or the last of these)."""
     import torch
+    if stream is not None:
+        return _on(stream, moe_forward, spec, pool, x, idx, w, shared, sgate, out, y_unreduced, flags)
     _check_spec(spec)
     x2 = _rows_of(spec, x)
     T, H, k = x2.shape[0], spec.hidden, spec.top_k
@@ -335,9 +345,7 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
     L.check(L.load().brx_mx_moe_forward(
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), idx.data_ptr(), ptr(w), ptr(shared),
         ptr(sgate), T, ptr(out), ptr(y_unreduced), 0 if flags is None else flags, ws.data_ptr(), ws.numel(),
-        _stream(stream)))
-    if stream is not None:
-        _keep(stream, ws, out, y_unreduced, x2)
+        _stream()))
     return out if w is not None else y_unreduced
 
 
@@ -356,6 +364,8 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
                   shared=None, stream=None) -> None:
     """`layer.forward_pairs` with MXFP4 activations (any `flags` give the same bits)."""
     import torch
+    if stream is not None:
+        return _on(stream, forward_pairs, spec, pool, x, pair_tok, pair_exp, pair_row, y_rows, flags, shared)
     _check_spec(spec)
     x2 = _rows_of(spec, x)
     n = pair_exp.numel()
@@ -374,6 +384,4 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
     L.check(L.load().brx_mx_moe_forward_pairs(
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), x2.shape[0], ptr(pair_tok), ptr(pair_exp),
         ptr(pair_row), n, y_rows.shape[0], ptr(shared), y_rows.data_ptr(), flags, ws.data_ptr(), ws.numel(),
-        _stream(stream)))
-    if stream is not None:
-        _keep(stream, ws, x2)
+        _stream()))

@@ -610,6 +610,69 @@ def test_two_streams(gpu, T):
             assert np.array_equal(bits(g), want[s])
 
 
+def test_a_given_stream_has_the_whole_call(gpu):
+    """Given a stream, a call takes its memory there (not a block that the current stream's queued work may
+    still read), and copies a strided x there, behind the work that makes it."""
+    import torch
+    spec, lay, sw, pool = built("swiglu", gpu)
+    s = torch.cuda.Stream()
+    x = to_dev_bits(acts(64, spec.hidden, 3), gpu)
+    idx, w = routing(spec, 64, 3)
+    idd, wd = dev(idx, gpu), dev(w, gpu)
+    want = bits(mx.moe_forward(spec, pool, x, idd, wd))
+    rows = mx.quantize(x)
+    torch.cuda.synchronize()
+    calls = {"quantize": lambda: mx.quantize(x, stream=s).codes,
+             "dequantize": lambda: mx.dequantize(rows, stream=s),
+             "forward": lambda: mx.moe_forward(spec, pool, x, idd, wd, stream=s)}
+    for what, call in calls.items():
+        got = call()
+        torch.cuda.synchronize()
+        size = got.numel() * got.element_size()
+        del got
+        torch.cuda.empty_cache()
+        freed = torch.empty(size, dtype=torch.uint8, device=gpu)
+        at = freed.data_ptr()
+        del freed
+        assert call().data_ptr() != at, what
+        torch.cuda.synchronize()
+    late = torch.zeros((64, 2 * spec.hidden), dtype=torch.bfloat16, device=gpu)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)
+        late[:, :spec.hidden] = x
+    got = mx.moe_forward(spec, pool, late[:, :spec.hidden], idd, wd, stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    assert np.array_equal(bits(got), want)
+
+
+@pytest.mark.parametrize("T", [3, 20, 90])
+def test_pairs_with_the_shared_expert(gpu, T):
+    """The pairs form with the shared expert's id among them, in shuffled rows: the layer call's rows and the
+    shared expert's, whichever kernels run; rows no pair names stay."""
+    import torch
+    spec, lay, sw, pool = built("shared", gpu)
+    E, k = spec.n_experts, spec.top_k
+    x, idx, w, _ = _layer_inputs(spec, lay, gpu, T, seed=70 + T)
+    xd = to_dev_bits(x, gpu)
+    tok = np.concatenate([np.repeat(np.arange(T), k), np.arange(T)]).astype(np.int32)
+    ex = np.concatenate([idx.reshape(-1), np.full(T, E)]).astype(np.int32)
+    row = np.random.default_rng(T).permutation(tok.size + 5)[:tok.size].astype(np.int32)
+    got = []
+    for f in (0, L.FWD_FORCE_PREFILL) + ((L.FWD_FORCE_DECODE,) if T <= 8 else ()):
+        y = torch.full((tok.size + 5, spec.hidden), 3.0, dtype=torch.bfloat16, device=gpu)
+        mx.forward_pairs(spec, pool, xd, dev(tok, gpu), dev(ex, gpu), dev(row, gpu), y, f, shared=sw.shared)
+        got.append(bits(y))
+        assert np.array_equal(got[-1], got[0])
+    assert (f64(np.delete(got[0], row, 0)) == 3.0).all()
+    routed = bits(mx.moe_forward(spec, pool, xd, dev(idx, gpu))).reshape(T * k, spec.hidden)
+    assert np.array_equal(got[0][row[:T * k]], routed)
+    # weight 0 for the routed experts leaves the shared expert's rows (times one)
+    zero, one = torch.zeros((T, k), device=gpu), torch.ones(T, device=gpu)
+    alone = bits(mx.moe_forward(spec, pool, xd, dev(idx, gpu), zero, shared=sw.shared, sgate=one))
+    assert np.array_equal(f64(got[0][row[T * k:]]), f64(alone))
+
+
 @pytest.mark.parametrize("T", [1, 8, 30])
 def test_captured_graphs(gpu, T):
     """Two captured layers (rows quantised and read back beside them), replayed in turn and with eager
