@@ -26,11 +26,12 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
-from dataclasses import dataclass
+from typing import NamedTuple
+
+import torch
 
 from . import formats as F
 from . import lib as L
-from .layer import _stream
 from .pool import ExpertPool
 from .spec import LayerSpec
 
@@ -39,8 +40,14 @@ MAX_PAIRS = 1 << 21     # (token, expert) pairs of one call
 FEW_PAIRS = 64          # pairs an expert product runs without scratch
 
 
-@dataclass(frozen=True)
-class MXRows:
+# the current device and its current stream's handle (read without building a Stream object, where this
+# torch has the calls for it)
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_handle = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+class MXRows(NamedTuple):
     """Rows [..., K] in MXFP4: `codes` uint8 [..., K / 2], `scales` uint8 [..., K / 32]."""
     codes: object
     scales: object
@@ -52,27 +59,25 @@ class MXRows:
 
 @functools.lru_cache(maxsize=None)
 def _dtype(t) -> int:
-    import torch
     dt = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}.get(t)
     if dt is None:
         raise ValueError(f"{t}: MXFP4 rows are made of float32, bfloat16 or float16 values")
     return dt
 
 
-def _on_device(*tensors) -> None:
-    """Every tensor given is on the current device."""
-    import torch
-    cur = None
+def _on_device(*tensors) -> int:
+    """The current device; every tensor given is on it."""
+    cur = -1
     for t in tensors:
-        if t is None:
-            continue
-        d = t.get_device()
-        if d != cur:
-            if not t.is_cuda:
-                raise ValueError("tensors must be on the GPU")
-            cur = torch.cuda.current_device()
-            if d != cur:
-                raise ValueError(f"tensor on {t.device}, the current device is cuda:{cur}")
+        if t is not None:
+            d = t.get_device()
+            if d != cur or d < 0:
+                if d < 0:
+                    raise ValueError("tensors must be on the GPU")
+                if d != _current():
+                    raise ValueError(f"tensor on {t.device}, the current device is cuda:{_current()}")
+                cur = d
+    return cur
 
 
 def _matrices(t, what: str):
@@ -102,7 +107,6 @@ def _matrices(t, what: str):
 
 def _packed(t, what: str):
     """(batch, rows, batch stride) of packed bytes [..., rows, n] whose matrices are contiguous."""
-    import torch
     if t.dtype != torch.uint8:
         raise ValueError(f"{what} are uint8, got {t.dtype}")
     b, r, bs, rs = _matrices(t, what)
@@ -114,7 +118,6 @@ def _packed(t, what: str):
 def _on(stream, call, *args):
     """call(*args) with `stream` current (memory that the current stream's last work may still use is
     not handed to it, nor its results' memory reused under readers on the current stream)."""
-    import torch
     here = torch.cuda.current_stream()
     with torch.cuda.stream(stream):
         got = call(*args)
@@ -128,41 +131,44 @@ def quantize(x, stream=None) -> MXRows:
     per group of 32, e = floor(log2(max |v|)) - 2 and codes v / 2^e rounded to nearest even,
     saturating at 6 -- the codes of `formats.quantize_mxfp4`. A group with a NaN or an infinity is
     held as NaN (scale byte 255)."""
-    import torch
     if stream is not None:
         return _on(stream, quantize, x)
-    _on_device(x)
+    device = _on_device(x)
     dt = _dtype(x.dtype)
     shape = x.shape
     if not shape or shape[-1] % 32:
         raise ValueError(f"rows of {tuple(shape)}: the innermost dimension must be a multiple of 32")
     K = shape[-1]
-    b, r, bs, rs = _matrices(x, "x")
+    n = x.numel()
+    if n and x.is_contiguous():
+        b, r, bs, rs = 1, n // K, 0, K
+    else:
+        b, r, bs, rs = _matrices(x, "x")
     lead = shape[:-1]
-    codes = x.new_empty(lead + (K // 2,), dtype=torch.uint8)
-    scales = x.new_empty(lead + (K // 32,), dtype=torch.uint8)
+    codes = x.new_empty((*lead, K // 2), dtype=torch.uint8)
+    scales = x.new_empty((*lead, K // 32), dtype=torch.uint8)
     if b:
         L.check(L.load().brx_mx_quantize(x.data_ptr(), dt, b, r, K, bs, rs, codes.data_ptr(), r * (K // 2),
-                                         scales.data_ptr(), r * (K // 32), _stream()))
+                                         scales.data_ptr(), r * (K // 32), _handle(device)))
     return MXRows(codes, scales)
 
 
 def dequantize(q: MXRows, dtype=None, stream=None):
     """The values of q as a contiguous [..., K] tensor of `dtype` (default bfloat16; exact in
     float32 and bfloat16, rounded to nearest even in float16)."""
-    import torch
     if stream is not None:
         return _on(stream, dequantize, q, dtype)
     dtype = torch.bfloat16 if dtype is None else dtype
     dt = _dtype(dtype)
-    codes, scales = q.codes, q.scales
-    _on_device(codes, scales)
-    lead = codes.shape[:-1]
-    K = 2 * codes.shape[-1] if codes.dim() else 0
+    codes, scales = q
+    device = _on_device(codes, scales)
+    shape = codes.shape
+    lead = shape[:-1]
+    K = 2 * shape[-1] if shape else 0
     if K % 32 or scales.shape != lead + (K // 32,):
         raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not "
                          f"[..., K / 2] and [..., K / 32] of one K")
-    out = codes.new_empty(lead + (K,), dtype=dtype)
+    out = codes.new_empty((*lead, K), dtype=dtype)
     n = out.numel()
     if n == 0:
         return out
@@ -177,7 +183,7 @@ def dequantize(q: MXRows, dtype=None, stream=None):
             else:
                 sbs = r * (K // 32)
     L.check(L.load().brx_mx_dequantize(codes.data_ptr(), cbs, scales.data_ptr(), sbs, b, r, K, dt,
-                                       out.data_ptr(), _stream()))
+                                       out.data_ptr(), _handle(device)))
     return out
 
 
@@ -186,7 +192,6 @@ def pack_experts(spec: LayerSpec, weights: dict, biases: dict | None = None, sha
     """uint8 [E, bytes_per_expert]: the packed MXFP4 experts of a layer whose unquantized weights
     are weights[projection] [E, n_out, n_in] (and biases[projection] [E, n_out]), in the layout
     `ExpertPool.admit_device` and `HostStore` take. `shared`: the shared expert's width."""
-    import torch
     if stream is not None:
         return _on(stream, pack_experts, spec, weights, biases, shared)
     if spec.quant.mode != "mxfp4":
@@ -205,7 +210,7 @@ def pack_experts(spec: LayerSpec, weights: dict, biases: dict | None = None, sha
         if biases and tuple(biases[p].shape) != (E, n):
             raise ValueError(f"{p}: bias {tuple(biases[p].shape)}, the layer has {(E, n)}")
         _dtype(weights[p].dtype)
-    _on_device(*weights.values(), *(biases or {}).values())
+    device = _on_device(*weights.values(), *(biases or {}).values())
     offs, per = F.spec_offsets(es), F.spec_bytes(es)
     out = torch.empty((E, per), dtype=torch.uint8, device=next(iter(weights.values())).device)
     for p in es:
@@ -219,7 +224,7 @@ def pack_experts(spec: LayerSpec, weights: dict, biases: dict | None = None, sha
         if out.numel():
             L.check(L.load().brx_mx_quantize(w.data_ptr(), _dtype(w.dtype), *args,
                                              out.data_ptr() + offs[(p, "weight")], per,
-                                             out.data_ptr() + offs[(p, "scales")], per, _stream()))
+                                             out.data_ptr() + offs[(p, "scales")], per, _handle(device)))
         if biases:
             o = offs[(p, "bias")]
             b16 = biases[p].to(torch.bfloat16).contiguous().view(torch.uint8)
@@ -234,15 +239,13 @@ def _check_spec(spec: LayerSpec) -> None:
 
 
 def _index(t, n: int, what: str):
-    import torch
     if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {n} entries, got "
                          f"{t.dtype} {tuple(t.shape)}")
 
 
-def _workspace(spec: LayerSpec, T: int, pairs: int, shared: bool, product: bool, device):
-    """Scratch for one call, from torch's allocator."""
-    import torch
+def _workspace(spec: LayerSpec, T: int, pairs: int, shared: bool, product: bool, like):
+    """Scratch for one call, from torch's allocator (on the device of tensor `like`)."""
     known = spec.__dict__.setdefault("_mx_workspace", {})     # sizes, not memory
     key = (T, pairs, shared, product)
     n = known.get(key)
@@ -253,7 +256,7 @@ def _workspace(spec: LayerSpec, T: int, pairs: int, shared: bool, product: bool,
         if len(known) > 4096:
             known.clear()
         n = known[key] = out.value
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return like.new_empty(n, dtype=torch.uint8)
 
 
 _PROJ = {"gate_proj": 0, "up_proj": 1, "down_proj": 2}
@@ -268,7 +271,6 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
     lists). With `out` [n_rows, n_out] and pair_row (distinct rows), row pair_row[i] is written and
     the others are left as they are. Up to 64 pairs run as one launch, more as two and with scratch;
     the rows are the same bits."""
-    import torch
     if stream is not None:
         return _on(stream, expert_product, spec, pool, q, pair_token, pair_expert, proj, pair_row, out)
     _check_spec(spec)
@@ -276,9 +278,9 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
     if j is None:
         raise ValueError(f"projection {proj!r} not in {list(_PROJ if spec.gated else _MLP_PROJ)}")
     n_out, n_in = (spec.hidden, spec.inter) if j == 2 else (spec.inter, spec.hidden)
-    codes, scales = q.codes, q.scales
+    codes, scales = q
     n = pair_expert.numel()
-    _on_device(codes, scales, pair_token, pair_expert, pair_row, out)
+    device = _on_device(codes, scales, pair_token, pair_expert, pair_row, out)
     T = codes.shape[0] if codes.dim() else 0
     if codes.shape != (T, n_in // 2) or scales.shape != (T, n_in // 32):
         raise ValueError(f"activations {tuple(codes.shape)} / {tuple(scales.shape)}: {proj} takes rows "
@@ -293,19 +295,18 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
         if out is None:
             raise ValueError("pair_row names rows of an `out` that is not given")
     if out is None:
-        out = torch.empty((n, n_out), dtype=torch.bfloat16, device=codes.device)
+        out = codes.new_empty((n, n_out), dtype=torch.bfloat16)
     elif out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[1] != n_out or not out.is_contiguous():
         raise ValueError(f"out must be contiguous bfloat16 [n_rows, {n_out}]")
-    ws = _workspace(spec, T, n, False, True, codes.device) if n > FEW_PAIRS else None
+    ws = _workspace(spec, T, n, False, True, codes) if n > FEW_PAIRS else None
     L.check(L.load().brx_mx_expert_product(
         C.byref(spec.c_desc), pool.device.handle, codes.data_ptr(), scales.data_ptr(), T, pair_token.data_ptr(),
         pair_expert.data_ptr(), None if pair_row is None else pair_row.data_ptr(), n, out.shape[0], j,
-        out.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream()))
+        out.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _handle(device)))
     return out
 
 
 def _rows_of(spec: LayerSpec, x):
-    import torch
     if x.dtype != torch.bfloat16 or not x.shape or x.shape[-1] != spec.hidden:
         raise ValueError(f"x must be bfloat16 [..., {spec.hidden}], got {x.dtype} {tuple(x.shape)}")
     return x if x.dim() == 2 and x.is_contiguous() else x.reshape(-1, spec.hidden).contiguous()
@@ -319,13 +320,12 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
     be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`. Up to 8 tokens and 64 pairs run
     as two launches, some more as three and the rest as the grouped GEMM; the outputs are the same bits
     (`flags`: BRX_FWD_FORCE_DECODE or BRX_FWD_FORCE_PREFILL for the first or the last of these)."""
-    import torch
     if stream is not None:
         return _on(stream, moe_forward, spec, pool, x, idx, w, shared, sgate, out, y_unreduced, flags)
     _check_spec(spec)
     x2 = _rows_of(spec, x)
     T, H, k = x2.shape[0], spec.hidden, spec.top_k
-    _on_device(x2, idx, w, shared, sgate, out, y_unreduced)
+    device = _on_device(x2, idx, w, shared, sgate, out, y_unreduced)
     _index(idx, T * k, "idx")
     if w is not None and (w.dtype != torch.float32 or w.numel() != T * k or not w.is_contiguous()):
         raise ValueError(f"w must be contiguous float32 [{T}, {k}]")
@@ -337,20 +337,19 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
         if t is not None and (t.dtype != torch.bfloat16 or t.numel() != n or not t.is_contiguous()):
             raise ValueError(f"out and y_unreduced must be contiguous bfloat16 [{T}, {H}] and [{T}, {k}, {H}]")
     if w is not None and out is None:
-        out = torch.empty((T, H), dtype=torch.bfloat16, device=x2.device)
+        out = x2.new_empty((T, H))
     if w is None and y_unreduced is None:
-        y_unreduced = torch.empty((T, k, H), dtype=torch.bfloat16, device=x2.device)
-    ws = _workspace(spec, T, T * k, shared is not None, False, x2.device)
+        y_unreduced = x2.new_empty((T, k, H))
+    ws = _workspace(spec, T, T * k, shared is not None, False, x2)
     ptr = L.ptr
     L.check(L.load().brx_mx_moe_forward(
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), idx.data_ptr(), ptr(w), ptr(shared),
         ptr(sgate), T, ptr(out), ptr(y_unreduced), 0 if flags is None else flags, ws.data_ptr(), ws.numel(),
-        _stream()))
+        _handle(device)))
     return out if w is not None else y_unreduced
 
 
 def _check_shared(spec: LayerSpec, shared) -> None:
-    import torch
     if not spec.shared_inter:
         raise ValueError("the layer has no shared expert")
     per = spec.__dict__.get("_mx_shared_bytes")
@@ -363,13 +362,12 @@ def _check_shared(spec: LayerSpec, shared) -> None:
 def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair_row, y_rows, flags: int,
                   shared=None, stream=None) -> None:
     """`layer.forward_pairs` with MXFP4 activations (any `flags` give the same bits)."""
-    import torch
     if stream is not None:
         return _on(stream, forward_pairs, spec, pool, x, pair_tok, pair_exp, pair_row, y_rows, flags, shared)
     _check_spec(spec)
     x2 = _rows_of(spec, x)
     n = pair_exp.numel()
-    _on_device(x2, pair_tok, pair_exp, pair_row, y_rows, shared)
+    device = _on_device(x2, pair_tok, pair_exp, pair_row, y_rows, shared)
     _index(pair_tok, n, "pair_tok")
     _index(pair_exp, n, "pair_exp")
     if pair_row is not None:
@@ -379,9 +377,9 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
     if (y_rows.dtype != torch.bfloat16 or y_rows.dim() != 2 or y_rows.shape[1] != spec.hidden or
             not y_rows.is_contiguous()):
         raise ValueError(f"y_rows must be contiguous bfloat16 [n_rows, {spec.hidden}]")
-    ws = _workspace(spec, x2.shape[0], n, shared is not None, False, x2.device)
+    ws = _workspace(spec, x2.shape[0], n, shared is not None, False, x2)
     ptr = L.ptr
     L.check(L.load().brx_mx_moe_forward_pairs(
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), x2.shape[0], ptr(pair_tok), ptr(pair_exp),
         ptr(pair_row), n, y_rows.shape[0], ptr(shared), y_rows.data_ptr(), flags, ws.data_ptr(), ws.numel(),
-        _stream()))
+        _handle(device)))
