@@ -6,10 +6,17 @@
 //                 (a wave holds whole groups), in bucketed order.
 //   k_mx_gemm<1>  down: A = h rows; + bias, each pair's bf16 row at its (token, k) position.
 //   k_mx_gemm<2>  one projection of the pairs' token rows (the expert product), stored as <1>.
-// The pairs are bucketed per expert and cut into M tiles by k_bucket (k_prefill.hip).
+// The pairs are bucketed per expert and cut into M tiles by bucket.h: in k_mx_prepare, which rounds x beside it
+// (a layer), or in k_bucket (a product).
 //
 // y[n][m] = sum over K groups g of 2^(es_w[m][g] + es_x[n][g] - 254) * sum_k w[m][k] x[n][k], exact
 // products, fp32 sums in steps of 128 K in order. A row's bits do not depend on its tile.
+//
+// What bounds it. 512 tokens of the gpt-oss shape (16 pairs an expert, 1.70 GB of weights): the weight stream,
+// 227 + 123 us, 5.0 TB/s, where a copy of 1 GiB reaches 5.1. 2048 tokens of the Qwen3 shape under a Zipf law
+// (128 pairs an expert on average, 155 GFLOP): 89 + 66 us, 1000 TFLOP/s; matrix instructions fill 15% of
+// the time and vector ones half, and the rest is the wait for each chunk's weights: with 64 pairs a tile a wave
+// has 64 + 64 registers of sums and weights, and a second set of weights does not fit.
 #include <type_traits>
 
 #include "bucket.h"
@@ -73,18 +80,21 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
     // piece 4 g + m % 4 of row 4 (m / 4) + t in load t, and the four transpose (mx_transpose).
     const uint32_t vw = (uint32_t)P0.w + (uint32_t)(cr + 8 * (l16 >> 2)) * (uint32_t)(K / 2);
     const uint32_t dw = gated ? (uint32_t)(P1.w - P0.w) : 16u * (uint32_t)K;
-    struct Chunk {
-        mx_u32x4 w[4][4];
+    // A chunk comes in two halves of two fragments, each requested as soon as the one before it in its registers
+    // is used (both at the end of a chunk: 512 tokens of the gpt-oss shape 355 us a layer, 349 so).
+    struct Half {
+        mx_u32x4 w[2][4];
     };
-    // (pieces past the row's end read its last one: their A codes are zero)
-    auto issue = [&](int ch, Chunk& q) __attribute__((always_inline)) {
-        const uint32_t v = vw + 16u * (uint32_t)min(16 * ch + 4 * g + (l16 & 3), G - 1);
+    // (pieces past the row's end read its last one: their A codes are zero; past the last chunk the request is
+    // out of the buffer's range, wherever the scalar offset counts, and costs no memory access -- under a branch
+    // the registers spilled)
+    auto issue = [&](int ch, Half& q, uint32_t d) __attribute__((always_inline)) {
+        const uint32_t v = 16 * ch < G ? vw + 16u * (uint32_t)min(16 * ch + 4 * g + (l16 & 3), G - 1) : 0x80000000u;
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
+        for (int f = 0; f < 2; ++f) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-                q.w[f][t] = __builtin_amdgcn_raw_buffer_load_b128(
-                    rw, v, (f >> 1) * dw + (f & 1) * 2u * K + t * (uint32_t)(K / 2), 0);
+                q.w[f][t] = __builtin_amdgcn_raw_buffer_load_b128(rw, v, d + f * 2u * K + t * (uint32_t)(K / 2), 0);
         }
     };
 
@@ -121,8 +131,9 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
             bias[h] = __builtin_amdgcn_raw_buffer_load_b128(
                 rw, (uint32_t)P0.bias + 2u * (uint32_t)(cr + 8 * g), gated ? h * (P1.bias - P0.bias) : 64 * h, 0);
     }
-    Chunk q;
-    issue(0, q);
+    Half qa, qb;
+    issue(0, qa, 0);
+    issue(0, qb, dw);
     asm volatile("" ::: "memory");
     uint32_t va[NC], vx[NS];
     int lc[NC], ls[NS];
@@ -169,38 +180,45 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
         if (ch + 1 < nch) issue_a(ch + 1);         // (every wave is done with the chunk that was there)
         asm volatile("" ::: "memory");
         const uint8_t* const buf = smem + (ch & 1) * kMxBuf<MP>;
-        uint32_t ws[4];
         // groups past the row's end: zeros (another row's byte might be a NaN)
         const int left = G - (16 * ch + 4 * g);
         const uint32_t in = left >= 4 ? 0xFFFFFFFFu : left >= 2 ? 0xFFFFu : 0u;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-            const uint16_t* const t =
-                reinterpret_cast<const uint16_t*>(tbl + (32 * (f >> 1) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3)) * G + 16 * ch + 4 * g);
-            ws[f] = (t[0] | ((uint32_t)t[1] << 16)) & in;
-            mx_transpose(q.w[f]);
-        }
         uint32_t xe[MP];       // the lane's four scales of its pairs' rows
 #pragma unroll
         for (int p = 0; p < MP; ++p) {
             const u32x2_t v = *reinterpret_cast<const u32x2_t*>(buf + kMxA<MP> + p * 512 + l16 * 32 + 8 * g);
             xe[p] = v[0] | (v[1] << 16);
         }
-        auto step = [&](auto t_) __attribute__((always_inline)) {
-            constexpr int t = decltype(t_)::value;
+        auto half = [&](Half& q, auto h_) __attribute__((always_inline)) {
+            constexpr int h = decltype(h_)::value;
+            uint32_t ws[2];
 #pragma unroll
-            for (int p = 0; p < MP; ++p) {
-                const mx_u32x4 xv = *reinterpret_cast<const mx_u32x4*>(buf + p * 4096 + l16 * 256 + 16 * ((4 * g + t) ^ l16));
-#pragma unroll
-                for (int f = 0; f < 4; ++f) acc[p][f] = mx_mfma<t>(q.w[f][t], ws[f], xv, xe[p], acc[p][f]);
+            for (int f = 0; f < 2; ++f) {
+                const uint16_t* const t =
+                    reinterpret_cast<const uint16_t*>(tbl + (32 * h + 8 * (l16 >> 2) + 4 * f + (l16 & 3)) * G + 16 * ch + 4 * g);
+                ws[f] = (t[0] | ((uint32_t)t[1] << 16)) & in;
+                mx_transpose(q.w[f]);
             }
+            auto step = [&](auto t_) __attribute__((always_inline)) {
+                constexpr int t = decltype(t_)::value;
+#pragma unroll
+                for (int p = 0; p < MP; ++p) {
+                    const mx_u32x4 xv = *reinterpret_cast<const mx_u32x4*>(buf + p * 4096 + l16 * 256 + 16 * ((4 * g + t) ^ l16));
+#pragma unroll
+                    for (int f = 0; f < 2; ++f) acc[p][2 * h + f] = mx_mfma<t>(q.w[f][t], ws[f], xv, xe[p], acc[p][2 * h + f]);
+                }
+            };
+            step(std::integral_constant<int, 0>{});
+            step(std::integral_constant<int, 1>{});
+            step(std::integral_constant<int, 2>{});
+            step(std::integral_constant<int, 3>{});
         };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
-        step(std::integral_constant<int, 2>{});
-        step(std::integral_constant<int, 3>{});
-        if (ch + 1 == nch) break;                  // (a request past the last chunk: 3% of a call)
-        issue(ch + 1, q);
+        half(qa, std::integral_constant<int, 0>{});
+        issue(ch + 1, qa, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        half(qb, std::integral_constant<int, 1>{});
+        if (ch + 1 == nch) break;
+        issue(ch + 1, qb, dw);
         __builtin_amdgcn_sched_barrier(0);
         // the next chunk of A has landed (the weights were issued after its copies), and every wave is done
         // reading this one
