@@ -849,7 +849,7 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
 
 static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T, int P, const int32_t* pexp,
                       const int32_t* ptok, const int32_t* prow, int yrows, const float* w, const void* shared_expert,
-                      const float* shared_gate, void* out, void* y_rows, unsigned flags, void* workspace,
+                      const float* shared_gate, void* out, void* y_rows, float* rows32, unsigned flags, void* workspace,
                       size_t workspace_bytes, void* stream) {
     if (!x) return fail(BRX_EINVAL, "x is required");
     if ((uintptr_t)x & 15) return fail(BRX_EINVAL, "x must be 16-byte aligned");
@@ -866,7 +866,7 @@ static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T
         return fail(BRX_EINVAL, "the decode path takes at most 8 token rows and 64 pairs (T=%d, P=%d)", T, P);
     const int rc = mx_begin(p, mx_workspace_bytes(a, true, path), workspace, workspace_bytes, s);
     if (rc) return rc;
-    return mx_end(p, launch_mx_layer(a, path, workspace, s), s);
+    return mx_end(p, launch_mx_layer(a, path, rows32, workspace, s), s);
 }
 
 int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, const int32_t* idx, const float* w,
@@ -883,20 +883,39 @@ int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, cons
     if (((uintptr_t)out | (uintptr_t)y_unreduced) & 15) return fail(BRX_EINVAL, "out and y_unreduced must be 16-byte aligned");
     if (shared_expert && out && !shared_gate) return fail(BRX_EINVAL, "shared expert given without its gate values");
     return mx_forward(d, p, x, T, T * d->top_k, idx, nullptr, nullptr, T * d->top_k, w, shared_expert, shared_gate, out,
-                      y_unreduced, flags, workspace, workspace_bytes, stream);
+                      y_unreduced, nullptr, flags, workspace, workspace_bytes, stream);
 }
 
 int brx_mx_moe_forward_pairs(const brx_layer_desc* d, brx_pool* p, const void* x, int T, const int32_t* pair_token,
                              const int32_t* pair_expert, const int32_t* pair_row, int n_pairs, int n_rows,
-                             const void* shared_expert, void* y_rows, unsigned flags, void* workspace,
+                             const void* shared_expert, void* y_rows, int y_dtype, unsigned flags, void* workspace,
                              size_t workspace_bytes, void* stream) {
     int rc = check_mx_forward(d, p);
     if (rc) return rc;
     if ((rc = check_mx_sizes(T, n_pairs, false))) return rc;
+    if (y_dtype != BRX_DT_BF16 && y_dtype != BRX_DT_F32) return fail(BRX_EINVAL, "y_dtype %d: rows are bf16 or fp32", y_dtype);
     if (n_pairs == 0) return BRX_OK;
+    const bool wide = y_dtype == BRX_DT_F32;
     if ((rc = check_pairs(T, n_pairs, n_rows, pair_token, pair_expert, pair_row, y_rows))) return rc;
     return mx_forward(d, p, x, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, shared_expert, nullptr,
-                      nullptr, y_rows, flags, workspace, workspace_bytes, stream);
+                      nullptr, wide ? nullptr : y_rows, wide ? (float*)y_rows : nullptr, flags, workspace, workspace_bytes,
+                      stream);
+}
+
+int brx_mx_combine(const brx_layer_desc* d, const float* y_routed, const float* w, const float* y_shared,
+                   const float* shared_gate, int T, void* out, void* stream) {
+    int rc = check_desc(d);
+    if (rc) return rc;
+    if ((rc = ensure_device())) return rc;
+    if (T < 0 || T > 65535) return fail(BRX_EINVAL, "T %d outside [0, 65535]", T);
+    if (T == 0) return BRX_OK;
+    if (!y_routed || !w || !out) return fail(BRX_EINVAL, "y_routed, w and out are required");
+    if (y_shared && !shared_gate) return fail(BRX_EINVAL, "shared rows given without their gate values");
+    if (((uintptr_t)y_routed | (uintptr_t)y_shared | (uintptr_t)out) & 15)
+        return fail(BRX_EINVAL, "y_routed, y_shared and out must be 16-byte aligned");
+    hipError_t e = launch_mx_combine(y_routed, y_shared, w, shared_gate, T, d->top_k, d->hidden, (uint16_t*)out, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "combine launch");
+    return BRX_OK;
 }
 
 int brx_combine(const brx_layer_desc* d, const void* y_routed, const float* w, const void* y_shared,

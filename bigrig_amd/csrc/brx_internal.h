@@ -682,11 +682,13 @@ hipError_t launch_mx_dequantize(const MxRows& m, int dtype, hipStream_t s);
 enum MxPath { kMxFew, kMxMid, kMxMany };
 MxPath mx_path(const FwdArgs& a);
 size_t mx_workspace_bytes(const FwdArgs& a, bool layer, MxPath path);
-hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, void* ws, hipStream_t s);
+hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, float* rows32, void* ws, hipStream_t s);
+hipError_t launch_mx_combine(const float* y, const float* y_shared, const float* w, const float* sg, int T, int k, int H,
+                             uint16_t* out, hipStream_t s);
 hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, void* ws,
                              hipStream_t s);
 size_t mx_few_workspace_bytes(const FwdArgs& a, bool tiles);
-hipError_t launch_mx_few_layer(const FwdArgs& a, bool tiles, void* ws, hipStream_t s);
+hipError_t launch_mx_few_layer(const FwdArgs& a, bool tiles, float* rows32, void* ws, hipStream_t s);
 hipError_t launch_mx_few_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, hipStream_t s);
 hipError_t launch_combine(const uint16_t* y_routed, const uint16_t* y_shared, const float* w,
                           const float* sg, int T, int k, int H, uint16_t* out, hipStream_t s);

@@ -264,12 +264,10 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
             }
         }
     } else {
-        uint16_t* dst[MP];
+        int row[MP];
 #pragma unroll
-        for (int p = 0; p < MP; ++p) {
-            const int d = KIND == 2 || pd[p] < a.P ? pair_row(a, pd[p]) : -2 - (pd[p] - a.P);
-            dst[p] = p * 16 + l16 >= rows ? nullptr : d >= 0 ? m.y_routed + (int64_t)d * N : m.y_shared + (int64_t)(-2 - d) * N;
-        }
+        for (int p = 0; p < MP; ++p)
+            row[p] = p * 16 + l16 >= rows ? -1 : KIND == 2 || pd[p] < a.P ? pair_row(a, pd[p]) : pd[p];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int col = c0 + 32 * h + 8 * g;
@@ -280,8 +278,14 @@ __device__ __forceinline__ void mx_tile(const FwdArgs& a, const MxArgs& m, uint8
                 float y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = absent ? nan : acc[p][2 * h + (i >> 2)][i & 3] + b[i];
-                if (dst[p])
-                    *reinterpret_cast<u32x4_t*>(dst[p] + col) =
+                if (row[p] < 0) continue;
+                if (KIND == 1 && m.y32) {              // uniform
+                    f32x4_t* const to = reinterpret_cast<f32x4_t*>(m.y32 + (int64_t)row[p] * N + col);
+                    to[0] = f32x4_t{y[0], y[1], y[2], y[3]};
+                    to[1] = f32x4_t{y[4], y[5], y[6], y[7]};
+                }
+                if ((KIND == 2 || m.y16) && row[p] < a.yrows)    // (no bf16 rows of the shared pairs)
+                    *reinterpret_cast<u32x4_t*>(m.y16 + (int64_t)row[p] * N + col) =
                         u32x4_t{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3]), pk_bf16(y[4], y[5]), pk_bf16(y[6], y[7])};
             }
         }
@@ -331,7 +335,7 @@ struct MxWs {
     uint8_t *xq, *xs, *hq, *hs;
     int32_t *order, *offsets, *tile_start;
     int4* tinfo;
-    uint16_t *y_routed, *y_shared;
+    float* y32;
     int mt_pad, tile, group, Imax;
     size_t bytes;
 };
@@ -358,8 +362,7 @@ MxWs carve(const FwdArgs& a, bool layer, void* ws) {
         w.xs = (uint8_t*)take((size_t)a.T * (a.H / 32));
         w.hq = (uint8_t*)take((size_t)P_ext * (w.Imax / 2));
         w.hs = (uint8_t*)take((size_t)P_ext * (w.Imax / 32));
-        w.y_routed = (uint16_t*)take(a.yun ? 0 : (size_t)a.P * a.H * 2);
-        w.y_shared = (uint16_t*)take((size_t)T_sh * a.H * 2);
+        w.y32 = (float*)take(a.out || !a.yun ? (size_t)P_ext * a.H * 4 : 0);   // (neither: a call's size is asked for)
     }
     w.bytes = off;
     return w;
@@ -432,6 +435,37 @@ __global__ __launch_bounds__(kBucketThreads) void k_mx_prepare(const int32_t* __
     if ((i & 3) == 0) xs[i >> 2] = (uint8_t)sb;
 }
 
+// out[t] = sum_j w[t, j] y[t, j] (+ sg[t] y_shared[t]) over fp32 rows, j in order, four columns a thread.
+__global__ __launch_bounds__(kMxThreads) void k_mx_combine(const float* __restrict__ y, const float* __restrict__ y_shared,
+                                                           const float* __restrict__ w, const float* __restrict__ sg,
+                                                           int k, int H, uint16_t* __restrict__ out) {
+    const int t = blockIdx.y, n = (blockIdx.x * kMxThreads + threadIdx.x) * 4;
+    if (n >= H) return;
+    constexpr int U = 8;                           // rows in flight
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    f32x4_t sh{0.f, 0.f, 0.f, 0.f};
+    if (y_shared) sh = *reinterpret_cast<const f32x4_t*>(y_shared + (int64_t)t * H + n);
+    for (int j0 = 0; j0 < k; j0 += U) {
+        f32x4_t v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const f32x4_t*>(y + ((int64_t)t * k + min(j0 + u, k - 1)) * H + n);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (j0 + u >= k) break;                // uniform
+            const float wj = w[t * k + j0 + u];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(wj, v[u][i], o[i]);
+        }
+    }
+    if (y_shared) {
+        const float g = sg[t];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(g, sh[i], o[i]);
+    }
+    *reinterpret_cast<u32x2_t*>(out + (int64_t)t * H + n) =
+        u32x2_t{f2bf(o[0]) | (f2bf(o[1]) << 16), f2bf(o[2]) | (f2bf(o[3]) << 16)};
+}
+
 hipError_t prepare(const FwdArgs& a, const MxWs& w, hipStream_t s) {
     const int E_ext = a.E + (a.shared ? 1 : 0), T_sh = a.auto_shared ? a.T : 0;
     const int lcap = bucket_list(a.P + T_sh);
@@ -468,8 +502,15 @@ size_t mx_workspace_bytes(const FwdArgs& a, bool layer, MxPath path) {
     return layer && path != kMxMany ? mx_few_workspace_bytes(a, path == kMxMid) : carve(a, layer, nullptr).bytes;
 }
 
-hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, void* ws, hipStream_t s) {
-    if (path != kMxMany) return launch_mx_few_layer(a, path == kMxMid, ws, s);
+hipError_t launch_mx_combine(const float* y, const float* y_shared, const float* w, const float* sg, int T, int k, int H,
+                             uint16_t* out, hipStream_t s) {
+    hipLaunchKernelGGL(k_mx_combine, dim3((H / 4 + kMxThreads - 1) / kMxThreads, T), dim3(kMxThreads), 0, s, y, y_shared, w,
+                       sg, k, H, out);
+    return hipGetLastError();
+}
+
+hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, float* rows32, void* ws, hipStream_t s) {
+    if (path != kMxMany) return launch_mx_few_layer(a, path == kMxMid, rows32, ws, s);
     const MxWs w = carve(a, true, ws);
     hipError_t e = prepare(a, w, s);
     if (e != hipSuccess) return e;
@@ -479,12 +520,12 @@ hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, void* ws, hipStream_t 
     m.hq = w.hq;
     m.hs = w.hs;
     m.hstride = w.Imax;
-    m.y_routed = a.yun ? a.yun : w.y_routed;
-    m.y_shared = w.y_shared;
+    m.y16 = a.yun;
+    m.y32 = rows32 ? rows32 : a.out ? w.y32 : nullptr;
     if ((e = launch_gemm<0>(a, m, w, a.H, w.Imax, s)) != hipSuccess) return e;
     if ((e = launch_gemm<1>(a, m, w, w.Imax, a.H, s)) != hipSuccess) return e;
     if (!a.out) return hipSuccess;
-    return launch_combine(m.y_routed, a.auto_shared ? w.y_shared : nullptr, a.w, a.sgate, a.T, a.k, a.H, a.out, s);
+    return launch_mx_combine(w.y32, a.auto_shared ? w.y32 + (int64_t)a.P * a.H : nullptr, a.w, a.sgate, a.T, a.k, a.H, a.out, s);
 }
 
 hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, void* ws,
@@ -496,7 +537,7 @@ hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8
     MxArgs m = gemm_args(a, w);
     m.xq = codes;
     m.xs = scales;
-    m.y_routed = a.yun;
+    m.y16 = a.yun;
     m.proj = proj;
     return launch_gemm<2>(a, m, w, proj == 2 ? w.Imax : a.H, proj == 2 ? a.H : w.Imax, s);
 }

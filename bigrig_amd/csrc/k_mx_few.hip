@@ -398,7 +398,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_mx_few_rows(FwdArgs a, MxArg
                         *reinterpret_cast<f32x4_t*>(&ys[pl[v].pair][4 * g]) = f32x4_t{y[0], y[1], y[2], y[3]};
                     } else {
                         const int N = m.proj == 2 ? a.H : a.I;
-                        *reinterpret_cast<u32x2_t*>(m.y_routed + (int64_t)pair_row(a, pl[v].pair) * N + c0 + 4 * g) =
+                        *reinterpret_cast<u32x2_t*>(m.y16 + (int64_t)pair_row(a, pl[v].pair) * N + c0 + 4 * g) =
                             u32x2_t{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
                     }
                 }
@@ -411,8 +411,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_mx_few_rows(FwdArgs a, MxArg
     }
     if constexpr (DOWN) {
         lds_barrier();
-        // two columns a thread, each pair's row rounded to bf16
+        // two columns a thread
         const int c = 2 * (tid & 7);
+        if (m.y32) {
+            for (int q = tid >> 3; q < a.P; q += 8 * kRowWaves) {
+                typedef float f32x2_t __attribute__((ext_vector_type(2)));
+                *reinterpret_cast<f32x2_t*>(m.y32 + (int64_t)pair_row(a, q) * a.H + c0 + c) = f32x2_t{ys[q][c], ys[q][c + 1]};
+            }
+        }
         if (a.yun) {
             for (int q = tid >> 3; q < a.P; q += 8 * kRowWaves)
                 *reinterpret_cast<uint32_t*>(a.yun + (int64_t)pair_row(a, q) * a.H + c0 + c) = pk_bf16(ys[q][c], ys[q][c + 1]);
@@ -421,9 +427,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_mx_few_rows(FwdArgs a, MxArg
             const int t = tid >> 3;
             float o0 = 0.f, o1 = 0.f;
             auto add = [&](float w, int q) __attribute__((always_inline)) {
-                const uint32_t v = pk_bf16(ys[q][c], ys[q][c + 1]);
-                o0 = fmaf(w, bf2f(v & 0xFFFFu), o0);
-                o1 = fmaf(w, bf2f(v >> 16), o1);
+                o0 = fmaf(w, ys[q][c], o0);
+                o1 = fmaf(w, ys[q][c + 1], o1);
             };
             for (int j = 0; j < a.k; ++j) add(a.w[t * a.k + j], t * a.k + j);
             if (a.auto_shared && a.sgate) add(a.sgate[t], a.P + t);
@@ -472,12 +477,13 @@ inline int few_batch(int K) { const int nch = (K + 511) / 512; return nch <= 2 ?
 
 size_t mx_few_workspace_bytes(const FwdArgs& a, bool tiles) { return carve_few(a, tiles, nullptr).bytes; }
 
-hipError_t launch_mx_few_layer(const FwdArgs& a, bool tiles, void* ws, hipStream_t s) {
+hipError_t launch_mx_few_layer(const FwdArgs& a, bool tiles, float* rows32, void* ws, hipStream_t s) {
     const FewWs w = carve_few(a, tiles, ws);
     MxArgs m{};
     m.hq = w.hq;
     m.hs = w.hs;
     m.hstride = w.Imax;
+    m.y32 = rows32;
     m.E_ext = a.E + (a.shared ? 1 : 0);
     hipError_t e = hipSuccess;
     if (tiles) {
@@ -521,7 +527,7 @@ hipError_t launch_mx_few_product(const FwdArgs& a, const uint8_t* codes, const u
     MxArgs m{};
     m.xq = codes;
     m.xs = scales;
-    m.y_routed = a.yun;
+    m.y16 = a.yun;
     m.proj = proj;
     const dim3 grid((proj == 2 ? a.H : a.I) / 16, (a.P + kRowWaves - 1) / kRowWaves);
 #define BRX_ROWS(NB) hipLaunchKernelGGL((k_mx_few_rows<false, NB, 1>), grid, dim3(64 * kRowWaves), 0, s, a, m, (const MxTable*)nullptr)

@@ -34,8 +34,8 @@ struct MxArgs {
     const int32_t* order;
     const int32_t* tile_start;
     const int4* tinfo;
-    uint16_t* y_routed;
-    uint16_t* y_shared;
+    uint16_t* y16;              // bf16 rows, a routed pair's at its row of the caller's, or null
+    float* y32;                 // fp32 rows, likewise (every token's shared pair at its index), or null
     int32_t hstride;            // values between h rows
     int32_t E_ext, ntn;
     int32_t group;              // M tiles an XCD takes together

@@ -336,15 +336,19 @@ class StreamingSwitchGLU:
             self._forward(x2, idx, w, shared, sgate, out=out, flags=flags, stream=stream)
             return out
         self.chunked_calls += 1
-        y = torch.empty((T * k, H), dtype=torch.bfloat16, device=x2.device)
+        join, rows = combine, torch.bfloat16
+        if self.activations == "mxfp4":       # (whose fused sum takes the rows before any rounding)
+            from . import mx
+            join, rows = mx.combine, torch.float32
+        y = torch.empty((T * k, H), dtype=rows, device=x2.device)
         self._spans(x2, gi, y, flags, stream)
         ysh = None
         if shared is not None:
-            ysh = torch.empty((T, H), dtype=torch.bfloat16, device=x2.device)
+            ysh = torch.empty((T, H), dtype=rows, device=x2.device)
             tt = torch.arange(T, dtype=torch.int32, device=x2.device)
             te = torch.full((T,), self.spec.n_experts, dtype=torch.int32, device=x2.device)
             self._forward_pairs(x2, tt, te, None, ysh, flags, shared=shared, stream=stream)
-        combine(self.spec, y, w, out, ysh, sgate, stream=stream)
+        join(self.spec, y, w, out, ysh, sgate, stream=stream)
         return out
 
 

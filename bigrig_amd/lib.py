@@ -33,7 +33,7 @@ EXPORTS = (
     "brx_pool_admit_async", "brx_pool_refill_range_async", "brx_pool_check",
     "brx_moe_block_forward_noalloc", "brx_mx_quantize", "brx_mx_dequantize",
     "brx_mx_workspace_bytes", "brx_mx_expert_product", "brx_mx_moe_forward",
-    "brx_mx_moe_forward_pairs",
+    "brx_mx_moe_forward_pairs", "brx_mx_combine",
 )
 
 
@@ -106,7 +106,8 @@ _SIGS = {
     "brx_mx_moe_forward": ([C.POINTER(LayerDesc), _vp, _vp, _vp, _vp, _vp, _vp, C.c_int, _vp, _vp,
                             C.c_uint, _vp, C.c_size_t, _vp], C.c_int),
     "brx_mx_moe_forward_pairs": ([C.POINTER(LayerDesc), _vp, _vp, C.c_int, _vp, _vp, _vp, C.c_int,
-                                  C.c_int, _vp, _vp, C.c_uint, _vp, C.c_size_t, _vp], C.c_int),
+                                  C.c_int, _vp, _vp, C.c_int, C.c_uint, _vp, C.c_size_t, _vp], C.c_int),
+    "brx_mx_combine": ([C.POINTER(LayerDesc), _vp, _vp, _vp, _vp, C.c_int, _vp, _vp], C.c_int),
     "brx_combine": ([C.POINTER(LayerDesc), _vp, _vp, _vp, _vp, C.c_int, _vp, _vp], C.c_int),
     "brx_dequant": ([C.POINTER(LayerDesc), _vp, C.c_int, C.c_int, _vp, _vp], C.c_int),
     "brx_sort_pairs": ([C.POINTER(LayerDesc), _vp, C.c_int, _vp, _vp, _vp], C.c_int),

@@ -11,7 +11,8 @@ of two.
 * `pack_experts`: unquantized expert weights into the packed bytes of MXFP4 experts, on the GPU
   (`formats.quantize_mxfp4` of every projection, in blob layout);
 * `expert_product`: one projection's rows for a list of (token, expert) pairs;
-* `moe_forward` / `forward_pairs`: the layer forms of `layer.moe_forward` / `layer.forward_pairs`.
+* `moe_forward` / `forward_pairs`: the layer forms of `layer.moe_forward` / `layer.forward_pairs`;
+* `combine`: the weighted sum of float32 rows that `moe_forward` makes, for rows of `forward_pairs`.
 
 A row [K] is K / 2 bytes of e2m1 codes (two a byte, the low nibble first) and K / 32 e8m0 scale
 bytes, as an expert's `weight` and `scales` components hold it. A group that holds a NaN or an
@@ -316,7 +317,8 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
                 y_unreduced=None, flags=None, stream=None):
     """The routed experts of tokens x [T, H] (bf16) under a routing idx [T, k] (int32) with both
     projections' activations in MXFP4. With weights w [T, k] (fp32): out [T, H] = sum_j w[t, j] *
-    y[t, j] (+ sgate[t] * shared(x_t)); without: the unreduced rows [T, k, H]. The pool's table must
+    y[t, j] (+ sgate[t] * shared(x_t)) over the float32 rows y; without: the unreduced rows [T, k, H] in
+    bfloat16. The pool's table must
     be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`. Up to 8 tokens and 64 pairs run
     as two launches, some more as three and the rest as the grouped GEMM; the outputs are the same bits
     (`flags`: BRX_FWD_FORCE_DECODE or BRX_FWD_FORCE_PREFILL for the first or the last of these)."""
@@ -361,7 +363,8 @@ def _check_shared(spec: LayerSpec, shared) -> None:
 
 def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair_row, y_rows, flags: int,
                   shared=None, stream=None) -> None:
-    """`layer.forward_pairs` with MXFP4 activations (any `flags` give the same bits)."""
+    """`layer.forward_pairs` with MXFP4 activations (any `flags` give the same bits); y_rows bfloat16, or
+    float32 for `combine`."""
     if stream is not None:
         return _on(stream, forward_pairs, spec, pool, x, pair_tok, pair_exp, pair_row, y_rows, flags, shared)
     _check_spec(spec)
@@ -374,12 +377,29 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
         _index(pair_row, n, "pair_row")
     if shared is not None:
         _check_shared(spec, shared)
-    if (y_rows.dtype != torch.bfloat16 or y_rows.dim() != 2 or y_rows.shape[1] != spec.hidden or
-            not y_rows.is_contiguous()):
-        raise ValueError(f"y_rows must be contiguous bfloat16 [n_rows, {spec.hidden}]")
+    if (y_rows.dtype not in (torch.bfloat16, torch.float32) or y_rows.dim() != 2 or
+            y_rows.shape[1] != spec.hidden or not y_rows.is_contiguous()):
+        raise ValueError(f"y_rows must be contiguous bfloat16 or float32 [n_rows, {spec.hidden}]")
     ws = _workspace(spec, x2.shape[0], n, shared is not None, False, x2)
     ptr = L.ptr
     L.check(L.load().brx_mx_moe_forward_pairs(
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), x2.shape[0], ptr(pair_tok), ptr(pair_exp),
-        ptr(pair_row), n, y_rows.shape[0], ptr(shared), y_rows.data_ptr(), flags, ws.data_ptr(), ws.numel(),
+        ptr(pair_row), n, y_rows.shape[0], ptr(shared), y_rows.data_ptr(), _dtype(y_rows.dtype), flags, ws.data_ptr(), ws.numel(),
         _handle(device)))
+
+
+def combine(spec: LayerSpec, y_routed, w, out, y_shared=None, sgate=None, stream=None) -> None:
+    """out[t] = sum_j w[t, j] * y_routed[t, j] (+ sgate[t] * y_shared[t]): rows float32 [T k, H] and
+    [T, H], w and sgate float32, out bfloat16 [T, H]."""
+    if stream is not None:
+        return _on(stream, combine, spec, y_routed, w, out, y_shared, sgate)
+    T, H, k = out.shape[0], spec.hidden, spec.top_k
+    device = _on_device(out, y_routed, w, y_shared, sgate)
+    if out.dtype != torch.bfloat16 or out.shape != (T, H) or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous bfloat16 [T, {H}]")
+    for t, n, what in ((y_routed, T * k * H, "y_routed"), (w, T * k, "w"), (y_shared, T * H, "y_shared"), (sgate, T, "sgate")):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"{what} must be {n} contiguous float32 values")
+    ptr = L.ptr
+    L.check(L.load().brx_mx_combine(C.byref(spec.c_desc), ptr(y_routed), ptr(w), ptr(y_shared), ptr(sgate), T,
+                                    out.data_ptr(), _handle(device)))

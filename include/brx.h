@@ -356,7 +356,7 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
 /* brx_moe_forward with MXFP4 activations, for layers of MXFP4 experts: x is rounded to MXFP4, the
  * activation is applied to the fp32 sums and its result h rounded to MXFP4 (once, from fp32), so
  *   y[t, j] = down(Q(act(gate(Q(x_t)), up(Q(x_t)))))
- * and out / y_unreduced as there. T at most 65535; x, out and y_unreduced 16-byte, workspace 256-byte aligned.
+ * and out / y_unreduced as there, but that out is the sum of the fp32 rows. T at most 65535; x, out and y_unreduced 16-byte, workspace 256-byte aligned.
  * Every output is the same bits whichever kernels run, so no flag is needed: FORCE_DECODE asks for the
  * two-launch kernels (at most 8 token rows and 64 pairs, BRX_EINVAL above), FORCE_PREFILL for the grouped
  * GEMM, any other flag is BRX_EINVAL. */
@@ -364,12 +364,17 @@ int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, cons
                        const float* w, const void* shared_expert, const float* shared_gate, int T,
                        void* out, void* y_unreduced, unsigned flags, void* workspace,
                        size_t workspace_bytes, void* stream);
-/* brx_moe_forward_pairs with MXFP4 activations (flags as in brx_mx_moe_forward). */
+/* brx_moe_forward_pairs with MXFP4 activations (flags as in brx_mx_moe_forward); y_rows in y_dtype,
+ * BRX_DT_BF16 or, for brx_mx_combine, BRX_DT_F32. */
 int brx_mx_moe_forward_pairs(const brx_layer_desc* d, brx_pool* p, const void* x, int T,
                              const int32_t* pair_token, const int32_t* pair_expert,
                              const int32_t* pair_row, int n_pairs, int n_rows,
-                             const void* shared_expert, void* y_rows, unsigned flags, void* workspace,
-                             size_t workspace_bytes, void* stream);
+                             const void* shared_expert, void* y_rows, int y_dtype, unsigned flags,
+                             void* workspace, size_t workspace_bytes, void* stream);
+/* brx_combine over fp32 rows: the sums brx_mx_moe_forward makes. y_routed [T, k, H], y_shared [T, H] or
+ * NULL, out [T, H] bf16, all 16-byte aligned. */
+int brx_mx_combine(const brx_layer_desc* d, const float* y_routed, const float* w, const float* y_shared,
+                   const float* shared_gate, int T, void* out, void* stream);
 
 /* The caller's router-weighted combine of unreduced rows (stream.py:1523-1525):
  *   out[t] = bf16( sum_j w[t, j] * y_routed[t, j]  (+ shared_gate[t] * y_shared[t]) )

@@ -128,8 +128,8 @@ def expert_rows(spec, blob, xq, shared=False):
 
 
 def layer(spec, experts, x, idx, w=None, shared=None, sgate=None):
-    """(y [T, k, H], bound, out [T, H] or None, bound): x float64 [T, H]. The bounds hold for kernels
-    that round y to bf16 before the weighted sum as for those that do not."""
+    """(y [T, k, H], bound, out [T, H] or None, bound): x float64 [T, H]. y is rounded to bf16, out is the
+    sum of the rows as they were before, rounded once."""
     T, k = idx.shape
     xq = held(x)
     y, dy = np.zeros((T, k, spec.hidden)), np.zeros((T, k, spec.hidden))
@@ -141,12 +141,12 @@ def layer(spec, experts, x, idx, w=None, shared=None, sgate=None):
         return y, dy16, None, None
     w = w.astype(np.float64)
     out = (w[..., None] * y).sum(1)
-    dout = (np.abs(w)[..., None] * dy16).sum(1)
+    dout = (np.abs(w)[..., None] * dy).sum(1)
     mag = (np.abs(w)[..., None] * np.abs(y)).sum(1)
     if shared is not None:
         s, ds = expert_rows(spec, shared, xq, True)
         sg = sgate.astype(np.float64)[:, None]
         out, mag = out + sg * s, mag + np.abs(sg * s)
-        dout = dout + np.abs(sg) * (ds + 2.0 ** -8 * (np.abs(s) + ds))
+        dout = dout + np.abs(sg) * ds
     dout = dout + (k + 2) * 2.0 ** -23 * mag
     return y, dy16, out, dout + 2.0 ** -8 * (np.abs(out) + dout)

@@ -543,12 +543,8 @@ def test_bounded_pool_and_host_served(gpu, T):
         s = StreamingSwitchGLU(p, PinnedFetcher(store), shared=sw.shared, host_served=host, activations="mxfp4")
         for _ in range(3):
             assert np.array_equal(bits(s(xd, idd)), want_rows)
-            got = bits(s.forward_combined(xd, idd, wd, sgd))
-            if host:
-                assert np.array_equal(got, want)
-            else:      # spans: y rounded to bf16 before the sum
-                _, _, ref, bound = O.layer(spec, lay.experts, f64(x), idx, w, lay.shared, sg)
-                close(f64(got), ref, bound, f"spans T={T}")
+            assert np.array_equal(bits(s.forward_combined(xd, idd, wd, sgd)), want)
+        assert host or s.chunked_calls > 0
         torch.cuda.synchronize()
         p.close()
 
@@ -608,6 +604,36 @@ def test_two_streams(gpu, T):
     for s in range(2):
         for g in got[s]:
             assert np.array_equal(bits(g), want[s])
+
+
+@pytest.mark.parametrize("name, T", [("shared", 1), ("shared", 33), ("clamped", 7), ("mlp", 70)])
+def test_combine_of_float32_rows(gpu, name, T):
+    """The pairs' float32 rows and their combine: the layer call's sums, bit for bit; rounded, its bf16 rows."""
+    import torch
+    spec, lay, sw, pool = built(name, gpu)
+    E, k, H = spec.n_experts, spec.top_k, spec.hidden
+    x, idx, w, sg = _layer_inputs(spec, lay, gpu, T, seed=80 + T)
+    xd, idd, wd = to_dev_bits(x, gpu), dev(idx, gpu), dev(w, gpu)
+    sgd = None if sg is None else dev(sg, gpu)
+    want = bits(mx.moe_forward(spec, pool, xd, idd, wd, shared=sw.shared, sgate=sgd))
+    tok = torch.arange(T, dtype=torch.int32, device=gpu)
+    for f in (0, L.FWD_FORCE_PREFILL):
+        y = torch.empty((T * k, H), device=gpu)
+        mx.forward_pairs(spec, pool, xd, tok.repeat_interleave(k), idd.view(-1), None, y, f)
+        ysh = None
+        if sw.shared is not None:
+            ysh = torch.empty((T, H), device=gpu)
+            mx.forward_pairs(spec, pool, xd, tok, torch.full_like(tok, E), None, ysh, f, shared=sw.shared)
+        out = torch.empty((T, H), dtype=torch.bfloat16, device=gpu)
+        mx.combine(spec, y, wd, out, ysh, sgd)
+        assert np.array_equal(bits(out), want)
+        assert np.array_equal(bits(y.bfloat16()), bits(mx.moe_forward(spec, pool, xd, idd)).reshape(T * k, H))
+    for kw, what in ((dict(y_routed=y.bfloat16()), "y_routed"), (dict(w=wd[:0]), "w must"), (dict(out=out.float()), "out"),
+                     (dict(y_shared=y[:0]), "y_shared"), (dict(sgate=wd.view(-1)[:0]), "sgate")):
+        with pytest.raises(ValueError, match=what):
+            mx.combine(**dict(dict(spec=spec, y_routed=y, w=wd, out=out), **kw))
+    with pytest.raises(L.BrxError, match="gate"):
+        mx.combine(spec, y, wd, out, torch.zeros((T, H), device=gpu))
 
 
 def test_a_given_stream_has_the_whole_call(gpu):
