@@ -4,8 +4,10 @@
 //   k_mx_gemm<0>  gate/up: A rows are the pairs' token rows, weight rows the gate and up rows of 32
 //                 features a wave; the epilogue applies act() in fp32 and rounds h to MXFP4 in place
 //                 (a wave holds whole groups), in bucketed order.
-//   k_mx_gemm<1>  down: A = h rows; + bias, each pair's bf16 row at its (token, k) position.
-//   k_mx_gemm<2>  one projection of the pairs' token rows (the expert product), stored as <1>.
+//   k_mx_gemm<1>  down: A = h rows; + bias, each pair's row at its (token, k) position in fp32 (for a sum), in
+//                 bf16 (unreduced rows), or both.
+//   k_mx_gemm<2>  one projection of the pairs' token rows (the expert product), in bf16.
+//   k_mx_combine  the routing-weighted sums of the fp32 rows.
 // The pairs are bucketed per expert and cut into M tiles by bucket.h: in k_mx_prepare, which rounds x beside it
 // (a layer), or in k_bucket (a product).
 //
@@ -14,9 +16,10 @@
 //
 // What bounds it. 512 tokens of the gpt-oss shape (16 pairs an expert, 1.70 GB of weights): the weight stream,
 // 227 + 123 us, 5.0 TB/s, where a copy of 1 GiB reaches 5.1. 2048 tokens of the Qwen3 shape under a Zipf law
-// (128 pairs an expert on average, 155 GFLOP): 89 + 66 us, 1000 TFLOP/s; matrix instructions fill 15% of
-// the time and vector ones half, and the rest is the wait for each chunk's weights: with 64 pairs a tile a wave
-// has 64 + 64 registers of sums and weights, and a second set of weights does not fit.
+// (128 pairs an expert on average, 155 GFLOP): 86 + 76 us, 950 TFLOP/s, and 21 us for the sums (135 MB, 6.4
+// TB/s); matrix instructions fill 15% of the time and vector ones half, and the rest is the wait for each chunk's
+// weights: with 64 pairs a tile a wave has 64 + 64 registers of sums and weights, and a second set of weights
+// does not fit.
 #include <type_traits>
 
 #include "bucket.h"

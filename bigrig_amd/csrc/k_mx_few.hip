@@ -10,9 +10,12 @@
 // expert's comes last. The arithmetic is k_mx_gemm's to the bit: the same 512-K chunks in the same order, the
 // same roundings.
 //
-// What bounds it: the weights are read once, and a wave requests the whole of its 16 rows (up to 6 chunks,
-// 24 KB) before it multiplies anything, so a call is a few dependent round trips -- the routing, the
-// table, the weights -- and little else.
+// What bounds it: the weights are read once, and a wave requests the whole of its 16 rows (up to 4 chunks,
+// 16 KB; wider rows three chunks at a time) before it multiplies anything, so a call is a few dependent round trips -- the routing, the
+// table, the weights -- and little else. One token of the gpt-oss shape (53 MB) takes 12.7 + 7.1 us (2.7
+// TB/s), 8 tokens of 256 experts and a shared one (59 MB) 15.8 + 8.8. The gate and up rows are split by
+// entry, the down rows are not (a block has every entry's 16 columns), so that the sum over a token's
+// experts is in one block's LDS and needs neither atomics nor a third launch.
 #include <type_traits>
 
 #include "mx_common.h"

@@ -699,6 +699,23 @@ def test_pairs_with_the_shared_expert(gpu, T):
     assert np.array_equal(f64(got[0][row[T * k:]]), f64(alone))
 
 
+@pytest.mark.parametrize("T", [3, 12, 150])
+def test_sums_and_rows_of_one_call(gpu, T):
+    """Both outputs at once, into tensors given: those of a call each."""
+    import torch
+    spec, lay, sw, pool = built("shared", gpu)
+    x, idx, w, sg = _layer_inputs(spec, lay, gpu, T, seed=33)
+    xd, idd, wd, sgd = to_dev_bits(x, gpu), dev(idx, gpu), dev(w, gpu), dev(sg, gpu)
+    kw = dict(shared=sw.shared, sgate=sgd)
+    out = torch.empty((T, spec.hidden), dtype=torch.bfloat16, device=gpu)
+    rows = torch.empty((T, spec.top_k, spec.hidden), dtype=torch.bfloat16, device=gpu)
+    assert mx.moe_forward(spec, pool, xd, idd, wd, out=out, y_unreduced=rows, **kw) is out
+    assert np.array_equal(bits(out), bits(mx.moe_forward(spec, pool, xd, idd, wd, **kw)))
+    assert np.array_equal(bits(rows), bits(mx.moe_forward(spec, pool, xd, idd)))
+    with pytest.raises(ValueError, match="y_rows"):
+        mx.forward_pairs(spec, pool, xd, idd.view(-1)[:T], idd.view(-1)[:T], None, rows[:, 0].half().contiguous(), 0)
+
+
 @pytest.mark.parametrize("T", [1, 8, 30])
 def test_captured_graphs(gpu, T):
     """Two captured layers (rows quantised and read back beside them), replayed in turn and with eager
