@@ -316,7 +316,8 @@ int brx_moe_block_forward_noalloc(const brx_layer_desc* d, brx_pool* p, const vo
  * holds a NaN or an infinity gets scale byte 255 and zero codes: it reads as NaN, and so does every
  * product it enters. None of these calls uses the library workspace: scratch comes from the caller,
  * so calls on several streams and captured graphs do not meet as long as their scratch does not. (A
- * pool's refills wait for the last call issued on it: the calls of a pool under refill go to one stream.) */
+ * pool's refills wait for the last call issued on it: the calls of a pool under refill go to one stream.
+ * The stream of a pool's last call has to outlive the pool's next refill, sync or check.) */
 
 /* Round `batch` matrices of rows x cols values to MXFP4.
  *   x       device, BRX_DT_* values; matrix b's row r starts x_batch_stride * b + x_row_stride * r

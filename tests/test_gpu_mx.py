@@ -9,6 +9,7 @@ from bigrig_amd import formats as F
 from bigrig_amd import lib as L
 from bigrig_amd import mx
 from bigrig_amd.layer import MoELayer, StreamingSwitchGLU
+from bigrig_amd.layer import moe_forward as _bf16_forward
 from bigrig_amd.pool import ExpertPool, HostStore, PinnedFetcher
 from bigrig_amd.spec import E256_SHARED, GPT_OSS_120B, OLMOE_1B_7B, QWEN3_30B_A3B
 from tests import mx_oracle as O
@@ -66,6 +67,14 @@ def built(name, gpu):
         pool.g2s_device(torch.cuda.current_stream().cuda_stream)
         _LAYERS[name] = (lay.spec, lay, sw, pool)
     return _LAYERS[name]
+
+
+def layer_forward(spec, pool, x, idx, w):
+    """The layer with bf16 activations."""
+    import torch
+    out = torch.empty((x.shape[0], spec.hidden), dtype=torch.bfloat16, device=x.device)
+    _bf16_forward(spec, pool, x, idx, w, out=out)
+    return out
 
 
 def close(got, want, bound, what):
@@ -697,6 +706,50 @@ def test_pairs_with_the_shared_expert(gpu, T):
     zero, one = torch.zeros((T, k), device=gpu), torch.ones(T, device=gpu)
     alone = bits(mx.moe_forward(spec, pool, xd, dev(idx, gpu), zero, shared=sw.shared, sgate=one))
     assert np.array_equal(f64(got[0][row[T * k:]]), f64(alone))
+
+
+@pytest.mark.parametrize("T", [2, 40])
+def test_refill_waits_for_a_resident_pools_calls(gpu, T):
+    """A slot is refilled behind a queued call that reads it, on a copy stream; the pool's sync waits for the
+    call; a bf16 forward and an MXFP4 call on two streams are both waited for."""
+    import torch
+    lay = make_layer(SWIGLU, seed=77, expert_std=0.05)
+    _, sw, pool, _ = build_gpu_layer(lay, gpu)
+    spec, lib, h = lay.spec, L.load(), pool.device.handle
+    pool.g2s_device(torch.cuda.current_stream().cuda_stream)
+    x, idx, w, _ = _layer_inputs(spec, lay, gpu, T, seed=61)
+    xd, idd, wd = to_dev_bits(x, gpu), dev(idx, gpu), dev(w, gpu)
+    old = bits(mx.moe_forward(spec, pool, xd, idd, wd))
+    plain = bits(layer_forward(spec, pool, xd, idd, wd))
+    blobs = [bytes_dev(b, gpu) for b in lay.experts]
+    slots = pool.g2s
+    torch.cuda.synchronize()
+    run, other, copy = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.Stream()
+    for both in (False, True):
+        with torch.cuda.stream(other):
+            if both:
+                torch.cuda._sleep(40_000_000)
+                p16 = layer_forward(spec, pool, xd, idd, wd)
+        with torch.cuda.stream(run):
+            torch.cuda._sleep(20_000_000)
+            got = mx.moe_forward(spec, pool, xd, idd, wd)
+        for e in range(spec.n_experts):      # every expert's slot takes the next expert's bytes
+            b = blobs[(e + 1) % spec.n_experts]
+            L.check(lib.brx_pool_refill_from_device_async(h, int(slots[e]), b.data_ptr(), b.numel(), copy.cuda_stream))
+        torch.cuda.synchronize()
+        assert np.array_equal(bits(got), old)
+        assert not both or np.array_equal(bits(p16), plain)
+        assert not np.array_equal(bits(mx.moe_forward(spec, pool, xd, idd, wd)), old)
+        for e in range(spec.n_experts):
+            L.check(lib.brx_pool_refill_from_device_async(h, int(slots[e]), blobs[e].data_ptr(), blobs[e].numel(), copy.cuda_stream))
+        assert np.array_equal(bits(mx.moe_forward(spec, pool, xd, idd, wd)), old)
+    with torch.cuda.stream(run):
+        torch.cuda._sleep(20_000_000)
+        mx.moe_forward(spec, pool, xd, idd, wd)
+    L.check(lib.brx_pool_sync(h))
+    assert run.query()
+    pool.device.check()
+    pool.close()
 
 
 @pytest.mark.parametrize("T", [3, 12, 150])
