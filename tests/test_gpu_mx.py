@@ -188,6 +188,20 @@ def test_strided_and_misaligned_rows(gpu, kind):
         mx.quantize(t.double())
 
 
+def test_offsets_past_32_bits(gpu):
+    """4.6 G values (one row again and again, by a row stride of zero): every row is the first one's."""
+    import torch
+    row = to_dev_bits(acts(1, 65536, 12), gpu)
+    q = mx.quantize(row.expand(70000, 65536))
+    one = mx.quantize(row)
+    assert torch.equal(q.codes[0], one.codes[0]) and torch.equal(q.scales[0], one.scales[0])
+    for at in range(0, 70000, 10000):
+        assert bool((q.codes[at:at + 10000] == one.codes).all()) and bool((q.scales[at:at + 10000] == one.scales).all())
+    back, want = mx.dequantize(q), mx.dequantize(one)
+    for at in range(0, 70000, 10000):
+        assert bool((back[at:at + 10000] == want).all())
+
+
 @pytest.mark.parametrize("name", ["clamped", "mlp", "swiglu", "shared"])
 def test_pack_experts(gpu, name):
     import torch
