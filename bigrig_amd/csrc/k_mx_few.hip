@@ -42,6 +42,7 @@ struct MxTable {
 struct MxPlan {
     int e, slot, n, pair, entries;
 };
+constexpr int kIdBits = 10;                        // expert ids, the shared one's among them, are at most 512
 constexpr int kSlotRegs = 8;                       // the slot table of up to 512 experts, 64 a register
 __device__ __forceinline__ bool mx_plan(const FwdArgs& a, int u, int32_t* s_pair, MxPlan& o) {
     const int lane = threadIdx.x & 63;
@@ -52,12 +53,12 @@ __device__ __forceinline__ bool mx_plan(const FwdArgs& a, int u, int32_t* s_pair
 #pragma unroll
     for (int i = 0; i < kSlotRegs; ++i) slots[i] = 64 * i < a.E ? a.g2s[min(lane + 64 * i, a.E - 1)] : 0;
     const int e = lane < P ? min(max(raw, 0), emax) : -1 - lane;
-    uint64_t same = 0;
-    for (uint64_t rest = __ballot(lane < P); rest;) {      // one round an expert of the step
-        const int v = __builtin_amdgcn_readlane(e, __builtin_ctzll(rest));
-        const uint64_t b = __ballot(e == v);
-        if (e == v) same = b;
-        rest &= ~b;
+    // the pairs of a lane's expert, an id bit at a time
+    uint64_t same = __ballot(lane < P);
+#pragma unroll
+    for (int i = 0; i < kIdBits; ++i) {
+        const uint64_t one = __ballot((e >> i) & 1);
+        same &= (e >> i) & 1 ? one : ~one;
     }
     const uint64_t below = (1ull << lane) - 1ull;
     const int rank = __popcll(same & below);
