@@ -897,7 +897,7 @@ static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T
     FwdArgs a = make_args(d, p, x, T, P, pexp, ptok, prow, yrows, w, shared_expert, shared_gate, out, y_rows);
     hipStream_t s = (hipStream_t)stream;
     const MxPath path = flags & BRX_FWD_FORCE_PREFILL ? kMxMany : mx_path(a);
-    if ((flags & BRX_FWD_FORCE_DECODE) && path != kMxFew)
+    if ((flags & BRX_FWD_FORCE_DECODE) && (T > 8 || P > 64))
         return fail(BRX_EINVAL, "the decode path takes at most 8 token rows and 64 pairs (T=%d, P=%d)", T, P);
     const int rc = mx_begin(p, mx_workspace_bytes(a, true, path), workspace, workspace_bytes, s);
     if (rc) return rc;

@@ -491,14 +491,16 @@ hipError_t prepare(const FwdArgs& a, const MxWs& w, hipStream_t s) {
 
 // The few-pair kernels have a block for every run of an expert's rows: they win while launches and round trips
 // set the time. The line past 8 tokens is the pairs times an expert's bytes (what the pairs could read), these
-// kernels against the grouped GEMM, three layers in turn: 2048 x 768, top-8, 9 tokens (180 MB) 36.8 / 38.9 us, 12
-// (241 MB) 41.5 / 42.8, 16 (321 MB) 45.6 / 45.4; 2048 x 512, 256 experts and a shared one, 16 tokens (214 MB)
-// 39.5 / 40.2, 24 (321 MB) 46.2 / 46.1; 2048 x 1024, top-8, 9 tokens (241 MB) 48.4 / 47.3; a 1024 x 256 MLP, 33 tokens
-// (19 MB) 16.5 / 17.8. Up to 8 tokens they lose only past that: 2880 x 2880, top-4, 7 tokens (371 MB) 92.2 / 95.5, 8
-// (424 MB) 103.3 / 99.8.
+// kernels against the grouped GEMM, three layers in turn: 2048 x 768, top-8, 9 tokens (180 MB) 34.8 / 38.0 us, 12
+// (241 MB) 38.8 / 41.8, 24 (477 MB) 44.0 / 44.0; 2048 x 512, 256 experts and a shared one, 12 tokens (160 MB) 31.9 /
+// 33.3, 16 (214 MB) 40.4 / 40.2; 2048 x 1024, top-8, 9 tokens (241 MB) 47.3 / 47.2; a 1024 x 256 MLP, 33 tokens (19
+// MB) 14.2 / 18.0. Up to 8 tokens they lose only past that: 2880 x 2880, top-4, 7 tokens (371 MB) 92.2 / 95.5, 8
+// (424 MB) 103.3 / 99.8. Up to 128 pairs every block plans the step (bucketed first: the MLP 16.2, 12 tokens of 2048
+// x 768 40.8).
 MxPath mx_path(const FwdArgs& a) {
     if (a.T <= kMxFewTokens && a.P <= kMxFewPairs) return kMxFew;
-    return a.T <= kMxMidTokens && a.P <= kMxMidPairs && a.P * a.lay.bytes <= 260 * 1000 * 1000 ? kMxMid : kMxMany;
+    if (a.T > kMxMidTokens || a.P > kMxMidPairs || a.P * a.lay.bytes > 260 * 1000 * 1000) return kMxMany;
+    return a.P <= kMxPlanPairs ? kMxFew : kMxMid;
 }
 
 size_t mx_workspace_bytes(const FwdArgs& a, bool layer, MxPath path) {

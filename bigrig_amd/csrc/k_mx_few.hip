@@ -44,41 +44,79 @@ struct MxPlan {
 };
 constexpr int kIdBits = 10;                        // expert ids, the shared one's among them, are at most 512
 constexpr int kSlotRegs = 8;                       // the slot table of up to 512 experts, 64 a register
+template <int R>                                   // pairs a lane: up to 64 R in all
 __device__ __forceinline__ bool mx_plan(const FwdArgs& a, int u, int32_t* s_pair, MxPlan& o) {
     const int lane = threadIdx.x & 63;
     const int P = a.P, emax = a.shared ? a.E : a.E - 1;
     // the slot table comes with the routing, not a round trip after it
-    const int raw = a.pexp[min(lane, P - 1)];
+    int e[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) e[r] = a.pexp[min(lane + 64 * r, P - 1)];
     int slots[kSlotRegs];
 #pragma unroll
     for (int i = 0; i < kSlotRegs; ++i) slots[i] = 64 * i < a.E ? a.g2s[min(lane + 64 * i, a.E - 1)] : 0;
-    const int e = lane < P ? min(max(raw, 0), emax) : -1 - lane;
-    // the pairs of a lane's expert, an id bit at a time
-    uint64_t same = __ballot(lane < P);
+    // same[r][c]: the pairs of register c that have the expert of the lane's pair r, found an id bit at a time
+    uint64_t same[R][R], live[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        e[r] = min(max(e[r], 0), emax);
+        live[r] = __ballot(lane + 64 * r < P);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < R; ++c) same[r][c] = live[c];
 #pragma unroll
     for (int i = 0; i < kIdBits; ++i) {
-        const uint64_t one = __ballot((e >> i) & 1);
-        same &= (e >> i) & 1 ? one : ~one;
+        uint64_t one[R];
+#pragma unroll
+        for (int c = 0; c < R; ++c) one[c] = __ballot((e[c] >> i) & 1);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < R; ++c) same[r][c] &= (e[r] >> i) & 1 ? one[c] : ~one[c];
     }
+    // an expert's 1st, 17th, .. pair leads an entry
     const uint64_t below = (1ull << lane) - 1ull;
-    const int rank = __popcll(same & below);
-    const uint64_t leads = __ballot(lane < P && (rank & 15) == 0);
-    const int routed = __popcll(leads);
-    o.entries = routed + (a.auto_shared ? 1 : 0);
+    int rank[R];
+    uint64_t leads[R];
+    int routed = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        rank[r] = __popcll(same[r][r] & below);
+#pragma unroll
+        for (int c = 0; c < r; ++c) rank[r] += __popcll(same[r][c]);
+        leads[r] = __ballot(lane + 64 * r < P && (rank[r] & 15) == 0);
+        routed += __popcll(leads[r]);
+    }
+    o.entries = routed + (a.auto_shared ? (a.T + 15) / 16 : 0);
     if (u >= o.entries) return false;
-    if (u == routed) {                             // every token of the shared expert (at most 8)
+    if (u >= routed) {                             // 16 tokens of the shared expert
+        const int t0 = 16 * (u - routed);
         o.e = a.E;
         o.slot = -1;
-        o.n = a.T;
-        o.pair = P + min(lane & 15, a.T - 1);
+        o.n = min(16, a.T - t0);
+        o.pair = P + t0 + min(lane & 15, o.n - 1);
         return true;
     }
-    const int lead = __builtin_ctzll(__ballot(((leads >> lane) & 1) && __popcll(leads & below) == u));
-    o.e = __builtin_amdgcn_readlane(e, lead);
-    const int r0 = __builtin_amdgcn_readlane(rank, lead);
-    const bool in = e == o.e && rank >= r0 && rank < r0 + 16;
-    o.n = __popcll(__ballot(in));
-    if (in) s_pair[rank - r0] = lane;              // (the wave's own words)
+    int r0 = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int n = __popcll(leads[r]);
+        if (u >= 0 && u < n) {                     // uniform
+            const int lead = __builtin_ctzll(__ballot(((leads[r] >> lane) & 1) && __popcll(leads[r] & below) == u));
+            o.e = __builtin_amdgcn_readlane(e[r], lead);
+            r0 = __builtin_amdgcn_readlane(rank[r], lead);
+        }
+        u -= n;
+    }
+    o.n = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const bool in = lane + 64 * r < P && e[r] == o.e && rank[r] >= r0 && rank[r] < r0 + 16;
+        o.n += __popcll(__ballot(in));
+        if (in) s_pair[rank[r] - r0] = lane + 64 * r;      // (the wave's own words)
+    }
     __builtin_amdgcn_wave_barrier();
     o.pair = s_pair[min(lane & 15, o.n - 1)];
     int v = 0;
@@ -135,8 +173,9 @@ __device__ __forceinline__ void few_mul(mx_u32x4 (&w)[4], uint32_t s, int ch, in
 __host__ __device__ inline int few_code_pitch(int nch) { return nch * 256 + 16; }
 __host__ __device__ inline int few_scale_pitch(int nch) { return nch * 16 + 4; }
 
-// TILES: the entries are the tiles of 16 pairs that k_bucket made; else every block plans the step itself.
-template <int NB, bool TILES>
+// R = 0: the entries are the tiles of 16 pairs that k_bucket made; else every block plans the step itself, R pairs
+// a lane.
+template <int NB, int R>
 __global__ __launch_bounds__(64 * kUpWaves) void k_mx_few_up(FwdArgs a, MxArgs m, MxTable* __restrict__ table) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ __attribute__((aligned(16))) f32x4_t red[4][64];
@@ -147,7 +186,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_mx_few_up(FwdArgs a, MxArgs m
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, l16 = lane & 15;
     MxPlan pl;
-    if constexpr (TILES) {
+    if constexpr (R == 0) {
         const int u = blockIdx.y;
         pl.entries = m.tile_start[m.E_ext];
         const int4 ti = m.tinfo[u];                // (the list is at least as long as the grid)
@@ -156,7 +195,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_mx_few_up(FwdArgs a, MxArgs m
         pl.n = __builtin_amdgcn_readfirstlane(ti.z);
         pl.slot = pl.e >= a.E ? -1 : __builtin_amdgcn_readfirstlane(ti.w);
         pl.pair = m.order[ti.y + min(lane & 15, pl.n - 1)];
-    } else if (!mx_plan(a, blockIdx.y, s_pair[wv], pl)) {
+    } else if (!mx_plan<R>(a, blockIdx.y, s_pair[wv], pl)) {
         return;
     }
     const bool gated = a.act != BRX_ACT_SILU_MLP, sh = pl.e >= a.E;
@@ -317,7 +356,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_mx_few_rows(FwdArgs a, MxArg
         for (int v = 0; v < NE; ++v) entry(wv + kRowWaves * v, pl[v]);
         entries = __builtin_amdgcn_readfirstlane(entries);
     } else {
-        if (!mx_plan(a, blockIdx.y * kRowWaves + wv, s_pair[wv], pl[0])) return;
+        if (!mx_plan<1>(a, blockIdx.y * kRowWaves + wv, s_pair[wv], pl[0])) return;
     }
     for (int u0 = DOWN ? wv : 0; u0 < entries; u0 += kRowWaves * NE) {
         FewW<NB> q[NE];
@@ -448,7 +487,7 @@ struct FewWs {
     uint8_t *hq, *hs;
     int32_t *order, *offsets, *tile_start;         // tiles only
     int4* tinfo;
-    int Imax, tiles;                               // at most so many tiles
+    int Imax, tiles;                               // at most so many tiles (entries)
     size_t bytes;
 };
 FewWs carve_few(const FwdArgs& a, bool tiles, void* ws) {
@@ -456,7 +495,7 @@ FewWs carve_few(const FwdArgs& a, bool tiles, void* ws) {
     w.Imax = a.shared && a.I_sh > a.I ? a.I_sh : a.I;
     const int rows = a.P + (a.auto_shared ? a.T : 0), E_ext = a.E + (a.shared ? 1 : 0);
     w.tiles = rows / 16 + (E_ext < rows ? E_ext : rows);
-    if (w.tiles > rows) w.tiles = rows;
+    if (w.tiles > rows) w.tiles = rows;            // (an entry has a pair)
     uint8_t* b = reinterpret_cast<uint8_t*>(ws);
     size_t off = 0;
     auto take = [&](size_t n) { uint8_t* p = b + off; off = align256(off + n); return p; };
@@ -501,11 +540,12 @@ hipError_t launch_mx_few_layer(const FwdArgs& a, bool tiles, float* rows32, void
     const int per = a.act == BRX_ACT_SILU_MLP ? 64 : 32, nch = (a.H + 511) / 512;
     int most = a.P < 16 ? a.P : 16;                // pairs of an entry, at most
     if (a.auto_shared && a.T > most) most = a.T < 16 ? a.T : 16;
-    const dim3 grid((w.Imax + per - 1) / per, tiles ? w.tiles : a.P + (a.auto_shared ? 1 : 0));
+    const dim3 grid((w.Imax + per - 1) / per, w.tiles);
     const size_t lds = (size_t)most * (few_code_pitch(nch) + few_scale_pitch(nch));
 #define BRX_UP(NB) \
-    if (tiles) hipLaunchKernelGGL((k_mx_few_up<NB, true>), grid, dim3(64 * kUpWaves), lds, s, a, m, w.table); \
-    else hipLaunchKernelGGL((k_mx_few_up<NB, false>), grid, dim3(64 * kUpWaves), lds, s, a, m, w.table)
+    if (tiles) hipLaunchKernelGGL((k_mx_few_up<NB, 0>), grid, dim3(64 * kUpWaves), lds, s, a, m, w.table); \
+    else if (a.P > 64) hipLaunchKernelGGL((k_mx_few_up<NB, 2>), grid, dim3(64 * kUpWaves), lds, s, a, m, w.table); \
+    else hipLaunchKernelGGL((k_mx_few_up<NB, 1>), grid, dim3(64 * kUpWaves), lds, s, a, m, w.table)
     switch (few_batch(a.H)) {
         case 1: BRX_UP(1); break;
         case 2: BRX_UP(2); break;

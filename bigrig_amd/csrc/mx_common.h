@@ -20,9 +20,10 @@
 
 namespace brx {
 
-// Most tokens and (token, expert) pairs of a step that every block of the few-pair kernels plans itself (one
-// wave, a pair a lane), and of one that is bucketed for them first.
+// Most tokens and (token, expert) pairs of a step that always runs on the few-pair kernels; of one that may, and
+// whose blocks plan it themselves (a pair or two a lane) or have it bucketed first.
 constexpr int kMxFewTokens = 8, kMxFewPairs = 64;
+constexpr int kMxPlanPairs = 128;
 constexpr int kMxMidTokens = 64, kMxMidPairs = 256;
 
 // What the GEMM launches take beside the forward's arguments (FwdArgs::x is unused).

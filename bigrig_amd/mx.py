@@ -319,9 +319,9 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
     projections' activations in MXFP4. With weights w [T, k] (fp32): out [T, H] = sum_j w[t, j] *
     y[t, j] (+ sgate[t] * shared(x_t)) over the float32 rows y; without: the unreduced rows [T, k, H] in
     bfloat16. The pool's table must
-    be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`. Up to 8 tokens and 64 pairs run
-    as two launches, some more as three and the rest as the grouped GEMM; the outputs are the same bits
-    (`flags`: BRX_FWD_FORCE_DECODE or BRX_FWD_FORCE_PREFILL for the first or the last of these)."""
+    be uploaded (`ExpertPool.g2s_device`), as for `layer.moe_forward`. Few pairs run
+    as two or three launches, the rest as the grouped GEMM; the outputs are the same bits (`flags`:
+    BRX_FWD_FORCE_DECODE for the first, up to 8 tokens and 64 pairs, BRX_FWD_FORCE_PREFILL for the last)."""
     if stream is not None:
         return _on(stream, moe_forward, spec, pool, x, idx, w, shared, sgate, out, y_unreduced, flags)
     _check_spec(spec)
