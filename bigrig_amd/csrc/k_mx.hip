@@ -536,7 +536,12 @@ hipError_t launch_mx_layer(const FwdArgs& a, MxPath path, float* rows32, void* w
 
 hipError_t launch_mx_product(const FwdArgs& a, const uint8_t* codes, const uint8_t* scales, int proj, void* ws,
                              hipStream_t s) {
-    if (a.P <= kMxFewPairs) return launch_mx_few_product(a, codes, scales, proj, s);
+    // Past 64 pairs the one launch wins while the pairs' projections are at most so many bytes (against the two):
+    // 2048 x 768, 72 pairs (60 MB) 13.5 / 15.9 us, 96 (80 MB) 16.2 / 16.3, 128 (107 MB) 17.3 / 16.9; 2048 x 512, 72
+    // pairs of 256 experts (40 MB) 10.0 / 15.3, 128 (71 MB) 14.5 / 16.4; 1024 x 256, 128 (18 MB) 5.7 / 10.2; 2880 x
+    // 2880, 68 (300 MB) 62.4 / 59.1.
+    if (a.P <= kMxFewPairs || (a.P <= kMxPlanPairs && (int64_t)a.P * a.I * a.H / 32 * 17 <= 75 * 1000 * 1000))
+        return launch_mx_few_product(a, codes, scales, proj, s);
     const MxWs w = carve(a, false, ws);
     hipError_t e = bucket(a, w, s);
     if (e != hipSuccess) return e;

@@ -331,8 +331,8 @@ __global__ __launch_bounds__(64 * kUpWaves) void k_mx_few_up(FwdArgs a, MxArgs m
 }
 
 // DOWN: the second launch of a layer, over the entry table, NE entries of NB chunks a wave at once; else one
-// projection's rows.
-template <bool DOWN, int NB, int NE>
+// projection's rows of a list that every block plans, R pairs a lane.
+template <bool DOWN, int NB, int NE, int R = 1>
 __global__ __launch_bounds__(64 * kRowWaves) void k_mx_few_rows(FwdArgs a, MxArgs m, const MxTable* __restrict__ table) {
     __shared__ __attribute__((aligned(16))) float ys[DOWN ? kMxMidPairs + kMxMidTokens : 1][16];
     __shared__ int32_t s_pair[kRowWaves][16];
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void k_mx_few_rows(FwdArgs a, MxArg
         for (int v = 0; v < NE; ++v) entry(wv + kRowWaves * v, pl[v]);
         entries = __builtin_amdgcn_readfirstlane(entries);
     } else {
-        if (!mx_plan<1>(a, blockIdx.y * kRowWaves + wv, s_pair[wv], pl[0])) return;
+        if (!mx_plan<R>(a, blockIdx.y * kRowWaves + wv, s_pair[wv], pl[0])) return;
     }
     for (int u0 = DOWN ? wv : 0; u0 < entries; u0 += kRowWaves * NE) {
         FewW<NB> q[NE];
@@ -573,8 +573,11 @@ hipError_t launch_mx_few_product(const FwdArgs& a, const uint8_t* codes, const u
     m.xs = scales;
     m.y16 = a.yun;
     m.proj = proj;
-    const dim3 grid((proj == 2 ? a.H : a.I) / 16, (a.P + kRowWaves - 1) / kRowWaves);
-#define BRX_ROWS(NB) hipLaunchKernelGGL((k_mx_few_rows<false, NB, 1>), grid, dim3(64 * kRowWaves), 0, s, a, m, (const MxTable*)nullptr)
+    const int most = a.P / 16 + (a.E + 1 < a.P ? a.E + 1 : a.P), entries = most < a.P ? most : a.P;   // at most
+    const dim3 grid((proj == 2 ? a.H : a.I) / 16, (entries + kRowWaves - 1) / kRowWaves);
+#define BRX_ROWS(NB) \
+    if (a.P > 64) hipLaunchKernelGGL((k_mx_few_rows<false, NB, 1, 2>), grid, dim3(64 * kRowWaves), 0, s, a, m, (const MxTable*)nullptr); \
+    else hipLaunchKernelGGL((k_mx_few_rows<false, NB, 1, 1>), grid, dim3(64 * kRowWaves), 0, s, a, m, (const MxTable*)nullptr)
     switch (few_batch(proj == 2 ? a.I : a.H)) { case 1: BRX_ROWS(1); break; case 2: BRX_ROWS(2); break; case 4: BRX_ROWS(4); break; default: BRX_ROWS(3); }
 #undef BRX_ROWS
     return hipGetLastError();

@@ -270,8 +270,8 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
     "up_proj", "down_proj"; "fc1", "fc2"), bf16 [n_pairs, n_out]. q: the activations [T, n_in];
     pair_token and pair_expert int32 [n_pairs] (entries outside are clamped, as in the layer's pair
     lists). With `out` [n_rows, n_out] and pair_row (distinct rows), row pair_row[i] is written and
-    the others are left as they are. Up to 64 pairs run as one launch, more as two and with scratch;
-    the rows are the same bits."""
+    the others are left as they are. Up to 64 pairs run as one launch and without scratch, more
+    as one or two; the rows are the same bits."""
     if stream is not None:
         return _on(stream, expert_product, spec, pool, q, pair_token, pair_expert, proj, pair_row, out)
     _check_spec(spec)

@@ -473,10 +473,10 @@ def test_every_kernel_family_gives_the_same_bits(gpu, name, T):
 @pytest.mark.parametrize("name, proj", [("swiglu", "down_proj"), ("clamped", "gate_proj"), ("mlp", "fc1"), ("wide", "up_proj"),
                                         ("long", "down_proj")])
 def test_short_and_long_lists_give_the_same_bits(gpu, name, proj):
-    spec, pool, q, tok, ex, _, _ = _product(gpu, name, proj, 11, 80, seed=6)
+    spec, pool, q, tok, ex, _, _ = _product(gpu, name, proj, 11, 200, seed=6)
     t, e = dev(tok, gpu), dev(ex, gpu)
     want = bits(mx.expert_product(spec, pool, q, t, e, proj))
-    for a, b in ((0, 64), (3, 4), (10, 47)):
+    for a, b in ((0, 64), (3, 4), (10, 47), (0, 65), (72, 200)):
         got = bits(mx.expert_product(spec, pool, q, t[a:b].contiguous(), e[a:b].contiguous(), proj))
         assert np.array_equal(got, want[a:b])
 
