@@ -540,7 +540,10 @@ hipError_t launch_mx_few_layer(const FwdArgs& a, bool tiles, float* rows32, void
     const int per = a.act == BRX_ACT_SILU_MLP ? 64 : 32, nch = (a.H + 511) / 512;
     int most = a.P < 16 ? a.P : 16;                // pairs of an entry, at most
     if (a.auto_shared && a.T > most) most = a.T < 16 ? a.T : 16;
-    const dim3 grid((w.Imax + per - 1) / per, w.tiles);
+    // planned by the blocks: the entries of the routed pairs, and of the shared expert
+    const int routed = a.P / 16 + a.E + (a.shared ? 1 : 0);
+    const int planned = (routed < a.P ? routed : a.P) + (a.auto_shared ? (a.T + 15) / 16 : 0);
+    const dim3 grid((w.Imax + per - 1) / per, tiles ? w.tiles : planned);
     const size_t lds = (size_t)most * (few_code_pitch(nch) + few_scale_pitch(nch));
 #define BRX_UP(NB) \
     if (tiles) hipLaunchKernelGGL((k_mx_few_up<NB, 0>), grid, dim3(64 * kUpWaves), lds, s, a, m, w.table); \
