@@ -790,6 +790,13 @@ static int check_mx_desc(const brx_layer_desc* d) {
     return BRX_OK;
 }
 
+// Activation rows are addressed by 32-bit offsets of their codes (k_mx.hip): T rows of `cols` values.
+static int check_mx_rows(int T, int64_t cols) {
+    if ((int64_t)T * (cols / 2) >= (int64_t)0xFFFFFF00)
+        return fail(BRX_EINVAL, "%d rows of %lld values: codes of less than 2^32 - 256 bytes", T, (long long)cols);
+    return BRX_OK;
+}
+
 static int check_mx_sizes(int T, int64_t n_pairs, bool shared) {
     if (T < 0 || n_pairs < 0) return fail(BRX_EINVAL, "negative size (T=%d, n_pairs=%lld)", T, (long long)n_pairs);
     if (n_pairs + (shared ? T : 0) > kMxMaxPairs)
@@ -803,6 +810,7 @@ int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int 
     if (!out) return fail(BRX_EINVAL, "out is NULL");
     if (shared && !d->shared_inter) return fail(BRX_EINVAL, "layer descriptor has no shared expert");
     if ((rc = check_mx_sizes(T, n_pairs, shared != 0))) return rc;
+    if (!product && n_pairs && (rc = check_mx_rows(T, d->hidden))) return rc;
     // a layer call and the pairs form (whose shared pairs are among n_pairs) share the count
     brx_pool none{};
     none.d = *d;
@@ -873,8 +881,7 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
     if (!codes || !scales) return fail(BRX_EINVAL, "codes and scales are required");
     if (((uintptr_t)codes & 15) || ((uintptr_t)scales & 1)) return fail(BRX_EINVAL, "codes must be 16-byte, scales 2-byte aligned");
     if ((rc = check_pairs(T, n_pairs, n_rows, pair_token, pair_expert, pair_row, y_rows))) return rc;
-    const int64_t k_in = proj == 2 ? d->inter : d->hidden;
-    if ((int64_t)T * (k_in / 2) >= (int64_t)0xFFFFFF00) return fail(BRX_EINVAL, "%d rows of %lld values: codes of at most 4 GB", T, (long long)k_in);
+    if ((rc = check_mx_rows(T, proj == 2 ? d->inter : d->hidden))) return rc;
     FwdArgs a = make_args(d, p, nullptr, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, nullptr, nullptr,
                           nullptr, y_rows);
     hipStream_t s = (hipStream_t)stream;
@@ -930,6 +937,7 @@ int brx_mx_moe_forward_pairs(const brx_layer_desc* d, brx_pool* p, const void* x
     if ((rc = check_mx_sizes(T, n_pairs, false))) return rc;
     if (y_dtype != BRX_DT_BF16 && y_dtype != BRX_DT_F32) return fail(BRX_EINVAL, "y_dtype %d: rows are bf16 or fp32", y_dtype);
     if (n_pairs == 0) return BRX_OK;
+    if ((rc = check_mx_rows(T, d->hidden))) return rc;
     const bool wide = y_dtype == BRX_DT_F32;
     if ((rc = check_pairs(T, n_pairs, n_rows, pair_token, pair_expert, pair_row, y_rows))) return rc;
     return mx_forward(d, p, x, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, shared_expert, nullptr,

@@ -37,7 +37,8 @@ from .pool import ExpertPool
 from .spec import LayerSpec
 
 MAX_TOKENS = 65535      # token rows of one layer call
-MAX_PAIRS = 1 << 21     # (token, expert) pairs of one call
+MAX_PAIRS = 1 << 21     # (token, expert) pairs of one call (a layer's shared ones too)
+MAX_CODES = (1 << 32) - 257   # bytes of the codes of one call's activations
 FEW_PAIRS = 64          # pairs an expert product runs without scratch
 
 
@@ -239,6 +240,14 @@ def _check_spec(spec: LayerSpec) -> None:
         raise ValueError(f"MXFP4 activations need MXFP4 experts, the layer's are {spec.quant.mode}")
 
 
+def _check_sizes(T: int, n: int, width: int) -> None:
+    """T activation rows of `width` values, n pairs: what the kernels' 32-bit counts and offsets hold."""
+    if n > MAX_PAIRS:
+        raise ValueError(f"{n} pairs in one call: at most {MAX_PAIRS}")
+    if n and T * (width // 2) > MAX_CODES:
+        raise ValueError(f"{T} rows of {width} values in one call: at most {MAX_CODES // (width // 2)}")
+
+
 def _index(t, n: int, what: str):
     if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous int32 tensor of {n} entries, got "
@@ -281,8 +290,9 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
     n_out, n_in = (spec.hidden, spec.inter) if j == 2 else (spec.inter, spec.hidden)
     codes, scales = q
     n = pair_expert.numel()
-    device = _on_device(codes, scales, pair_token, pair_expert, pair_row, out)
     T = codes.shape[0] if codes.dim() else 0
+    _check_sizes(T, n, n_in)
+    device = _on_device(codes, scales, pair_token, pair_expert, pair_row, out)
     if codes.shape != (T, n_in // 2) or scales.shape != (T, n_in // 32):
         raise ValueError(f"activations {tuple(codes.shape)} / {tuple(scales.shape)}: {proj} takes rows "
                          f"of {n_in} values")
@@ -327,6 +337,9 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
     _check_spec(spec)
     x2 = _rows_of(spec, x)
     T, H, k = x2.shape[0], spec.hidden, spec.top_k
+    if T > MAX_TOKENS:
+        raise ValueError(f"{T} tokens in one call: at most {MAX_TOKENS}")
+    _check_sizes(T, T * k, H)
     device = _on_device(x2, idx, w, shared, sgate, out, y_unreduced)
     _index(idx, T * k, "idx")
     if w is not None and (w.dtype != torch.float32 or w.numel() != T * k or not w.is_contiguous()):
@@ -370,6 +383,7 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
     _check_spec(spec)
     x2 = _rows_of(spec, x)
     n = pair_exp.numel()
+    _check_sizes(x2.shape[0], n, spec.hidden)
     device = _on_device(x2, pair_tok, pair_exp, pair_row, y_rows, shared)
     _index(pair_tok, n, "pair_tok")
     _index(pair_exp, n, "pair_exp")

@@ -366,7 +366,8 @@ int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, cons
                        void* out, void* y_unreduced, unsigned flags, void* workspace,
                        size_t workspace_bytes, void* stream);
 /* brx_moe_forward_pairs with MXFP4 activations (flags as in brx_mx_moe_forward); y_rows in y_dtype,
- * BRX_DT_BF16 or, for brx_mx_combine, BRX_DT_F32. */
+ * BRX_DT_BF16 or, for brx_mx_combine, BRX_DT_F32. At most 2^21 pairs, and T * hidden / 2 less than
+ * 2^32 - 256 (the bytes of x's codes). */
 int brx_mx_moe_forward_pairs(const brx_layer_desc* d, brx_pool* p, const void* x, int T,
                              const int32_t* pair_token, const int32_t* pair_expert,
                              const int32_t* pair_row, int n_pairs, int n_rows,

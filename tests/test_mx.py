@@ -136,3 +136,29 @@ def test_switch_refuses_activations():
         StreamingSwitchGLU(Pool(), None, activations="mxfp4")
     Pool.spec = GPT_OSS_120B
     assert StreamingSwitchGLU(Pool(), None, activations="mxfp4").activations == "mxfp4"
+
+
+def test_rows_past_32_bit_offsets_are_refused():
+    """Activations whose codes pass 4 GB, which the kernels' offsets do not reach: refused by size, whatever the
+    form of the call, and the widest that fit are not."""
+    import torch
+    spec = small(GPT_OSS_120B, hidden=8192, inter=64, n_experts=4, top_k=2)
+    most = mx.MAX_CODES // 4096
+    assert most == (1 << 20) - 1
+    assert _ws(spec, most, 8)[0] == 0
+    assert _ws(spec, most + 1, 8)[0] == L.BRX_EINVAL and "2^32 - 256" in _err()
+    assert _ws(spec, most + 1, 0)[0] == 0            # (no pairs: nothing is addressed)
+    i32 = torch.empty(8, dtype=torch.int32, device="meta")
+    for T in (most + 1, 1 << 31, (1 << 32) + 5):     # (the last two have other values in 32 bits)
+        rows = mx.MXRows(torch.empty(T, 4096, dtype=torch.uint8, device="meta"),
+                         torch.empty(T, 256, dtype=torch.uint8, device="meta"))
+        with pytest.raises(ValueError, match="rows of 8192 values"):
+            mx.expert_product(spec, None, rows, i32, i32, "gate_proj")
+        with pytest.raises(ValueError, match="rows of 8192 values"):
+            mx.forward_pairs(spec, None, torch.empty(T, 8192, dtype=torch.bfloat16, device="meta"), i32, i32, None,
+                             None, 0)
+    with pytest.raises(ValueError, match="tokens"):
+        mx.moe_forward(spec, None, torch.empty(mx.MAX_TOKENS + 1, 8192, dtype=torch.bfloat16, device="meta"), None)
+    many = torch.empty(mx.MAX_PAIRS + 1, dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="pairs in one call"):
+        mx.forward_pairs(spec, None, torch.empty(4, 8192, dtype=torch.bfloat16, device="meta"), many, many, None, None, 0)
