@@ -182,23 +182,19 @@ class StreamingSwitchGLU:
 
     # -- the kernels of the chosen activations ------------------------------------------------
     def _forward(self, x2, idx, w=None, shared=None, sgate=None, out=None, y_unreduced=None,
-                 flags=None, stream=None):
+                 flags=None):
         if self.activations == "mxfp4":
             from . import mx      # (its kernels agree bit for bit: no flag holds a chunk to one of them)
-            mx.moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced,
-                           stream=stream)
+            mx.moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced)
         else:
-            moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced, flags,
-                        stream)
+            moe_forward(self.spec, self._pool, x2, idx, w, shared, sgate, out, y_unreduced, flags)
 
-    def _forward_pairs(self, x2, pair_tok, pair_exp, pair_row, y_rows, flags, shared=None, stream=None):
+    def _forward_pairs(self, x2, pair_tok, pair_exp, pair_row, y_rows, flags, shared=None):
         if self.activations == "mxfp4":
             from . import mx
-            mx.forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, 0, shared,
-                             stream)
+            mx.forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, 0, shared)
         else:
-            forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, flags, shared,
-                          stream)
+            forward_pairs(self.spec, self._pool, x2, pair_tok, pair_exp, pair_row, y_rows, flags, shared)
 
     # -- residency (stream.py:922-978) -------------------------------------------------------
     def ensure(self, indices, ranks=None) -> np.ndarray:
@@ -237,17 +233,17 @@ class StreamingSwitchGLU:
         self._sync_free = self._pool.full or self._serve is not None
         return self._sync_free
 
-    def _before(self, stream=None) -> None:
+    def _before(self) -> None:
         """Ahead of a sync-free forward: the table as residency left it (uploaded if it changed),
         or, host-served, the admissions decided from the routing that has come back since."""
         if self._serve is not None:
-            self._serve.service(stream)
+            self._serve.service()
         elif self._pool.table_stale:
-            self._pool.g2s_device(_stream(stream))
+            self._pool.g2s_device(_stream())
 
-    def _after(self, idx, stream=None) -> None:
+    def _after(self, idx) -> None:
         if self._serve is not None:
-            self._serve.record(idx, stream)
+            self._serve.record(idx)
 
     @staticmethod
     def _pair_chunks(sorted_experts: np.ndarray, C: int):
@@ -265,7 +261,7 @@ class StreamingSwitchGLU:
         self.sync_seconds += time.perf_counter() - t0
         return gi
 
-    def _spans(self, x2, flat: np.ndarray, y_rows, flags: int, stream=None) -> None:
+    def _spans(self, x2, flat: np.ndarray, y_rows, flags: int) -> None:
         """Expert-sorted spans (stream.py:1521-1561), each written to its unsorted rows."""
         import torch
         k = flat.shape[1]
@@ -277,14 +273,17 @@ class StreamingSwitchGLU:
         dev = x2.device
         for lo, hi in self._pair_chunks(spe, self._pool.capacity):
             self.ensure(spe[lo:hi], ranks=rank[lo:hi])
-            self._pool.g2s_device(_stream(stream))
+            self._pool.g2s_device(_stream())
             t_tok = torch.from_numpy(tok[lo:hi].astype(np.int32)).to(dev)
             t_exp = torch.from_numpy(spe[lo:hi].astype(np.int32)).to(dev)
             t_row = torch.from_numpy(order[lo:hi].astype(np.int32)).to(dev)
-            self._forward_pairs(x2, t_tok, t_exp, t_row, y_rows, flags, stream=stream)
+            self._forward_pairs(x2, t_tok, t_exp, t_row, y_rows, flags)
 
     def __call__(self, x, indices, stream=None):
-        """Unreduced expert rows [..., k, H] (bf16) for `indices` [..., k]."""
+        """Unreduced expert rows [..., k, H] (bf16) for `indices` [..., k]. Given a `stream`, the whole
+        call runs there (its allocations and copies too): the inputs have to be ready on it."""
+        if stream is not None:
+            return L.on_stream(stream, self.__call__, x, indices)
         import torch
         H, k = self.spec.hidden, self.spec.top_k
         x2 = x.reshape(-1, H).contiguous()
@@ -293,9 +292,9 @@ class StreamingSwitchGLU:
         idx = indices.reshape(-1, k).to(torch.int32).contiguous()
         y = torch.empty((T, k, H), dtype=torch.bfloat16, device=x2.device)
         if self._sync_free:
-            self._before(stream)
-            self._forward(x2, idx, y_unreduced=y, flags=flags, stream=stream)
-            self._after(idx, stream)
+            self._before()
+            self._forward(x2, idx, y_unreduced=y, flags=flags)
+            self._after(idx)
             return y.reshape(*indices.shape[:-1], k, H)
         gi = self._host_routing(idx)
         if k > self._pool.capacity:
@@ -304,16 +303,18 @@ class StreamingSwitchGLU:
                 f"{self._pool.capacity}. A single token cannot be served.")
         if len(np.unique(gi)) <= self._pool.capacity:
             self.ensure(gi)
-            self._pool.g2s_device(_stream(stream))
-            self._forward(x2, idx, y_unreduced=y, flags=flags, stream=stream)
+            self._pool.g2s_device(_stream())
+            self._forward(x2, idx, y_unreduced=y, flags=flags)
         else:
             self.chunked_calls += 1
-            self._spans(x2, gi, y.view(T * k, H), flags, stream)
+            self._spans(x2, gi, y.view(T * k, H), flags)
         return y.reshape(*indices.shape[:-1], k, H)
 
     def forward_combined(self, x2, idx, w, sgate=None, stream=None):
         """out [T, H] = sum_j w[t,j] * y[t,j] (+ sgate[t] * shared(x_t)), the block's combine
-        fused into the expert kernels whenever no span split is needed."""
+        fused into the expert kernels whenever no span split is needed. `stream` as in `__call__`."""
+        if stream is not None:
+            return L.on_stream(stream, self.forward_combined, x2, idx, w, sgate)
         import torch
         H, k = self.spec.hidden, self.spec.top_k
         T = x2.shape[0]
@@ -321,9 +322,9 @@ class StreamingSwitchGLU:
         out = torch.empty((T, H), dtype=torch.bfloat16, device=x2.device)
         shared = self.shared
         if self._sync_free:
-            self._before(stream)
-            self._forward(x2, idx, w, shared, sgate, out=out, flags=flags, stream=stream)
-            self._after(idx, stream)
+            self._before()
+            self._forward(x2, idx, w, shared, sgate, out=out, flags=flags)
+            self._after(idx)
             return out
         gi = self._host_routing(idx)
         if k > self._pool.capacity:
@@ -332,8 +333,8 @@ class StreamingSwitchGLU:
                 f"{self._pool.capacity}. A single token cannot be served.")
         if len(np.unique(gi)) <= self._pool.capacity:
             self.ensure(gi)
-            self._pool.g2s_device(_stream(stream))
-            self._forward(x2, idx, w, shared, sgate, out=out, flags=flags, stream=stream)
+            self._pool.g2s_device(_stream())
+            self._forward(x2, idx, w, shared, sgate, out=out, flags=flags)
             return out
         self.chunked_calls += 1
         join, rows = combine, torch.bfloat16
@@ -341,14 +342,14 @@ class StreamingSwitchGLU:
             from . import mx
             join, rows = mx.combine, torch.float32
         y = torch.empty((T * k, H), dtype=rows, device=x2.device)
-        self._spans(x2, gi, y, flags, stream)
+        self._spans(x2, gi, y, flags)
         ysh = None
         if shared is not None:
             ysh = torch.empty((T, H), dtype=rows, device=x2.device)
             tt = torch.arange(T, dtype=torch.int32, device=x2.device)
             te = torch.full((T,), self.spec.n_experts, dtype=torch.int32, device=x2.device)
-            self._forward_pairs(x2, tt, te, None, ysh, flags, shared=shared, stream=stream)
-        join(self.spec, y, w, out, ysh, sgate, stream=stream)
+            self._forward_pairs(x2, tt, te, None, ysh, flags, shared=shared)
+        join(self.spec, y, w, out, ysh, sgate)
         return out
 
 
@@ -369,12 +370,15 @@ class MoELayer:
                            self.shared_gate_w if self.switch.shared is not None else None, stream)
 
     def __call__(self, x, stream=None):
+        """The block's output, in x's shape. `stream` as in `StreamingSwitchGLU.__call__`."""
+        if stream is not None:
+            return L.on_stream(stream, self.__call__, x)
         x2 = x.reshape(-1, self.spec.hidden).contiguous()
         sw = self.switch
         if sw._sync_free and sw.activations == "bf16":
             # every expert resident (or served from host memory): routing, experts and combine
             # in one library call, the routing never waited for by the host (stream.py:1377-1394)
-            sw._before(stream)
+            sw._before()
             sgw = self.shared_gate_w if sw.shared is not None else None
             idx = None
             if sw._serve is not None:
@@ -382,10 +386,10 @@ class MoELayer:
                 idx = torch.empty((x2.shape[0], self.spec.top_k), dtype=torch.int32,
                                   device=x2.device)
             out = moe_block(self.spec, sw._pool, x2, self.router_w, self.router_bias, sgw,
-                            sw.shared, out_idx=idx, flags=path_flag(x2.shape[0], self.spec.top_k), stream=stream)
+                            sw.shared, out_idx=idx, flags=path_flag(x2.shape[0], self.spec.top_k))
             if idx is not None:
-                sw._after(idx, stream)
+                sw._after(idx)
             return out.reshape(x.shape)
-        idx, w, sg = self.route(x2, stream)
-        out = sw.forward_combined(x2, idx, w, sg, stream)
+        idx, w, sg = self.route(x2)
+        out = sw.forward_combined(x2, idx, w, sg)
         return out.reshape(x.shape)

@@ -164,3 +164,30 @@ def stream_ptr(stream=None) -> int | None:
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream or None
+
+
+def _device_tensors(v):
+    """The GPU tensors in v: a tensor, or tuples, lists and dicts of them."""
+    import torch
+    if isinstance(v, torch.Tensor):
+        if v.is_cuda:
+            yield v
+    elif isinstance(v, (tuple, list, dict)):
+        for u in v.values() if isinstance(v, dict) else v:
+            yield from _device_tensors(u)
+
+
+def on_stream(stream, call, *args):
+    """call(*args) with `stream` current, so that what it allocates, copies and launches is all ordered
+    there: no block that the current stream's queued work may still use is handed to it, and none of its own
+    temporaries to the current stream while `stream` uses them. The memory of the tensors given is not handed
+    out again before `stream` is done with them, nor the results' before the current stream is."""
+    import torch
+    here = torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        for t in _device_tensors(args):
+            t.record_stream(stream)
+        got = call(*args)
+    for t in _device_tensors(got):
+        t.record_stream(here)
+    return got

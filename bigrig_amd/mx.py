@@ -20,8 +20,9 @@ infinity is held as NaN.
 
 Tensors live on the current device. Scratch is allocated per call by torch, on the call's stream, so
 calls on several streams do not share any, and a captured graph keeps its own. Given a `stream`, the
-whole call runs there, its allocations and copies too; the inputs have to be ready on it, and its
-results may be read on the stream that was current once that waits for it.
+whole call runs there, its allocations and copies too; the inputs have to be ready on it (they may be freed
+as soon as the call returns), and its results may be read on the stream that was current once that waits
+for it.
 """
 from __future__ import annotations
 
@@ -117,24 +118,13 @@ def _packed(t, what: str):
     return b, r, bs
 
 
-def _on(stream, call, *args):
-    """call(*args) with `stream` current (memory that the current stream's last work may still use is
-    not handed to it, nor its results' memory reused under readers on the current stream)."""
-    here = torch.cuda.current_stream()
-    with torch.cuda.stream(stream):
-        got = call(*args)
-    for t in (got.codes, got.scales) if isinstance(got, MXRows) else () if got is None else (got,):
-        t.record_stream(here)
-    return got
-
-
 def quantize(x, stream=None) -> MXRows:
     """x [..., K] (float32, bfloat16 or float16; K a multiple of 32; rows may be strided) in MXFP4:
     per group of 32, e = floor(log2(max |v|)) - 2 and codes v / 2^e rounded to nearest even,
     saturating at 6 -- the codes of `formats.quantize_mxfp4`. A group with a NaN or an infinity is
     held as NaN (scale byte 255)."""
     if stream is not None:
-        return _on(stream, quantize, x)
+        return L.on_stream(stream, quantize, x)
     device = _on_device(x)
     dt = _dtype(x.dtype)
     shape = x.shape
@@ -159,7 +149,7 @@ def dequantize(q: MXRows, dtype=None, stream=None):
     """The values of q as a contiguous [..., K] tensor of `dtype` (default bfloat16; exact in
     float32 and bfloat16, rounded to nearest even in float16)."""
     if stream is not None:
-        return _on(stream, dequantize, q, dtype)
+        return L.on_stream(stream, dequantize, q, dtype)
     dtype = torch.bfloat16 if dtype is None else dtype
     dt = _dtype(dtype)
     codes, scales = q
@@ -195,7 +185,7 @@ def pack_experts(spec: LayerSpec, weights: dict, biases: dict | None = None, sha
     are weights[projection] [E, n_out, n_in] (and biases[projection] [E, n_out]), in the layout
     `ExpertPool.admit_device` and `HostStore` take. `shared`: the shared expert's width."""
     if stream is not None:
-        return _on(stream, pack_experts, spec, weights, biases, shared)
+        return L.on_stream(stream, pack_experts, spec, weights, biases, shared)
     if spec.quant.mode != "mxfp4":
         raise ValueError(f"the layer's experts are {spec.quant.mode}, not mxfp4")
     es = spec.expert_spec(shared)
@@ -282,7 +272,7 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
     the others are left as they are. Up to 64 pairs run as one launch and without scratch, more
     as one or two; the rows are the same bits."""
     if stream is not None:
-        return _on(stream, expert_product, spec, pool, q, pair_token, pair_expert, proj, pair_row, out)
+        return L.on_stream(stream, expert_product, spec, pool, q, pair_token, pair_expert, proj, pair_row, out)
     _check_spec(spec)
     j = (_PROJ if spec.gated else _MLP_PROJ).get(proj)
     if j is None:
@@ -333,7 +323,7 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
     as two or three launches, the rest as the grouped GEMM; the outputs are the same bits (`flags`:
     BRX_FWD_FORCE_DECODE for the first, up to 8 tokens and 64 pairs, BRX_FWD_FORCE_PREFILL for the last)."""
     if stream is not None:
-        return _on(stream, moe_forward, spec, pool, x, idx, w, shared, sgate, out, y_unreduced, flags)
+        return L.on_stream(stream, moe_forward, spec, pool, x, idx, w, shared, sgate, out, y_unreduced, flags)
     _check_spec(spec)
     x2 = _rows_of(spec, x)
     T, H, k = x2.shape[0], spec.hidden, spec.top_k
@@ -379,7 +369,7 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
     """`layer.forward_pairs` with MXFP4 activations (any `flags` give the same bits); y_rows bfloat16, or
     float32 for `combine`."""
     if stream is not None:
-        return _on(stream, forward_pairs, spec, pool, x, pair_tok, pair_exp, pair_row, y_rows, flags, shared)
+        return L.on_stream(stream, forward_pairs, spec, pool, x, pair_tok, pair_exp, pair_row, y_rows, flags, shared)
     _check_spec(spec)
     x2 = _rows_of(spec, x)
     n = pair_exp.numel()
@@ -406,7 +396,7 @@ def combine(spec: LayerSpec, y_routed, w, out, y_shared=None, sgate=None, stream
     """out[t] = sum_j w[t, j] * y_routed[t, j] (+ sgate[t] * y_shared[t]): rows float32 [T k, H] and
     [T, H], w and sgate float32, out bfloat16 [T, H]."""
     if stream is not None:
-        return _on(stream, combine, spec, y_routed, w, out, y_shared, sgate)
+        return L.on_stream(stream, combine, spec, y_routed, w, out, y_shared, sgate)
     T, H, k = out.shape[0], spec.hidden, spec.top_k
     device = _on_device(out, y_routed, w, y_shared, sgate)
     if out.dtype != torch.bfloat16 or out.shape != (T, H) or not out.is_contiguous():
