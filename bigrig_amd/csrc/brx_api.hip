@@ -137,6 +137,17 @@ int ws_reserve(size_t bytes, hipStream_t s, void** out) {
 
 }  // namespace
 
+// The MXFP4 calls of one stream, as a pool's refills see them. With every expert resident refills are rare, and
+// whoever is to wait for the calls records the event (one behind every call costs a call 3.5 us).
+struct ReadMark {
+    hipStream_t stream;
+    hipEvent_t done;            // behind the calls that were there when it was last recorded
+    bool pending, recorded;     // calls with no event behind them; an event to wait for
+    uint64_t refills;           // refills that the calls wait for (brx_pool::refills)
+};
+// Streams told apart; the calls of another one wait for those of the oldest, whose mark covers both from then on.
+constexpr int kReadMarks = 8;
+
 struct brx_pool {
     brx_layer_desc d;
     Layout lay;
@@ -155,11 +166,10 @@ struct brx_pool {
     bool refill_recorded;
     bool refill_pending;
     bool g2s_recorded;
-    // MXFP4 calls of a pool with every expert resident: the stream of the last one, whose work an event is
-    // recorded behind when somebody is to wait for it
-    hipStream_t mx_stream;
-    hipEvent_t mx_read;
-    bool mx_pending, mx_recorded;
+    std::mutex mu;              // the marks, and what orders refills with the calls they stand for
+    ReadMark marks[kReadMarks];
+    int n_marks, next_mark;
+    uint64_t refills;           // refills so far that calls wait for
 };
 
 extern "C" {
@@ -229,7 +239,6 @@ int brx_pool_create(const brx_layer_desc* d, int capacity, brx_pool** out) {
     if (e == hipSuccess) e = hipMemset(p->err_dev, 0, 2 * sizeof(int32_t));
     if (e == hipSuccess) e = hipHostMalloc(&p->g2s_pinned, sizeof(int32_t) * d->n_experts, hipHostMallocDefault);
     if (e == hipSuccess) e = hipEventCreateWithFlags(&p->last_read, hipEventDisableTiming);
-    if (e == hipSuccess) e = hipEventCreateWithFlags(&p->mx_read, hipEventDisableTiming);
     if (e == hipSuccess) e = hipEventCreateWithFlags(&p->refill_done, hipEventDisableTiming);
     if (e == hipSuccess) e = hipEventCreateWithFlags(&p->g2s_uploaded, hipEventDisableTiming);
     if (e != hipSuccess) {
@@ -248,7 +257,7 @@ int brx_pool_destroy(brx_pool* p) {
     if (p->err_dev) (void)hipFree(p->err_dev);
     if (p->g2s_pinned) (void)hipHostFree(p->g2s_pinned);
     if (p->last_read) (void)hipEventDestroy(p->last_read);
-    if (p->mx_read) (void)hipEventDestroy(p->mx_read);
+    for (int i = 0; i < p->n_marks; ++i) (void)hipEventDestroy(p->marks[i].done);
     if (p->refill_done) (void)hipEventDestroy(p->refill_done);
     if (p->g2s_uploaded) (void)hipEventDestroy(p->g2s_uploaded);
     delete p;
@@ -270,22 +279,68 @@ int brx_pool_g2s_ptr(brx_pool* p, int32_t** out) {
     return BRX_OK;
 }
 
-// The event behind the MXFP4 calls that left none.
-static int settle_reads(brx_pool* p) {
-    if (p->mx_pending) {
-        HIP_TRY(hipEventRecord(p->mx_read, p->mx_stream));
-        p->mx_pending = false;
-        p->mx_recorded = true;
-    }
+// Whether work given to `s` is captured into a graph. (A captured call neither waits for refills nor holds them
+// back: its replays are the caller's to order with them.)
+static int capturing(hipStream_t s, bool* out) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(s, &st));
+    *out = st != hipStreamCaptureStatusNone;
     return BRX_OK;
 }
 
-// Write-after-read: `cs` waits for the forwards issued so far.
+// The event behind a stream's calls that have none. An event recorded in a capture stands for nothing outside it.
+static int settle(ReadMark& m) {
+    if (!m.pending) return BRX_OK;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    hipError_t e = hipStreamIsCapturing(m.stream, &st);
+    if (e == hipErrorStreamCaptureImplicit || st != hipStreamCaptureStatusNone) {
+        (void)hipGetLastError();
+        return fail(BRX_ESTATE, "MXFP4 calls of this pool are on a stream that is being captured: end the capture first");
+    }
+    if (e == hipSuccess) e = hipEventRecord(m.done, m.stream);
+    if (e == hipSuccess) {
+        m.recorded = true;
+    } else {                    // (no such stream any more)
+        (void)hipGetLastError();
+        HIP_TRY(hipDeviceSynchronize());
+        m.recorded = false;
+    }
+    m.pending = false;
+    return BRX_OK;
+}
+static int settle_reads(brx_pool* p) {
+    for (int i = 0; i < p->n_marks; ++i)
+        if (const int rc = settle(p->marks[i])) return rc;
+    return BRX_OK;
+}
+
+// Write-after-read: `cs` waits for the forwards issued so far, on whatever streams.
 static int wait_reads(brx_pool* p, hipStream_t cs) {
-    const int rc = settle_reads(p);
-    if (rc) return rc;
+    if (const int rc = settle_reads(p)) return rc;
     if (p->read_recorded) HIP_TRY(hipStreamWaitEvent(cs, p->last_read, 0));
-    if (p->mx_recorded) HIP_TRY(hipStreamWaitEvent(cs, p->mx_read, 0));
+    for (int i = 0; i < p->n_marks; ++i)
+        if (p->marks[i].recorded) HIP_TRY(hipStreamWaitEvent(cs, p->marks[i].done, 0));
+    return BRX_OK;
+}
+
+// The mark of stream `s`, which has none.
+static int take_mark(brx_pool* p, hipStream_t s, ReadMark** out) {
+    ReadMark* m;
+    if (p->n_marks < kReadMarks) {
+        hipEvent_t done;
+        HIP_TRY(hipEventCreateWithFlags(&done, hipEventDisableTiming));
+        m = &p->marks[p->n_marks++];
+        *m = ReadMark{};
+        m->done = done;
+    } else {
+        m = &p->marks[p->next_mark];
+        if (const int rc = settle(*m)) return rc;
+        if (m->recorded) HIP_TRY(hipStreamWaitEvent(s, m->done, 0));
+        p->next_mark = (p->next_mark + 1) % kReadMarks;
+        m->refills = 0;
+    }
+    m->stream = s;
+    *out = m;
     return BRX_OK;
 }
 
@@ -297,11 +352,13 @@ static int refill(brx_pool* p, int slot, const void* src, size_t nbytes, void* c
         return fail(BRX_EINVAL, "the layout accounts for %lld bytes but the region supplied %zu. "
                     "Refusing to write a partially-filled slot.", (long long)p->lay.bytes, nbytes);
     hipStream_t cs = (hipStream_t)copy_stream;
+    std::lock_guard<std::mutex> lk(p->mu);
     if (const int rc = wait_reads(p, cs)) return rc;
     HIP_TRY(hipMemcpyAsync(p->slots + (int64_t)slot * p->stride, src, nbytes, kind, cs));
     HIP_TRY(hipEventRecord(p->refill_done, cs));
     p->refill_pending = true;
     p->refill_recorded = true;
+    ++p->refills;
     return BRX_OK;
 }
 
@@ -319,6 +376,7 @@ int brx_pool_refill_range_async(brx_pool* p, int slot0, int n, const void* host_
                     "Refusing to write a partially-filled slot.", (long long)p->lay.bytes, nbytes);
     if (host_stride < (int64_t)nbytes) return fail(BRX_EINVAL, "host stride %lld is below the expert size", (long long)host_stride);
     hipStream_t cs = (hipStream_t)copy_stream;
+    std::lock_guard<std::mutex> lk(p->mu);
     if (const int rc = wait_reads(p, cs)) return rc;
     uint8_t* dst = p->slots + (int64_t)slot0 * p->stride;
     const uint8_t* src = (const uint8_t*)host_src;
@@ -334,6 +392,7 @@ int brx_pool_refill_range_async(brx_pool* p, int slot0, int n, const void* host_
     HIP_TRY(hipEventRecord(p->refill_done, cs));
     p->refill_pending = true;
     p->refill_recorded = true;
+    ++p->refills;
     return BRX_OK;
 }
 
@@ -368,7 +427,7 @@ int brx_pool_set_g2s(brx_pool* p, const int32_t* g2s_host, int n, void* stream) 
 int brx_pool_set_host_backing(brx_pool* p, const void* host_base, int64_t host_stride, size_t host_bytes) {
     if (!p || !host_base) return fail(BRX_EINVAL, "pool or host_base is NULL");
     if (p->host) return fail(BRX_EINVAL, "the pool already has host backing");
-    if (p->refill_recorded || p->g2s_recorded || p->read_recorded || p->mx_pending || p->mx_recorded)
+    if (p->refill_recorded || p->g2s_recorded || p->read_recorded || p->n_marks)
         return fail(BRX_EINVAL, "host backing is set on a fresh pool, before any refill, table upload or forward");
     const int E = p->d.n_experts;
     // the kernels address a host expert exactly as a slot: same stride, same alignment
@@ -439,6 +498,7 @@ int brx_pool_admit_async(brx_pool* p, int expert, int slot, const void* host_src
         return fail(BRX_EINVAL, "the layout accounts for %lld bytes but the region supplied %zu. "
                     "Refusing to write a partially-filled slot.", (long long)p->lay.bytes, nbytes);
     hipStream_t cs = (hipStream_t)copy_stream;
+    std::lock_guard<std::mutex> lk(p->mu);
     // write-after-read: every forward issued so far may still read the slot's old expert
     if (const int rc = wait_reads(p, cs)) return rc;
     HIP_TRY(hipMemcpyAsync(p->slots + (int64_t)slot * p->stride, host_src, nbytes, hipMemcpyHostToDevice, cs));
@@ -457,10 +517,17 @@ int brx_pool_admit_async(brx_pool* p, int expert, int slot, const void* host_src
 
 int brx_pool_sync(brx_pool* p) {
     if (!p) return fail(BRX_EINVAL, "pool is NULL");
-    if (const int rc = settle_reads(p)) return rc;
+    hipEvent_t calls[kReadMarks];
+    int n = 0;
+    {
+        std::lock_guard<std::mutex> lk(p->mu);
+        if (const int rc = settle_reads(p)) return rc;
+        for (int i = 0; i < p->n_marks; ++i)
+            if (p->marks[i].recorded) calls[n++] = p->marks[i].done;
+    }
     if (p->refill_recorded) HIP_TRY(hipEventSynchronize(p->refill_done));
     if (p->read_recorded) HIP_TRY(hipEventSynchronize(p->last_read));
-    if (p->mx_recorded) HIP_TRY(hipEventSynchronize(p->mx_read));
+    for (int i = 0; i < n; ++i) HIP_TRY(hipEventSynchronize(calls[i]));
     if (p->g2s_recorded) HIP_TRY(hipEventSynchronize(p->g2s_uploaded));
     return BRX_OK;
 }
@@ -824,29 +891,44 @@ int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int 
     return BRX_OK;
 }
 
-// Ahead of a call's launches: its workspace checked, the stream behind the pool's refills (as run_forward).
-static int mx_begin(brx_pool* p, size_t need, void* workspace, size_t workspace_bytes, hipStream_t s) {
+// Ahead of a call's launches (under the pool's lock, as mx_end): its workspace checked, its stream behind the pool's
+// refills. *mark: the stream's, or null where the call is captured and its stream has none.
+static int mx_begin(brx_pool* p, size_t need, void* workspace, size_t workspace_bytes, hipStream_t s, ReadMark** mark) {
     if (need && (!workspace || ((uintptr_t)workspace & 255))) return fail(BRX_EINVAL, "workspace must be a 256-byte aligned device buffer");
     if (workspace_bytes < need) return fail(BRX_EINVAL, "this call needs %zu bytes of workspace, %zu given", need, workspace_bytes);
-    if (p->refill_pending) {
+    ReadMark* m = nullptr;
+    for (int i = 0; i < p->n_marks && !m; ++i)
+        if (p->marks[i].stream == s) m = &p->marks[i];
+    *mark = m;
+    if (m && m->refills == p->refills) return BRX_OK;
+    bool captured = false;
+    int rc = capturing(s, &captured);
+    if (rc || captured) return rc;
+    if (!m && (rc = take_mark(p, s, &m))) return rc;
+    if (m->refills != p->refills) {
         HIP_TRY(hipStreamWaitEvent(s, p->refill_done, 0));
-        p->refill_pending = false;
+        m->refills = p->refills;
     }
+    *mark = m;
     return BRX_OK;
 }
 
-// After them: the pool marked read. With every expert resident refills are rare, and the event waits for one (it
-// costs a call 3.5 us: one token of the gpt-oss shape 22.1 -> 18.6); elsewhere a refill should wait for this
-// call and not for what is queued behind it.
-static int mx_end(brx_pool* p, hipError_t e, hipStream_t s) {
-    if (e != hipSuccess) return hip_fail(e, "MXFP4 launch");
-    if (!p->host && p->resident == p->d.n_experts) {
-        p->mx_stream = s;
-        p->mx_pending = true;
-        return BRX_OK;
+// After them: the stream's calls marked. With every expert resident the event waits for a refill (one token of the
+// gpt-oss shape 22.1 -> 18.6 us); elsewhere a refill should wait for this call and not for what is queued
+// behind it.
+static int mx_end(brx_pool* p, ReadMark* m, hipError_t e, hipStream_t s) {
+    if (m && !p->host && p->resident == p->d.n_experts) {
+        m->pending = true;
+    } else if (m) {
+        bool captured = false;
+        if (const int rc = capturing(s, &captured)) return rc;
+        if (!captured) {
+            HIP_TRY(hipEventRecord(m->done, s));
+            m->recorded = true;
+            m->pending = false;
+        }
     }
-    HIP_TRY(hipEventRecord(p->last_read, s));
-    p->read_recorded = true;
+    if (e != hipSuccess) return hip_fail(e, "MXFP4 launch");
     return BRX_OK;
 }
 
@@ -885,8 +967,10 @@ int brx_mx_expert_product(const brx_layer_desc* d, brx_pool* p, const void* code
     FwdArgs a = make_args(d, p, nullptr, T, n_pairs, pair_expert, pair_token, pair_row, n_rows, nullptr, nullptr, nullptr,
                           nullptr, y_rows);
     hipStream_t s = (hipStream_t)stream;
-    if ((rc = mx_begin(p, mx_workspace_bytes(a, false, kMxMany), workspace, workspace_bytes, s))) return rc;
-    return mx_end(p, launch_mx_product(a, (const uint8_t*)codes, (const uint8_t*)scales, proj, workspace, s), s);
+    std::lock_guard<std::mutex> lk(p->mu);
+    ReadMark* mark;
+    if ((rc = mx_begin(p, mx_workspace_bytes(a, false, kMxMany), workspace, workspace_bytes, s, &mark))) return rc;
+    return mx_end(p, mark, launch_mx_product(a, (const uint8_t*)codes, (const uint8_t*)scales, proj, workspace, s), s);
 }
 
 static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T, int P, const int32_t* pexp,
@@ -906,9 +990,11 @@ static int mx_forward(const brx_layer_desc* d, brx_pool* p, const void* x, int T
     const MxPath path = flags & BRX_FWD_FORCE_PREFILL ? kMxMany : mx_path(a);
     if ((flags & BRX_FWD_FORCE_DECODE) && (T > 8 || P > 64))
         return fail(BRX_EINVAL, "the decode path takes at most 8 token rows and 64 pairs (T=%d, P=%d)", T, P);
-    const int rc = mx_begin(p, mx_workspace_bytes(a, true, path), workspace, workspace_bytes, s);
+    std::lock_guard<std::mutex> lk(p->mu);
+    ReadMark* mark;
+    const int rc = mx_begin(p, mx_workspace_bytes(a, true, path), workspace, workspace_bytes, s, &mark);
     if (rc) return rc;
-    return mx_end(p, launch_mx_layer(a, path, rows32, workspace, s), s);
+    return mx_end(p, mark, launch_mx_layer(a, path, rows32, workspace, s), s);
 }
 
 int brx_mx_moe_forward(const brx_layer_desc* d, brx_pool* p, const void* x, const int32_t* idx, const float* w,

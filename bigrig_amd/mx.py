@@ -23,6 +23,10 @@ calls on several streams do not share any, and a captured graph keeps its own. G
 whole call runs there, its allocations and copies too; the inputs have to be ready on it (they may be freed
 as soon as the call returns), and its results may be read on the stream that was current once that waits
 for it.
+
+A pool's admissions and its calls wait for each other on whatever streams they are (a stream of torch's; one made
+elsewhere has to outlive the pool's next admission, sync or check). Replays of captured calls are the
+caller's to order with admissions.
 """
 from __future__ import annotations
 

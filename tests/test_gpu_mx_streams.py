@@ -3,12 +3,13 @@ import numpy as np
 import pytest
 
 from bigrig_amd import formats as F
+from bigrig_amd import lib as L
+from bigrig_amd import mx
 from bigrig_amd.layer import MoELayer, StreamingSwitchGLU
 from bigrig_amd.pool import ExpertPool, HostStore, PinnedFetcher
-from tests.gpu_util import bits, to_dev_bits
-from tests.test_gpu_mx import SHARED, _layer_inputs, dev
-from tests.gpu_util import build_gpu_layer
+from tests.gpu_util import bits, build_gpu_layer, bytes_dev, to_dev_bits
 from tests.helpers import make_layer
+from tests.test_gpu_mx import SHARED, SWIGLU, _layer_inputs, dev, layer_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -73,4 +74,151 @@ def test_layer_calls_on_a_given_stream(gpu, kind, activations, T):
             torch.cuda.current_stream().wait_stream(s)
             assert np.array_equal(bits(got), want[n]), (n, strided)
     torch.cuda.synchronize()
+    pool.close()
+
+
+# ------------------------------------------------------------------ a pool's refills and its calls
+def _pool(gpu, kind, T, seed):
+    """(layer, pool, its blobs on the device, inputs of T tokens): every expert resident, or the first three of
+    six, which the routing keeps to."""
+    import torch
+    lay = make_layer(SWIGLU, seed=seed, expert_std=0.05)
+    n = SWIGLU.n_experts if kind == "resident" else 3
+    store = HostStore()
+    store.add_layer(0, lay.experts)
+    pool = ExpertPool(0, lay.spec, n).build()
+    for e in range(n):
+        pool.touch([e], [0])
+        pool.admit(e, store.region(0, e))
+    pool.g2s_device(torch.cuda.current_stream().cuda_stream)
+    x, idx, w, _ = _layer_inputs(lay.spec, lay, gpu, T, seed=seed + T)
+    if kind != "resident":
+        idx = np.stack([np.arange(T) % 3, (np.arange(T) + 1) % 3], 1).astype(np.int32)
+    ins = to_dev_bits(x, gpu), dev(idx, gpu), dev(w, gpu)
+    blobs = [bytes_dev(b, gpu) for b in lay.experts[:n]]
+    torch.cuda.synchronize()
+    return lay, pool, blobs, ins
+
+
+def _refill(pool, blobs, shift, copy):
+    """Expert e's slot takes the bytes of expert e + shift."""
+    for e in range(len(blobs)):
+        b = blobs[(e + shift) % len(blobs)]
+        L.check(L.load().brx_pool_refill_from_device_async(pool.device.handle, int(pool.g2s[e]), b.data_ptr(), b.numel(),
+                                                           copy.cuda_stream))
+
+
+def _queued(streams, call, slow):
+    """call() on each stream, the ones of `slow` behind some milliseconds of other work."""
+    import torch
+    got = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            if i in slow:
+                torch.cuda._sleep(20_000_000)
+            got.append(call())
+    return got
+
+
+@pytest.mark.parametrize("kind", ["resident", "bounded"])
+@pytest.mark.parametrize("n, slow", [(2, [0]), (3, [1]), (11, [0, 2, 9])])
+@pytest.mark.parametrize("T", [2, 80])
+def test_calls_on_every_stream_are_waited_for(gpu, kind, n, slow, T):
+    """The pool's sync and its refills wait for the calls of every stream, the slowest not the last."""
+    import torch
+    lay, pool, blobs, ins = _pool(gpu, kind, T, 300 + n)
+    spec, copy = lay.spec, torch.cuda.Stream()
+    streams = [torch.cuda.Stream() for _ in range(n)]
+    old = bits(mx.moe_forward(spec, pool, *ins))
+    torch.cuda.synchronize()
+    call = lambda: mx.moe_forward(spec, pool, *ins)   # noqa: E731
+    got = _queued(streams, call, slow)
+    pool.device.sync()
+    assert all(s.query() for s in streams)
+    got += _queued(streams, call, slow)
+    _refill(pool, blobs, 1, copy)
+    torch.cuda.synchronize()
+    for g in got:
+        assert np.array_equal(bits(g), old)
+    new = bits(call())
+    assert not np.array_equal(new, old)
+    _refill(pool, blobs, 0, copy)
+    assert np.array_equal(bits(call()), old)
+    pool.device.check()
+    pool.close()
+
+
+@pytest.mark.parametrize("n", [2, 10])
+@pytest.mark.parametrize("T", [2, 80])
+def test_a_refill_is_waited_for_on_every_stream(gpu, n, T):
+    """Calls issued behind a queued refill see its bytes, the second stream's as the first's, products and bf16
+    forwards too."""
+    import torch
+    lay, pool, blobs, ins = _pool(gpu, "resident", T, 400 + n)
+    spec, copy = lay.spec, torch.cuda.Stream()
+    streams = [torch.cuda.Stream() for _ in range(n)]
+    plain = torch.cuda.Stream()
+    q = mx.quantize(ins[0])
+    tok = torch.arange(T, dtype=torch.int32, device=gpu).repeat_interleave(spec.top_k)
+    call = lambda: mx.moe_forward(spec, pool, *ins)   # noqa: E731
+    rows = lambda: mx.expert_product(spec, pool, q, tok, ins[1].view(-1), "up_proj")   # noqa: E731
+    want = []
+    for shift in (0, 1, 2):
+        _refill(pool, blobs, shift, copy)
+        torch.cuda.synchronize()
+        want.append((bits(call()), bits(rows()), bits(layer_forward(spec, pool, *ins))))
+        torch.cuda.synchronize()
+    for shift in (0, 1, 2):
+        with torch.cuda.stream(copy):
+            torch.cuda._sleep(20_000_000)
+        _refill(pool, blobs, shift, copy)
+        got = _queued(streams, call if shift else rows, [])
+        with torch.cuda.stream(plain):
+            p16 = layer_forward(spec, pool, *ins)
+        torch.cuda.synchronize()
+        for g in got:
+            assert np.array_equal(bits(g), want[shift][0 if shift else 1])
+        assert np.array_equal(bits(p16), want[shift][2])
+    pool.close()
+
+
+@pytest.mark.parametrize("T", [2, 80])
+def test_capture_and_refills(gpu, T):
+    """A capture on a stream the pool has not seen, straight after a refill, then one on a stream with calls of its
+    own; the pool is not synchronized inside the second, and is after it. Replays against eager calls, around
+    refills that the program orders."""
+    import torch
+    lay, pool, blobs, ins = _pool(gpu, "resident", T, 500)
+    spec, copy = lay.spec, torch.cuda.Stream()
+    call = lambda: mx.moe_forward(spec, pool, *ins)   # noqa: E731
+    _refill(pool, blobs, 1, copy)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    for s in (torch.cuda.Stream(), side):
+        if s is side:
+            with torch.cuda.stream(side):
+                call()
+            pool.device.sync()
+            torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(call())
+            if s is side:
+                with pytest.raises(L.BrxError, match="captured"):
+                    pool.device.sync()
+        graphs.append(g)
+    pool.device.sync()
+    for shift in (0, 1, 2, 0):
+        _refill(pool, blobs, shift, copy)
+        torch.cuda.synchronize()
+        for o in outs:
+            o.zero_()
+        for g in graphs:
+            g.replay()
+        want = bits(call())
+        torch.cuda.synchronize()
+        for o in outs:
+            assert np.array_equal(bits(o), want), shift
+    pool.device.check()
     pool.close()
