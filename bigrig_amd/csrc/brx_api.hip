@@ -871,20 +871,22 @@ static int check_mx_sizes(int T, int64_t n_pairs, bool shared) {
     return BRX_OK;
 }
 
-int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int shared, int product, size_t* out) {
+int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int shared, int call, size_t* out) {
     int rc = check_mx_desc(d);
     if (rc) return rc;
     if (!out) return fail(BRX_EINVAL, "out is NULL");
     if (shared && !d->shared_inter) return fail(BRX_EINVAL, "layer descriptor has no shared expert");
     if ((rc = check_mx_sizes(T, n_pairs, shared != 0))) return rc;
+    if (call < BRX_MX_LAYER || call > BRX_MX_ROWS) return fail(BRX_EINVAL, "call %d unknown", call);
+    const bool product = call == BRX_MX_PRODUCT;
     if (!product && n_pairs && (rc = check_mx_rows(T, d->hidden))) return rc;
     // a layer call and the pairs form (whose shared pairs are among n_pairs) share the count
     brx_pool none{};
     none.d = *d;
     none.lay = make_layout(*d, d->inter);
-    static const uint8_t some = 0;
+    static uint8_t some = 0;
     FwdArgs a = make_args(d, &none, nullptr, T, (int)n_pairs, nullptr, nullptr, nullptr, 0, nullptr,
-                          shared ? &some : nullptr, nullptr, nullptr, nullptr);
+                          shared ? &some : nullptr, nullptr, call == BRX_MX_LAYER ? &some : nullptr, nullptr);
     // (of whichever kernels a call may take)
     const size_t all = mx_workspace_bytes(a, !product, kMxMany), own = mx_workspace_bytes(a, !product, mx_path(a));
     *out = own > all ? own : all;

@@ -365,7 +365,7 @@ MxWs carve(const FwdArgs& a, bool layer, void* ws) {
         w.xs = (uint8_t*)take((size_t)a.T * (a.H / 32));
         w.hq = (uint8_t*)take((size_t)P_ext * (w.Imax / 2));
         w.hs = (uint8_t*)take((size_t)P_ext * (w.Imax / 32));
-        w.y32 = (float*)take(a.out || !a.yun ? (size_t)P_ext * a.H * 4 : 0);   // (neither: a call's size is asked for)
+        w.y32 = (float*)take(a.out ? (size_t)P_ext * a.H * 4 : 0);             // (rows alone go where the caller has them)
     }
     w.bytes = off;
     return w;

@@ -19,6 +19,7 @@ ACT_SWIGLU, ACT_SWIGLU_CLAMPED = 0, 1
 ROUTE_SOFTMAX_TOPK, ROUTE_SOFTMAX_TOPK_RENORM, ROUTE_TOPK_SOFTMAX = 0, 1, 2
 ROUTE_SIGMOID_TOPK, ROUTE_SIGMOID_TOPK_RENORM = 3, 4
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+MX_LAYER, MX_PRODUCT, MX_ROWS = 0, 1, 2
 FWD_FORCE_DECODE, FWD_FORCE_PREFILL, FWD_PHASE_A, FWD_PHASE_B, FWD_PHASE_R = 1, 2, 4, 8, 16
 ABI_VERSION = 2         # brx_abi_version() of the library this binding matches (BRX_ABI_VERSION)
 NOALLOC_SCRATCH_BYTES = 16 << 20

@@ -248,15 +248,15 @@ def _index(t, n: int, what: str):
                          f"{t.dtype} {tuple(t.shape)}")
 
 
-def _workspace(spec: LayerSpec, T: int, pairs: int, shared: bool, product: bool, like):
-    """Scratch for one call, from torch's allocator (on the device of tensor `like`)."""
+def _workspace(spec: LayerSpec, T: int, pairs: int, shared: bool, call: int, like):
+    """Scratch for one call (L.MX_*), from torch's allocator (on the device of tensor `like`)."""
     known = spec.__dict__.setdefault("_mx_workspace", {})     # sizes, not memory
-    key = (T, pairs, shared, product)
+    key = (T, pairs, shared, call)
     n = known.get(key)
     if n is None:
         out = C.c_size_t()
         L.check(L.load().brx_mx_workspace_bytes(C.byref(spec.c_desc), T, pairs, int(shared),
-                                                int(product), C.byref(out)))
+                                                call, C.byref(out)))
         if len(known) > 4096:
             known.clear()
         n = known[key] = out.value
@@ -303,7 +303,7 @@ def expert_product(spec: LayerSpec, pool: ExpertPool, q: MXRows, pair_token, pai
         out = codes.new_empty((n, n_out), dtype=torch.bfloat16)
     elif out.dtype != torch.bfloat16 or out.dim() != 2 or out.shape[1] != n_out or not out.is_contiguous():
         raise ValueError(f"out must be contiguous bfloat16 [n_rows, {n_out}]")
-    ws = _workspace(spec, T, n, False, True, codes) if n > FEW_PAIRS else None
+    ws = _workspace(spec, T, n, False, L.MX_PRODUCT, codes) if n > FEW_PAIRS else None
     L.check(L.load().brx_mx_expert_product(
         C.byref(spec.c_desc), pool.device.handle, codes.data_ptr(), scales.data_ptr(), T, pair_token.data_ptr(),
         pair_expert.data_ptr(), None if pair_row is None else pair_row.data_ptr(), n, out.shape[0], j,
@@ -349,7 +349,7 @@ def moe_forward(spec: LayerSpec, pool: ExpertPool, x, idx, w=None, shared=None, 
         out = x2.new_empty((T, H))
     if w is None and y_unreduced is None:
         y_unreduced = x2.new_empty((T, k, H))
-    ws = _workspace(spec, T, T * k, shared is not None, False, x2)
+    ws = _workspace(spec, T, T * k, shared is not None, L.MX_ROWS if out is None else L.MX_LAYER, x2)
     ptr = L.ptr
     L.check(L.load().brx_mx_moe_forward(
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), idx.data_ptr(), ptr(w), ptr(shared),
@@ -388,7 +388,7 @@ def forward_pairs(spec: LayerSpec, pool: ExpertPool, x, pair_tok, pair_exp, pair
     if (y_rows.dtype not in (torch.bfloat16, torch.float32) or y_rows.dim() != 2 or
             y_rows.shape[1] != spec.hidden or not y_rows.is_contiguous()):
         raise ValueError(f"y_rows must be contiguous bfloat16 or float32 [n_rows, {spec.hidden}]")
-    ws = _workspace(spec, x2.shape[0], n, shared is not None, False, x2)
+    ws = _workspace(spec, x2.shape[0], n, shared is not None, L.MX_ROWS, x2)
     ptr = L.ptr
     L.check(L.load().brx_mx_moe_forward_pairs(
         C.byref(spec.c_desc), pool.device.handle, x2.data_ptr(), x2.shape[0], ptr(pair_tok), ptr(pair_exp),

@@ -339,10 +339,13 @@ int brx_mx_dequantize(const void* codes, int64_t codes_batch_stride, const void*
                       int64_t scales_batch_stride, int64_t batch, int64_t rows, int64_t cols, int dtype,
                       void* out, void* stream);
 
-/* Bytes of scratch the calls below need for T token rows and n_pairs routed pairs (a layer: T * top_k):
- * `product` nonzero for brx_mx_expert_product, zero for the layer calls (shared != 0: given a shared
- * expert). What a call needs never exceeds this; a product of at most 64 pairs needs none. */
-int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int shared, int product,
+/* Bytes of scratch the calls below need for T token rows and n_pairs routed pairs (a layer: T * top_k;
+ * shared != 0: given a shared expert). `call`: BRX_MX_LAYER a layer call of any outputs, BRX_MX_PRODUCT
+ * brx_mx_expert_product, BRX_MX_ROWS a layer call without `out` or the pairs form, which keep no fp32 rows to
+ * sum (n_pairs * hidden * 4 bytes less). What a call needs never exceeds this; a product of at most 64
+ * pairs needs none. */
+enum { BRX_MX_LAYER = 0, BRX_MX_PRODUCT = 1, BRX_MX_ROWS = 2 };
+int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int shared, int call,
                            size_t* out);
 
 /* One projection's rows for a list of (token, expert) pairs, activations already quantized:

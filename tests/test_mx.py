@@ -162,3 +162,16 @@ def test_rows_past_32_bit_offsets_are_refused():
     many = torch.empty(mx.MAX_PAIRS + 1, dtype=torch.int32, device="meta")
     with pytest.raises(ValueError, match="pairs in one call"):
         mx.forward_pairs(spec, None, torch.empty(4, 8192, dtype=torch.bfloat16, device="meta"), many, many, None, None, 0)
+
+
+def test_workspace_of_rows_has_no_rows_to_sum():
+    """Unreduced rows and the pairs form write where the caller says: no fp32 row a pair in their scratch."""
+    spec = small(E256_SHARED, quant=MX)
+    for T, shared in ((64, 0), (2048, 0), (2048, 1)):
+        pairs = T * spec.top_k
+        sums, rows = _ws(spec, T, pairs, shared, L.MX_LAYER)[1], _ws(spec, T, pairs, shared, L.MX_ROWS)[1]
+        assert sums - rows == (pairs + shared * T) * spec.hidden * 4
+        # x and h rows, four bytes a pair and the tile list
+        assert rows < (T * spec.hidden + (pairs + T) * spec.inter) * 17 // 32 + 64 * (pairs + T) + 64 * 1024
+    assert _ws(spec, 64, 512, 0, 3)[0] == L.BRX_EINVAL and "call 3" in _err()
+    assert _ws(spec, 64, 512, 0, -1)[0] == L.BRX_EINVAL
