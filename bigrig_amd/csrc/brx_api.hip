@@ -137,13 +137,16 @@ int ws_reserve(size_t bytes, hipStream_t s, void** out) {
 
 }  // namespace
 
-// The MXFP4 calls of one stream, as a pool's refills see them. With every expert resident refills are rare, and
-// whoever is to wait for the calls records the event (one behind every call costs a call 3.5 us).
-struct ReadMark {
+// Work of one stream that others may have to wait for. Where that is rare, whoever has to records the event (one
+// behind every call costs a call 3.5 us).
+struct Mark {
     hipStream_t stream;
-    hipEvent_t done;            // behind the calls that were there when it was last recorded
-    bool pending, recorded;     // calls with no event behind them; an event to wait for
-    uint64_t refills;           // refills that the calls wait for (brx_pool::refills)
+    hipEvent_t done;            // behind the work that was there when it was last recorded
+    bool pending, recorded;     // work with no event behind it; an event to wait for
+};
+// The MXFP4 calls of one stream, and the refills and table changes they wait for (brx_pool::refills, tables).
+struct ReadMark : Mark {
+    uint64_t refills, tables;
 };
 // Streams told apart; the calls of another one wait for those of the oldest, whose mark covers both from then on.
 constexpr int kReadMarks = 8;
@@ -166,10 +169,11 @@ struct brx_pool {
     bool refill_recorded;
     bool refill_pending;
     bool g2s_recorded;
-    std::mutex mu;              // the marks, and what orders refills with the calls they stand for
+    std::mutex mu;              // the marks, and what orders refills and the table with the calls they stand for
     ReadMark marks[kReadMarks];
     int n_marks, next_mark;
-    uint64_t refills;           // refills so far that calls wait for
+    Mark table;                 // the table's last change
+    uint64_t refills, tables;   // refills that calls wait for, and changes of the table, so far
 };
 
 extern "C" {
@@ -239,6 +243,7 @@ int brx_pool_create(const brx_layer_desc* d, int capacity, brx_pool** out) {
     if (e == hipSuccess) e = hipMemset(p->err_dev, 0, 2 * sizeof(int32_t));
     if (e == hipSuccess) e = hipHostMalloc(&p->g2s_pinned, sizeof(int32_t) * d->n_experts, hipHostMallocDefault);
     if (e == hipSuccess) e = hipEventCreateWithFlags(&p->last_read, hipEventDisableTiming);
+    if (e == hipSuccess) e = hipEventCreateWithFlags(&p->table.done, hipEventDisableTiming);
     if (e == hipSuccess) e = hipEventCreateWithFlags(&p->refill_done, hipEventDisableTiming);
     if (e == hipSuccess) e = hipEventCreateWithFlags(&p->g2s_uploaded, hipEventDisableTiming);
     if (e != hipSuccess) {
@@ -258,6 +263,7 @@ int brx_pool_destroy(brx_pool* p) {
     if (p->g2s_pinned) (void)hipHostFree(p->g2s_pinned);
     if (p->last_read) (void)hipEventDestroy(p->last_read);
     for (int i = 0; i < p->n_marks; ++i) (void)hipEventDestroy(p->marks[i].done);
+    if (p->table.done) (void)hipEventDestroy(p->table.done);
     if (p->refill_done) (void)hipEventDestroy(p->refill_done);
     if (p->g2s_uploaded) (void)hipEventDestroy(p->g2s_uploaded);
     delete p;
@@ -288,14 +294,14 @@ static int capturing(hipStream_t s, bool* out) {
     return BRX_OK;
 }
 
-// The event behind a stream's calls that have none. An event recorded in a capture stands for nothing outside it.
-static int settle(ReadMark& m) {
+// The event behind a stream's work that has none. An event recorded in a capture stands for nothing outside it.
+static int settle(Mark& m) {
     if (!m.pending) return BRX_OK;
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     hipError_t e = hipStreamIsCapturing(m.stream, &st);
     if (e == hipErrorStreamCaptureImplicit || st != hipStreamCaptureStatusNone) {
         (void)hipGetLastError();
-        return fail(BRX_ESTATE, "MXFP4 calls of this pool are on a stream that is being captured: end the capture first");
+        return fail(BRX_ESTATE, "work of this pool is on a stream that is being captured: end the capture first");
     }
     if (e == hipSuccess) e = hipEventRecord(m.done, m.stream);
     if (e == hipSuccess) {
@@ -323,6 +329,22 @@ static int wait_reads(brx_pool* p, hipStream_t cs) {
     return BRX_OK;
 }
 
+// `s` behind the work of a mark, if it is another stream's.
+static int wait_mark(Mark& m, hipStream_t s) {
+    if (m.stream == s) return BRX_OK;
+    if (const int rc = settle(m)) return rc;
+    if (m.recorded) HIP_TRY(hipStreamWaitEvent(s, m.done, 0));
+    return BRX_OK;
+}
+
+// Ahead of a change of the table on `s`: behind the last one (so the last one's mark stands for all).
+static int table_begin(brx_pool* p, hipStream_t s) { return wait_mark(p->table, s); }
+static void table_end(brx_pool* p, hipStream_t s) {
+    p->table.stream = s;
+    p->table.pending = true;
+    ++p->tables;
+}
+
 // The mark of stream `s`, which has none.
 static int take_mark(brx_pool* p, hipStream_t s, ReadMark** out) {
     ReadMark* m;
@@ -334,10 +356,9 @@ static int take_mark(brx_pool* p, hipStream_t s, ReadMark** out) {
         m->done = done;
     } else {
         m = &p->marks[p->next_mark];
-        if (const int rc = settle(*m)) return rc;
-        if (m->recorded) HIP_TRY(hipStreamWaitEvent(s, m->done, 0));
+        if (const int rc = wait_mark(*m, s)) return rc;
         p->next_mark = (p->next_mark + 1) % kReadMarks;
-        m->refills = 0;
+        m->refills = m->tables = 0;
     }
     m->stream = s;
     *out = m;
@@ -408,6 +429,11 @@ int brx_pool_set_g2s(brx_pool* p, const int32_t* g2s_host, int n, void* stream) 
         if (g2s_host[e] >= p->capacity)
             return fail(BRX_ERANGE, "expert %d maps to slot %d outside [0, %d)", e, g2s_host[e], p->capacity);
     hipStream_t s = (hipStream_t)stream;
+    std::lock_guard<std::mutex> lk(p->mu);
+    // calls on other streams still read the entries this replaces
+    for (int i = 0; i < p->n_marks; ++i)
+        if (const int rc = wait_mark(p->marks[i], s)) return rc;
+    if (const int rc = table_begin(p, s)) return rc;
     // the staging copy of the previous upload must have been consumed before it is rewritten
     if (p->g2s_recorded) HIP_TRY(hipEventSynchronize(p->g2s_uploaded));
     // -1 stays -1 (absent): with host backing the kernels read the expert from host memory,
@@ -421,6 +447,7 @@ int brx_pool_set_g2s(brx_pool* p, const int32_t* g2s_host, int n, void* stream) 
     HIP_TRY(hipMemcpyAsync(p->g2s_dev, p->g2s_pinned, sizeof(int32_t) * n, hipMemcpyHostToDevice, s));
     HIP_TRY(hipEventRecord(p->g2s_uploaded, s));
     p->g2s_recorded = true;
+    table_end(p, s);
     return BRX_OK;
 }
 
@@ -473,6 +500,8 @@ int brx_pool_publish_async(brx_pool* p, int n, const int32_t* experts, const int
         for (int j = 0; j < i; ++j)
             if (experts[j] == experts[i]) return fail(BRX_EINVAL, "expert %d appears twice", experts[i]);
     }
+    std::lock_guard<std::mutex> lk(p->mu);
+    if (const int rc = table_begin(p, (hipStream_t)stream)) return rc;
     for (int i0 = 0; i0 < n; i0 += kMaxTableEdits) {
         TableEdits ed{};
         ed.n = n - i0 < kMaxTableEdits ? n - i0 : kMaxTableEdits;
@@ -483,6 +512,7 @@ int brx_pool_publish_async(brx_pool* p, int n, const int32_t* experts, const int
         hipError_t e = launch_table_set(p->g2s_dev, ed, (hipStream_t)stream);
         if (e != hipSuccess) return hip_fail(e, "table update");
     }
+    if (n) table_end(p, (hipStream_t)stream);
     return BRX_OK;
 }
 
@@ -894,7 +924,7 @@ int brx_mx_workspace_bytes(const brx_layer_desc* d, int T, int64_t n_pairs, int 
 }
 
 // Ahead of a call's launches (under the pool's lock, as mx_end): its workspace checked, its stream behind the pool's
-// refills. *mark: the stream's, or null where the call is captured and its stream has none.
+// refills and the table's changes. *mark: the stream's, or null where the call is captured and its stream has none.
 static int mx_begin(brx_pool* p, size_t need, void* workspace, size_t workspace_bytes, hipStream_t s, ReadMark** mark) {
     if (need && (!workspace || ((uintptr_t)workspace & 255))) return fail(BRX_EINVAL, "workspace must be a 256-byte aligned device buffer");
     if (workspace_bytes < need) return fail(BRX_EINVAL, "this call needs %zu bytes of workspace, %zu given", need, workspace_bytes);
@@ -902,7 +932,7 @@ static int mx_begin(brx_pool* p, size_t need, void* workspace, size_t workspace_
     for (int i = 0; i < p->n_marks && !m; ++i)
         if (p->marks[i].stream == s) m = &p->marks[i];
     *mark = m;
-    if (m && m->refills == p->refills) return BRX_OK;
+    if (m && m->refills == p->refills && m->tables == p->tables) return BRX_OK;
     bool captured = false;
     int rc = capturing(s, &captured);
     if (rc || captured) return rc;
@@ -910,6 +940,10 @@ static int mx_begin(brx_pool* p, size_t need, void* workspace, size_t workspace_
     if (m->refills != p->refills) {
         HIP_TRY(hipStreamWaitEvent(s, p->refill_done, 0));
         m->refills = p->refills;
+    }
+    if (m->tables != p->tables) {
+        if ((rc = wait_mark(p->table, s))) return rc;
+        m->tables = p->tables;
     }
     *mark = m;
     return BRX_OK;

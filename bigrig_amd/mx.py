@@ -24,9 +24,9 @@ whole call runs there, its allocations and copies too; the inputs have to be rea
 as soon as the call returns), and its results may be read on the stream that was current once that waits
 for it.
 
-A pool's admissions and its calls wait for each other on whatever streams they are (a stream of torch's; one made
-elsewhere has to outlive the pool's next admission, sync or check). Replays of captured calls are the
-caller's to order with admissions.
+A pool's admissions, its table and its calls wait for each other on whatever streams they are (a stream of torch's;
+one made elsewhere has to outlive the pool's next admission, upload, sync or check). Replays of captured
+calls are the caller's to order with them.
 """
 from __future__ import annotations
 

@@ -316,11 +316,12 @@ int brx_moe_block_forward_noalloc(const brx_layer_desc* d, brx_pool* p, const vo
  * holds a NaN or an infinity gets scale byte 255 and zero codes: it reads as NaN, and so does every
  * product it enters. None of these calls uses the library workspace: scratch comes from the caller,
  * so calls on several streams and captured graphs do not meet as long as their scratch does not. A call
- * waits for the refills of its pool issued before it, and a pool's refills, sync and check wait for the
- * calls issued on it, on whatever streams (calls on more than eight streams may wait for each other). The
- * stream of a call has to outlive the pool's next refill, sync or check, or the pool. A captured call takes
- * no part in this: its replays are the caller's to order with refills, and none is issued, nor the pool
- * synchronized or checked, while a stream of its calls is being captured (BRX_ESTATE). */
+ * waits for the refills of its pool and the changes of its table issued before it, and refills, table
+ * uploads, sync and check wait for the calls issued on the pool, on whatever streams (calls on more than
+ * eight streams may wait for each other). The stream of a call or of a change of the table has to outlive
+ * the pool's next refill, upload, sync or check, or the pool. A captured call takes no part in this: its
+ * replays are the caller's to order with refills, and none is issued, nor the pool synchronized or
+ * checked, while a stream of its calls is being captured (BRX_ESTATE). */
 
 /* Round `batch` matrices of rows x cols values to MXFP4.
  *   x       device, BRX_DT_* values; matrix b's row r starts x_batch_stride * b + x_row_stride * r

@@ -222,3 +222,79 @@ def test_capture_and_refills(gpu, T):
             assert np.array_equal(bits(o), want), shift
     pool.device.check()
     pool.close()
+
+
+@pytest.mark.parametrize("T", [2, 80])
+def test_the_table_and_the_calls_of_other_streams(gpu, T):
+    """Residency moves while a call on one stream is still queued: it reads the experts it was issued with. A
+    call on a stream other than the upload's, which is still queued, reads the new ones."""
+    import torch
+    lay = make_layer(SWIGLU, seed=77, expert_std=0.05)
+    spec = lay.spec
+    _, _, whole, _ = build_gpu_layer(lay, gpu)
+    whole.g2s_device(torch.cuda.current_stream().cuda_stream)
+    x, _, w, _ = _layer_inputs(spec, lay, gpu, T, seed=12)
+    xd, wd = to_dev_bits(x, gpu), dev(w, gpu)
+    low = np.stack([np.arange(T) % 3, (np.arange(T) + 1) % 3], 1).astype(np.int32)
+    ids = [dev(low, gpu), dev(low + 3, gpu)]
+    want = [bits(mx.moe_forward(spec, whole, xd, i, wd)) for i in ids]
+    store = HostStore()
+    store.add_layer(0, lay.experts)
+    pool = ExpertPool(0, spec, 3).build()
+    sw = StreamingSwitchGLU(pool, PinnedFetcher(store), activations="mxfp4")
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for step in range(6):
+        i = step % 2
+        sw.ensure(low + 3 * i)
+        with torch.cuda.stream(b):
+            torch.cuda._sleep(10_000_000)
+            pool.g2s_device(b.cuda_stream)
+        with torch.cuda.stream(a):          # (behind the upload)
+            if step % 3:
+                torch.cuda._sleep(10_000_000)
+            one = mx.moe_forward(spec, pool, xd, ids[i], wd)
+        sw.ensure(low + 3 * (1 - i))        # (the slots' next experts wait for the call, and so does the table)
+        with torch.cuda.stream(b):
+            pool.g2s_device(b.cuda_stream)
+            two = mx.moe_forward(spec, pool, xd, ids[1 - i], wd)
+        torch.cuda.synchronize()
+        assert np.array_equal(bits(one), want[i]) and np.array_equal(bits(two), want[1 - i]), step
+    pool.device.check()
+    pool.close()
+    whole.close()
+
+
+@pytest.mark.parametrize("kind", ["bounded", "host"])
+@pytest.mark.parametrize("T", [2, 90])
+def test_a_bounded_switch_on_streams_in_turn(gpu, kind, T):
+    """Steps of one bounded layer on three streams in turn, some with work ahead of them, each step with a routing of
+    its own: the resident layer's bits."""
+    import torch
+    lay = make_layer(SHARED, seed=92, expert_std=0.05)
+    whole, wpool = _switch(lay, gpu, "resident", "mxfp4")
+    sw, pool = _switch(lay, gpu, kind, "mxfp4")
+    if kind == "host":
+        sw._serve.depth = 2        # (the routing of a step two behind is waited for and acted on)
+    steps = []
+    for k in range(18):
+        x, _, w, sg = _layer_inputs(lay.spec, lay, gpu, T, seed=200 + k)
+        # three experts a step, other ones each time (a step of more leaves no slot of three to give up)
+        idx = ((np.argsort(np.random.default_rng(k).random((T, 3)), 1) + k) % lay.spec.n_experts).astype(np.int32)
+        steps.append((to_dev_bits(x, gpu), dev(idx, gpu), dev(w, gpu), dev(sg, gpu)))
+    want = [bits(whole.forward_combined(*s)) for s in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for k, s in enumerate(steps):
+        if k % 4 == 1:
+            with torch.cuda.stream(streams[k % 3]):
+                torch.cuda._sleep(5_000_000)
+        got.append(sw.forward_combined(*s, stream=streams[k % 3]))
+    torch.cuda.synchronize()
+    for k in range(len(steps)):
+        assert np.array_equal(bits(got[k]), want[k]), k
+    assert pool.evicts > 0
+    pool.device.check()
+    pool.close()
+    wpool.close()
