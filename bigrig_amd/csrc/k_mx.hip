@@ -15,8 +15,8 @@
 // products, fp32 sums in steps of 128 K in order. A row's bits do not depend on its tile.
 //
 // What bounds it. 512 tokens of the gpt-oss shape (16 pairs an expert, 1.70 GB of weights): the weight stream,
-// 227 + 123 us, 5.0 TB/s, where a copy of 1 GiB reaches 5.1. 2048 tokens of the Qwen3 shape under a Zipf law
-// (128 pairs an expert on average, 155 GFLOP): 86 + 76 us, 950 TFLOP/s, and 21 us for the sums (135 MB, 6.4
+// 223 + 126 us, 4.9 TB/s, where a copy of 1 GiB reaches 4.8 to 5.1. 2048 tokens of the Qwen3 shape under a Zipf law
+// (128 pairs an expert on average, 155 GFLOP): 88 + 78 us, 930 TFLOP/s, and 22 us for the sums (135 MB, 6.1
 // TB/s); matrix instructions fill 15% of the time and vector ones half, and the rest is the wait for each chunk's
 // weights: with 64 pairs a tile a wave has 64 + 64 registers of sums and weights, and a second set of weights
 // does not fit.
