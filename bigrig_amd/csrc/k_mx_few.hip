@@ -13,9 +13,9 @@
 // What bounds it: the weights are read once, and a wave requests the whole of its 16 rows (up to 4 chunks,
 // 16 KB; wider rows three chunks at a time) before it multiplies anything, so a call is a few dependent round
 // trips -- the routing, the table, the weights (of rows wider than four chunks once more: the second three are
-// requested behind the first three's products) -- and little else. One token of the gpt-oss shape (53 MB) takes 12.9 + 7.1 us (2.7
-// TB/s), 8 tokens of 256 experts and a shared one (59 MB) 14.4 + 9.2. The gate and up rows are split by
-// entry, the down rows are not (a block has every entry's 16 columns), so that the sum over a token's
+// requested behind the first three's products) -- and little else. One token of the gpt-oss shape (53 MB) takes
+// 12.9 + 7.1 us (2.7 TB/s), 8 tokens of 256 experts and a shared one (59 MB) 14.4 + 9.2. The gate and up rows are
+// split by entry, the down rows are not (a block has every entry's 16 columns), so that the sum over a token's
 // experts is in one block's LDS and needs neither atomics nor a third launch.
 #include <type_traits>
 

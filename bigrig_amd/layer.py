@@ -283,7 +283,7 @@ class StreamingSwitchGLU:
         """Unreduced expert rows [..., k, H] (bf16) for `indices` [..., k]. Given a `stream`, the whole
         call runs there (its allocations and copies too): the inputs have to be ready on it."""
         if stream is not None:
-            return L.on_stream(stream, self.__call__, x, indices)
+            return L.on_stream(stream, StreamingSwitchGLU.__call__, self, x, indices)
         import torch
         H, k = self.spec.hidden, self.spec.top_k
         x2 = x.reshape(-1, H).contiguous()
@@ -314,7 +314,7 @@ class StreamingSwitchGLU:
         """out [T, H] = sum_j w[t,j] * y[t,j] (+ sgate[t] * shared(x_t)), the block's combine
         fused into the expert kernels whenever no span split is needed. `stream` as in `__call__`."""
         if stream is not None:
-            return L.on_stream(stream, self.forward_combined, x2, idx, w, sgate)
+            return L.on_stream(stream, StreamingSwitchGLU.forward_combined, self, x2, idx, w, sgate)
         import torch
         H, k = self.spec.hidden, self.spec.top_k
         T = x2.shape[0]
@@ -372,7 +372,7 @@ class MoELayer:
     def __call__(self, x, stream=None):
         """The block's output, in x's shape. `stream` as in `StreamingSwitchGLU.__call__`."""
         if stream is not None:
-            return L.on_stream(stream, self.__call__, x)
+            return L.on_stream(stream, MoELayer.__call__, self, x)
         x2 = x.reshape(-1, self.spec.hidden).contiguous()
         sw = self.switch
         if sw._sync_free and sw.activations == "bf16":

@@ -106,3 +106,32 @@ def test_memory_is_recorded_on_both_streams(streams, monkeypatch):
     got = L.on_stream("side", call, 3, a, (b, None), {"c": c})
     assert got == [out, None]
     assert marks == [("a", "side"), ("b", "side"), ("c", "side"), ("o", "own")]
+
+
+def test_a_subclass_that_names_its_stream(streams, monkeypatch):
+    """A block or switch whose own call passes a stream on is entered once."""
+    import torch
+    seen = []
+
+    class Switch(ops.StreamingSwitchGLU):
+        def __call__(self, x, indices):
+            return super().__call__(x, indices, stream="side")
+
+        def forward_combined(self, x2, idx, w, sgate=None):
+            return super().forward_combined(x2, idx, w, sgate, stream="side")
+
+    class Block(ops.MoELayer):
+        def __call__(self, x):
+            return super().__call__(x, stream="outer")
+    sw = Switch(_Pool(4, seen, streams), None)
+    assert sw.refresh()
+    monkeypatch.setattr(sw, "_forward", lambda *a, **kw: seen.append(streams[0]))
+    monkeypatch.setattr(ops, "router_topk", lambda *a: (idx, w, None))
+    idx, w = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, 2)
+    x = torch.zeros(1, 64, dtype=torch.bfloat16)
+    sw(x, idx)
+    sw.forward_combined(x, idx, w)
+    sw.activations = "mxfp4"
+    Block(SPEC, None, sw)(x)
+    assert [s for s in seen if not isinstance(s, tuple)] == ["side", "side", "side"]
+    assert streams[0] == "own"
