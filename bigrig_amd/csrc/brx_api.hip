@@ -137,6 +137,19 @@ int ws_reserve(size_t bytes, hipStream_t s, void** out) {
 
 }  // namespace
 
+// For entry points defined elsewhere (block_ops.h).
+namespace brx {
+int api_fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+int api_ready() { return ensure_device(); }
+}  // namespace brx
+
 // Work of one stream that others may have to wait for. Where that is rare, whoever has to records the event (one
 // behind every call costs a call 3.5 us).
 struct Mark {

@@ -358,8 +358,11 @@ class MoELayer:
     operator is installed in (stream.py:1884-1889)."""
 
     def __init__(self, spec: LayerSpec, router_w, switch: StreamingSwitchGLU, router_bias=None,
-                 shared_gate_w=None):
+                 shared_gate_w=None, norms=None):
+        """norms: a `norm.BlockNorms`; the call then takes the residual stream and returns it behind the
+        block, x + scale * gate * n(block(n(x))), instead of the block's output."""
         self.spec = spec
+        self.norms = norms
         self.router_w = router_w
         self.router_bias = router_bias
         self.switch = switch
@@ -370,10 +373,16 @@ class MoELayer:
                            self.shared_gate_w if self.switch.shared is not None else None, stream)
 
     def __call__(self, x, stream=None):
-        """The block's output, in x's shape. `stream` as in `StreamingSwitchGLU.__call__`."""
+        """The block's output (with `norms`: the residual stream behind it), in x's shape. `stream`
+        as in `StreamingSwitchGLU.__call__`."""
         if stream is not None:
             return L.on_stream(stream, MoELayer.__call__, self, x)
         x2 = x.reshape(-1, self.spec.hidden).contiguous()
+        if self.norms is not None:
+            return self.norms.around(self._block, x2).reshape(x.shape)
+        return self._block(x2).reshape(x.shape)
+
+    def _block(self, x2):
         sw = self.switch
         if sw._sync_free and sw.activations == "bf16":
             # every expert resident (or served from host memory): routing, experts and combine
@@ -389,7 +398,6 @@ class MoELayer:
                             sw.shared, out_idx=idx, flags=path_flag(x2.shape[0], self.spec.top_k))
             if idx is not None:
                 sw._after(idx)
-            return out.reshape(x.shape)
+            return out
         idx, w, sg = self.route(x2)
-        out = sw.forward_combined(x2, idx, w, sg)
-        return out.reshape(x.shape)
+        return sw.forward_combined(x2, idx, w, sg)

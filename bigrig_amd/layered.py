@@ -29,12 +29,14 @@ from .spec import LayerSpec
 @dataclass
 class MoEWeights:
     """One MoE block's non-expert weights (device tensors) and where its experts are in the
-    host store: router [E, H], optional logit bias [E], optional shared expert and its gate."""
+    host store: router [E, H], optional logit bias [E], optional shared expert and its gate,
+    optional norms around the block (`norm.BlockNorms`)."""
     layer: int
     router: object
     router_bias: object = None
     shared: object = None
     shared_gate_w: object = None
+    norms: object = None
 
 
 class _SlotSet:
@@ -95,18 +97,22 @@ def prefill(spec: LayerSpec, layers: list, store: HostStore, chunks: list, ring:
     """Run the hidden states `chunks` ([T_j, H] bf16 device tensors, the prompt's chunks in
     order) through the MoE blocks `layers` (MoEWeights, in model order), layer by layer.
 
-    With `residual`, a block's output is added to its input (h <- h + moe(h)); otherwise it
-    replaces it. With `read_ahead` (default), layer i + 1's experts are queued for copying
-    before layer i's chunks, so the copy overlaps their compute; without it, a layer's copy
-    starts only once the previous layer's compute has finished (the serial schedule, for
-    comparison). `progress(done, total)` is called after each layer. Returns the chunks after
-    the last block (new tensors)."""
+    With `residual`, a block's output is added to its input (h <- h + moe(h), or with the block's
+    `norms` h <- h + scale * gate * n(moe(n(h))), the next block's pre-norm made in the same pass);
+    otherwise it replaces it, and norms are refused. With `read_ahead` (default), layer i + 1's
+    experts are queued for copying before layer i's chunks, so the copy overlaps their compute;
+    without it, a layer's copy starts only once the previous layer's compute has finished (the
+    serial schedule, for comparison). `progress(done, total)` is called after each layer. Returns
+    the chunks after the last block (new tensors)."""
     import torch
 
     from . import layer as ops
     if not layers:
         return list(chunks)
+    if not residual and any(lw.norms is not None for lw in layers):
+        raise ValueError("norms around a block are of its residual sum: residual=False has none")
     h = list(chunks)
+    entered = [None] * len(h)       # n(h; the next block's pre-norm), where the block before has made it
     n = len(layers)
     for i, lw in enumerate(layers):
         s = ring.set_for(i)
@@ -116,10 +122,17 @@ def prefill(spec: LayerSpec, layers: list, store: HostStore, chunks: list, ring:
             ring.load(i, store, lw.layer)
         if read_ahead and i + 1 < n and ring.set_for(i + 1).layer != layers[i + 1].layer:
             ring.load(i + 1, store, layers[i + 1].layer)
+        nm = lw.norms
+        after = layers[i + 1].norms if i + 1 < n else None
         for j, x in enumerate(h):
+            if nm is not None:
+                x = entered[j] if entered[j] is not None else nm.enter(x)
             out = ops.moe_block(spec, s, x, lw.router, lw.router_bias, lw.shared_gate_w, lw.shared,
                                 flags=ops.path_flag(x.shape[0], spec.top_k))
-            h[j] = out + x if residual else out
+            if nm is None:
+                h[j] = out + x if residual else out
+            else:
+                h[j], entered[j] = nm.leave(out, h[j], after)
         if progress is not None:
             progress(i + 1, n)
     return h

@@ -34,7 +34,11 @@ EXPORTS = (
     "brx_pool_admit_async", "brx_pool_refill_range_async", "brx_pool_check",
     "brx_moe_block_forward_noalloc", "brx_mx_quantize", "brx_mx_dequantize",
     "brx_mx_workspace_bytes", "brx_mx_expert_product", "brx_mx_moe_forward",
-    "brx_mx_moe_forward_pairs", "brx_mx_combine",
+    "brx_mx_moe_forward_pairs", "brx_mx_combine", "brx_pairs_workspace_bytes",
+    "brx_pairs_plan", "brx_pairs_dispatch", "brx_pairs_combine", "brx_pairs_combine_backward",
+    "brx_grouped_product", "brx_grouped_product_backward_rows",
+    "brx_grouped_product_backward_weight", "brx_norm_forward", "brx_norm_workspace_bytes",
+    "brx_norm_backward",
 )
 
 
@@ -112,6 +116,25 @@ _SIGS = {
     "brx_combine": ([C.POINTER(LayerDesc), _vp, _vp, _vp, _vp, C.c_int, _vp, _vp], C.c_int),
     "brx_dequant": ([C.POINTER(LayerDesc), _vp, C.c_int, C.c_int, _vp, _vp], C.c_int),
     "brx_sort_pairs": ([C.POINTER(LayerDesc), _vp, C.c_int, _vp, _vp, _vp], C.c_int),
+    "brx_pairs_workspace_bytes": ([_i64, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "brx_pairs_plan": ([_vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, C.c_size_t, _vp], C.c_int),
+    "brx_pairs_dispatch": ([_vp, _i64, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp], C.c_int),
+    "brx_pairs_combine": ([_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp], C.c_int),
+    "brx_pairs_combine_backward": ([_vp, _i64, _vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp,
+                                    _vp, _vp], C.c_int),
+    "brx_grouped_product": ([_vp, _vp, _i64, _i64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                             _vp, _vp], C.c_int),
+    "brx_grouped_product_backward_rows": ([_vp, _vp, _i64, _i64, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
+                                           C.c_int, _vp, _vp], C.c_int),
+    "brx_grouped_product_backward_weight": ([_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                             _vp, _vp, _vp], C.c_int),
+    "brx_norm_forward": ([_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, C.c_int, _vp, C.c_int, C.c_int, _vp,
+                          C.c_int, C.c_float, C.c_float, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp],
+                         C.c_int),
+    "brx_norm_workspace_bytes": ([C.c_int, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "brx_norm_backward": ([_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, C.c_int, _vp, C.c_int, C.c_int, _vp,
+                           C.c_int, C.c_float, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                           _vp, _vp, C.c_size_t, _vp], C.c_int),
 }
 
 

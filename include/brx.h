@@ -403,6 +403,71 @@ int brx_dequant(const brx_layer_desc* d, const void* expert, int proj, int share
 int brx_sort_pairs(const brx_layer_desc* d, const int32_t* idx, int T, int32_t* out_order,
                    int32_t* out_offsets, void* stream);
 
+/* ---- around a block's experts
+ * Pairs sorted by expert and back, products of the sorted rows, norms at both ends of a block, each with its
+ * gradient. The reference has no counterpart (its sort is np.argsort on the host, stream.py:1526-1530, and it
+ * trains nothing). None of these calls uses the library workspace: scratch comes from the caller, so calls on
+ * several streams and captured graphs do not meet as long as their scratch does not. Results are the same bits
+ * on every run. `dtype` is that of the values (BRX_DT_*); sums and statistics are fp32. Tensors are contiguous
+ * where no stride is named; outputs overlap neither inputs nor each other. */
+
+/* Plan of a routing: idx [T, k] int32, of E experts. Pairs of an expert outside [0, E) are dropped.
+ *   offsets  [E + 1]  start of each expert's run of rows; entry E: the pairs kept
+ *   order    [T k]    the pair in each row, by expert, stable; -1 behind the last
+ *   position [T, k]   the row of each pair; a dropped pair's is -1 - r, r one of the rows behind the last
+ * E at most 512, k at most 64, T k at most 2^24. workspace: brx_pairs_workspace_bytes (0 up to 16384 pairs). */
+int brx_pairs_workspace_bytes(int64_t n_pairs, int n_experts, size_t* out);
+int brx_pairs_plan(const int32_t* idx, int T, int k, int E, int32_t* order, int32_t* position, int32_t* offsets,
+                   void* workspace, size_t workspace_bytes, void* stream);
+/* rows[position[t, j]] = x[t]; the rows of dropped pairs are cleared. x [T, H], its rows x_row values apart. */
+int brx_pairs_dispatch(const void* x, int64_t x_row, const int32_t* position, int T, int k, int H, int dtype,
+                       void* rows, void* stream);
+/* out[t] = sum_j w[t, j] rows[position[t, j]], fp32, j in order, rounded once; w [T, k] fp32 or NULL (ones: the
+ * gradient of brx_pairs_dispatch). */
+int brx_pairs_combine(const void* rows, const float* w, const int32_t* position, int T, int k, int H, int dtype,
+                      void* out, void* stream);
+/* The gradient of brx_pairs_combine: drows[position[t, j]] = w[t, j] dout[t] (dropped pairs' cleared), dw[t, j] =
+ * <dout[t], rows[position[t, j]]> (dropped: 0). drows or dw may be NULL; rows only where dw is not. */
+int brx_pairs_combine_backward(const void* dout, int64_t dout_row, const void* rows, const float* w,
+                               const int32_t* position, int T, int k, int H, int dtype, void* drows, float* dw,
+                               void* stream);
+
+/* out[r] = W[e] rows[r] (+ bias[e]) for the rows of expert e's run, offsets[e] <= r < offsets[e + 1] (offsets[0] is
+ * taken as 0), and 0 behind the last run. rows [P, K], weight [E, N, K] (w_expert and w_row values between its
+ * experts and rows), bias [E, N] or NULL, offsets [E + 1] int32, out [P, N]; BRX_DT_BF16 or BRX_DT_F16, K and N
+ * multiples of 8 up to 8192, E at most 512, P at most 2^24; rows, weight and out 16-byte aligned, w_row and w_expert
+ * multiples of 8, w_row at most 2^20. Offsets outside [0, P] or out of order name no memory outside the tensors. */
+int brx_grouped_product(const void* rows, const void* weight, int64_t w_expert, int64_t w_row, const void* bias,
+                        const int32_t* offsets, int P, int E, int K, int N, int dtype, void* out, void* stream);
+/* Its gradients: drows[r] = W[e]^T dout[r] (0 behind the last run), and dweight [E, N, K] = sum over e's run of
+ * dout[r] rows[r]^T (0 for an empty run), dbias [E, N] = sum over e's run of dout[r], either NULL. */
+int brx_grouped_product_backward_rows(const void* dout, const void* weight, int64_t w_expert, int64_t w_row,
+                                      const int32_t* offsets, int P, int E, int K, int N, int dtype, void* drows,
+                                      void* stream);
+int brx_grouped_product_backward_weight(const void* dout, const void* rows, const int32_t* offsets, int P, int E, int K,
+                                        int N, int dtype, void* dweight, void* dbias, void* stream);
+
+/* Norms at both ends of a block, n(v; w) = v / sqrt(mean(v^2) + eps) * w:
+ *   u = n(y; post), or y without post;  new_r = r + scale * gate * u;  h = n(new_r; next)
+ * y [T, H] of y_dtype and r [T, H] of r_dtype (y's type, or BRX_DT_F32), rows y_row / r_row values apart. Without y
+ * (NULL): h = n(r; next) alone (next NULL: no weights). new_r is rounded to r_dtype before h is made of it; h has
+ * y_dtype, NULL: not made. post, next [H] and gate have types of their own; gate_form: 0 none, 1 [H], 2 [T], 3
+ * [T, H]. rstd_y, rstd_n [T]: the reciprocal roots, for the gradient, or NULL. H at most 8192, eps at least 2^-126. */
+int brx_norm_forward(const void* y, int64_t y_row, int y_dtype, const void* r, int64_t r_row, int r_dtype,
+                     const void* post, int post_dtype, const void* gate, int gate_form, int gate_dtype,
+                     const void* next, int next_dtype, float scale, float eps, int T, int H, void* new_r, void* h,
+                     float* rstd_y, float* rstd_n, void* stream);
+/* Its gradient. r: what h was made of (new_r; without y: r), rows r_row apart; d_new (r_dtype) and d_h (y_dtype)
+ * contiguous, either NULL; rstd_y (with post) and rstd_n (with d_h) of the forward call. Outputs, each may be NULL: dy
+ * (y_dtype), dr (r_dtype), dgate, dpost, dnext (their tensors' types and shapes). workspace:
+ * brx_norm_workspace_bytes (column sums). */
+int brx_norm_workspace_bytes(int T, int H, size_t* out);
+int brx_norm_backward(const void* y, int64_t y_row, int y_dtype, const void* r, int64_t r_row, int r_dtype,
+                      const void* post, int post_dtype, const void* gate, int gate_form, int gate_dtype,
+                      const void* next, int next_dtype, float scale, int T, int H, const float* rstd_y,
+                      const float* rstd_n, const void* d_new, const void* d_h, void* dy, void* dr, void* dgate,
+                      void* dpost, void* dnext, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
