@@ -40,15 +40,15 @@ __device__ __forceinline__ int y_key(int k) { return 4 * (k & 3); }
 
 // 16 bytes a lane from byte offset `at` of the buffer at p (`bytes` long; past them: zeros) into the 1 KB at `to`. In assembly:
 // where the compiler knows of a copy into LDS in flight, it waits for all of them before each transposing load. It has
-// no result register; whoever reads `to` waits for it (copies_left).
+// no result register; whoever reads `to` waits for it (copies_left). m0, which holds the LDS address, is put back.
 __device__ __forceinline__ void copy16(const void* p, uint32_t bytes, uint32_t at, const void* to) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     const uint64_t base = (uint64_t)(uintptr_t)p;
     const u32x4 r = {(uint32_t)base, (uint32_t)(base >> 32) & 0xFFFFu, bytes, 0x00020000u};
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"((uint32_t)(uintptr_t)(LDS_PTR)to), "v"(at), "s"(r) : "memory", "m0");
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "s"((uint32_t)(uintptr_t)(LDS_PTR)to), "v"(at), "s"(r) : "memory");
 }
-#pragma clang diagnostic pop
 
 // One operand of a tile: `M` values along the output, laid out X or Y, of which wave w of W copies its share.
 template <bool Y, int M, int W>

@@ -23,16 +23,16 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / kWave;
-constexpr int kPlanOne = 16384;       // pairs one block sorts by itself
-constexpr int kPlanBlocks = 64;       // blocks of a longer list, at most
-constexpr int kGroup = 4;             // groups of 64 pairs a wave has in flight
+constexpr int kCopies = 4;            // counters that all lanes add to come so often, 16 neighbouring pairs to one: a popular
+                                      // expert is among each token's (Zipf, 16384 pairs of 128 experts: 11.0 -> 7.0 us)
+constexpr int kPlanSelf = 16384;      // pairs of a list whose blocks count all of it themselves
 
-// Pairs of one block: a multiple of the 64 kGroup a wave takes at a time, over all waves.
-inline int plan_chunk(int64_t n) {
-    const int64_t unit = (int64_t)kPlanThreads * kGroup;
-    if (n <= kPlanOne) return (int)((n + kPlanThreads - 1) / kPlanThreads) * kPlanThreads;
-    const int64_t per = (n + kPlanBlocks - 1) / kPlanBlocks;
-    return (int)((per + unit - 1) / unit * unit);
+// Groups of 64 pairs a wave holds: few, so that a list is spread over CUs, more where there are so many blocks that adding up
+// their counts costs more.
+inline int plan_groups(int64_t n) { return n <= kPlanSelf ? 1 : n <= 64 * 4 * kPlanThreads ? 4 : 16; }
+inline int plan_blocks(int64_t n) {
+    const int64_t chunk = (int64_t)plan_groups(n) * kPlanThreads;
+    return (int)((n + chunk - 1) / chunk);
 }
 
 // Lanes of the wave whose value is this lane's (values below 2^bits).
@@ -49,93 +49,132 @@ __device__ __forceinline__ uint64_t same_lanes(int v, int bits) {
 // Keeps a wave's LDS accesses in the order they are written (they execute in it).
 __device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
-enum { kPlanWhole, kPlanCount, kPlanPlace };
+static_assert((kPlanWaves + 2 * kCopies) * (kMaxExperts + 1) * 4 <= 65536 - 1024, "the counters fit a block's LDS");
 
-// A stable counting sort. A block takes a contiguous chunk of the pairs, wave w of it the w-th contiguous part,
-// so a pair's place is (pairs of lower experts) + (the same expert's pairs in earlier blocks, earlier waves,
-// earlier groups of this wave, lower lanes). A wave's 64 pairs meet their equals by ballots of the id's bits,
-// and one lane of each set of equals counts for all of it, so the counters need no atomics across lanes.
-// Dropped pairs count as expert E. MODE: a list of one block, or the counts of each block and then the places.
-// 8192 / 16384 pairs of 128 experts ... us in one block, 65536 ... us in two launches.
-template <int MODE>
-__global__ __launch_bounds__(kPlanThreads) void k_pairs_plan(PairsPlan p, int chunk) {
-    extern __shared__ int32_t lds[];
+enum { kPlanAlone, kPlanCount, kPlanPlace };
+
+// A stable counting sort. A block takes a contiguous chunk of the pairs, its waves (only as many as the chunk fills) contiguous
+// parts of it, held in registers, so a pair's place is (pairs of lower experts) + (the same expert's pairs in earlier
+// blocks, earlier waves, earlier groups of this wave, lower lanes). A wave's 64 pairs meet their equals by ballots of the
+// id's bits, and one lane of each set of equals counts for all of it, so no order of atomics decides anything. Dropped
+// pairs count as expert E. MODE: alone, each block counting all pairs (one launch), or the counts of each block and then the
+// places.
+template <int MODE, int G>
+__global__ __launch_bounds__(kPlanThreads) void k_pairs_plan(PairsPlan p) {
+    extern __shared__ int32_t hist[];                 // [waves, E1]
     const int E1 = p.E + 1;
-    int32_t* hist = lds;                              // [waves, E1]
     __shared__ int32_t wtot[kPlanWaves];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int n = p.n, base = blockIdx.x * chunk, per = chunk / kPlanWaves, lo = base + wv * per;
+    const int n = p.n, base = blockIdx.x * (G * kPlanThreads), mine_n = min(n - base, G * kPlanThreads);
+    const int waves = MODE == kPlanCount ? kCopies : (mine_n + G * kWave - 1) / (G * kWave);
+    const int lo = base + wv * (G * kWave);
     const int bits = 32 - __builtin_clz(p.E);
-    for (int i = tid; i < kPlanWaves * E1; i += kPlanThreads) hist[i] = 0;
+    int e[G];
+    if (lo < n) {                                     // (whole waves)
+#pragma unroll
+        for (int g = 0; g < G; ++g) e[g] = p.idx[min(lo + g * kWave + lane, n - 1)];
+    }
+    for (int i = tid; i < waves * E1; i += kPlanThreads) hist[i] = 0;
     __syncthreads();
+    if constexpr (MODE == kPlanCount) {
+        if (lo < n) {
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+                if (lo + g * kWave + lane < n) atomicAdd(&hist[(lane >> 4) * E1 + ((unsigned)e[g] < (unsigned)p.E ? e[g] : p.E)], 1);
+        }
+        __syncthreads();
+        if (tid < E1) {
+            int v = 0;
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) v += hist[c * E1 + tid];
+            p.counts[blockIdx.x * E1 + tid] = v;
+        }
+        return;
+    }
+    int32_t* const all = hist + kPlanWaves * E1;      // (alone, of several blocks) counts of earlier blocks' pairs, and of the rest
+    int32_t* const earlier = all + kCopies * E1;
+    const bool several = MODE == kPlanAlone && gridDim.x > 1;
+    if (several) {                                    // uniform
+        for (int i = tid; i < 2 * kCopies * E1; i += kPlanThreads) all[i] = 0;
+        __syncthreads();
+        int v[kPlanSelf / kPlanThreads];              // (all requested at once)
+#pragma unroll
+        for (int i = 0; i < kPlanSelf / kPlanThreads; ++i) v[i] = p.idx[min(i * kPlanThreads + tid, n - 1)];
+#pragma unroll
+        for (int i = 0; i < kPlanSelf / kPlanThreads; ++i) {
+            const int q = i * kPlanThreads + tid, x = (unsigned)v[i] < (unsigned)p.E ? v[i] : p.E;
+            if (q < n) atomicAdd((q < base ? earlier : all) + (lane >> 4) * E1 + x, 1);
+        }
+    }
     int32_t* mine = hist + wv * E1;
-    auto load = [&](int g, int (&e)[kGroup]) __attribute__((always_inline)) {
+    uint64_t m[G];
+    if (lo < n) {
 #pragma unroll
-        for (int u = 0; u < kGroup; ++u) e[u] = p.idx[min(lo + (g + u) * kWave + lane, n - 1)];
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u) e[u] = (unsigned)e[u] < (unsigned)p.E ? e[u] : p.E;
-    };
-    const int groups = per / kWave;
-    for (int g = 0; g < groups; g += kGroup) {
-        int e[kGroup];
-        load(g, e);
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-            const bool in = g + u < groups && lo + (g + u) * kWave + lane < n;
-            const uint64_t m = same_lanes(e[u], bits) & __ballot(in);
-            if (in && lane == __builtin_ctzll(m)) mine[e[u]] += __popcll(m);
-            wave_order();
+        for (int g = 0; g < G; ++g) {
+            e[g] = (unsigned)e[g] < (unsigned)p.E ? e[g] : p.E;
+            const bool in = lo + g * kWave + lane < n;
+            m[g] = same_lanes(e[g], bits) & __ballot(in);
+            if (in && lane == __builtin_ctzll(m[g])) atomicAdd(&mine[e[g]], __popcll(m[g]));
         }
     }
     __syncthreads();
-    // thread e: the waves' counts of expert e into prefixes, their sum, what earlier blocks have of it
+    // thread e: what of expert e the waves have, and earlier blocks
     int total = 0, before = 0;
     if (tid < E1) {
-        for (int w = 0; w < kPlanWaves; ++w) {
-            const int v = hist[w * E1 + tid];
-            hist[w * E1 + tid] = total;
-            total += v;
-        }
-        if constexpr (MODE == kPlanCount) p.counts[blockIdx.x * E1 + tid] = total;
         if constexpr (MODE == kPlanPlace) {
-            total = 0;
+#pragma unroll 8
             for (int b = 0; b < (int)gridDim.x; ++b) {
                 const int v = p.counts[b * E1 + tid];
                 before += b < (int)blockIdx.x ? v : 0;
                 total += v;
             }
+        } else if (several) {
+#pragma unroll
+            for (int c = 0; c < kCopies; ++c) {
+                before += earlier[c * E1 + tid];
+                total += all[c * E1 + tid];
+            }
+            total += before;
+        } else {
+#pragma unroll 4
+            for (int w = 0; w < waves; ++w) total += hist[w * E1 + tid];
         }
     }
-    if constexpr (MODE == kPlanCount) return;
     const int incl = wave_incl_scan(total);
     if (lane == 63) wtot[wv] = incl;
     __syncthreads();
     int off = incl - total;
-    for (int w = 0; w < wv; ++w) off += wtot[w];
+#pragma unroll
+    for (int w = 0; w < kMaxExperts / kWave; ++w) off += w < wv ? wtot[w] : 0;
     if (tid < E1) {
-        if (blockIdx.x == 0) p.offsets[tid] = off;     // (entry E: where the dropped ones start, the pairs kept)
-        for (int w = 0; w < kPlanWaves; ++w) hist[w * E1 + tid] += off + before;
+        if (blockIdx.x == 0) p.offsets[tid] = off;    // (entry E: where the dropped ones start, the pairs kept)
+        int at = off + before;
+#pragma unroll 4
+        for (int w = 0; w < waves; ++w) {
+            const int v = hist[w * E1 + tid];
+            hist[w * E1 + tid] = at;
+            at += v;
+        }
     }
     __syncthreads();
-    for (int g = 0; g < groups; g += kGroup) {
-        int e[kGroup];
-        load(g, e);
+    if (lo >= n) return;
+    int at[G];
 #pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-            const int q = lo + (g + u) * kWave + lane;
-            const bool in = g + u < groups && q < n;
-            const uint64_t m = same_lanes(e[u], bits) & __ballot(in);
-            const int at = mine[e[u]];
-            wave_order();
-            if (in) {
-                const int r = at + __popcll(m & ((1ull << lane) - 1ull));
-                const bool kept = e[u] < p.E;
-                p.position[q] = kept ? r : -1 - r;
-                p.order[r] = kept ? q : -1;
-                if (lane == __builtin_ctzll(m)) mine[e[u]] = at + __popcll(m);
-            }
-            wave_order();
-        }
+    for (int g = 0; g < G; ++g) {
+        const bool in = lo + g * kWave + lane < n;
+        at[g] = mine[e[g]];
+        wave_order();
+        if (in && lane == __builtin_ctzll(m[g])) atomicAdd(&mine[e[g]], __popcll(m[g]));
+        wave_order();
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const int q = lo + g * kWave + lane;
+        if (q >= n) break;
+        const int r = at[g] + __popcll(m[g] & ((1ull << lane) - 1ull));
+        const bool kept = e[g] < p.E;
+        p.position[q] = kept ? r : -1 - r;
+        p.order[r] = kept ? q : -1;
     }
 }
 
@@ -333,24 +372,26 @@ inline int row_lanes(int H, int vec) {
 }  // namespace
 
 size_t pairs_plan_workspace(int64_t n, int E) {
-    if (n <= kPlanOne) return 0;
-    const int chunk = plan_chunk(n);
-    return (size_t)((n + chunk - 1) / chunk) * (E + 1) * sizeof(int32_t);
+    return n <= kPlanSelf ? 0 : (size_t)plan_blocks(n) * (E + 1) * sizeof(int32_t);
+}
+
+template <int MODE>
+static hipError_t plan_launch(const PairsPlan& p, hipStream_t s) {
+    const int groups = plan_groups(p.n), per = groups * kWave, blocks = p.n ? plan_blocks(p.n) : 1;
+    // counters: of each wave (a list of one block has only as many as it fills), and the two of a list whose blocks count it all
+    const int sets = MODE == kPlanCount ? kCopies
+                     : blocks == 1 ? (p.n ? (p.n + per - 1) / per : 1) : kPlanWaves + (MODE == kPlanAlone ? 2 * kCopies : 0);
+    const size_t lds = (size_t)sets * (p.E + 1) * sizeof(int32_t);
+    if constexpr (MODE == kPlanAlone) hipLaunchKernelGGL((k_pairs_plan<MODE, 1>), dim3(blocks), dim3(kPlanThreads), lds, s, p);
+    else if (groups == 4) hipLaunchKernelGGL((k_pairs_plan<MODE, 4>), dim3(blocks), dim3(kPlanThreads), lds, s, p);
+    else hipLaunchKernelGGL((k_pairs_plan<MODE, 16>), dim3(blocks), dim3(kPlanThreads), lds, s, p);
+    return hipGetLastError();
 }
 
 hipError_t launch_pairs_plan(const PairsPlan& p, hipStream_t s) {
-    const int chunk = plan_chunk(p.n);
-    const int blocks = (p.n + chunk - 1) / chunk;
-    const size_t lds = (size_t)kPlanWaves * (p.E + 1) * sizeof(int32_t);
-    if (p.n <= kPlanOne) {
-        hipLaunchKernelGGL(k_pairs_plan<kPlanWhole>, dim3(1), dim3(kPlanThreads), lds, s, p, chunk);
-        return hipGetLastError();
-    }
-    hipLaunchKernelGGL(k_pairs_plan<kPlanCount>, dim3(blocks), dim3(kPlanThreads), lds, s, p, chunk);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_pairs_plan<kPlanPlace>, dim3(blocks), dim3(kPlanThreads), lds, s, p, chunk);
-    return hipGetLastError();
+    if (p.n <= kPlanSelf) return plan_launch<kPlanAlone>(p, s);
+    const hipError_t e = plan_launch<kPlanCount>(p, s);
+    return e != hipSuccess ? e : plan_launch<kPlanPlace>(p, s);
 }
 
 #define BRX_ROWS(KERNEL, DT)                                                                                           \

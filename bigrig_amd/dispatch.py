@@ -83,9 +83,10 @@ def plan(idx, n_experts: int, stream=None) -> Dispatch:
     offsets = idx.new_empty(n_experts + 1)
     need = _plan_bytes(n, n_experts)
     ws = idx.new_empty(need // 4) if need else None
-    L.check(L.load().brx_pairs_plan(idx.data_ptr(), T, k, n_experts, order.data_ptr(), position.data_ptr(),
-                                    offsets.data_ptr(), None if ws is None else ws.data_ptr(), need,
-                                    _handle(device)))
+    rc = L.load().brx_pairs_plan(idx.data_ptr(), T, k, n_experts, order.data_ptr(), position.data_ptr(),
+                                 offsets.data_ptr(), None if ws is None else ws.data_ptr(), need, _handle(device))
+    if rc:
+        L.check(rc)
     return Dispatch(order, position, offsets)
 
 
@@ -109,8 +110,10 @@ def _gather(x, position, T: int, k: int):
     device = _on_device(x, position)
     H = x.shape[1]
     rows = x.new_empty((T * k, H))
-    L.check(L.load().brx_pairs_dispatch(x.data_ptr(), x.stride(0) if T > 1 else H, position.data_ptr(), T, k, H,
-                                        _TYPES[x.dtype], rows.data_ptr(), _handle(device)))
+    rc = L.load().brx_pairs_dispatch(x.data_ptr(), x.stride(0) if T > 1 else H, position.data_ptr(), T, k, H,
+                                     _TYPES[x.dtype], rows.data_ptr(), _handle(device))
+    if rc:
+        L.check(rc)
     return rows
 
 
@@ -118,8 +121,10 @@ def _sum(rows, w, position, T: int, k: int):
     device = _on_device(rows, w, position)
     H = rows.shape[1]
     out = rows.new_empty((T, H))
-    L.check(L.load().brx_pairs_combine(rows.data_ptr(), None if w is None else w.data_ptr(), position.data_ptr(), T, k,
-                                       H, _TYPES[rows.dtype], out.data_ptr(), _handle(device)))
+    rc = L.load().brx_pairs_combine(rows.data_ptr(), None if w is None else w.data_ptr(), position.data_ptr(), T, k, H,
+                                    _TYPES[rows.dtype], out.data_ptr(), _handle(device))
+    if rc:
+        L.check(rc)
     return out
 
 

@@ -142,7 +142,11 @@ def _backward(y, r, post, gate, form, nxt, scale, rstd_y, rstd_n, d_new, d_h, ne
 
 
 def _grads(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _check_count(T: int) -> None:

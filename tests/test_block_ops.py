@@ -117,7 +117,7 @@ def call(name, *args):
 def test_workspace_sizes():
     out = C.c_size_t()
     lib = L.load()
-    for n, E, want in ((0, 4, 0), (16384, 512, 0), (16385, 4, 5 * 4 * 5), (1 << 24, 512, 64 * 513 * 4)):
+    for n, E, want in ((0, 4, 0), (16384, 512, 0), (16385, 4, 5 * 5 * 4), (1 << 24, 512, 1024 * 513 * 4)):
         L.check(lib.brx_pairs_workspace_bytes(n, E, C.byref(out)))
         assert out.value == want, (n, E)
     for bad in ((-1, 4), ((1 << 24) + 1, 4), (8, 0), (8, 513)):

@@ -43,7 +43,8 @@ def check_plan(D, idx, E):
 
 @pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 128), (0, 4, 8), (7, 8, 256), (63, 1, 3), (64, 2, 5), (65, 4, 512),
                                    (333, 8, 60), (2048, 8, 128), (2049, 8, 128), (4097, 4, 512), (40000, 2, 17),
-                                   (70001, 8, 128), (3, 64, 100), (50, 3, 2)])
+                                   (70001, 8, 128), (3, 64, 100), (50, 3, 2), (2000, 8, 512), (129, 8, 512), (128, 8, 511),
+                                   (2048, 8, 512)])
 @pytest.mark.parametrize("drop", [0.0, 0.4])
 def test_plan(D, T, k, E, drop):
     check_plan(D, routing(T, k, E, T + k, drop), E)

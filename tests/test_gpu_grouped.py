@@ -90,6 +90,57 @@ def test_wide(G):
     check(G, [40, 3], 264, 8192, torch.float16, bias=True)
 
 
+@pytest.mark.parametrize("dtype,bias", [(torch.bfloat16, True), (torch.float16, False)])
+@pytest.mark.parametrize("N,K", [(4104, 72), (72, 4104)])
+def test_enough_rows_for_the_persistent_tiles(G, dtype, bias, N, K):
+    # 17 whole tiles of 256 rows by 17 of 256 columns (forward, or the rows' gradient): tiles of 1 to 4 fragments a wave, runs
+    # that end in each, empty ones, rows behind the last; sums of one stage, of several, and ending inside one
+    counts = [0, 1, 64, 65, 128, 129, 192, 193, 256, 257, 0, 700, 1500, 33, 1000, 0]
+    check(G, counts, N, K, dtype, bias=bias, behind=300)
+
+
+def test_persistent_tiles_of_more_than_the_cus(G):
+    # every block takes several tiles, short sums among long ones
+    g = torch.Generator().manual_seed(3)
+    counts = torch.randint(0, 300, (200,), generator=g).tolist()
+    check(G, counts, 1032, 200, torch.bfloat16, bias=True, behind=5)
+    check(G, counts, 1032, 56, torch.float16, bias=False)
+
+
+def test_persistent_tiles_keep_a_nan_in_its_row(G):
+    N, K = 4104, 72
+    offsets, at = offsets_of([3, 500, 130, 0, 4000])
+    rows, w = rand((at[-1], K), torch.bfloat16, 1), rand((5, N, K), torch.bfloat16, 2)
+    ref = G.product(rows, w, offsets)
+    bad = rows.clone()
+    bad[[2, 3, 502, 700]] = float("nan")
+    out = G.product(bad, w, offsets)
+    keep = torch.ones(at[-1], dtype=torch.bool, device="cuda")
+    keep[[2, 3, 502, 700]] = False
+    assert torch.isnan(out[~keep]).all() and torch.equal(out[keep], ref[keep])
+    wr = w.clone().requires_grad_()
+    d = rand((at[-1], N), torch.bfloat16, 3)
+    bad = rows.clone()
+    bad[2] = float("nan")
+    (g,) = torch.autograd.grad(G.product(bad, wr, offsets), wr, d)
+    assert torch.isnan(g[0]).all() and torch.isfinite(g[1:].float()).all() and not g[3].any()
+
+
+def test_thin_and_square_tiles_agree_with_the_persistent_ones_row_by_row(G):
+    # a row's value does not depend on how many others there are, up to the order of its fp32 sum
+    N, K = 4104, 264
+    w = rand((4, N, K), torch.bfloat16, 1, scale=0.1)
+    rows = rand((4800, K), torch.bfloat16, 2)
+    full = G.product(rows, w, offsets_of([1200] * 4)[0])
+    for take in (1, 5, 8, 40, 300):
+        pick = torch.cat([torch.arange(e * 1200, e * 1200 + take) for e in range(4)]).cuda()
+        part = G.product(rows[pick], w, offsets_of([take] * 4)[0])
+        m = rows[pick].double().cpu().abs() @ torch.ones(K, dtype=torch.float64)
+        # (weights are below 0.6 in size: 0.1 times normal values below 6; two fp32 sums and the other's rounding)
+        close(part, full[pick].double().cpu(), 2 * K * SUM_U * 0.6 * m[:, None] + 2.0 ** -8 * full[pick].double().cpu().abs(),
+              f"{take}")
+
+
 def test_a_long_run_beside_short_ones(G):
     check(G, [1, 3000, 1], 136, 72, torch.bfloat16)
 
