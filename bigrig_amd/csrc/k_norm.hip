@@ -11,8 +11,8 @@
 // Column sums are made in two steps, each block's over the rows it took and then those of the blocks, in a fixed
 // order.
 //
-// Bound: memory, each input read once and each output written once. A row stays in registers, 8 values a
-// run: one wave a row up to 1024 values, a block of four beyond.
+// Bound: memory, each input read once and each output written once; a row stays in registers, 8 values a run. 16384 x 2048,
+// bf16 with an fp32 residual, both norms and a gate: 74 us (5.4 TB/s), its gradient 126 us (4.8 TB/s).
 #include "block_ops.h"
 
 namespace brx {
@@ -188,32 +188,49 @@ __global__ __launch_bounds__(kThreads) void k_norm_backward(NormArgs a) {
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int i = 0; i < V; ++i) sum_post[c][i] = sum_gate[c][i] = sum_next[c][i] = 0.f;
+    // the columns' weights, in registers where these suffice
+    constexpr bool kKeep = NC <= 2;
+    float w_post[kKeep ? NC : 1][V], w_next[kKeep ? NC : 1][V], w_gate[kKeep ? NC : 1][V];
+    if constexpr (kKeep) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) w_post[c][i] = w_next[c][i] = w_gate[c][i] = 1.0f;
+            if (a.post) load8_any(a.post, a.post_dt, 0, rn[c], H, w_post[c]);
+            if (a.next) load8_any(a.next, a.next_dt, 0, rn[c], H, w_next[c]);
+            if (a.gate_form == kGateChannel) load8_any(a.gate, a.gate_dt, 0, rn[c], H, w_gate[c]);
+        }
+    }
     for (int t = blockIdx.x * kRows + group; t < a.T; t += gridDim.x * kRows) {
-        float D[NC][V], y[NC][V];
+        float D[NC][V], y[NC][V], x[NC][V], g[NC][V];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
 #pragma unroll
             for (int i = 0; i < V; ++i) D[c][i] = 0.f;
             if (a.d_new) load8<RD>(a.d_new, (int64_t)t * H, rn[c], H, D[c]);
             if (a.y) load8<YD>(a.y, (int64_t)t * a.y_row, rn[c], H, y[c]);
-        }
-        if (a.d_h) {
-            float x[NC][V], g[NC][V], s = 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
+            if (a.d_h) {
                 load8<RD>(a.r, (int64_t)t * a.r_row, rn[c], H, x[c]);
                 load8<YD>(a.d_h, (int64_t)t * H, rn[c], H, g[c]);
             }
+        }
+        if (a.d_h) {
+            float s = 0.f;
             const float rstd = a.rstd_n[t];
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 float w[V];
-                if (a.next) load8_any(a.next, a.next_dt, 0, rn[c], H, w);
+                if constexpr (!kKeep) {
+                    if (a.next) load8_any(a.next, a.next_dt, 0, rn[c], H, w);
+                    else
+#pragma unroll
+                        for (int i = 0; i < V; ++i) w[i] = 1.0f;
+                }
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     x[c][i] *= rstd;
                     sum_next[c][i] = __builtin_fmaf(g[c][i], x[c][i], sum_next[c][i]);
-                    if (a.next) g[c][i] *= w[i];
+                    g[c][i] *= kKeep ? w_next[c][i] : w[i];
                     s = counts(rn[c], H, i) ? __builtin_fmaf(g[c][i], x[c][i], s) : s;
                 }
             }
@@ -236,21 +253,29 @@ __global__ __launch_bounds__(kThreads) void k_norm_backward(NormArgs a) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             float w[V], g[V], dg[V];
-            if (a.post) load8_any(a.post, a.post_dt, 0, rn[c], H, w);
+            if constexpr (!kKeep) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) g[i] = g_row;
-            if (a.gate_form == kGateChannel) load8_any(a.gate, a.gate_dt, 0, rn[c], H, g);
-            if (a.gate_form == kGateFull) load8_any(a.gate, a.gate_dt, (int64_t)t * H, rn[c], H, g);
+                for (int i = 0; i < V; ++i) w[i] = 1.0f;
+                if (a.post) load8_any(a.post, a.post_dt, 0, rn[c], H, w);
+            }
+            if (a.gate_form == kGateFull) {
+                load8_any(a.gate, a.gate_dt, (int64_t)t * H, rn[c], H, g);
+            } else if (!kKeep && a.gate_form == kGateChannel) {
+                load8_any(a.gate, a.gate_dt, 0, rn[c], H, g);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[i] = kKeep && a.gate_form == kGateChannel ? w_gate[c][i] : g_row;
+            }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                const float wp = kKeep ? w_post[c][i] : w[i];
                 y[c][i] *= rstd;                                                // y^ (or y)
-                const float u = a.post ? y[c][i] * w[i] : y[c][i];
-                dg[i] = a.scale * u * D[c][i];
+                dg[i] = a.scale * (y[c][i] * wp) * D[c][i];
                 sum_gate[c][i] += dg[i];
                 gs = counts(rn[c], H, i) ? gs + dg[i] : gs;
                 const float du = a.scale * g[i] * D[c][i];
                 sum_post[c][i] = __builtin_fmaf(du, y[c][i], sum_post[c][i]);
-                D[c][i] = a.post ? du * w[i] : du;                              // q
+                D[c][i] = du * wp;                                              // q
                 s = counts(rn[c], H, i) ? __builtin_fmaf(D[c][i], y[c][i], s) : s;
             }
             if (a.gate_form == kGateFull && a.dgate) {
@@ -331,48 +356,55 @@ __global__ __launch_bounds__(kColThreads) void k_norm_columns(NormArgs a, int bl
     }
 }
 
-// Threads of a row: a wave up to 1024 values, else a block.
-inline int row_threads(int H) { return H <= 1024 ? kWave : kThreads; }
+// Threads of a row: a wave up to 1024 values, else a block; of a gradient's, whose block sums columns over its rows, a wave up
+// to 512 (4999 x 1001, fp16: a wave a row 26 us, a block 17.6).
+constexpr int kWaveRow = 1024, kWaveRowBack = 512;
+inline int threads_of(int H, int wave_row) { return H <= wave_row ? kWave : kThreads; }
+
+// Blocks of a gradient: as many as its registers let run at once, three a CU (16384 x 2048, bf16 with an fp32 residual, out of
+// cold memory, us: 512 blocks 163, 768 150, 1024 182; 4999 x 1001 26, 22, 28).
+constexpr int kBackBlocks = 768;
 
 }  // namespace
 
 int norm_blocks(int T, int H) {
-    const int per = kThreads / row_threads(H);
+    const int per = kThreads / threads_of(H, kWaveRowBack);
     const int most = (T + per - 1) / per;
-    return most < 1024 ? most : 1024;
+    return most < kBackBlocks ? most : kBackBlocks;
 }
 
-#define BRX_SHAPE(KERNEL, YD, RD, GRID, LDS)                                                                           \
+#define BRX_SHAPE(KERNEL, YD, RD, WAVE_ROW, GRID, LDS)                                                                 \
     do {                                                                                                               \
-        const int nc = (a.H + row_threads(a.H) * V - 1) / (row_threads(a.H) * V);                                      \
         if (a.H <= 512) hipLaunchKernelGGL((KERNEL<YD, RD, kWave, 1>), GRID, dim3(kThreads), LDS, s, a);               \
-        else if (a.H <= 1024) hipLaunchKernelGGL((KERNEL<YD, RD, kWave, 2>), GRID, dim3(kThreads), LDS, s, a);         \
-        else if (nc == 1) hipLaunchKernelGGL((KERNEL<YD, RD, kThreads, 1>), GRID, dim3(kThreads), 0, s, a);            \
-        else if (nc == 2) hipLaunchKernelGGL((KERNEL<YD, RD, kThreads, 2>), GRID, dim3(kThreads), 0, s, a);            \
+        else if (WAVE_ROW > 512 && a.H <= 1024)                                                                        \
+            hipLaunchKernelGGL((KERNEL<YD, RD, WAVE_ROW <= 512 ? kThreads : kWave, WAVE_ROW <= 512 ? 1 : 2>), GRID,    \
+                               dim3(kThreads), 0, s, a);                                                               \
+        else if (a.H <= kThreads * V) hipLaunchKernelGGL((KERNEL<YD, RD, kThreads, 1>), GRID, dim3(kThreads), 0, s, a);\
+        else if (a.H <= 2 * kThreads * V) hipLaunchKernelGGL((KERNEL<YD, RD, kThreads, 2>), GRID, dim3(kThreads), 0, s, a);\
         else hipLaunchKernelGGL((KERNEL<YD, RD, kThreads, 4>), GRID, dim3(kThreads), 0, s, a);                         \
     } while (0)
 // (y's type, r's type: equal, or r fp32)
-#define BRX_TYPES(KERNEL, GRID, LDS)                                                                                   \
+#define BRX_TYPES(KERNEL, W, GRID, LDS)                                                                                \
     do {                                                                                                               \
-        if (y_dt == BRX_DT_F32) BRX_SHAPE(KERNEL, BRX_DT_F32, BRX_DT_F32, GRID, LDS);                                  \
-        else if (y_dt == BRX_DT_BF16 && r_dt == y_dt) BRX_SHAPE(KERNEL, BRX_DT_BF16, BRX_DT_BF16, GRID, LDS);          \
-        else if (y_dt == BRX_DT_BF16) BRX_SHAPE(KERNEL, BRX_DT_BF16, BRX_DT_F32, GRID, LDS);                           \
-        else if (r_dt == y_dt) BRX_SHAPE(KERNEL, BRX_DT_F16, BRX_DT_F16, GRID, LDS);                                   \
-        else BRX_SHAPE(KERNEL, BRX_DT_F16, BRX_DT_F32, GRID, LDS);                                                     \
+        if (y_dt == BRX_DT_F32) BRX_SHAPE(KERNEL, BRX_DT_F32, BRX_DT_F32, W, GRID, LDS);                               \
+        else if (y_dt == BRX_DT_BF16 && r_dt == y_dt) BRX_SHAPE(KERNEL, BRX_DT_BF16, BRX_DT_BF16, W, GRID, LDS);       \
+        else if (y_dt == BRX_DT_BF16) BRX_SHAPE(KERNEL, BRX_DT_BF16, BRX_DT_F32, W, GRID, LDS);                        \
+        else if (r_dt == y_dt) BRX_SHAPE(KERNEL, BRX_DT_F16, BRX_DT_F16, W, GRID, LDS);                                \
+        else BRX_SHAPE(KERNEL, BRX_DT_F16, BRX_DT_F32, W, GRID, LDS);                                                  \
     } while (0)
 
 hipError_t launch_norm_forward(const NormArgs& a, int y_dt, int r_dt, hipStream_t s) {
-    const int per = kThreads / row_threads(a.H);
+    const int per = kThreads / threads_of(a.H, kWaveRow);
     const dim3 grid((a.T + per - 1) / per);
-    BRX_TYPES(k_norm_forward, grid, 0);
+    BRX_TYPES(k_norm_forward, kWaveRow, grid, 0);
     return hipGetLastError();
 }
 
 hipError_t launch_norm_backward(const NormArgs& a, int y_dt, int r_dt, hipStream_t s) {
     const int blocks = norm_blocks(a.T, a.H);
     const dim3 grid(blocks);
-    const size_t lds = (size_t)a.H * sizeof(float);     // (where a block has several row groups)
-    BRX_TYPES(k_norm_backward, grid, lds);
+    const size_t lds = (size_t)a.H * sizeof(float);     // (blocks of several rows)
+    BRX_TYPES(k_norm_backward, kWaveRowBack, grid, lds);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (!a.dpost && !a.dnext && !(a.dgate && a.gate_form == kGateChannel)) return hipSuccess;
