@@ -6,7 +6,7 @@ using namespace brx;
 
 namespace {
 
-constexpr int64_t kMaxRows = (int64_t)1 << 24;      // pairs, sorted rows or tokens of one call
+constexpr int64_t kMaxRows = (int64_t)1 << 23;      // pairs, sorted rows or tokens of one call: a grid of a block a row stays under 2^32 threads
 constexpr int64_t kMaxRowStride = (int64_t)1 << 20; // of a weight: a tile's offsets stay inside 31 bits
 
 int hip_result(hipError_t e, const char* what) {

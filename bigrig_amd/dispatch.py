@@ -28,7 +28,7 @@ import torch
 from . import lib as L
 from .mx import _handle, _on_device
 
-MAX_PAIRS = 1 << 24     # (token, expert) pairs of one call
+MAX_PAIRS = 1 << 23     # (token, expert) pairs of one call
 MAX_EXPERTS = 512
 MAX_TOP_K = 64
 MAX_WIDTH = 8192        # values of a row

@@ -111,6 +111,10 @@ def prefill(spec: LayerSpec, layers: list, store: HostStore, chunks: list, ring:
         return list(chunks)
     if not residual and any(lw.norms is not None for lw in layers):
         raise ValueError("norms around a block are of its residual sum: residual=False has none")
+    if any(lw.norms is not None for lw in layers) and any(lw.norms is None for lw in layers):
+        for x in chunks:
+            if x.dtype != torch.bfloat16:
+                raise ValueError(f"chunks of {x.dtype} through a block without norms, which reads bfloat16")
     h = list(chunks)
     entered = [None] * len(h)       # n(h; the next block's pre-norm), where the block before has made it
     n = len(layers)

@@ -415,7 +415,7 @@ int brx_sort_pairs(const brx_layer_desc* d, const int32_t* idx, int T, int32_t* 
  *   offsets  [E + 1]  start of each expert's run of rows; entry E: the pairs kept
  *   order    [T k]    the pair in each row, by expert, stable; -1 behind the last
  *   position [T, k]   the row of each pair; a dropped pair's is -1 - r, r one of the rows behind the last
- * E at most 512, k at most 64, T k at most 2^24. workspace: brx_pairs_workspace_bytes (0 up to 16384 pairs). */
+ * E at most 512, k at most 64, T k at most 2^23. workspace: brx_pairs_workspace_bytes (0 up to 16384 pairs). */
 int brx_pairs_workspace_bytes(int64_t n_pairs, int n_experts, size_t* out);
 int brx_pairs_plan(const int32_t* idx, int T, int k, int E, int32_t* order, int32_t* position, int32_t* offsets,
                    void* workspace, size_t workspace_bytes, void* stream);
@@ -435,7 +435,7 @@ int brx_pairs_combine_backward(const void* dout, int64_t dout_row, const void* r
 /* out[r] = W[e] rows[r] (+ bias[e]) for the rows of expert e's run, offsets[e] <= r < offsets[e + 1] (offsets[0] is
  * taken as 0), and 0 behind the last run. rows [P, K], weight [E, N, K] (w_expert and w_row values between its
  * experts and rows), bias [E, N] or NULL, offsets [E + 1] int32, out [P, N]; BRX_DT_BF16 or BRX_DT_F16, K and N
- * multiples of 8 up to 8192, E at most 512, P at most 2^24; rows, weight and out 16-byte aligned, w_row and w_expert
+ * multiples of 8 up to 8192, E at most 512, P at most 2^23; rows, weight and out 16-byte aligned, w_row and w_expert
  * multiples of 8, w_row at most 2^20. Offsets outside [0, P] or out of order name no memory outside the tensors. */
 int brx_grouped_product(const void* rows, const void* weight, int64_t w_expert, int64_t w_row, const void* bias,
                         const int32_t* offsets, int P, int E, int K, int N, int dtype, void* out, void* stream);
@@ -452,7 +452,7 @@ int brx_grouped_product_backward_weight(const void* dout, const void* rows, cons
  * y [T, H] of y_dtype and r [T, H] of r_dtype (y's type, or BRX_DT_F32), rows y_row / r_row values apart. Without y
  * (NULL): h = n(r; next) alone (next NULL: no weights). new_r is rounded to r_dtype before h is made of it; h has
  * y_dtype, NULL: not made. post, next [H] and gate have types of their own; gate_form: 0 none, 1 [H], 2 [T], 3
- * [T, H]. rstd_y, rstd_n [T]: the reciprocal roots, for the gradient, or NULL. H at most 8192, eps at least 2^-126. */
+ * [T, H]. rstd_y, rstd_n [T]: the reciprocal roots, for the gradient, or NULL. H at most 8192, T at most 2^23, eps at least 2^-126. */
 int brx_norm_forward(const void* y, int64_t y_row, int y_dtype, const void* r, int64_t r_row, int r_dtype,
                      const void* post, int post_dtype, const void* gate, int gate_form, int gate_dtype,
                      const void* next, int next_dtype, float scale, float eps, int T, int H, void* new_r, void* h,

@@ -28,7 +28,7 @@ def plan(T=4, k=2, E=3):
     (torch.zeros((4, 2), dtype=torch.int64), 4, "int32"), (torch.zeros(8, dtype=I), 4, "T, k"),
     (torch.zeros((4, 2), dtype=I), 0, "experts"), (torch.zeros((4, 2), dtype=I), 513, "experts"),
     (torch.zeros((4, 0), dtype=I), 4, "a token"), (torch.zeros((1, 65), dtype=I), 128, "a token"),
-    (meta(1 << 21, 9, dtype=I), 16, "pairs"), (torch.zeros((4, 2), dtype=I), 4, "GPU")])
+    (meta(1 << 20, 9, dtype=I), 16, "pairs"), (torch.zeros((4, 2), dtype=I), 4, "GPU")])
 def test_plan_refuses(idx, E, what):
     with pytest.raises(ValueError, match=what):
         D.plan(idx, E)
@@ -40,7 +40,7 @@ def test_plan_refuses(idx, E, what):
     (torch.zeros((4, 8)), plan(), "GPU"),
     (torch.zeros((4, 8)), plan()._replace(position=torch.zeros((4, 2))), "int32"),
     (torch.zeros((4, 8)), plan()._replace(position=torch.zeros((2, 4), dtype=I).t()), "contiguous"),
-    (meta(1 << 21, 8), plan()._replace(position=meta(1 << 21, 9, dtype=I)), "at most")])
+    (meta(1 << 20, 8), plan()._replace(position=meta(1 << 20, 9, dtype=I)), "at most")])
 def test_dispatch_refuses(x, p, what):
     with pytest.raises(ValueError, match=what):
         D.dispatch(x, p)
@@ -66,7 +66,7 @@ def off(E):
     (meta(4, 16), meta(2, 8, 8), off(2), None, "E, N, K"), (meta(4, 8), meta(8, 8), off(2), None, "E, N, K"),
     (meta(4, 12), meta(2, 8, 12), off(2), None, "multiple of 8"), (meta(4, 8), meta(2, 20, 8), off(2), None, "multiple of 8"),
     (meta(4, 8), meta(2, 8200, 8), off(2), None, "8192"), (meta(4, 8), meta(0, 8, 8), off(0), None, "experts"),
-    (meta(4, 8), meta(513, 8, 8), off(513), None, "experts"), (meta((1 << 24) + 1, 8), meta(2, 8, 8), off(2), None, "rows"),
+    (meta(4, 8), meta(513, 8, 8), off(513), None, "experts"), (meta((1 << 23) + 1, 8), meta(2, 8, 8), off(2), None, "rows"),
     (meta(4, 8), meta(2, 8, 8), off(3), None, "offsets"), (meta(4, 8), meta(2, 8, 8), off(2).long(), None, "offsets"),
     (meta(4, 8), meta(2, 8, 8), off(2), meta(2, 16), "bias"),
     (meta(4, 8), meta(2, 8, 8).transpose(1, 2), off(2), None, "contiguous"),
@@ -82,7 +82,7 @@ def test_product_refuses(rows, weight, offsets, bias, what):
     (torch.zeros((4, 8), dtype=B), dict(dtype=S), "own type"), (torch.zeros(()), {}, "dimensions"),
     (torch.zeros((4, 8200)), {}, "8192"), (torch.zeros((4, 0)), {}, "values"), (torch.zeros((4, 8)), dict(eps=0.0), "eps"),
     (torch.zeros((4, 8)), dict(eps=float("nan")), "eps"), (torch.zeros((4, 8)), dict(weight=torch.zeros(7)), "weight"),
-    (torch.zeros((4, 8)), dict(weight=torch.zeros(8, dtype=I)), "weight"), (meta((1 << 24) + 1, 8), {}, "rows"),
+    (torch.zeros((4, 8)), dict(weight=torch.zeros(8, dtype=I)), "weight"), (meta((1 << 23) + 1, 8), {}, "rows"),
     (torch.zeros((4, 8)), {}, "GPU")])
 def test_enter_refuses(x, kw, what):
     with pytest.raises(ValueError, match=what):
@@ -108,6 +108,11 @@ def test_prefill_refuses_norms_without_a_residual_sum():
         prefill(None, [MoEWeights(0, None, norms=M.BlockNorms())], None, [], None, residual=False)
 
 
+def test_prefill_refuses_other_types_through_a_block_without_norms():
+    with pytest.raises(ValueError, match="bfloat16"):
+        prefill(None, [MoEWeights(0, None, norms=M.BlockNorms()), MoEWeights(1, None)], None, [torch.zeros((2, 8))], None)
+
+
 # ------------------------------------------------------------------ the C-ABI
 def call(name, *args):
     rc = getattr(L.load(), name)(*args)
@@ -117,15 +122,15 @@ def call(name, *args):
 def test_workspace_sizes():
     out = C.c_size_t()
     lib = L.load()
-    for n, E, want in ((0, 4, 0), (16384, 512, 0), (16385, 4, 5 * 5 * 4), (1 << 24, 512, 1024 * 513 * 4)):
+    for n, E, want in ((0, 4, 0), (16384, 512, 0), (16385, 4, 5 * 5 * 4), (1 << 23, 512, 512 * 513 * 4)):
         L.check(lib.brx_pairs_workspace_bytes(n, E, C.byref(out)))
         assert out.value == want, (n, E)
-    for bad in ((-1, 4), ((1 << 24) + 1, 4), (8, 0), (8, 513)):
+    for bad in ((-1, 4), ((1 << 23) + 1, 4), (8, 0), (8, 513)):
         assert lib.brx_pairs_workspace_bytes(*bad, C.byref(out)) == L.BRX_EINVAL
     assert lib.brx_pairs_workspace_bytes(8, 4, None) == L.BRX_EINVAL
     L.check(lib.brx_norm_workspace_bytes(7, 100, C.byref(out)))
     assert out.value >= 3 * 100 * 4
-    for bad in ((-1, 8), (4, 0), (4, 8193), ((1 << 24) + 1, 8)):
+    for bad in ((-1, 8), (4, 0), (4, 8193), ((1 << 23) + 1, 8)):
         assert lib.brx_norm_workspace_bytes(*bad, C.byref(out)) == L.BRX_EINVAL
 
 
@@ -141,17 +146,17 @@ def test_c_calls_check_their_arguments():
     bad = [
         ("brx_pairs_plan", p, -1, 2, 4, p, p, p, None, 0, None), ("brx_pairs_plan", p, 4, 0, 4, p, p, p, None, 0, None),
         ("brx_pairs_plan", p, 4, 65, 4, p, p, p, None, 0, None), ("brx_pairs_plan", p, 4, 2, 0, p, p, p, None, 0, None),
-        ("brx_pairs_plan", p, 4, 2, 513, p, p, p, None, 0, None), ("brx_pairs_plan", p, 1 << 24, 2, 4, p, p, p, None, 0, None),
+        ("brx_pairs_plan", p, 4, 2, 513, p, p, p, None, 0, None), ("brx_pairs_plan", p, 1 << 23, 2, 4, p, p, p, None, 0, None),
         ("brx_pairs_dispatch", p, 8, p, -1, 2, 8, 1, p, None), ("brx_pairs_dispatch", p, 8, p, 4, 2, 0, 1, p, None),
         ("brx_pairs_dispatch", p, 8, p, 4, 2, 8193, 1, p, None), ("brx_pairs_dispatch", p, 8, p, 4, 2, 8, 3, p, None),
-        ("brx_pairs_combine", p, p, p, 4, 65, 8, 1, p, None), ("brx_pairs_combine", p, p, p, 1 << 24, 2, 8, 1, p, None),
+        ("brx_pairs_combine", p, p, p, 4, 65, 8, 1, p, None), ("brx_pairs_combine", p, p, p, 1 << 23, 2, 8, 1, p, None),
         ("brx_pairs_combine_backward", p, 8, p, p, p, 4, 2, 8, -1, p, p, None),
         ("brx_grouped_product", p, p, 64, 8, None, p, -1, 2, 8, 8, 1, p, None),
         ("brx_grouped_product", p, p, 64, 8, None, p, 4, 0, 8, 8, 1, p, None),
         ("brx_grouped_product", p, p, 64, 8, None, p, 4, 2, 12, 8, 1, p, None),
         ("brx_grouped_product", p, p, 64, 8, None, p, 4, 2, 8, 8200, 1, p, None),
         ("brx_grouped_product", p, p, 64, 8, None, p, 4, 2, 8, 8, 0, p, None),
-        ("brx_grouped_product_backward_rows", p, p, 64, 8, p, (1 << 24) + 1, 2, 8, 8, 1, p, None),
+        ("brx_grouped_product_backward_rows", p, p, 64, 8, p, (1 << 23) + 1, 2, 8, 8, 1, p, None),
         ("brx_grouped_product_backward_weight", p, p, p, 4, 513, 8, 8, 1, p, None, None),
         ("brx_norm_forward", p, 8, 0, p, 8, 1, None, 0, None, 0, 0, None, 0, 1.0, 1e-6, 4, 8, p, None, None, None, None),
         ("brx_norm_forward", p, 8, 5, p, 8, 5, None, 0, None, 0, 0, None, 0, 1.0, 1e-6, 4, 8, p, None, None, None, None),

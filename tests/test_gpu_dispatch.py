@@ -226,6 +226,16 @@ def test_streams_and_graphs(D):
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, ref) and torch.equal(p2.order, plan.order)
 
+    # gradients of calls given a stream
+    gx, gw = x.clone().requires_grad_(), w.clone().requires_grad_()
+    d = rand((T, H), torch.bfloat16, 60)
+    want = torch.autograd.grad(D.combine(D.dispatch(gx, plan), plan, gw), (gx, gw), d)
+    s.wait_stream(torch.cuda.current_stream())
+    rows = D.dispatch(gx, plan, stream=s)
+    out = D.combine(rows, plan, gw, stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, (gx, gw), d), want))
+
     sx, si, sw, sd = x.clone(), idx.clone(), w.clone(), rand((T, H), torch.bfloat16, 29)
 
     def step():

@@ -260,6 +260,11 @@ def test_streams_and_graphs(G):
     got = G.product(rows, w, offsets, b, stream=s)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, ref[0])
+    lr, lw, lb = (t.clone().requires_grad_() for t in (rows, w, b))
+    s.wait_stream(torch.cuda.current_stream())
+    out = G.product(lr, lw, offsets, lb, stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(out, (lr, lw, lb), d), ref[1:]))
     with torch.cuda.stream(s):
         step()
     torch.cuda.current_stream().wait_stream(s)

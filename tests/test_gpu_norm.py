@@ -269,6 +269,11 @@ def test_streams_and_graphs(M):
     h = M.enter(ts[0], ts[2], stream=s)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1]) and torch.equal(h, M.enter(ts[0], ts[2]))
+    v = [t.clone().requires_grad_() for t in ts]
+    s.wait_stream(torch.cuda.current_stream())
+    got = M.leave(*v[:4], 0.5, v[4], stream=s)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(got, v, d), ref[2:]))
     with torch.cuda.stream(s):
         step()
     torch.cuda.current_stream().wait_stream(s)
