@@ -158,35 +158,33 @@ int brx_grouped_product(const void* rows, const void* weight, int64_t w_expert, 
     return hip_result(launch_grouped_rows(g, false, dtype, (hipStream_t)stream), "grouped product launch");
 }
 
-int brx_grouped_product_backward_rows(const void* dout, const void* weight, int64_t w_expert, int64_t w_row,
-                                      const int32_t* offsets, int P, int E, int K, int N, int dtype, void* drows, void* stream) {
-    int rc = check_grouped(P, E, K, N, dtype);
-    if (rc) return rc;
-    if ((rc = check_weight(w_expert, w_row, K))) return rc;
-    if (!P) return BRX_OK;
-    if ((rc = check_16({dout, weight, drows}, "dout, weight and drows"))) return rc;
-    if (!offsets) return api_fail(BRX_EINVAL, "offsets are required");
-    // (the reduction runs over W's N rows, the output over its K columns)
-    const GroupedArgs g{(const uint16_t*)dout, (const uint16_t*)weight, nullptr, (uint16_t*)drows, offsets, w_expert, w_row, P, E, N, K};
-    return hip_result(launch_grouped_rows(g, true, dtype, (hipStream_t)stream), "grouped product row gradient launch");
-}
-
-int brx_grouped_product_backward_weight(const void* dout, const void* rows, const int32_t* offsets, int P, int E, int K, int N,
-                                        int dtype, void* dweight, void* dbias, void* stream) {
+int brx_grouped_product_backward(const void* dout, const void* rows, const void* weight, int64_t w_expert, int64_t w_row,
+                                 const int32_t* offsets, int P, int E, int K, int N, int dtype, void* drows, void* dweight,
+                                 void* dbias, void* stream) {
     int rc = check_grouped(P, E, K, N, dtype);
     if (rc) return rc;
     if (!offsets) return api_fail(BRX_EINVAL, "offsets are required");
     if (P && (!dout || ((uintptr_t)dout & 15))) return api_fail(BRX_EINVAL, "dout is required, 16-byte aligned");
+    if (drows && P) {
+        if ((rc = check_weight(w_expert, w_row, K))) return rc;
+        if ((rc = check_16({weight, drows}, "weight and drows"))) return rc;
+    }
+    if (dweight && (((uintptr_t)dweight & 15) || (P && (!rows || ((uintptr_t)rows & 15)))))
+        return api_fail(BRX_EINVAL, "rows and dweight must be 16-byte aligned, and rows given");
+    if ((uintptr_t)dbias & 1) return api_fail(BRX_EINVAL, "dbias must be aligned to its type");
+    const hipStream_t s = (hipStream_t)stream;
+    if (drows && P) {
+        // (the reduction runs over W's N rows, the output over its K columns)
+        const GroupedArgs g{(const uint16_t*)dout, (const uint16_t*)weight, nullptr, (uint16_t*)drows, offsets, w_expert, w_row, P, E, N, K};
+        if ((rc = hip_result(launch_grouped_rows(g, true, dtype, s), "grouped product row gradient launch"))) return rc;
+    }
     if (dweight) {
-        if (((uintptr_t)dweight & 15) || (P && (!rows || ((uintptr_t)rows & 15))))
-            return api_fail(BRX_EINVAL, "rows and dweight must be 16-byte aligned, and rows given");
         const GroupedArgs g{(const uint16_t*)dout, (const uint16_t*)rows, nullptr, (uint16_t*)dweight, offsets, 0, 0, P, E, N, K};
-        if ((rc = hip_result(launch_grouped_weight(g, dtype, (hipStream_t)stream), "grouped product weight gradient launch"))) return rc;
+        if ((rc = hip_result(launch_grouped_weight(g, dtype, s), "grouped product weight gradient launch"))) return rc;
     }
     if (dbias) {
-        if ((uintptr_t)dbias & 1) return api_fail(BRX_EINVAL, "dbias must be aligned to its type");
         const GroupedArgs g{(const uint16_t*)dout, nullptr, nullptr, (uint16_t*)dbias, offsets, 0, 0, P, E, N, 0};
-        return hip_result(launch_grouped_bias(g, dtype, (hipStream_t)stream), "grouped product bias gradient launch");
+        return hip_result(launch_grouped_bias(g, dtype, s), "grouped product bias gradient launch");
     }
     return BRX_OK;
 }

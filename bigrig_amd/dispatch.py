@@ -188,12 +188,14 @@ class _Combine(torch.autograd.Function):
         rows, w, position = ctx.saved_tensors
         T, k, H = ctx.sizes
         dout = _strided(dout)
-        device = _on_device(dout, rows, w, position)
         drows = dout.new_empty((T * k, H)) if ctx.needs_input_grad[0] else None
         dw = w.new_empty((T, k)) if ctx.needs_input_grad[1] else None
-        L.check(L.load().brx_pairs_combine_backward(
-            dout.data_ptr(), dout.stride(0) if T > 1 else H, L.ptr(rows), L.ptr(w), position.data_ptr(), T, k, H,
-            _TYPES[dout.dtype], L.ptr(drows), L.ptr(dw), _handle(device)))
+        ptr = L.ptr
+        rc = L.load().brx_pairs_combine_backward(
+            dout.data_ptr(), dout.stride(0) if T > 1 else H, ptr(rows), ptr(w), position.data_ptr(), T, k, H,
+            _TYPES[dout.dtype], ptr(drows), ptr(dw), _handle(dout.get_device()))
+        if rc:
+            L.check(rc)
         return drows, dw, None, None, None
 
 

@@ -58,21 +58,17 @@ class _Product(torch.autograd.Function):
         rows, weight, offsets = ctx.saved_tensors
         E, N, K = ctx.sizes
         dout = _aligned(dout)
-        P, dt = dout.shape[0], _TYPES[dout.dtype]
-        device = _on_device(dout, rows, weight, offsets)
-        lib, stream = L.load(), _handle(device)
-        drows = dweight = dbias = None
-        if ctx.needs_input_grad[0]:
-            drows = dout.new_empty((P, K))
-            L.check(lib.brx_grouped_product_backward_rows(dout.data_ptr(), weight.data_ptr(), *_strides(weight),
-                                                          offsets.data_ptr(), P, E, K, N, dt, drows.data_ptr(), stream))
-        if ctx.needs_input_grad[1]:
-            dweight = dout.new_empty((E, N, K))
-        if ctx.needs_input_grad[3]:
-            dbias = dout.new_empty((E, N))
-        if dweight is not None or dbias is not None:
-            L.check(lib.brx_grouped_product_backward_weight(dout.data_ptr(), L.ptr(rows), offsets.data_ptr(), P, E, K, N,
-                                                            dt, L.ptr(dweight), L.ptr(dbias), stream))
+        P = dout.shape[0]
+        need_rows, need_weight, _, need_bias = ctx.needs_input_grad
+        drows = dout.new_empty((P, K)) if need_rows else None
+        dweight = dout.new_empty((E, N, K)) if need_weight else None
+        dbias = dout.new_empty((E, N)) if need_bias else None
+        ptr = L.ptr
+        rc = L.load().brx_grouped_product_backward(
+            dout.data_ptr(), ptr(rows), ptr(weight), *(_strides(weight) if need_rows else (0, K)), offsets.data_ptr(), P, E,
+            K, N, _TYPES[dout.dtype], ptr(drows), ptr(dweight), ptr(dbias), _handle(dout.get_device()))
+        if rc:
+            L.check(rc)
         return drows, dweight, None, dbias
 
 

@@ -36,9 +36,8 @@ EXPORTS = (
     "brx_mx_workspace_bytes", "brx_mx_expert_product", "brx_mx_moe_forward",
     "brx_mx_moe_forward_pairs", "brx_mx_combine", "brx_pairs_workspace_bytes",
     "brx_pairs_plan", "brx_pairs_dispatch", "brx_pairs_combine", "brx_pairs_combine_backward",
-    "brx_grouped_product", "brx_grouped_product_backward_rows",
-    "brx_grouped_product_backward_weight", "brx_norm_forward", "brx_norm_workspace_bytes",
-    "brx_norm_backward",
+    "brx_grouped_product", "brx_grouped_product_backward", "brx_norm_forward",
+    "brx_norm_workspace_bytes", "brx_norm_backward",
 )
 
 
@@ -124,10 +123,8 @@ _SIGS = {
                                     _vp, _vp], C.c_int),
     "brx_grouped_product": ([_vp, _vp, _i64, _i64, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                              _vp, _vp], C.c_int),
-    "brx_grouped_product_backward_rows": ([_vp, _vp, _i64, _i64, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
-                                           C.c_int, _vp, _vp], C.c_int),
-    "brx_grouped_product_backward_weight": ([_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
-                                             _vp, _vp, _vp], C.c_int),
+    "brx_grouped_product_backward": ([_vp, _vp, _vp, _i64, _i64, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
+                                      C.c_int, _vp, _vp, _vp, _vp], C.c_int),
     "brx_norm_forward": ([_vp, _i64, C.c_int, _vp, _i64, C.c_int, _vp, C.c_int, _vp, C.c_int, C.c_int, _vp,
                           C.c_int, C.c_float, C.c_float, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp],
                          C.c_int),

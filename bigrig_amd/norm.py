@@ -121,7 +121,6 @@ def _forward(y, r, post, gate, form, nxt, scale, eps, make_h, h_type, stats):
 
 def _backward(y, r, post, gate, form, nxt, scale, rstd_y, rstd_n, d_new, d_h, needs, y_type):
     """Gradients (dy, dr, dpost, dgate, dnext), None where `needs` is false."""
-    device = _on_device(y, r, post, gate, nxt, d_new, d_h)
     T, H = r.shape
     dy = r.new_empty((T, H), dtype=y_type) if needs[0] else None
     dr = r.new_empty((T, H)) if needs[1] else None
@@ -137,7 +136,7 @@ def _backward(y, r, post, gate, form, nxt, scale, rstd_y, rstd_n, d_new, d_h, ne
     L.check(L.load().brx_norm_backward(
         ptr(y), 0 if y is None else _stride(y, T, H), _TYPES[y_type], r.data_ptr(), _stride(r, T, H), _TYPES[r.dtype],
         ptr(post), _type(post), ptr(gate), form, _type(gate), ptr(nxt), _type(nxt), scale, T, H, ptr(rstd_y), ptr(rstd_n),
-        ptr(d_new), ptr(d_h), ptr(dy), ptr(dr), ptr(dgate), ptr(dpost), ptr(dnext), ptr(ws), need, _handle(device)))
+        ptr(d_new), ptr(d_h), ptr(dy), ptr(dr), ptr(dgate), ptr(dpost), ptr(dnext), ptr(ws), need, _handle(r.get_device())))
     return dy, dr, dpost, dgate, dnext
 
 

@@ -439,13 +439,12 @@ int brx_pairs_combine_backward(const void* dout, int64_t dout_row, const void* r
  * multiples of 8, w_row at most 2^20. Offsets outside [0, P] or out of order name no memory outside the tensors. */
 int brx_grouped_product(const void* rows, const void* weight, int64_t w_expert, int64_t w_row, const void* bias,
                         const int32_t* offsets, int P, int E, int K, int N, int dtype, void* out, void* stream);
-/* Its gradients: drows[r] = W[e]^T dout[r] (0 behind the last run), and dweight [E, N, K] = sum over e's run of
- * dout[r] rows[r]^T (0 for an empty run), dbias [E, N] = sum over e's run of dout[r], either NULL. */
-int brx_grouped_product_backward_rows(const void* dout, const void* weight, int64_t w_expert, int64_t w_row,
-                                      const int32_t* offsets, int P, int E, int K, int N, int dtype, void* drows,
-                                      void* stream);
-int brx_grouped_product_backward_weight(const void* dout, const void* rows, const int32_t* offsets, int P, int E, int K,
-                                        int N, int dtype, void* dweight, void* dbias, void* stream);
+/* Its gradients, each NULL where it is not wanted: drows[r] = W[e]^T dout[r] (0 behind the last run), dweight [E, N, K] =
+ * sum over e's run of dout[r] rows[r]^T (0 for an empty run), dbias [E, N] = sum over e's run of dout[r]. weight is
+ * read only for drows, rows only for dweight. */
+int brx_grouped_product_backward(const void* dout, const void* rows, const void* weight, int64_t w_expert, int64_t w_row,
+                                 const int32_t* offsets, int P, int E, int K, int N, int dtype, void* drows,
+                                 void* dweight, void* dbias, void* stream);
 
 /* Norms at both ends of a block, n(v; w) = v / sqrt(mean(v^2) + eps) * w:
  *   u = n(y; post), or y without post;  new_r = r + scale * gate * u;  h = n(new_r; next)

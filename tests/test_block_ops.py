@@ -156,8 +156,8 @@ def test_c_calls_check_their_arguments():
         ("brx_grouped_product", p, p, 64, 8, None, p, 4, 2, 12, 8, 1, p, None),
         ("brx_grouped_product", p, p, 64, 8, None, p, 4, 2, 8, 8200, 1, p, None),
         ("brx_grouped_product", p, p, 64, 8, None, p, 4, 2, 8, 8, 0, p, None),
-        ("brx_grouped_product_backward_rows", p, p, 64, 8, p, (1 << 23) + 1, 2, 8, 8, 1, p, None),
-        ("brx_grouped_product_backward_weight", p, p, p, 4, 513, 8, 8, 1, p, None, None),
+        ("brx_grouped_product_backward", p, p, p, 64, 8, p, (1 << 23) + 1, 2, 8, 8, 1, p, p, p, None),
+        ("brx_grouped_product_backward", p, p, p, 64, 8, p, 4, 513, 8, 8, 1, p, p, p, None),
         ("brx_norm_forward", p, 8, 0, p, 8, 1, None, 0, None, 0, 0, None, 0, 1.0, 1e-6, 4, 8, p, None, None, None, None),
         ("brx_norm_forward", p, 8, 5, p, 8, 5, None, 0, None, 0, 0, None, 0, 1.0, 1e-6, 4, 8, p, None, None, None, None),
         ("brx_norm_forward", p, 8, 1, p, 8, 1, None, 0, None, 0, 0, None, 0, 1.0, 1e-6, 4, 8193, p, None, None, None, None),
@@ -183,8 +183,7 @@ def test_c_calls_need_a_device_first():
         ("brx_pairs_combine", p, p, p, 4, 2, 8, 1, p, None),
         ("brx_pairs_combine_backward", p, 8, p, p, p, 4, 2, 8, 1, p, p, None),
         ("brx_grouped_product", p, p, 64, 8, None, p, 4, 2, 8, 8, 1, p, None),
-        ("brx_grouped_product_backward_rows", p, p, 64, 8, p, 4, 2, 8, 8, 1, p, None),
-        ("brx_grouped_product_backward_weight", p, p, p, 4, 2, 8, 8, 1, p, None, None),
+        ("brx_grouped_product_backward", p, p, p, 64, 8, p, 4, 2, 8, 8, 1, p, p, p, None),
         ("brx_norm_forward", p, 8, 1, p, 8, 1, None, 0, None, 0, 0, None, 0, 1.0, 1e-6, 4, 8, p, None, None, None, None),
         ("brx_norm_backward", p, 8, 1, p, 8, 1, None, 0, None, 0, 0, None, 0, 1.0, 4, 8, None, None, p, None, p, p, None, None,
          None, None, 0, None),
