@@ -832,16 +832,30 @@ inline int64_t row_tiles(const GroupedArgs& g, int BM) {
     return g.P / BM + (runs < g.P ? runs : g.P);
 }
 
-typedef Shape<2, 2, 2, 2, 2> Square;      // 128 x 128
+typedef Shape<2, 2, 2, 2, 2> Square;      // 128 x 128, four waves: two blocks a CU
+typedef Shape<1, 2, 2, 2, 3> Half;        // 64 x 128, one stage more ahead: one block a CU, alone with its latency
+typedef Shape<1, 2, 4, 2, 2> Eight;       // 128 x 128, eight waves
 
 // Which kernel. Products of rows: thin tiles for up to 32 rows; the persistent kernel where whole tiles of 256 x 256 give each
-// CU one; 128 x 128 tiles, two blocks a CU, between. bf16, 128 experts of 2048 -> 1536, us (thin / 128 / 256):
+// CU one; between, 128 x 128 tiles, two blocks a CU, or tiles of half the rows where the whole ones cannot give each CU one.
+// bf16, us, 128 experts of 2048 -> 1536 (thin / 128 / 256):
 //      8 rows 14.3 / 25.2 / 77,  32 rows 29.2 / 30.5 / 42,  64 rows 38.6 / 36.2 / 77,  1024 rows 172 / 168 / 171
 //   8192 rows 199 / 199,  16384 rows 231 / 212,  32768 rows 340 / 294  (128 / 256; rows^T 171 / 162, 230 / 177, 352 / 268)
-// and 64 experts of 512 -> 512: 4096 rows 12.6 / 19.8, 32768 rows 43.0 / 41.9. Products over the runs write every tile in any
-// case: the persistent kernel where those are as many as the CUs (128 / 256: 64 x 512 x 512 of 4096 rows 18.0 / 18.2, 60 x 712 x
-// 1000 34.3 / 29.8, 128 x 1536 x 2048 of 1024 rows 231 / 162, of 32768 478 / 343; 8 x 1024 x 1024 of 1000 rows 12.0 / 16.3).
+// 64 experts of 512 -> 512 (128 / 256): 4096 rows 12.6 / 19.8, 32768 rows 43.0 / 41.9.
+// 8 experts (half / whole): 1000 rows 1024 -> 1024 13.7 / 16.6, 2048 -> 1024 20.5 / 26.1, 1024 -> 2048 (256 whole tiles) 21.7 /
+// 18.2; 4000 rows 1024 -> 1024 49 / 32.
+// Products over the runs write every tile in any case: the persistent kernel where those are as many as the CUs (128 by four
+// waves / 256: 64 x 512 x 512 of 4096 rows 18.0 / 18.2, 60 x 712 x 1000 of 2804 34.3 / 29.8, 128 x 1536 x 2048 of 1024 231 / 162,
+// of 32768 478 / 343), else 128 x 128 by eight waves (by four / by eight / 256: 8 x 1024 x 1024 of 1000 rows 12.0 / 11.8 / 16.3,
+// 8 x 1024 x 2048 of 4000 33.3 / 28.7 / 28.6).
 constexpr int kThinMost = 32;
+
+template <int DT, bool BY, class S>
+hipError_t launch_tiles(const GroupedArgs& g, hipStream_t s) {
+    const int mt = (int)row_tiles(g, S::BM), nt = (g.N + S::BN - 1) / S::BN;
+    hipLaunchKernelGGL((k_grouped_rows<DT, BY, S>), dim3((mt + kXcd - 1) / kXcd * kXcd * nt), dim3(S::kThreads), 0, s, g, mt, nt);
+    return hipGetLastError();
+}
 
 template <int DT, bool BY>
 hipError_t launch_rows(const GroupedArgs& g, hipStream_t s) {
@@ -856,10 +870,8 @@ hipError_t launch_rows(const GroupedArgs& g, hipStream_t s) {
         hipLaunchKernelGGL((k_grouped_tall<DT, kind>), dim3(kCus), dim3(kTallThreads), 0, s, g, tall_nt, 0);
         return hipGetLastError();
     }
-    typedef Square S;
-    const int mt = (int)row_tiles(g, S::BM), nt = (g.N + S::BN - 1) / S::BN;
-    hipLaunchKernelGGL((k_grouped_rows<DT, BY, S>), dim3((mt + kXcd - 1) / kXcd * kXcd * nt), dim3(S::kThreads), 0, s, g, mt, nt);
-    return hipGetLastError();
+    if (row_tiles(g, Square::BM) * ((g.N + Square::BN - 1) / Square::BN) < kCus) return launch_tiles<DT, BY, Half>(g, s);
+    return launch_tiles<DT, BY, Square>(g, s);
 }
 
 template <int DT>
@@ -869,7 +881,7 @@ hipError_t launch_weight(const GroupedArgs& g, hipStream_t s) {
         hipLaunchKernelGGL((k_grouped_tall<DT, kWeight>), dim3(kCus), dim3(kTallThreads), 0, s, g, tall_nt, tall_mt);
         return hipGetLastError();
     }
-    typedef Square S;
+    typedef Eight S;
     const int mt = (g.K + S::BM - 1) / S::BM, nt = (g.N + S::BN - 1) / S::BN;
     hipLaunchKernelGGL((k_grouped_weight<DT, S>), dim3(mt * nt, g.E), dim3(S::kThreads), 0, s, g, mt, nt);
     return hipGetLastError();

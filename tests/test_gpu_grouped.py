@@ -99,6 +99,12 @@ def test_enough_rows_for_the_persistent_tiles(G, dtype, bias, N, K):
     check(G, counts, N, K, dtype, bias=bias, behind=300)
 
 
+@pytest.mark.parametrize("dtype,bias", [(torch.float16, True), (torch.bfloat16, False)])
+def test_enough_rows_for_whole_tiles_of_128(G, dtype, bias):
+    # (23 + 10) row tiles by 9 column tiles of 128 both ways, more than the CUs; 11 by 5 of 256, fewer
+    check(G, [0, 700, 1, 128, 129, 900, 0, 1000, 127], 1032, 1096, dtype, bias=bias, behind=40)
+
+
 def test_persistent_tiles_of_more_than_the_cus(G):
     # every block takes several tiles, short sums among long ones
     g = torch.Generator().manual_seed(3)
