@@ -56,8 +56,7 @@ struct NormArgs {
     float scale, eps;
     int T, H;
     int gate_form;
-    int post_dt, next_dt, gate_dt;          // BRX_DT_*
-    int dy_dt;                              // (the kernels' y type: dtype of dpost / dnext / dgate follows *_dt)
+    int post_dt, next_dt, gate_dt;          // BRX_DT_*, of their gradients too
 };
 int norm_blocks(int T, int H);              // blocks of a backward launch
 hipError_t launch_norm_forward(const NormArgs& a, int y_dt, int r_dt, hipStream_t s);
@@ -89,14 +88,6 @@ __device__ __forceinline__ v4u_t get16(const void* p) {
 __device__ __forceinline__ void set16(void* p, const v4u_t& v) {
     typedef v4u_t __attribute__((aligned(2))) V;
     *reinterpret_cast<V*>(p) = v;
-}
-__device__ __forceinline__ v4u_t get16_nt(const void* p) {
-    typedef v4u_t __attribute__((aligned(2))) V;
-    return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
-}
-__device__ __forceinline__ void set16_nt(void* p, const v4u_t& v) {
-    typedef v4u_t __attribute__((aligned(2))) V;
-    __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
 }
 
 template <int DT>

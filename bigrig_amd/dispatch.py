@@ -15,7 +15,9 @@ A pair of an expert outside [0, n_experts) -- padding, another device's expert: 
 `dispatch` and `combine` have gradients (taken once: create_graph=True is refused). Sums are float32, over a
 token's pairs in their order, rounded once, and every result is the same bits on every run. Tensors live on
 the current device; scratch is allocated per call by torch, on the call's stream. Given a `stream`, the whole call
-runs there (and its gradient): the inputs have to be ready on it.
+runs there (and its gradient): the inputs have to be ready on it. A gradient that is captured into a graph is taken of
+leaves that no eager graph holds meanwhile (`detach().requires_grad_()` inside the capture): torch ends the process
+where an eager graph's leaf on another stream is met in a capture.
 """
 from __future__ import annotations
 
