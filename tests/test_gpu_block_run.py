@@ -104,6 +104,36 @@ def test_a_captured_block_step(ops):
             assert torch.equal(a, b), i
 
 
+def test_blocks_on_two_streams_at_once(ops):
+    # calls share nothing: steps of two blocks, queued in turn on two streams with no wait between them
+    E, k = 8, 3
+    near = lambda shape, seed: (rand(shape, S, seed) * 0.1 + 1.0).to(B)
+    jobs = []
+    for T, H, I, seed in ((3000, 256, 136, 0), (40, 128, 72, 50)):
+        weights = [near((H,), seed + 1), rand((E, H), B, seed + 2, scale=0.1), rand((E, 2 * I, H), B, seed + 3, scale=0.1),
+                   rand((E, H, I), B, seed + 4, scale=0.1), near((H,), seed + 5), near((H,), seed + 6)]
+        jobs.append((weights, rand((T, H), B, seed + 7), routing(T, k, E, seed), [rand((T, H), B, seed + 8 + i) for i in range(2)]))
+
+    def step(job):
+        weights, x, idx, d = job
+        leaves = [t.detach().requires_grad_() for t in (x, *weights)]
+        outs = expert_block(ops, leaves[0], leaves[1:], E, k, idx)
+        return [*(o.detach() for o in outs), *torch.autograd.grad(outs, leaves, d)]
+
+    want = [step(j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(jobs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i])), i
+
+
 def test_sorted_rows_through_the_pair_forms(ops):
     # the plan's rows, as pairs of one token each, through the library's own experts: the layer's rows, bit for bit
     from bigrig_amd import layer as ly
