@@ -70,6 +70,7 @@ struct GroupedArgs {
     const int32_t* offsets;       // [E + 1]
     int64_t b_expert, b_row;      // values between experts and rows of b (weights)
     int P, E, K, N;               // rows, experts, reduction (row products) and output widths
+    bool past_cache;              // (set by the launch) the output is stored past the caches
 };
 hipError_t launch_grouped_rows(const GroupedArgs& g, bool transposed, int dtype, hipStream_t s);
 hipError_t launch_grouped_weight(const GroupedArgs& g, int dtype, hipStream_t s);

@@ -154,7 +154,7 @@ int brx_grouped_product(const void* rows, const void* weight, int64_t w_expert, 
     if (!P) return BRX_OK;
     if ((rc = check_16({rows, weight, out}, "rows, weight and out"))) return rc;
     if (!offsets || ((uintptr_t)bias & 1)) return api_fail(BRX_EINVAL, "offsets are required, bias aligned to its type");
-    const GroupedArgs g{(const uint16_t*)rows, (const uint16_t*)weight, (const uint16_t*)bias, (uint16_t*)out, offsets, w_expert, w_row, P, E, K, N};
+    const GroupedArgs g{(const uint16_t*)rows, (const uint16_t*)weight, (const uint16_t*)bias, (uint16_t*)out, offsets, w_expert, w_row, P, E, K, N, false};
     return hip_result(launch_grouped_rows(g, false, dtype, (hipStream_t)stream), "grouped product launch");
 }
 
@@ -175,15 +175,15 @@ int brx_grouped_product_backward(const void* dout, const void* rows, const void*
     const hipStream_t s = (hipStream_t)stream;
     if (drows && P) {
         // (the reduction runs over W's N rows, the output over its K columns)
-        const GroupedArgs g{(const uint16_t*)dout, (const uint16_t*)weight, nullptr, (uint16_t*)drows, offsets, w_expert, w_row, P, E, N, K};
+        const GroupedArgs g{(const uint16_t*)dout, (const uint16_t*)weight, nullptr, (uint16_t*)drows, offsets, w_expert, w_row, P, E, N, K, false};
         if ((rc = hip_result(launch_grouped_rows(g, true, dtype, s), "grouped product row gradient launch"))) return rc;
     }
     if (dweight) {
-        const GroupedArgs g{(const uint16_t*)dout, (const uint16_t*)rows, nullptr, (uint16_t*)dweight, offsets, 0, 0, P, E, N, K};
+        const GroupedArgs g{(const uint16_t*)dout, (const uint16_t*)rows, nullptr, (uint16_t*)dweight, offsets, 0, 0, P, E, N, K, false};
         if ((rc = hip_result(launch_grouped_weight(g, dtype, s), "grouped product weight gradient launch"))) return rc;
     }
     if (dbias) {
-        const GroupedArgs g{(const uint16_t*)dout, nullptr, nullptr, (uint16_t*)dbias, offsets, 0, 0, P, E, N, 0};
+        const GroupedArgs g{(const uint16_t*)dout, nullptr, nullptr, (uint16_t*)dbias, offsets, 0, 0, P, E, N, 0, false};
         return hip_result(launch_grouped_bias(g, dtype, s), "grouped product bias gradient launch");
     }
     return BRX_OK;

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kG = 64;                // reduction steps of a stage
 constexpr uint32_t kPast = 0x80000000u;   // a byte offset past every buffer
+constexpr int kNonTemporal = 2;       // cache policy of a buffer store: not kept
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
@@ -750,8 +751,10 @@ __device__ __forceinline__ void tall_tile(TallState<KIND>& c, const TallTile& ds
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = (2 * m + c.wm) * 32 + (l32 & 28) + i;
-            __builtin_amdgcn_raw_buffer_store_b128(v4u_t{q[i][0], q[i][1], q[i][2], q[i][3]}, ro,
-                                                   in && row < dst.rows ? (uint32_t)(row * c.g.N + col) * 2 : kPast, 0, 0);
+            const v4u_t v = {q[i][0], q[i][1], q[i][2], q[i][3]};
+            const uint32_t to = in && row < dst.rows ? (uint32_t)(row * c.g.N + col) * 2 : kPast;
+            if (KIND == kWeight && c.g.past_cache) __builtin_amdgcn_raw_buffer_store_b128(v, ro, to, 0, kNonTemporal);
+            else __builtin_amdgcn_raw_buffer_store_b128(v, ro, to, 0, 0);
         }
     }
     c.stores = 4 * NF;
@@ -850,6 +853,12 @@ typedef Shape<1, 2, 4, 2, 2> Eight;       // 128 x 128, eight waves
 // 8 x 1024 x 2048 of 4000 33.3 / 28.7 / 28.6).
 constexpr int kThinMost = 32;
 
+// Gradients of the matrices that are larger than the chip's last cache, and whose rows are whole lines, are stored past the
+// caches (128 x 1536 x 2048, 805 MB, of 32768 rows: 378 -> 323 us, a read of them right behind it included 700 -> 676,
+// a whole pass with both other products 1015 -> 985). Of what fits,
+// that read finds less (24 x 1024 x 2048, 101 MB: 86 -> 80, with the read 115 -> 121), and parts of lines cost more (60 x 712 x 1000: 30 -> 46).
+constexpr int64_t kCacheBytes = 256ll << 20;
+
 template <int DT, bool BY, class S>
 hipError_t launch_tiles(const GroupedArgs& g, hipStream_t s) {
     const int mt = (int)row_tiles(g, S::BM), nt = (g.N + S::BN - 1) / S::BN;
@@ -878,7 +887,9 @@ template <int DT>
 hipError_t launch_weight(const GroupedArgs& g, hipStream_t s) {
     const int tall_mt = (g.K + kTall - 1) / kTall, tall_nt = (g.N + kTall - 1) / kTall;
     if ((int64_t)g.E * tall_mt * tall_nt >= kCus) {
-        hipLaunchKernelGGL((k_grouped_tall<DT, kWeight>), dim3(kCus), dim3(kTallThreads), 0, s, g, tall_nt, tall_mt);
+        GroupedArgs a = g;
+        a.past_cache = (int64_t)g.E * g.K * g.N * 2 > kCacheBytes && g.N % 64 == 0;
+        hipLaunchKernelGGL((k_grouped_tall<DT, kWeight>), dim3(kCus), dim3(kTallThreads), 0, s, a, tall_nt, tall_mt);
         return hipGetLastError();
     }
     typedef Eight S;

@@ -233,6 +233,22 @@ def test_offsets_out_of_order_or_range_touch_nothing_else(G):
     torch.cuda.synchronize()
 
 
+def test_matrix_gradients_larger_than_the_caches(G):
+    E, N, K = 65, 2056, 1088         # 291 MB of whole lines, tiles of 8 rows at their end
+    counts = [0 if e % 9 == 4 else e % 7 * 13 + 1 for e in range(E)]
+    offsets, at = offsets_of(counts)
+    rows, dout = rand((at[-1], K), torch.bfloat16, 1), rand((at[-1], N), torch.bfloat16, 2)
+    w = torch.zeros((E, N, K), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    for _ in range(2):
+        (dw,) = torch.autograd.grad(G.product(rows, w, offsets), w, dout)
+        for e in range(E):
+            if not counts[e]:
+                assert not dw[e].any(), e
+            elif e % 8 == 0 or e == E - 1:
+                x, d = (t[at[e]:at[e + 1]].cpu().double() for t in (rows, dout))
+                close(dw[e], d.T @ x, counts[e] * SUM_U * (d.abs().T @ x.abs()), f"dweight of {e}")
+
+
 def test_rows_past_two_to_the_thirty_one_bytes(G):
     P, K, N = 600000, 2048, 8        # 2.5 GB of rows, one expert
     offsets, _ = offsets_of([10, P - 10])
