@@ -81,7 +81,13 @@ __device__ __forceinline__ void store8(void* base, int64_t row_at, const Run& r,
 // elements that count: owned, and inside a row of fewer than 8
 __device__ __forceinline__ bool counts(const Run& r, int H, int i) { return i >= r.own && i < H; }
 
-__device__ __forceinline__ float rsqrt_of(float v) { return __builtin_amdgcn_rsqf(v); }
+// v^(-1/2): the instruction's value is off by up to a step of its last place, which every value of the row would be off by; one
+// Newton step on it leaves its own rounding. (An infinite v, of a sum that overflowed, keeps its 0.)
+__device__ __forceinline__ float rsqrt_of(float v) {
+    const float r = __builtin_amdgcn_rsqf(v), t = v * r;
+    const float e = __builtin_fmaf(-t, r, 1.0f) - __builtin_fmaf(v, r, -t) * r;      // 1 - v r^2
+    return v < __builtin_inff() ? __builtin_fmaf(0.5f * r, e, r) : r;
+}
 
 // Sum over the threads of a row. Across waves: one slot a wave in `s`, two sets of slots in turn, so one barrier a
 // sum suffices.
