@@ -836,22 +836,29 @@ inline int64_t row_tiles(const GroupedArgs& g, int BM) {
 }
 
 typedef Shape<2, 2, 2, 2, 2> Square;      // 128 x 128, four waves: two blocks a CU
-typedef Shape<1, 2, 2, 2, 3> Half;        // 64 x 128, one stage more ahead: one block a CU, alone with its latency
+typedef Shape<1, 1, 2, 4, 3> Half;        // 64 x 128, eight waves, one stage more ahead
+typedef Shape<1, 1, 1, 4, 4> Low;         // 32 x 128, four waves, two stages more ahead
 typedef Shape<1, 2, 4, 2, 2> Eight;       // 128 x 128, eight waves
 
-// Which kernel. Products of rows: thin tiles for up to 32 rows; the persistent kernel where whole tiles of 256 x 256 give each
-// CU one; between, 128 x 128 tiles, two blocks a CU, or tiles of half the rows where the whole ones cannot give each CU one.
-// bf16, us, 128 experts of 2048 -> 1536 (thin / 128 / 256):
-//      8 rows 14.3 / 25.2 / 77,  32 rows 29.2 / 30.5 / 42,  64 rows 38.6 / 36.2 / 77,  1024 rows 172 / 168 / 171
-//   8192 rows 199 / 199,  16384 rows 231 / 212,  32768 rows 340 / 294  (128 / 256; rows^T 171 / 162, 230 / 177, 352 / 268)
-// 64 experts of 512 -> 512 (128 / 256): 4096 rows 12.6 / 19.8, 32768 rows 43.0 / 41.9.
-// 8 experts (half / whole): 1000 rows 1024 -> 1024 13.7 / 16.6, 2048 -> 1024 20.5 / 26.1, 1024 -> 2048 (256 whole tiles) 21.7 /
-// 18.2; 4000 rows 1024 -> 1024 49 / 32.
+// Which kernel. Products of rows, by what bounds them. Where runs are short, by the matrices' bytes: thin tiles for up to 8 rows,
+// 32 x 128 up to 16 rows a run on average, 64 x 128 up to 48 (and where 128 x 128 could not give each CU one): lower tiles
+// leave LDS for more of the matrices in flight. Where whole tiles of 256 x 256 give each CU one: the persistent kernel. Between:
+// 128 x 128, two blocks a CU. bf16, us, thin / 32 / 64 / 128 / 256 (rows; rows^T in brackets):
+//   128 experts of 2048 -> 1536   8 rows 14.6 / 16.6 / 20 / 25 / -        16 rows 20.4 / 19.3 / 20 / - / -
+//                               512 rows 131 / 125 / 132 / 147 / - (- / 115 / 117 / 133)
+//                              2048 rows - / 157 / 170 / 189 / - (- / 146 / 146 / 150)
+//                              6144 rows - / 225 / 172 / 195 / 194 (- / 233 / 161 / 164 / 152)
+//                              8192 rows - / 272 / 190 / 202 / 202 (- / 271 / 184 / 171 / 162)
+//                             32768 rows - / - / - / 340 / 294 (- / - / - / 352 / 268)
+//   64 experts, thin / 32: 8 rows 2048 -> 2048 16.5 / 16.5, 4096 -> 1024 21 / 25, 2880 -> 2880 27 / 24; 32 rows 41 / 39, 52 / 40, 88 / 84
+//   256 experts of 2048 -> 4096 8192 rows - / 872 / 806 / 914 / 902 (- / 909 / 750 / 750 / 705: the persistent kernel before 64 x 128)
+//   64 experts of 512 -> 512    4096 rows - / 19.4 / 14.1 / 13.0 / 20.1,  32768 rows - / - / - / 43.0 / 41.9
+//   8 experts, 1000 rows   1024 -> 1024 - / 19.6 / 13.0 / 17.0 / 52,  1024 -> 2048 (256 tiles of 128) - / 29 / 21.4 / 19.3 / 54
 // Products over the runs write every tile in any case: the persistent kernel where those are as many as the CUs (128 by four
 // waves / 256: 64 x 512 x 512 of 4096 rows 18.0 / 18.2, 60 x 712 x 1000 of 2804 34.3 / 29.8, 128 x 1536 x 2048 of 1024 231 / 162,
 // of 32768 478 / 343), else 128 x 128 by eight waves (by four / by eight / 256: 8 x 1024 x 1024 of 1000 rows 12.0 / 11.8 / 16.3,
 // 8 x 1024 x 2048 of 4000 33.3 / 28.7 / 28.6).
-constexpr int kThinMost = 32;
+constexpr int kThinMost = 8, kLowRun = 16, kHalfRun = 48;
 
 // Gradients of the matrices that are larger than the chip's last cache, and whose rows are whole lines, are stored past the
 // caches (128 x 1536 x 2048, 805 MB, of 32768 rows: 378 -> 323 us, a read of them right behind it included 700 -> 676,
@@ -874,13 +881,14 @@ hipError_t launch_rows(const GroupedArgs& g, hipStream_t s) {
         return hipGetLastError();
     }
     const int tall_nt = (g.N + kTall - 1) / kTall;
-    if ((int64_t)(g.P / kTall) * tall_nt >= kCus) {
-        constexpr int kind = BY ? kRowsT : kRows;
-        hipLaunchKernelGGL((k_grouped_tall<DT, kind>), dim3(kCus), dim3(kTallThreads), 0, s, g, tall_nt, 0);
-        return hipGetLastError();
-    }
-    if (row_tiles(g, Square::BM) * ((g.N + Square::BN - 1) / Square::BN) < kCus) return launch_tiles<DT, BY, Half>(g, s);
-    return launch_tiles<DT, BY, Square>(g, s);
+    const bool tall = (int64_t)(g.P / kTall) * tall_nt >= kCus;
+    if (g.P <= kLowRun * g.E) return launch_tiles<DT, BY, Low>(g, s);
+    if ((g.P <= kHalfRun * g.E && !(BY && tall)) || row_tiles(g, Square::BM) * ((g.N + Square::BN - 1) / Square::BN) < kCus)
+        return launch_tiles<DT, BY, Half>(g, s);
+    if (!tall) return launch_tiles<DT, BY, Square>(g, s);
+    constexpr int kind = BY ? kRowsT : kRows;
+    hipLaunchKernelGGL((k_grouped_tall<DT, kind>), dim3(kCus), dim3(kTallThreads), 0, s, g, tall_nt, 0);
+    return hipGetLastError();
 }
 
 template <int DT>
