@@ -134,6 +134,51 @@ def test_blocks_on_two_streams_at_once(ops):
             assert all(torch.equal(a, b) for a, b in zip(g, want[i])), i
 
 
+def test_the_largest_calls(ops):
+    # 2^23 pairs, rows and tokens of small whole numbers, which every type and sum holds exactly
+    D, G, M = ops
+    T, k, E, H = 1 << 20, 8, 512, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    idx = torch.randint(-1, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    x = torch.randint(-2, 3, (T, H), generator=g, device="cuda").to(B).requires_grad_()
+    weight = torch.randint(0, 2, (E, H, H), generator=g, device="cuda").to(B).requires_grad_()
+    plan = D.plan(idx, E)
+    flat = idx.reshape(-1)
+    kept = flat >= 0
+    by = torch.where(kept, flat, E).long().argsort(stable=True)
+    n = int(kept.sum())
+    assert torch.equal(plan.order[:n].long(), by[:n]) and (plan.order[n:] == -1).all()
+    assert torch.equal(plan.offsets[1:].long(), torch.bincount(flat[kept].long(), minlength=E).cumsum(0))
+    rows = D.dispatch(x, plan)
+    assert torch.equal(rows[:n], x[by[:n] // k]) and not rows[n:].any()
+    y = G.product(rows, weight, plan.offsets)
+    e = flat.long().clamp(min=0).view(T, k)
+    want = torch.zeros((T, H), device="cuda")
+    for j in range(k):      # (products of tokens' rows one pair at a time, exact)
+        for c in range(H):
+            want[:, c] += torch.where(idx[:, j] >= 0, (x.float() * weight.float()[:, c][e[:, j]]).sum(-1), 0.0)
+    out = D.combine(y, plan)
+    assert torch.equal(out, want.to(B))
+    dx, dw = torch.autograd.grad(out, (x, weight), torch.ones_like(out))
+    hit = torch.where((idx >= 0)[:, :, None], weight.float().sum(1)[e], 0.0).sum(1)
+    assert torch.equal(dx, hit.to(B))
+    sums = torch.zeros((E + 1, H), device="cuda", dtype=torch.float64)
+    sums.index_add_(0, torch.where(kept, flat, E).long(), x.detach().double().repeat_interleave(k, 0))
+    # (sums of some 16000 small whole numbers, exact in fp32, rounded once)
+    assert torch.equal(dw, sums[:E, None].expand(E, H, H).float().to(B))
+    with pytest.raises(ValueError, match="at most"):
+        D.plan(torch.zeros((T + 1, k), dtype=torch.int32, device="cuda"), E)
+
+    T = 1 << 23
+    r = torch.ones((T, H), dtype=B, device="cuda")
+    r[-1], r[12345678 % T] = 4.0, 2.0
+    w = torch.ones(H, dtype=S, device="cuda", requires_grad=True)
+    new, h = M.leave(r, r, w, next_weight=w)
+    assert torch.equal(h, torch.ones_like(h)) and (new[-1] == 5).all() and (new[0] == 2).all() and (new[12345678 % T] == 3).all()
+    (dw,) = torch.autograd.grad(h, w, torch.ones_like(h))
+    assert torch.isfinite(dw).all()
+
+
 def test_sorted_rows_through_the_pair_forms(ops):
     # the plan's rows, as pairs of one token each, through the library's own experts: the layer's rows, bit for bit
     from bigrig_amd import layer as ly
