@@ -421,7 +421,6 @@ constexpr int kTallThreads = 512, kTallWaves = 8;
 constexpr int kTall = 256, kHalf = 128;      // rows and columns of a tile, rows of its halves
 constexpr int kUnitB = kTall * kG * 2, kUnitA = kHalf * kG * 2;
 constexpr int kTallRing = 2 * kUnitB + 5 * kUnitA;      // b and the first rows twice, the other rows three times
-constexpr int kOwnRun = 2;                   // row tiles an XCD takes before the next XCD's
 
 // One operand's copies: `M` values along the output, rows or steps `ld` values apart.
 template <bool Y, int M>
@@ -534,53 +533,70 @@ __device__ __forceinline__ int last_at_most(const int32_t* v, int n, int x) {
     return __builtin_amdgcn_readfirstlane(at);
 }
 
+// The tiles of a call in one sequence, two row tiles by all columns (of the runs' products: one by all) after another. A round
+// gives each block one, each XCD neighbours, which share operands. The last round's, where they are few, are cut into two or
+// four by their rows. (XCDs with sequences of their own, nothing cut: 8192 rows of 8 x 2048 x 2048 110 us against 99, 32768 of 64 x 512 x 512
+// 41.7 / 38.4, 24000 of 8 x 2048 x 2048 173 / 179.)
 template <int KIND>
 struct TallList {
     const GroupedArgs& g;
     const TallTable& t;
     int ntiles, mtiles;       // column tiles; row tiles (in all, or of an expert's matrix)
-    int xcd, per;             // this block's XCD; blocks an XCD
-    int at;                   // place in the XCD's sequence
+    int xcd, place, per;      // this block's XCD, its place there; blocks an XCD
+    int round, rounds;        // of whole rounds
+    int last, cut;            // tiles of the last round, cut 2^cut times
+
+    __device__ __forceinline__ void init() {
+        const int blocks = per * kXcd;
+        const int all = mtiles * ntiles * (KIND == kWeight ? g.E : 1);      // (2^21 at most)
+        round = 0;
+        rounds = all / blocks;
+        last = all - rounds * blocks;
+        cut = 4 * last <= blocks ? 2 : 2 * last <= blocks ? 1 : 0;
+    }
 
     // The next tile of this block; false behind the last.
     __device__ __forceinline__ bool next(TallTile& o) {
+        int at = round * per * kXcd, part = 0, rows = kTall;
+        if (round < rounds) {
+            at += xcd * per + place;
+        } else {
+            const int n = last << cut, share = (n + kXcd - 1) / kXcd, v = xcd * share + place;
+            if (round > rounds || place >= share || v >= n) return false;
+            at += v >> cut;
+            part = v & ((1 << cut) - 1);
+            rows = kTall >> cut;
+        }
+        ++round;
         if constexpr (KIND == kWeight) {
-            const int u = at / ntiles * kXcd + xcd, nt = at % ntiles;
-            if (u >= g.E * mtiles) return false;
-            at += per;
-            const int e = __builtin_amdgcn_readfirstlane(t.order[u / mtiles]), m0 = u % mtiles * kTall, n0 = nt * kTall;
+            const int u = at / ntiles, nt = at - u * ntiles;
+            const int e = __builtin_amdgcn_readfirstlane(t.order[u / mtiles]), m0 = u % mtiles * kTall + part * rows, n0 = nt * kTall;
             const int lo = t.first[e], hi = t.first[e + 1];
             const int l = __builtin_amdgcn_readfirstlane(lo), h = __builtin_amdgcn_readfirstlane(max(hi, lo));
             o.a = g.a + (int64_t)l * g.K + m0;
             o.b = g.b + (int64_t)l * g.N + n0;
             o.bias = nullptr;
             o.out = g.out + ((int64_t)e * g.K + m0) * g.N + n0;
-            o.rows = g.K - m0;
+            o.rows = min(g.K - m0, rows);
             o.cols = g.N - n0;
             o.steps = h - l;
-            return true;
         } else {
-            for (;;) {
-                const int run = at / (kOwnRun * ntiles), rem = at % (kOwnRun * ntiles);
-                const int m_run = (run * kXcd + xcd) * kOwnRun;
-                if (m_run >= mtiles) return false;
-                at += per;
-                const int mt = m_run + rem % kOwnRun, nt = rem / kOwnRun;
-                if (mt >= mtiles) continue;
-                const int e = last_at_most(t.tiles, g.E + 1, mt);
-                const int lo = __builtin_amdgcn_readfirstlane(t.first[e]), hi = __builtin_amdgcn_readfirstlane(t.first[e + 1]);
-                const int m0 = lo + (mt - __builtin_amdgcn_readfirstlane(t.tiles[e])) * kTall, n0 = nt * kTall;
-                const bool none = e >= g.E;
-                o.a = g.a + (int64_t)m0 * g.K;
-                o.b = g.b + (none ? 0 : (int64_t)e * g.b_expert) + (KIND == kRowsT ? n0 : (int64_t)n0 * g.b_row);
-                o.bias = g.bias && !none ? g.bias + (int64_t)e * g.N + n0 : nullptr;
-                o.out = g.out + (int64_t)m0 * g.N + n0;
-                o.rows = min(max(hi, lo) - m0, kTall);
-                o.cols = g.N - n0;
-                o.steps = none ? 0 : g.K;
-                return true;
-            }
+            const int run = at / (2 * ntiles), rem = at - run * (2 * ntiles);
+            const bool pair = 2 * run + 1 < mtiles;
+            const int mt = 2 * run + (pair ? rem & 1 : 0), nt = pair ? rem >> 1 : rem;
+            const int e = last_at_most(t.tiles, g.E + 1, mt);
+            const int lo = __builtin_amdgcn_readfirstlane(t.first[e]), hi = __builtin_amdgcn_readfirstlane(t.first[e + 1]);
+            const int m0 = lo + (mt - __builtin_amdgcn_readfirstlane(t.tiles[e])) * kTall + part * rows, n0 = nt * kTall;
+            const bool none = e >= g.E;
+            o.a = g.a + (int64_t)m0 * g.K;
+            o.b = g.b + (none ? 0 : (int64_t)e * g.b_expert) + (KIND == kRowsT ? n0 : (int64_t)n0 * g.b_row);
+            o.bias = g.bias && !none ? g.bias + (int64_t)e * g.N + n0 : nullptr;
+            o.out = g.out + (int64_t)m0 * g.N + n0;
+            o.rows = min(max(hi, lo) - m0, rows);
+            o.cols = g.N - n0;
+            o.steps = none ? 0 : g.K;
         }
+        return o.rows > 0;                   // (a part past the tile's rows: nothing is behind it)
     }
 };
 
@@ -771,7 +787,8 @@ void k_grouped_tall(GroupedArgs g, int ntiles, int mtiles) {
     tall_table(table, g.offsets, g.E, g.P);
     if constexpr (KIND == kWeight) tall_order(table, g.E);
     else mtiles = __builtin_amdgcn_readfirstlane(table.tiles[g.E + 1]);
-    TallList<KIND> list{g, table, ntiles, mtiles, (int)blockIdx.x % kXcd, (int)gridDim.x / kXcd, (int)blockIdx.x / kXcd};
+    TallList<KIND> list{g, table, ntiles, mtiles, (int)blockIdx.x % kXcd, (int)blockIdx.x / kXcd, (int)gridDim.x / kXcd};
+    list.init();
     TallState<KIND> c{g, list};
     c.lane = tid & 63;
     c.wv = __builtin_amdgcn_readfirstlane(tid >> 6);
