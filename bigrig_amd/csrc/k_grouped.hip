@@ -878,9 +878,10 @@ typedef Shape<1, 2, 4, 2, 2> Eight;       // 128 x 128, eight waves
 constexpr int kThinMost = 8, kLowRun = 16, kHalfRun = 48;
 
 // Gradients of the matrices that are larger than the chip's last cache, and whose rows are whole lines, are stored past the
-// caches (128 x 1536 x 2048, 805 MB, of 32768 rows: 378 -> 323 us, a read of them right behind it included 700 -> 676,
-// a whole pass with both other products 1015 -> 985). Of what fits,
-// that read finds less (24 x 1024 x 2048, 101 MB: 86 -> 80, with the read 115 -> 121), and parts of lines cost more (60 x 712 x 1000: 30 -> 46).
+// caches (128 x 1536 x 2048, 805 MB, of 32768 rows: 378 -> 323 us, a read of them right behind it included 700 -> 676; all three
+// products of 16000 rows of 128 x 1024 x 2048 482 -> 440, of the former no difference: other kernels wait for less that is
+// written back, and the clocks fall). Of what fits, the read finds less (24 x 1024 x 2048, 101 MB: 86 -> 80, with the read 115 ->
+// 121), and parts of lines cost more (60 x 712 x 1000: 30 -> 46).
 constexpr int64_t kCacheBytes = 256ll << 20;
 
 template <int DT, bool BY, class S>
