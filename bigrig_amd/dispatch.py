@@ -18,6 +18,9 @@ the current device; scratch is allocated per call by torch, on the call's stream
 runs there (and its gradient): the inputs have to be ready on it. A gradient that is captured into a graph is taken of
 leaves that no eager graph holds meanwhile (`detach().requires_grad_()` inside the capture): torch ends the process
 where an eager graph's leaf on another stream is met in a capture.
+
+There are no forward-mode derivatives: a tensor with a tangent is refused. So are the calls where torch's operations are
+recorded (`torch.jit.trace`, make_fx): the recorded program would not hold them.
 """
 from __future__ import annotations
 
@@ -26,6 +29,7 @@ import functools
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import lib as L
 from .mx import _handle, _on_device
@@ -55,6 +59,33 @@ def _dtype(t, what: str) -> int:
     return dt
 
 
+def _refuse_recorders() -> None:
+    """A recorder of torch's operations (`torch.jit.trace`, make_fx) sees a launch's allocations only: its program would read
+    memory that nothing wrote. (A trace would hold an autograd function, but not the checks of shapes before it.)"""
+    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack()
+                                  and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+        raise RuntimeError("torch's operations are being recorded: a recorded program would not hold this call")
+
+
+def _refuse_tangents(tensors) -> None:
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("a tensor with a tangent: there are no forward-mode derivatives")
+
+
+def _recorded(*tensors) -> bool:
+    """Whether a gradient is recorded of a call. It is refused where its result would silently lack a derivative or a
+    program the call."""
+    _refuse_recorders()
+    _refuse_tangents(tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 @functools.lru_cache(maxsize=1024)
 def _plan_bytes(n: int, E: int) -> int:
     out = C.c_size_t()
@@ -77,6 +108,7 @@ def plan(idx, n_experts: int, stream=None) -> Dispatch:
     n = T * k
     if n > MAX_PAIRS:
         raise ValueError(f"{n} pairs in one call: at most {MAX_PAIRS}")
+    _refuse_recorders()
     device = _on_device(idx)
     if not idx.is_contiguous():
         idx = idx.contiguous()
@@ -142,6 +174,7 @@ def _once(backward):
     def call(ctx, *grads):
         if torch.is_grad_enabled():
             raise RuntimeError("this gradient is taken once: create_graph=True is refused")
+        _refuse_tangents(grads)
         return backward(ctx, *grads)
     return call
 
@@ -171,7 +204,7 @@ def dispatch(x, plan: Dispatch, stream=None):
         raise ValueError(f"x {tuple(x.shape)}: the plan is of {T} tokens")
     _width(x.shape[1])
     x = _strided(x)
-    if x.requires_grad and torch.is_grad_enabled():
+    if _recorded(x):
         return _Dispatch.apply(x, position, T, k)
     return _gather(x, position, T, k)
 
@@ -217,6 +250,6 @@ def combine(rows, plan: Dispatch, w=None, stream=None):
     rows = rows.contiguous()
     if w is not None:
         w = w.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or (w is not None and w.requires_grad)):
+    if _recorded(rows, w):
         return _Combine.apply(rows, w, position, T, k)
     return _sum(rows, w, position, T, k)

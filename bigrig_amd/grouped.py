@@ -7,14 +7,14 @@ with the gradients that tuning them, or what stands before them, takes. Rows com
 `dispatch.dispatch`, with its plan's offsets; the order needs no host read, so a step can be captured.
 
 Products run on the matrix instructions, sums are float32 and rounded once. Gradients are taken once
-(create_graph=True is refused). Every result is the same bits on every run. Streams as in `dispatch`.
+(create_graph=True is refused). Every result is the same bits on every run. Streams, tangents and recorders as in `dispatch`.
 """
 from __future__ import annotations
 
 import torch
 
 from . import lib as L
-from .dispatch import MAX_EXPERTS, MAX_PAIRS, MAX_WIDTH, _once
+from .dispatch import MAX_EXPERTS, MAX_PAIRS, MAX_WIDTH, _once, _recorded
 from .mx import _handle, _on_device
 
 MAX_ROW_STRIDE = 1 << 20    # values between a matrix's rows
@@ -105,6 +105,6 @@ def product(rows, weight, offsets, bias=None, stream=None):
     offsets = offsets.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if _recorded(rows, weight, bias):
         return _Product.apply(rows, weight, offsets, bias)
     return _forward(rows, weight, offsets, bias)

@@ -8,8 +8,8 @@ With n(v; w) = v / sqrt(mean(v^2) + eps) * w (root mean square, over the last di
 
 `new` is rounded to the residual's type and h made of what was rounded, so `leave` with next_weight gives the
 bits that `leave` and `enter` give one after the other. Statistics and sums are float32, each result rounded once.
-Gradients are taken once (create_graph=True is refused) and are the same bits on every run. Streams as in
-`dispatch`. The reference leaves norms and residual sums to MLX (bigrig_engine/layered.py:110-121 calls a whole
+Gradients are taken once (create_graph=True is refused) and are the same bits on every run. Streams, tangents and recorders as
+in `dispatch`. The reference leaves norms and residual sums to MLX (bigrig_engine/layered.py:110-121 calls a whole
 decoder layer).
 
 `BlockNorms` puts both around a block of `layer.MoELayer` or `layered.prefill`.
@@ -24,7 +24,7 @@ import torch
 
 from . import lib as L
 from .dispatch import MAX_PAIRS as MAX_ROWS
-from .dispatch import _TYPES, _dtype, _once, _width
+from .dispatch import _TYPES, _dtype, _once, _recorded, _width
 from .mx import _handle, _on_device
 
 EPS = 1e-6
@@ -140,14 +140,6 @@ def _backward(y, r, post, gate, form, nxt, scale, rstd_y, rstd_n, d_new, d_h, ne
     return dy, dr, dpost, dgate, dnext
 
 
-def _grads(*tensors) -> bool:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
 def _check_count(T: int) -> None:
     if T > MAX_ROWS:
         raise ValueError(f"{T} rows in one call: at most {MAX_ROWS}")
@@ -194,7 +186,7 @@ def enter(x, weight=None, eps: float = EPS, dtype=None, stream=None):
         weight = _vector(weight, H, "weight")
     x2 = _rows(x, H)
     _check_count(x2.shape[0])
-    if _grads(x2, weight):
+    if _recorded(x2, weight):
         h = _Enter.apply(x2, weight, eps, dtype)
     else:
         h = _forward(None, x2, None, None, _NO_GATE, weight, 1.0, eps, True, dtype, False)[1]
@@ -252,7 +244,7 @@ def leave(y, residual, weight=None, gate=None, scale: float = 1.0, next_weight=N
         next_weight = _vector(next_weight, H, "next_weight")
     y2, r2 = _rows(y, H), _rows(residual, H)
     _check_count(y2.shape[0])
-    if _grads(y2, r2, weight, gate, next_weight):
+    if _recorded(y2, r2, weight, gate, next_weight):
         got = _Leave.apply(y2, r2, weight, gate, next_weight, form, scale, eps, make_h)
         new, h = got if make_h else (got, None)
     else:
