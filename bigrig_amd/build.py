@@ -1,7 +1,8 @@
-"""Build libbrx.so (the HIP kernels and C-ABI) for gfx950, in-tree, with hipcc, and the
-host-only trace-replay library libbrx_replay.so with g++.
+"""Build libbrx.so (the HIP kernels and C-ABI) for gfx950, in-tree, with hipcc, and, host code only,
+with g++: libbrx_torch.so (calls that record a gradient in torch's graph, over libbrx.so) and the
+trace-replay library libbrx_replay.so.
 
-    python -m bigrig_amd.build            # compile bigrig_amd/libbrx.so and libbrx_replay.so
+    python -m bigrig_amd.build            # compile the three into bigrig_amd/
     python -m bigrig_amd.build --incremental   # recompile only sources changed since their object
 
 The library is one hipcc invocation over every `csrc/*.hip` file. Packed FP32 instructions are
@@ -24,6 +25,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libbrx.so")
+TORCH_LIB = os.path.join(PKG, "libbrx_torch.so")
 REPLAY_LIB = os.path.join(PKG, "libbrx_replay.so")
 ARCH = "gfx950"
 
@@ -79,8 +81,25 @@ def build(verbose: bool = False, incremental: bool = False) -> str:
     _run([hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp], verbose,
          "hipcc link")
     os.replace(tmp, LIB)
+    build_torch(verbose)
     build_replay(verbose)
     return LIB
+
+
+def build_torch(verbose: bool = False) -> str:
+    """libbrx_torch.so: csrc/brx_torch.cpp against the installed torch and the libbrx.so beside it."""
+    import torch
+    at = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
+    tmp = TORCH_LIB + ".tmp"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", INCLUDE,
+           "-isystem", f"{at}/include", "-isystem", f"{at}/include/torch/csrc/api/include", "-isystem", f"{rocm}/include",
+           os.path.join(CSRC, "brx_torch.cpp"), "-o", tmp, "-L", PKG, "-lbrx", "-L", f"{at}/lib", "-lc10", "-lc10_hip",
+           "-ltorch_cpu", "-Wl,-rpath,$ORIGIN"]
+    _run(cmd, verbose, "g++")
+    os.replace(tmp, TORCH_LIB)
+    return TORCH_LIB
 
 
 def build_replay(verbose: bool = False) -> str:

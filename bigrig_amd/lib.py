@@ -9,7 +9,7 @@ import ctypes as C
 import os
 import threading
 
-from .build import LIB
+from .build import LIB, TORCH_LIB
 
 # ------------------------------------------------------------------ constants (brx.h)
 BRX_OK, BRX_EINVAL, BRX_ESTATE, BRX_EHIP, BRX_ENOMEM, BRX_ERANGE = 0, -1, -2, -3, -4, -5
@@ -65,6 +65,7 @@ class BrxError(RuntimeError):
 
 
 _lib = None
+_torch_ops = None
 _lock = threading.Lock()
 _init_device = None
 
@@ -156,6 +157,19 @@ def load(path: str | None = None):
         if path is None:
             _lib = lib
         return lib
+
+
+def load_torch():
+    """torch.ops.brx, the calls that record a gradient in C++: libbrx_torch.so, over the libbrx.so that `load` opens."""
+    global _torch_ops
+    with _lock:
+        if _torch_ops is None:
+            import torch
+            if not os.path.exists(TORCH_LIB):
+                raise RuntimeError(f"{TORCH_LIB} is missing: build it with `python -m bigrig_amd.build`")
+            torch.ops.load_library(TORCH_LIB)
+            _torch_ops = torch.ops.brx
+        return _torch_ops
 
 
 def check(rc: int) -> None:

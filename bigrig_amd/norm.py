@@ -16,7 +16,6 @@ decoder layer).
 """
 from __future__ import annotations
 
-import ctypes as C
 import functools
 from dataclasses import dataclass
 
@@ -24,7 +23,7 @@ import torch
 
 from . import lib as L
 from .dispatch import MAX_PAIRS as MAX_ROWS
-from .dispatch import _TYPES, _dtype, _once, _recorded, _width
+from .dispatch import _TYPES, _dtype, _recorded, _width
 from .mx import _handle, _on_device
 
 EPS = 1e-6
@@ -60,11 +59,12 @@ class BlockNorms:
         return self.leave(block(self.enter(x)), x)[0]
 
 
-@functools.lru_cache(maxsize=1024)
-def _columns_bytes(T: int, H: int) -> int:
-    out = C.c_size_t()
-    L.check(L.load().brx_norm_workspace_bytes(T, H, C.byref(out)))
-    return out.value
+@functools.cache
+def _with_gradients():
+    """The calls that record a gradient (csrc/brx_torch.cpp): (enter, leave, leave and enter). (The functions under torch's
+    operators: torch.compile breaks its graph at them, where it would run the operators on tensors without memory.)"""
+    ops = L.load_torch()
+    return ops.enter.default._op, ops.leave.default._op, ops.leave_enter.default._op
 
 
 def _vector(t, H: int, what: str):
@@ -103,41 +103,18 @@ def _stride(t, T: int, H: int) -> int:
     return t.stride(0) if T > 1 else H
 
 
-def _forward(y, r, post, gate, form, nxt, scale, eps, make_h, h_type, stats):
-    """(new_r or None, h or None, rstd_y, rstd_n) of rows r [T, H] and, for `leave`, y [T, H]."""
+def _forward(y, r, post, gate, form, nxt, scale, eps, make_h, h_type):
+    """(new_r or None, h or None) of rows r [T, H] and, for `leave`, y [T, H]; no gradient is recorded."""
     device = _on_device(y, r, post, gate, nxt)
     T, H = r.shape
     new = None if y is None else r.new_empty((T, H))
     h = r.new_empty((T, H), dtype=h_type) if make_h else None
-    rstd_y = r.new_empty(T, dtype=torch.float32) if stats and post is not None else None
-    rstd_n = r.new_empty(T, dtype=torch.float32) if stats and make_h else None
     ptr = L.ptr
     L.check(L.load().brx_norm_forward(
         ptr(y), 0 if y is None else _stride(y, T, H), _TYPES[h_type], r.data_ptr(), _stride(r, T, H), _TYPES[r.dtype],
         ptr(post), _type(post), ptr(gate), form, _type(gate), ptr(nxt), _type(nxt), scale, eps, T, H, ptr(new), ptr(h),
-        ptr(rstd_y), ptr(rstd_n), _handle(device)))
-    return new, h, rstd_y, rstd_n
-
-
-def _backward(y, r, post, gate, form, nxt, scale, rstd_y, rstd_n, d_new, d_h, needs, y_type):
-    """Gradients (dy, dr, dpost, dgate, dnext), None where `needs` is false."""
-    T, H = r.shape
-    dy = r.new_empty((T, H), dtype=y_type) if needs[0] else None
-    dr = r.new_empty((T, H)) if needs[1] else None
-    new = torch.empty_like if T else torch.zeros_like
-    dpost = new(post) if needs[2] else None
-    dgate = new(gate) if needs[3] else None
-    dnext = new(nxt) if needs[4] and d_h is not None else None
-    need = 0
-    if dpost is not None or dnext is not None or (dgate is not None and form == _CHANNEL):
-        need = _columns_bytes(T, H)
-    ws = r.new_empty(need, dtype=torch.uint8) if need else None
-    ptr = L.ptr
-    L.check(L.load().brx_norm_backward(
-        ptr(y), 0 if y is None else _stride(y, T, H), _TYPES[y_type], r.data_ptr(), _stride(r, T, H), _TYPES[r.dtype],
-        ptr(post), _type(post), ptr(gate), form, _type(gate), ptr(nxt), _type(nxt), scale, T, H, ptr(rstd_y), ptr(rstd_n),
-        ptr(d_new), ptr(d_h), ptr(dy), ptr(dr), ptr(dgate), ptr(dpost), ptr(dnext), ptr(ws), need, _handle(r.get_device())))
-    return dy, dr, dpost, dgate, dnext
+        None, None, _handle(device)))
+    return new, h
 
 
 def _check_count(T: int) -> None:
@@ -148,24 +125,6 @@ def _check_count(T: int) -> None:
 def _check_eps(eps: float) -> None:
     if not 1.17549435e-38 <= eps < 3.4e38:
         raise ValueError(f"eps {eps} must be a positive, normal float32 value")
-
-
-class _Enter(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, eps, dtype):
-        _, h, _, rstd = _forward(None, x, None, None, _NO_GATE, weight, 1.0, eps, True, dtype, True)
-        ctx.save_for_backward(x, weight, rstd)
-        ctx.dtype = dtype
-        return h
-
-    @staticmethod
-    @_once
-    def backward(ctx, dh):
-        x, weight, rstd = ctx.saved_tensors
-        needs = (False, ctx.needs_input_grad[0], False, False, ctx.needs_input_grad[1])
-        _, dx, _, _, dw = _backward(None, x, None, None, _NO_GATE, weight, 1.0, None, rstd, None, dh.contiguous(), needs,
-                                    ctx.dtype)
-        return dx, dw, None, None
 
 
 def enter(x, weight=None, eps: float = EPS, dtype=None, stream=None):
@@ -187,35 +146,11 @@ def enter(x, weight=None, eps: float = EPS, dtype=None, stream=None):
     x2 = _rows(x, H)
     _check_count(x2.shape[0])
     if _recorded(x2, weight):
-        h = _Enter.apply(x2, weight, eps, dtype)
+        _on_device(x2, weight)
+        h = _with_gradients()[0](x2, weight, eps, dtype)
     else:
-        h = _forward(None, x2, None, None, _NO_GATE, weight, 1.0, eps, True, dtype, False)[1]
+        h = _forward(None, x2, None, None, _NO_GATE, weight, 1.0, eps, True, dtype)[1]
     return h if h.shape == x.shape else h.view(x.shape)
-
-
-class _Leave(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, r, post, gate, nxt, form, scale, eps, make_h):
-        new, h, rstd_y, rstd_n = _forward(y, r, post, gate, form, nxt, scale, eps, make_h, y.dtype, True)
-        ctx.save_for_backward(y, new if make_h else None, post, gate, nxt, rstd_y, rstd_n)
-        ctx.form, ctx.scale, ctx.r_type = form, scale, r.dtype
-        ctx.set_materialize_grads(False)
-        return (new, h) if make_h else new
-
-    @staticmethod
-    @_once
-    def backward(ctx, d_new, d_h=None):
-        none = (None,) * 4
-        if d_new is None and d_h is None:
-            return (None,) * 5 + none
-        y, new, post, gate, nxt, rstd_y, rstd_n = ctx.saved_tensors
-        d_new = None if d_new is None else d_new.contiguous()
-        d_h = None if d_h is None else d_h.contiguous()
-        r = d_new if new is None else new      # (read only where there is an h)
-        got = _backward(y, r, post, gate, ctx.form, nxt, ctx.scale, rstd_y, rstd_n, d_new, d_h, ctx.needs_input_grad[:5],
-                        y.dtype)
-        dy, dr, dpost, dgate, dnext = got
-        return (dy, dr, dpost, dgate, dnext) + none
 
 
 def leave(y, residual, weight=None, gate=None, scale: float = 1.0, next_weight=None, eps: float = EPS, stream=None):
@@ -245,10 +180,13 @@ def leave(y, residual, weight=None, gate=None, scale: float = 1.0, next_weight=N
     y2, r2 = _rows(y, H), _rows(residual, H)
     _check_count(y2.shape[0])
     if _recorded(y2, r2, weight, gate, next_weight):
-        got = _Leave.apply(y2, r2, weight, gate, next_weight, form, scale, eps, make_h)
-        new, h = got if make_h else (got, None)
+        _on_device(y2, r2, weight, gate, next_weight)
+        if make_h:
+            new, h = _with_gradients()[2](y2, r2, weight, gate, form, scale, next_weight, eps)
+        else:
+            new, h = _with_gradients()[1](y2, r2, weight, gate, form, scale, eps), None
     else:
-        new, h, _, _ = _forward(y2, r2, weight, gate, form, next_weight, scale, eps, make_h, y.dtype, False)
+        new, h = _forward(y2, r2, weight, gate, form, next_weight, scale, eps, make_h, y.dtype)
     if new.shape != y.shape:
         new, h = new.view(y.shape), None if h is None else h.view(y.shape)
     return (new, h) if make_h else new
