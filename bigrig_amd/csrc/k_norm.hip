@@ -367,16 +367,18 @@ __global__ __launch_bounds__(kColThreads) void k_norm_columns(NormArgs a, int bl
 constexpr int kWaveRow = 1024, kWaveRowBack = 512;
 inline int threads_of(int H, int wave_row) { return H <= wave_row ? kWave : kThreads; }
 
-// Blocks of a gradient: as many as its registers let run at once, three a CU (16384 x 2048, bf16 with an fp32 residual, out of
-// cold memory, us: 512 blocks 163, 768 150, 1024 182; 4999 x 1001 26, 22, 28).
-constexpr int kBackBlocks = 768;
+// Blocks of a gradient: as many as its registers let run at once, so that none is left for a second round on a part of the
+// chip: of up to 2048 values (138 registers) three a CU, up to 4096 (221) two, beyond (402) one. bf16, us, 256 / 512 / 768 / 1024
+// blocks: 16384 x 2048 (fp32 residual) 206 / 136 / 129 / 156; 16384 x 2880 enter 195 / 119 / 152 / 127, leave 325 / 224 / 285 / 240;
+// 16384 x 4096 207 / 129 / 164 / 138, 350 / 258 / 323 / 277; 4096 x 8192 114 / 121 / 128 / 135, 248 / 269 / 290 / 310.
+inline int back_blocks(int H) { return H <= kThreads * V ? 768 : H <= 2 * kThreads * V ? 512 : 256; }
 
 }  // namespace
 
 int norm_blocks(int T, int H) {
     const int per = kThreads / threads_of(H, kWaveRowBack);
     const int most = (T + per - 1) / per;
-    return most < kBackBlocks ? most : kBackBlocks;
+    return most < back_blocks(H) ? most : back_blocks(H);
 }
 
 #define BRX_SHAPE(KERNEL, YD, RD, WAVE_ROW, GRID, LDS)                                                                 \
