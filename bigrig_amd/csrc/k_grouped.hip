@@ -13,6 +13,7 @@
 // what lies past the end comes from past the buffer's end, as zeros, in both operands, so that a NaN next to them does
 // not enter.
 #include "block_ops.h"
+#include "grouped_tiles.h"
 #include "pf_common.h"
 
 namespace brx {
@@ -238,9 +239,10 @@ __device__ __forceinline__ RowTile find_tile(const int32_t* __restrict__ offsets
         const int up = (i + 1) * kWave <= E ? __builtin_amdgcn_readlane(at[i + 1 < kChunks ? i + 1 : i], 0) : P;
         int hi = __builtin_amdgcn_ds_bpermute(min(lane + 1, 63) * 4, at[i]);
         hi = e >= E ? P : lane == 63 ? up : hi;
-        lo = min(max(lo, 0), P);
-        hi = e <= E ? min(max(hi, lo), P) : lo;
-        const int n = (hi - lo + BM - 1) / BM;
+        const RowRun own = run_between(lo, e <= E ? hi : lo, P);
+        lo = own.first;
+        hi = own.end;
+        const int n = run_tiles(own, BM);
         const int incl = wave_incl_scan(n);
         const uint64_t past = __ballot(run + incl > mt);
         if (past) {
@@ -276,10 +278,9 @@ template <int DT, class S>
 __global__ __launch_bounds__(S::kThreads) void k_grouped_weight(GroupedArgs g, int mtiles, int ntiles) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[S::kLds];
     const int e = blockIdx.y, m0 = blockIdx.x / ntiles * S::BM, n0 = blockIdx.x % ntiles * S::BN;
-    int lo = e == 0 ? 0 : g.offsets[e], hi = g.offsets[e + 1];
-    lo = min(max(lo, 0), g.P);
-    hi = min(max(hi, lo), g.P);
-    tile<DT, true, true, S>(lds, g.a + (int64_t)lo * g.K + m0, g.K, g.K - m0, g.b + (int64_t)lo * g.N + n0, g.N, g.N - n0, hi - lo,
+    const RowRun run = run_between(e == 0 ? 0 : g.offsets[e], g.offsets[e + 1], g.P);
+    const int64_t lo = run.first;
+    tile<DT, true, true, S>(lds, g.a + lo * g.K + m0, g.K, g.K - m0, g.b + lo * g.N + n0, g.N, g.N - n0, run.end - run.first,
                             nullptr, g.out + ((int64_t)e * g.K + m0) * g.N + n0, g.N);
 }
 
@@ -290,14 +291,12 @@ template <int DT>
 __global__ __launch_bounds__(kColThreads) void k_grouped_bias(GroupedArgs g) {
     __shared__ float s[kColRows][kColLanes * 8 + 4];
     const int e = blockIdx.y, lane = threadIdx.x % kColLanes, r0 = threadIdx.x / kColLanes;
-    int lo = e == 0 ? 0 : g.offsets[e], hi = g.offsets[e + 1];
-    lo = min(max(lo, 0), g.P);
-    hi = min(max(hi, lo), g.P);
+    const RowRun run = run_between(e == 0 ? 0 : g.offsets[e], g.offsets[e + 1], g.P);
     const int c0 = blockIdx.x * kColLanes * 8, col = c0 + lane * 8;
     const uint16_t* p = g.a + min(col, g.K - 8);
     float v[8] = {};
 #pragma unroll 4
-    for (int r = lo + r0; r < hi; r += kColRows) {
+    for (int r = run.first + r0; r < run.end; r += kColRows) {
         float x[8];
         unpack<DT>(get16(p + (int64_t)r * g.K), x);
 #pragma unroll
@@ -319,7 +318,7 @@ __global__ __launch_bounds__(kColThreads) void k_grouped_bias(GroupedArgs g) {
 // on the way, a lane's loads (16 bytes of a matrix row, 64 a row and instruction) go straight to the operands of
 // v_mfma_f32_16x16x32, many in flight. The reduction is dealt to the block's four waves in units of 64 steps (whole
 // lines), whose sums are joined in the waves' order.
-constexpr int kThinRows = 16, kThinCols = 32, kThinThreads = 256, kThinWaves = 4;
+constexpr int kThinCols = 32, kThinThreads = 256, kThinWaves = 4;
 constexpr int kThinAhead = 8;         // units a wave loads at a time
 
 template <int DT>
@@ -418,7 +417,7 @@ __device__ __forceinline__ void copies_left() {
 }
 
 constexpr int kTallThreads = 512, kTallWaves = 8;
-constexpr int kTall = 256, kHalf = 128;      // rows and columns of a tile, rows of its halves
+constexpr int kHalf = 128;                   // rows of a tile's halves
 constexpr int kUnitB = kTall * kG * 2, kUnitA = kHalf * kG * 2;
 constexpr int kTallRing = 2 * kUnitB + 5 * kUnitA;      // b and the first rows twice, the other rows three times
 
@@ -482,9 +481,10 @@ __device__ __forceinline__ void tall_table(TallTable& t, const int32_t* offsets,
     for (int e0 = 0; e0 <= E; e0 += kTallThreads) {
         const int e = e0 + tid;
         int lo = e == 0 ? 0 : offsets[min(e, E)], hi = e < E ? offsets[min(e + 1, E)] : P;
-        lo = min(max(lo, 0), P);
-        hi = e <= E ? min(max(hi, lo), P) : lo;
-        const int n = (hi - lo + kTall - 1) / kTall;
+        const RowRun own = run_between(lo, e <= E ? hi : lo, P);
+        lo = own.first;
+        hi = own.end;
+        const int n = run_tiles(own, kTall);
         const int incl = wave_incl_scan(n);
         __syncthreads();
         if (lane == 63) t.sums[wv] = incl;
@@ -543,31 +543,20 @@ struct TallList {
     const TallTable& t;
     int ntiles, mtiles;       // column tiles; row tiles (in all, or of an expert's matrix)
     int xcd, place, per;      // this block's XCD, its place there; blocks an XCD
-    int round, rounds;        // of whole rounds
-    int last, cut;            // tiles of the last round, cut 2^cut times
+    int round;
+    Rounds rounds;
 
     __device__ __forceinline__ void init() {
-        const int blocks = per * kXcd;
-        const int all = mtiles * ntiles * (KIND == kWeight ? g.E : 1);      // (2^21 at most)
         round = 0;
-        rounds = all / blocks;
-        last = all - rounds * blocks;
-        cut = 4 * last <= blocks ? 2 : 2 * last <= blocks ? 1 : 0;
+        rounds = rounds_of(mtiles * ntiles * (KIND == kWeight ? g.E : 1), per * kXcd);
     }
 
     // The next tile of this block; false behind the last.
     __device__ __forceinline__ bool next(TallTile& o) {
-        int at = round * per * kXcd, part = 0, rows = kTall;
-        if (round < rounds) {
-            at += xcd * per + place;
-        } else {
-            const int n = last << cut, share = (n + kXcd - 1) / kXcd, v = xcd * share + place;
-            if (round > rounds || place >= share || v >= n) return false;
-            at += v >> cut;
-            part = v & ((1 << cut) - 1);
-            rows = kTall >> cut;
-        }
+        const Dealt d = deal(rounds, round, xcd, place, per);
+        if (!d.rows) return false;
         ++round;
+        const int at = d.tile, part = d.part, rows = d.rows;
         if constexpr (KIND == kWeight) {
             const int u = at / ntiles, nt = at - u * ntiles;
             const int e = __builtin_amdgcn_readfirstlane(t.order[u / mtiles]), m0 = u % mtiles * kTall + part * rows, n0 = nt * kTall;
@@ -581,9 +570,8 @@ struct TallList {
             o.cols = g.N - n0;
             o.steps = h - l;
         } else {
-            const int run = at / (2 * ntiles), rem = at - run * (2 * ntiles);
-            const bool pair = 2 * run + 1 < mtiles;
-            const int mt = 2 * run + (pair ? rem & 1 : 0), nt = pair ? rem >> 1 : rem;
+            const RowColumn rc = row_column(at, mtiles, ntiles);
+            const int mt = rc.mt, nt = rc.nt;
             const int e = last_at_most(t.tiles, g.E + 1, mt);
             const int lo = __builtin_amdgcn_readfirstlane(t.first[e]), hi = __builtin_amdgcn_readfirstlane(t.first[e + 1]);
             const int m0 = lo + (mt - __builtin_amdgcn_readfirstlane(t.tiles[e])) * kTall + part * rows, n0 = nt * kTall;
@@ -846,12 +834,6 @@ BRX_TALL(BRX_DT_BF16);
 BRX_TALL(BRX_DT_F16);
 #undef BRX_TALL
 
-// Row tiles of BM rows a call can have: the whole ones, and one of each run that is not empty.
-inline int64_t row_tiles(const GroupedArgs& g, int BM) {
-    const int64_t runs = g.E + 1;
-    return g.P / BM + (runs < g.P ? runs : g.P);
-}
-
 typedef Shape<2, 2, 2, 2, 2> Square;      // 128 x 128, four waves: two blocks a CU
 typedef Shape<1, 1, 2, 4, 3> Half;        // 64 x 128, eight waves, one stage more ahead
 typedef Shape<1, 1, 1, 4, 4> Low;         // 32 x 128, four waves, two stages more ahead
@@ -875,7 +857,7 @@ typedef Shape<1, 2, 4, 2, 2> Eight;       // 128 x 128, eight waves
 // waves / 256: 64 x 512 x 512 of 4096 rows 18.0 / 18.2, 60 x 712 x 1000 of 2804 34.3 / 29.8, 128 x 1536 x 2048 of 1024 231 / 162,
 // of 32768 478 / 343), else 128 x 128 by eight waves (by four / by eight / 256: 8 x 1024 x 1024 of 1000 rows 12.0 / 11.8 / 16.3,
 // 8 x 1024 x 2048 of 4000 33.3 / 28.7 / 28.6).
-constexpr int kThinMost = 8, kLowRun = 16, kHalfRun = 48;
+static_assert(kChipCus == kCus && kChipXcds == kXcd, "");
 
 // Gradients of the matrices that are larger than the chip's last cache, and whose rows are whole lines, are stored past the
 // caches (128 x 1536 x 2048, 805 MB, of 32768 rows: 378 -> 323 us, a read of them right behind it included 700 -> 676; all three
@@ -886,26 +868,26 @@ constexpr int64_t kCacheBytes = 256ll << 20;
 
 template <int DT, bool BY, class S>
 hipError_t launch_tiles(const GroupedArgs& g, hipStream_t s) {
-    const int mt = (int)row_tiles(g, S::BM), nt = (g.N + S::BN - 1) / S::BN;
+    const int mt = (int)row_tiles(g.P, g.E, S::BM), nt = (g.N + S::BN - 1) / S::BN;
     hipLaunchKernelGGL((k_grouped_rows<DT, BY, S>), dim3((mt + kXcd - 1) / kXcd * kXcd * nt), dim3(S::kThreads), 0, s, g, mt, nt);
     return hipGetLastError();
 }
 
 template <int DT, bool BY>
 hipError_t launch_rows(const GroupedArgs& g, hipStream_t s) {
-    if (!BY && g.P <= kThinMost) {
-        const int nt = (g.N + kThinCols - 1) / kThinCols;
-        hipLaunchKernelGGL(k_grouped_thin<DT>, dim3((unsigned)(row_tiles(g, kThinRows) * nt)), dim3(kThinThreads), 0, s, g, nt);
-        return hipGetLastError();
+    const RowForm form = row_form(g.P, g.E, g.N, BY);
+    if constexpr (!BY) {
+        if (form == kFormThin) {
+            const int nt = (g.N + kThinCols - 1) / kThinCols;
+            hipLaunchKernelGGL(k_grouped_thin<DT>, dim3((unsigned)(row_tiles(g.P, g.E, kThinRows) * nt)), dim3(kThinThreads), 0, s, g, nt);
+            return hipGetLastError();
+        }
     }
-    const int tall_nt = (g.N + kTall - 1) / kTall;
-    const bool tall = (int64_t)(g.P / kTall) * tall_nt >= kCus;
-    if (g.P <= kLowRun * g.E) return launch_tiles<DT, BY, Low>(g, s);
-    if ((g.P <= kHalfRun * g.E && !(BY && tall)) || row_tiles(g, Square::BM) * ((g.N + Square::BN - 1) / Square::BN) < kCus)
-        return launch_tiles<DT, BY, Half>(g, s);
-    if (!tall) return launch_tiles<DT, BY, Square>(g, s);
+    if (form == kFormLow) return launch_tiles<DT, BY, Low>(g, s);
+    if (form == kFormHalf) return launch_tiles<DT, BY, Half>(g, s);
+    if (form == kFormSquare) return launch_tiles<DT, BY, Square>(g, s);
     constexpr int kind = BY ? kRowsT : kRows;
-    hipLaunchKernelGGL((k_grouped_tall<DT, kind>), dim3(kCus), dim3(kTallThreads), 0, s, g, tall_nt, 0);
+    hipLaunchKernelGGL((k_grouped_tall<DT, kind>), dim3(kCus), dim3(kTallThreads), 0, s, g, (g.N + kTall - 1) / kTall, 0);
     return hipGetLastError();
 }
 
