@@ -1,14 +1,26 @@
-"""Offsets of the grouped products that are out of order or range, on the GPU."""
+"""The persistent tiles of the grouped products where their last round is cut, and offsets that are out of order or range, on
+the GPU."""
 import ctypes as C
 
 import pytest
 import torch
 
 from tests.block_util import rand
-from tests.test_gpu_grouped import G  # noqa: F401
+from tests.grouped_util import CUT, NARROW, WIDE
+from tests.test_gpu_grouped import G, check  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 B = torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", [B, torch.float16])
+@pytest.mark.parametrize("name", CUT)
+@pytest.mark.parametrize("across", [False, True])
+def test_a_cut_last_round(G, name, across, dtype):  # noqa: F811
+    # (rounds and cuts of these calls: test_grouped_tiles.py)
+    counts, behind, _, _ = CUT[name]
+    N, K = (NARROW, WIDE) if across else (WIDE, NARROW)
+    check(G, counts, N, K, dtype, bias=dtype == B, behind=behind, seed=len(counts))
 
 
 GUARD = 1 << 16      # values on each side of an output

@@ -8,6 +8,8 @@ import subprocess
 
 import pytest
 
+from tests.grouped_util import CUT, NARROW, WIDE
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 SRC = r"""
@@ -195,3 +197,21 @@ def test_which_kernel(walk):
             (8192, 256, 4096, 1, tall), (32768, 128, 1536, 0, tall), (1000, 8, 2048, 0, square), (1000, 8, 1024, 0, half),
             (4000, 8, 2048, 0, square), (0, 4, 64, 1, low)):
         assert walk.form(P, E, N, across) == want, (P, E, N, across)
+
+
+@pytest.mark.parametrize("name", CUT)
+def test_calls_whose_last_round_is_cut(walk, name):
+    # what the GPU tests of the cut rounds are meant to run
+    counts, behind, rows, runs = CUT[name]
+    at, E = offsets_of(counts), len(counts)
+    P, out = at[-1] + behind, ints([0, 0, 0])
+    columns = -(-WIDE // 256)
+    for across in (0, 1):
+        assert walk.form(P, E, WIDE, across) == 4
+    walk.rounds(walk.count_row_tiles(ints(at), E, P, 256) * columns, out)
+    assert tuple(out) == rows
+    assert E * columns * (-(-NARROW // 256)) >= 256
+    walk.rounds(E * columns, out)
+    assert tuple(out) == runs
+    assert walk.walk_rows(ints(at), E, P, WIDE, 1) == 0
+    assert walk.walk_runs(E, WIDE, NARROW) == 0 and walk.walk_runs(E, NARROW, WIDE) == 0
