@@ -286,8 +286,8 @@ __global__ __launch_bounds__(kThreads) void k_pairs_combine(PairRows p, int lane
     }
 }
 
-// drows (out) and dw of a combine, one wave a token: dout's chunk is read once for kAhead pairs. Either output may
-// be null.
+// drows (out, or null) and dw of a combine, one wave a token: dout's chunk is read once for kAhead pairs. (drows alone are a
+// dispatch with the weights.)
 template <int DT>
 __global__ __launch_bounds__(kThreads) void k_pairs_combine_backward(PairRows p) {
     typedef typename Elem<DT>::T ET;
@@ -315,21 +315,16 @@ __global__ __launch_bounds__(kThreads) void k_pairs_combine_backward(PairRows p)
             if (p.H >= V) {
                 v4u_t q[kAhead];
                 const v4u_t dq = get16(d + c);
-                if (p.dw) {
 #pragma unroll
-                    for (int u = 0; u < kAhead; ++u)
-                        q[u] = get16(rows + (int64_t)((unsigned)at[u] < (unsigned)n ? at[u] : 0) * p.H + c);
-                }
+                for (int u = 0; u < kAhead; ++u) q[u] = get16(rows + (int64_t)((unsigned)at[u] < (unsigned)n ? at[u] : 0) * p.H + c);
                 float f[V];
                 unpack<DT>(dq, f);
 #pragma unroll
                 for (int u = 0; u < kAhead; ++u) {
-                    if (p.dw) {
-                        float v[V];
-                        unpack<DT>(q[u], v);
+                    float v[V];
+                    unpack<DT>(q[u], v);
 #pragma unroll
-                        for (int i = 0; i < V; ++i) dot[u] = i >= own ? __builtin_fmaf(f[i], v[i], dot[u]) : dot[u];
-                    }
+                    for (int i = 0; i < V; ++i) dot[u] = i >= own ? __builtin_fmaf(f[i], v[i], dot[u]) : dot[u];
                     const int r = row_of(at[u]);
                     if (out && j0 + u < p.k && r < n) {
                         float g[V];
@@ -345,18 +340,16 @@ __global__ __launch_bounds__(kThreads) void k_pairs_combine_backward(PairRows p)
                     for (int u = 0; u < kAhead; ++u) {
                         const int r = row_of(at[u]);
                         if (j0 + u >= p.k || r >= n) continue;
-                        if (p.dw && at[u] >= 0) dot[u] = __builtin_fmaf(f, to_f<DT>(rows[(int64_t)r * p.H + i]), dot[u]);
+                        if (at[u] >= 0) dot[u] = __builtin_fmaf(f, to_f<DT>(rows[(int64_t)r * p.H + i]), dot[u]);
                         if (out) out[(int64_t)r * p.H + i] = at[u] < 0 ? ET(0) : from_f<DT>(f * s[u]);
                     }
                 }
             }
         }
-        if (p.dw) {
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const float v = wave_sum(dot[u]);
-                if (lane == 0 && j0 + u < p.k) p.dw[(int64_t)t * p.k + j0 + u] = (unsigned)at[u] < (unsigned)n ? v : 0.f;
-            }
+        for (int u = 0; u < kAhead; ++u) {
+            const float v = wave_sum(dot[u]);
+            if (lane == 0 && j0 + u < p.k) p.dw[(int64_t)t * p.k + j0 + u] = (unsigned)at[u] < (unsigned)n ? v : 0.f;
         }
     }
 }
