@@ -25,7 +25,10 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / kWave;
 constexpr int kCopies = 4;            // counters that all lanes add to come so often, 16 neighbouring pairs to one: a popular
                                       // expert is among each token's (Zipf, 16384 pairs of 128 experts: 11.0 -> 7.0 us)
-constexpr int kPlanSelf = 16384;      // pairs of a list whose blocks count all of it themselves
+// Pairs of a list whose blocks count all of it themselves, in one launch. Zipf, 128 experts, us as a graph's nodes, one launch /
+// two: 4096 pairs 4.4 / 7.9, 16384 6.1 / 9.4, 24576 7.6 / 10.0, 32768 8.5 / 8.8 (60 experts 8.1 / 8.2, 512 8.6 / 10.1). The line is where
+// brx.h has it, which says that up to there a plan needs no scratch; past it a call from the host has a second launch's 4 us to pay.
+constexpr int kPlanSelf = 16384;
 
 // Groups of 64 pairs a wave holds: few, so that a list is spread over CUs, more where there are so many blocks that adding up
 // their counts costs more.
