@@ -69,10 +69,12 @@ struct NormBackward : torch::autograd::Node {
         auto rows = [&](const at::TensorOptions& o) { return at::empty({T, H}, o); };
         auto whole = [&](const Tensor& t) { return T ? at::empty_like(t) : at::zeros_like(t); };
         if (task_should_compute_output(kY)) got[kY] = rows(y_.options());
-        if (task_should_compute_output(kR)) got[kR] = rows(r_options);
+        // (without an h the residual's gradient is the one given)
+        if (task_should_compute_output(kR)) got[kR] = makes_h ? rows(r_options) : d_new;
         if (task_should_compute_output(kPost)) got[kPost] = whole(post_);
         if (task_should_compute_output(kGate)) got[kGate] = whole(gate_);
         if (task_should_compute_output(kNext) && d_h.defined()) got[kNext] = whole(next_);
+        if (!got[kY].defined() && !got[kPost].defined() && !got[kGate].defined() && !makes_h) return got;
         Tensor ws;
         size_t need = 0;
         if (got[kPost].defined() || got[kNext].defined() || (got[kGate].defined() && form == kGateChannel)) {
@@ -82,7 +84,7 @@ struct NormBackward : torch::autograd::Node {
         const int r_type = r_options.dtype() == at::kBFloat16 ? BRX_DT_BF16 : r_options.dtype() == at::kHalf ? BRX_DT_F16 : BRX_DT_F32;
         check(brx_norm_backward(from(y_), row_of(y_), leave ? type_of(y_) : type_of(d_h), from(r_), row_of(r_), r_type, from(post_),
                                 type_of(post_), from(gate_), form, type_of(gate_), from(next_), type_of(next_), (float)scale, T, H,
-                                floats(rstd_y), floats(rstd_n), from(d_new), from(d_h), to(got[kY]), to(got[kR]), to(got[kGate]),
+                                floats(rstd_y), floats(rstd_n), from(d_new), from(d_h), to(got[kY]), makes_h ? to(got[kR]) : nullptr, to(got[kGate]),
                                 to(got[kPost]), to(got[kNext]), to(ws), need, stream_on(r_options.device())));
         return got;
     }

@@ -158,3 +158,24 @@ def test_transforms_without_a_rule_are_refused(M):
         for call in (lambda: torch.func.grad(f)(x), lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.func.vmap(f)(x[None])):
             with pytest.raises(RuntimeError):
                 call()
+
+
+def test_the_residuals_gradient_without_a_next_norm(M):
+    # is the one given, whichever others are asked for
+    y, r, w = rand((30, 264), B, 1), rand((30, 264), S, 2), rand((264,), B, 3)
+    for d in (rand((30, 264), S, 4), rand((264, 30), S, 5).t(), torch.ones((1, 1), device="cuda").expand(30, 264)):
+        for needs in ((0, 1, 0), (1, 1, 0), (0, 1, 1), (1, 1, 1), (1, 0, 1)):
+            ts = [t.clone().requires_grad_(bool(n)) for t, n in zip((y, r, w), needs)]
+            asked = [t for t, n in zip(ts, needs) if n]
+            got = torch.autograd.grad(M.leave(*ts), asked, d)
+            whole = [t.clone().requires_grad_() for t in (y, r, w)]
+            want = torch.autograd.grad(M.leave(*whole), whole, d.clone())
+            assert all(torch.equal(a, b) for a, b in zip(got, (v for v, n in zip(want, needs) if n)))
+            if needs[1]:
+                assert torch.equal(got[needs[0]], d)
+    # added to what is there, it leaves the gradient that was given as it was
+    r2, d = r.clone().requires_grad_(), rand((30, 264), S, 6)
+    keep = d.clone()
+    for _ in range(2):
+        M.leave(y, r2).backward(d)
+    assert torch.equal(d, keep) and torch.equal(r2.grad, 2 * keep)
