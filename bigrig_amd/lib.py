@@ -162,6 +162,8 @@ def load(path: str | None = None):
 def load_torch():
     """torch.ops.brx, the calls that record a gradient in C++: libbrx_torch.so, over the libbrx.so that `load` opens."""
     global _torch_ops
+    if _torch_ops is None:
+        load()
     with _lock:
         if _torch_ops is None:
             import torch

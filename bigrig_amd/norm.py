@@ -17,6 +17,7 @@ decoder layer).
 from __future__ import annotations
 
 import functools
+import re
 from dataclasses import dataclass
 
 import torch
@@ -28,6 +29,8 @@ from .mx import _handle, _on_device
 
 EPS = 1e-6
 _NO_GATE, _CHANNEL, _ROW, _FULL = 0, 1, 2, 3
+_ENTER, _LEAVE, _LEAVE_ENTER = 0, 1, 2
+_ERROR = re.compile(r"libbrx error (-?\d+): (.*)")
 
 
 @dataclass
@@ -65,6 +68,16 @@ def _with_gradients():
     operators: torch.compile breaks its graph at them, where it would run the operators on tensors without memory.)"""
     ops = L.load_torch()
     return ops.enter.default._op, ops.leave.default._op, ops.leave_enter.default._op
+
+
+def _record(call: int, *args):
+    try:
+        return _with_gradients()[call](*args)
+    except RuntimeError as e:
+        found = _ERROR.match(str(e))
+        if found is None:
+            raise
+        raise L.BrxError(int(found[1]), found[2]) from None
 
 
 def _vector(t, H: int, what: str):
@@ -147,7 +160,7 @@ def enter(x, weight=None, eps: float = EPS, dtype=None, stream=None):
     _check_count(x2.shape[0])
     if _recorded(x2, weight):
         _on_device(x2, weight)
-        h = _with_gradients()[0](x2, weight, eps, dtype)
+        h = _record(_ENTER, x2, weight, eps, dtype)
     else:
         h = _forward(None, x2, None, None, _NO_GATE, weight, 1.0, eps, True, dtype)[1]
     return h if h.shape == x.shape else h.view(x.shape)
@@ -182,9 +195,9 @@ def leave(y, residual, weight=None, gate=None, scale: float = 1.0, next_weight=N
     if _recorded(y2, r2, weight, gate, next_weight):
         _on_device(y2, r2, weight, gate, next_weight)
         if make_h:
-            new, h = _with_gradients()[2](y2, r2, weight, gate, form, scale, next_weight, eps)
+            new, h = _record(_LEAVE_ENTER, y2, r2, weight, gate, form, scale, next_weight, eps)
         else:
-            new, h = _with_gradients()[1](y2, r2, weight, gate, form, scale, eps), None
+            new, h = _record(_LEAVE, y2, r2, weight, gate, form, scale, eps), None
     else:
         new, h = _forward(y2, r2, weight, gate, form, next_weight, scale, eps, make_h, y.dtype)
     if new.shape != y.shape:

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from bigrig_amd import lib as L
+from bigrig_amd import norm as M
 
 
 def test_calls_are_registered():
@@ -27,3 +28,16 @@ def test_a_missing_library_is_an_error(monkeypatch):
     monkeypatch.setattr(L, "TORCH_LIB", L.TORCH_LIB + ".missing")
     with pytest.raises(RuntimeError, match="missing"):
         L.load_torch()
+
+
+def test_its_errors_are_the_librarys(monkeypatch):
+    def fails(*args):
+        raise RuntimeError("libbrx error -2: brx_init was not called\nwhere it was raised")
+
+    monkeypatch.setattr(M, "_with_gradients", lambda: (fails,) * 3)
+    monkeypatch.setattr(M, "_on_device", lambda *t: 0)
+    x = torch.zeros((2, 8), requires_grad=True)
+    for call in (lambda: M.enter(x), lambda: M.leave(x, x), lambda: M.leave(x, x, next_weight=torch.ones(8))):
+        with pytest.raises(L.BrxError, match="brx_init") as e:
+            call()
+        assert e.value.code == L.BRX_ESTATE
