@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kThinThreads) void k_grouped_thin(GroupedArgs g, in
 //
 // Bound: the copies. 32768 rows of 8 experts of 4096 x 4096 take 890 us (1.24 PFLOP/s; 730 without copies, 690 without
 // products), of 128 experts of 1536 x 2048 (256 rows each) 290 (280 without products; the matrices alone, 805 MB, take 150).
-// One stage ahead instead of one and a half: 940 and 316. One tile a block, 128 x 128 with two blocks a CU: 1250 and 340.
+// (Timed in turn on one part; on another 942 and 297.) One stage ahead instead of one and a half: 940 and 316. One tile a block, 128 x 128 with two blocks a CU: 1250 and 340.
 #define BRX_FENCE() __builtin_amdgcn_sched_barrier(0)
 __device__ __forceinline__ void meet() {
     BRX_FENCE();
