@@ -59,26 +59,30 @@ def _dtype(t, what: str) -> int:
     return dt
 
 
+_is_tracing = torch._C._is_tracing
+_modes = torch._C._len_torch_dispatch_stack
+
+
 def _refuse_recorders() -> None:
     """A recorder of torch's operations (`torch.jit.trace`, make_fx) sees a launch's allocations only: its program would read
     memory that nothing wrote. (A trace would hold an autograd function, but not the checks of shapes before it.)"""
-    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack()
-                                  and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+    if _is_tracing() or (_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
         raise RuntimeError("torch's operations are being recorded: a recorded program would not hold this call")
 
 
 def _refuse_tangents(tensors) -> None:
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError("a tensor with a tangent: there are no forward-mode derivatives")
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("a tensor with a tangent: there are no forward-mode derivatives")
 
 
 def _recorded(*tensors) -> bool:
     """Whether a gradient is recorded of a call. It is refused where its result would silently lack a derivative or a
     program the call."""
-    _refuse_recorders()
-    _refuse_tangents(tensors)
+    if _is_tracing() or _modes():
+        _refuse_recorders()
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -174,7 +178,8 @@ def _once(backward):
     def call(ctx, *grads):
         if torch.is_grad_enabled():
             raise RuntimeError("this gradient is taken once: create_graph=True is refused")
-        _refuse_tangents(grads)
+        if forward_ad._current_level >= 0:
+            _refuse_tangents(grads)
         return backward(ctx, *grads)
     return call
 

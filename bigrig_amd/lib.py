@@ -139,6 +139,8 @@ _SIGS = {
 def load(path: str | None = None):
     """Open libbrx.so and declare its signatures (no GPU call is made)."""
     global _lib
+    if _lib is not None and path is None:       # (set once, whole)
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib
